@@ -35,6 +35,7 @@
 #ifndef MSX_SPARSE_H
 #define MSX_SPARSE_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -926,6 +927,152 @@ msx_status msx_csr_batched_spmm_cpu(msx_vtype vt, msx_itype it, int64_t n_rows,
                                     const void *data, const void *indices,
                                     const void *indptr, int64_t batch, int64_t k,
                                     const void *X, void *Y, int n_threads);
+
+/*
+ * Window attention with sinks.  Query i of a sequence stands at position
+ * p = i + lk - lq and sees key j iff 0 <= j <= p, j < n and
+ * (p - j < window or j < sinks), where n is the sequence's length (lk without
+ * `lengths`); a query with p < 0 or p >= n sees nothing.  Query head h reads
+ * kv head h / (heads / kv_heads).
+ *
+ *   out = sum_j softmax_j(scale * q.k_j) v_j,  zeros where nothing is seen
+ *
+ * The pattern is the CSR pattern of a band and a few dense columns; it is
+ * never stored.  Scores, softmax statistics and sums are float32 whatever the
+ * storage type.  Values of keys that no query of a sequence sees, and of
+ * tokens at or beyond n, are not used (they may be NaN).
+ */
+typedef struct msx_window_attention_desc {
+  int32_t vtype;         /* MSX_F32, MSX_F16 or MSX_BF16 */
+  int32_t lengths_itype; /* msx_itype of `lengths` */
+  int64_t batch, lq, lk; /* lq, lk < 2^30 */
+  int64_t heads, kv_heads;
+  int64_t dim;           /* 1 .. 256 */
+  int64_t window;        /* >= 1 */
+  int64_t sinks;         /* >= 0 */
+  double scale;
+  const void *lengths;   /* batch values, or NULL */
+  const void *q, *k, *v;
+  /* (sequence, token, head), in values; the values of a head are adjacent */
+  int64_t q_strides[3], k_strides[3], v_strides[3];
+} msx_window_attention_desc;
+
+/*
+ * Forward product: `out` is batch x lq x heads x dim, contiguous.  `lse`
+ * (NULL, or batch x heads x lq floats) gets what the backward pass needs of
+ * the softmax: the base-2 logarithm of its sum, +inf for a row without one.
+ */
+msx_status msx_window_attention(const msx_window_attention_desc *desc, void *out,
+                                float *lse, void *stream);
+
+/*
+ * Gradients of the product: `grad` is the gradient of `out`, with strides as
+ * q's; dq, dk and dv are contiguous and shaped as q, k and v.  `out` and
+ * `lse` come from the forward call.  `scratch` holds
+ * msx_window_attention_backward_scratch bytes.  Every gradient is summed in a
+ * fixed order (no atomics): the same inputs give the same bits.
+ */
+size_t msx_window_attention_backward_scratch(const msx_window_attention_desc *desc);
+msx_status msx_window_attention_backward(const msx_window_attention_desc *desc, const void *out,
+                                         const float *lse, const void *grad,
+                                         const int64_t *grad_strides, void *dq, void *dk,
+                                         void *dv, void *scratch, size_t scratch_bytes,
+                                         void *stream);
+
+/*
+ * One token of every sequence against its ring cache.  `lengths[b]` tokens
+ * came before it, so it stands at position p = lengths[b]; its key and value
+ * are written to the cache and the query attends to what it sees there.
+ * Position j lies in slot j while j < sinks and in slot
+ * sinks + (j - sinks) mod (slots - sinks) from there on; slots >= sinks +
+ * window.  A cache with a slot for every position never wraps.  A sequence of
+ * negative length is left alone and gets zeros.
+ */
+typedef struct msx_window_step_desc {
+  int32_t vtype;         /* MSX_F32, MSX_F16 or MSX_BF16 */
+  int32_t lengths_itype; /* msx_itype of `lengths` */
+  int64_t batch, heads, kv_heads, dim, slots, window, sinks;
+  double scale;
+  const void *lengths;
+  const void *q, *k, *v;
+  int64_t q_strides[2], k_strides[2], v_strides[2]; /* (sequence, head) */
+  void *cache_k, *cache_v;
+  int64_t cache_k_strides[3], cache_v_strides[3];   /* (sequence, slot, head) */
+} msx_window_step_desc;
+
+/* `out` is batch x heads x dim, contiguous; `scratch` holds
+ * msx_window_attention_step_scratch bytes. */
+size_t msx_window_attention_step_scratch(const msx_window_step_desc *desc);
+msx_status msx_window_attention_step(const msx_window_step_desc *desc, void *out, void *scratch,
+                                     size_t scratch_bytes, void *stream);
+
+/*
+ * A prompt's keys and values into the ring cache: the tokens at positions
+ * start[b] .. start[b] + length[b] - 1 that a query at the last of them or
+ * later can still see (`starts` NULL: 0; `lengths` NULL: all `tokens`).  Of
+ * the step's descriptor the fields vtype, batch, kv_heads, dim, slots, sinks
+ * and the caches are read; k and v are batch x tokens x kv_heads x dim with
+ * (sequence, token, head) strides.
+ */
+msx_status msx_window_cache_store(const msx_window_step_desc *desc, int64_t tokens, const void *k,
+                                  const int64_t *k_strides, const void *v,
+                                  const int64_t *v_strides, msx_itype itype, const void *starts,
+                                  const void *lengths, void *stream);
+
+/*
+ * Distillation from a teacher's top logits.  Row i of a CSR matrix holds the
+ * logits the teacher kept for token i; row i of `logits` (row stride ld) the
+ * student's.  With p the softmax of the kept logits / temperature and q the
+ * softmax of the whole row / temperature
+ *
+ *   losses[i] = temperature^2 sum_r p_r (ln p_r - ln q_r)
+ *   grad[i]   = weights[i] temperature (q - p)      (weights NULL: ones)
+ *
+ * grad is the gradient of sum_i weights[i] losses[i] in the logits, n_rows x
+ * n_cols with row stride ld_grad.  A row without a kept logit (none stored,
+ * all -inf, columns outside [0, n_cols)) has loss and gradient zero, a row of
+ * weight zero the gradient zero; its logits may be anything.  A column stored
+ * twice counts twice.  Sums and statistics are float32; the gradient is
+ * rounded once.  `lse` (n_rows floats, or NULL): written by the losses, read
+ * by msx_distill_grad, which computes the gradient alone.
+ */
+typedef struct msx_distill_desc {
+  int32_t vtype;         /* of logits and grad: MSX_F32, MSX_F16 or MSX_BF16 */
+  int32_t teacher_vtype; /* of the kept logits: one of the same three */
+  int32_t itype;         /* of indices and indptr */
+  int32_t reserved;
+  int64_t n_rows, n_cols, nnz, ld;
+  double temperature;    /* > 0 */
+  const void *logits;
+  const void *data, *indices, *indptr;
+  const float *weights;
+  int64_t weights_stride; /* 0: one weight for all rows */
+} msx_distill_desc;
+
+msx_status msx_distill_loss(const msx_distill_desc *desc, float *losses, float *lse, void *stream);
+msx_status msx_distill_grad(const msx_distill_desc *desc, const float *lse, void *grad,
+                            int64_t ld_grad, void *stream);
+msx_status msx_distill_loss_grad(const msx_distill_desc *desc, float *losses, void *grad,
+                                 int64_t ld_grad, void *stream);
+
+/* The same on the host: one row, head or token after the other, in float32
+ * sums, split over `n_threads` threads (0: msx_cpu_worker_count). */
+msx_status msx_window_attention_cpu(const msx_window_attention_desc *desc, void *out, float *lse,
+                                    int n_threads);
+msx_status msx_window_attention_backward_cpu(const msx_window_attention_desc *desc,
+                                             const void *out, const float *lse, const void *grad,
+                                             const int64_t *grad_strides, void *dq, void *dk,
+                                             void *dv, int n_threads);
+msx_status msx_window_attention_step_cpu(const msx_window_step_desc *desc, void *out,
+                                         int n_threads);
+msx_status msx_window_cache_store_cpu(const msx_window_step_desc *desc, int64_t tokens,
+                                      const void *k, const int64_t *k_strides, const void *v,
+                                      const int64_t *v_strides, msx_itype itype,
+                                      const void *starts, const void *lengths);
+msx_status msx_distill_loss_cpu(const msx_distill_desc *desc, float *losses, float *lse,
+                                int n_threads);
+msx_status msx_distill_grad_cpu(const msx_distill_desc *desc, const float *lse, void *grad,
+                                int64_t ld_grad, int n_threads);
 
 /*
  * CPU worker count resolved from the environment: MLX_SPARSE_CPU_THREADS,

@@ -1,0 +1,63 @@
+// msx_window.h - device-side view of window attention: the operands, and
+// which keys a query sees.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "msx_device.h"
+#include "msx_sparse.h"
+
+namespace msx {
+
+// Operands of one product, as the kernels take them (strides in values).
+struct WindowArgs {
+  int64_t batch;
+  int32_t lq, lk, heads, kv_heads, group, dim;
+  int32_t window, sinks;  // capped at lk: no wider span changes the pattern
+  float scale;            // scale * log2(e): scores are kept in base 2
+  float grad_scale;       // scale
+  const void *lengths;
+  int32_t lengths64;
+  const void *q, *k, *v;
+  int64_t qs[3], ks[3], vs[3];
+
+  // Tokens of sequence b that exist: [0, lk].
+  __device__ inline int32_t length(int64_t b) const {
+    if (lengths == nullptr) return lk;
+    const int64_t n = lengths64 ? static_cast<const int64_t *>(lengths)[b]
+                                : static_cast<const int32_t *>(lengths)[b];
+    return static_cast<int32_t>(n < 0 ? 0 : n > lk ? lk : n);
+  }
+};
+
+// Logarithms are base 2: exp2 is one instruction, and a score times log2(e)
+// costs nothing beside the scale.
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+
+__device__ inline float wave_max(float v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// The keys that the query at position p sees, numbered: the first `far` are
+// keys 0 .. far - 1, the others near .. p.
+struct Seen {
+  int32_t near, far;
+  __device__ inline Seen(int32_t p, int32_t window, int32_t sinks)
+      : near(p >= window ? p - window + 1 : 0), far(sinks < near ? sinks : near) {}
+  __device__ inline int32_t count(int32_t p) const { return far + p - near + 1; }
+  __device__ inline int32_t key(int32_t c) const { return c < far ? c : near + c - far; }
+};
+
+}  // namespace msx

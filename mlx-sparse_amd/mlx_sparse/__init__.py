@@ -6,8 +6,10 @@ hand-written gfx950 HIP kernels behind the C ABI in ``include/msx_sparse.h``.
 from __future__ import annotations
 
 from mlx_sparse import linalg, runtime
+from mlx_sparse._attention import window_attention, window_attention_step, window_cache_store
 from mlx_sparse._csr import CSRArray, csr_array
 from mlx_sparse._device import default_torch_device, use_cpu, use_device, use_gpu
+from mlx_sparse._distill import distill_loss, distill_value_and_grad
 from mlx_sparse._io import from_scipy, mminfo, mmread
 from mlx_sparse._ops import (
     csr_batched_matmul,
@@ -41,6 +43,8 @@ __all__ = [
     "csr_matvec",
     "csr_matvec_transpose",
     "default_torch_device",
+    "distill_loss",
+    "distill_value_and_grad",
     "from_scipy",
     "is_available",
     "linalg",
@@ -50,4 +54,7 @@ __all__ = [
     "use_cpu",
     "use_device",
     "use_gpu",
+    "window_attention",
+    "window_attention_step",
+    "window_cache_store",
 ]

@@ -1,0 +1,285 @@
+"""Window attention with sinks: attention over the sparse pattern of a band and
+a few dense columns.
+
+The query at position ``p`` sees the last ``window`` keys, its own among them,
+and the first ``sinks`` keys of its sequence.  As a CSR matrix that pattern
+would hold ``window + sinks`` columns a row, its scores would be one value
+gradient (a sampled product), its output one SpMM; here the two integers are
+the pattern, and scores and probabilities exist only inside the kernels.
+
+- :func:`window_attention`: a whole sequence, a prompt or a chunk of one, with
+  derivatives in queries, keys and values;
+- :func:`window_attention_step`: one token of every sequence against a ring
+  cache that holds no more than what can still be seen;
+- :func:`window_cache_store`: a prompt's keys and values into that cache.
+"""
+
+from __future__ import annotations
+
+import inspect
+import operator
+
+import torch
+from torch.autograd import forward_ad
+
+import mlx_sparse._native as _native
+from mlx_sparse._autograd import _call
+from mlx_sparse._device import default_torch_device
+from mlx_sparse._validation import ensure_array
+
+_REAL = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _span(name: str, window, sinks) -> tuple[int, int]:
+    window, sinks = operator.index(window), operator.index(sinks)
+    if window < 1:
+        raise ValueError(f"{name} window must be at least 1, got {window}.")
+    if sinks < 0:
+        raise ValueError(f"{name} sinks must be non-negative, got {sinks}.")
+    # no sequence is as long: wider spans are the same pattern
+    return min(window, 2**40), min(sinks, 2**40)
+
+
+def _operand(value, device) -> torch.Tensor:
+    """On ``device``, its own values in memory, the last dimension adjacent."""
+    t = ensure_array(value, device=device)
+    if t.is_neg():
+        t = t.resolve_neg()
+    if t.ndim and t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t
+
+
+def _counts(value, device) -> torch.Tensor | None:
+    return None if value is None else ensure_array(value, device=device).contiguous()
+
+
+def _check_dtypes(name: str, q: torch.Tensor, **others: torch.Tensor) -> None:
+    if q.dtype not in _REAL:
+        raise TypeError(f"{name} supports float32, float16 and bfloat16, got {q.dtype}.")
+    for other, t in others.items():
+        if t.dtype != q.dtype:
+            raise TypeError(f"{name} requires one dtype for all operands, got {q.dtype} and "
+                            f"{other} of {t.dtype}.")
+
+
+def _check_heads(name: str, heads: int, kv_heads: int, dim: int) -> None:
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{name} query heads ({heads}) must be a multiple of the key and value "
+                         f"heads ({kv_heads}).")
+    if not 1 <= dim <= 256:
+        raise ValueError(f"{name} head dimension must be between 1 and 256, got {dim}.")
+
+
+def _scale(scale, dim: int) -> float:
+    return dim ** -0.5 if scale is None else float(scale)
+
+
+def _tracked(*tensors: torch.Tensor) -> bool:
+    if torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+class _WindowAttention(torch.autograd.Function):
+    """``(out, lse)``; ``lse`` is the backward pass's and has no derivative."""
+
+    @staticmethod
+    def forward(q, k, v, lengths, window, sinks, scale):
+        return _native.window_attention(q, k, v, lengths, window, sinks, scale, True)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        q, k, v, lengths, window, sinks, scale = inputs
+        out, lse = output
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        ctx.pattern = (window, sinks, scale)
+        ctx.has_lengths = lengths is not None
+        ctx.save_for_backward(q, k, v, out, lse, *((lengths,) if ctx.has_lengths else ()))
+
+    @staticmethod
+    def backward(ctx, grad, _lse):
+        if grad is None:
+            return (None,) * 7
+        q, k, v, out, lse, *rest = ctx.saved_tensors
+        got = _call(_WindowGradients, q, k, v, rest[0] if ctx.has_lengths else None, out, lse,
+                    grad, *ctx.pattern)
+        return (*(g if needed else None for g, needed in zip(got, ctx.needs_input_grad)),
+                None, None, None, None)
+
+    @staticmethod
+    def vmap(info, in_dims, q, k, v, lengths, window, sinks, scale):
+        """The mapped axis joins the batch."""
+        n = info.batch_size
+
+        def folded(t, dim):
+            t = t.unsqueeze(0).expand(n, *t.shape) if dim is None else t.movedim(dim, 0)
+            return t.reshape(n * t.shape[1], *t.shape[2:])
+
+        q, k, v = (folded(t, d) for t, d in zip((q, k, v), in_dims))
+        if lengths is not None:
+            lengths = folded(lengths, in_dims[3]).contiguous()
+        out, lse = _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
+        return (out.reshape(n, -1, *out.shape[1:]), lse.reshape(n, -1, *lse.shape[1:])), (0, 0)
+
+
+class _WindowGradients(torch.autograd.Function):
+    """``(dq, dk, dv)``; no derivative of their own."""
+
+    @staticmethod
+    def forward(q, k, v, lengths, out, lse, grad, window, sinks, scale):
+        return _native.window_attention_backward(q, k, v, lengths, out, lse,
+                                                 _operand(grad, grad.device), window, sinks, scale)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError("second-order derivatives of window_attention are not supported.")
+
+
+for _function in (_WindowAttention, _WindowGradients):
+    _function.forward.__signature__ = inspect.signature(_function.forward)
+
+
+def window_attention(q, k, v, *, window: int, sinks: int = 0, scale: float | None = None,
+                     lengths=None) -> torch.Tensor:
+    """Attention of every query over the last ``window`` keys and the first
+    ``sinks`` keys of its sequence.
+
+    Query ``i`` stands at position ``p = i + k_tokens - q_tokens`` (a chunk of
+    a prompt ends where its keys end) and sees key ``j`` where ``j <= p`` and
+    either ``p - j < window`` or ``j < sinks``.  A query that sees nothing
+    gives zeros.
+
+    Args:
+        q: Queries, shape ``(batch, q_tokens, heads, dim)``.
+        k: Keys, shape ``(batch, k_tokens, kv_heads, dim)``; ``heads`` is a
+            multiple of ``kv_heads``, and consecutive query heads share one.
+        v: Values, shaped as ``k``.
+        window: Keys a query sees, its own position included.
+        sinks: First keys that stay visible.
+        scale: Factor of the scores, ``dim ** -0.5`` by default.
+        lengths: Tokens of each sequence, shape ``(batch,)``, int32 or int64:
+            keys and queries at or beyond them are padding (a padding query
+            gives zeros and takes no part in the gradients).
+
+    Returns:
+        Shape ``(batch, q_tokens, heads, dim)``, the dtype of ``q``.
+        Differentiable once in ``q``, ``k`` and ``v``.
+
+    Operands are float32, float16 or bfloat16, of one dtype, ``dim`` at most
+    256; any strides with adjacent head values are read in place.  Scores,
+    softmax and sums are float32; 16-bit operands round probabilities to their
+    own type for the products with values, which costs no more than the
+    rounding of the result.
+
+    Raises:
+        TypeError: dtypes differ or are unsupported.
+        ValueError: shapes, ``window`` or ``sinks`` are out of range.
+    """
+    window, sinks = _span("window_attention", window, sinks)
+    device = default_torch_device()
+    q, k, v = _operand(q, device), _operand(k, device), _operand(v, device)
+    lengths = _counts(lengths, device)
+    _check_dtypes("window_attention", q, k=k, v=v)
+    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape:
+        raise ValueError("window_attention expects q of shape (batch, q_tokens, heads, dim) and "
+                         "k and v of shape (batch, k_tokens, kv_heads, dim), got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}.")
+    if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("window_attention q and k differ in batch or head dimension: "
+                         f"{tuple(q.shape)} and {tuple(k.shape)}.")
+    _check_heads("window_attention", q.shape[2], k.shape[2], q.shape[3])
+    scale = _scale(scale, q.shape[3])
+    if _tracked(q, k, v):
+        return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)[0]
+    return _native.window_attention(q, k, v, lengths, window, sinks, scale, False)[0]
+
+
+def _cache(name: str, cache, device) -> torch.Tensor:
+    """Caches are written in place, so none is moved or copied."""
+    if not isinstance(cache, torch.Tensor):
+        raise TypeError(f"{name} caches must be torch tensors.")
+    if cache.device != device:
+        raise ValueError(f"{name} caches must be on {device}, got {cache.device}.")
+    if cache.requires_grad:
+        raise ValueError(f"{name} caches are updated in place and cannot require grad.")
+    return cache
+
+
+def window_attention_step(q, k, v, cache_k, cache_v, lengths, *, window: int, sinks: int = 0,
+                          scale: float | None = None) -> torch.Tensor:
+    """One token of every sequence: its key and value go into the ring cache,
+    its query attends to what it sees there.
+
+    Position ``j`` of a sequence lies in slot ``j`` while ``j < sinks`` and in
+    slot ``sinks + (j - sinks) % (slots - sinks)`` from there on, so ``sinks +
+    window`` slots serve a sequence of any length; a cache with a slot for
+    every position never wraps.
+
+    Args:
+        q: Queries, shape ``(batch, heads, dim)``.
+        k, v: The tokens' keys and values, shape ``(batch, kv_heads, dim)``.
+        cache_k, cache_v: Ring caches, shape ``(batch, slots, kv_heads,
+            dim)``, updated in place; on the selected device.
+        lengths: Tokens before this one, shape ``(batch,)``, int32 or int64
+            (not changed: one counter serves the caches of all layers).  A
+            negative length marks a slot of the batch without a sequence: its
+            caches are left alone and it gives zeros.
+        window, sinks, scale: As in :func:`window_attention`.
+
+    Returns:
+        Shape ``(batch, heads, dim)``, the dtype of ``q``.  Not
+        differentiable.
+    """
+    name = "window_attention_step"
+    window, sinks = _span(name, window, sinks)
+    device = default_torch_device()
+    q, k, v = (_operand(t, device).detach() for t in (q, k, v))
+    cache_k, cache_v = _cache(name, cache_k, device), _cache(name, cache_v, device)
+    lengths = _counts(lengths, device)
+    if lengths is None:
+        raise TypeError(f"{name} requires lengths.")
+    _check_dtypes(name, q, k=k, v=v, cache_k=cache_k, cache_v=cache_v)
+    if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape:
+        raise ValueError(f"{name} expects q of shape (batch, heads, dim) and k and v of shape "
+                         f"(batch, kv_heads, dim), got {tuple(q.shape)}, {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}.")
+    _check_heads(name, q.shape[1], k.shape[1], q.shape[2])
+    if cache_k.ndim == 4 and sinks + window > cache_k.shape[1]:
+        raise ValueError(f"{name} cache needs at least sinks + window = {sinks + window} slots, "
+                         f"got {cache_k.shape[1]}.")
+    out = _native.window_attention_step(q, k, v, cache_k, cache_v, lengths, window, sinks,
+                                        _scale(scale, q.shape[2]))
+    return out
+
+
+def window_cache_store(k, v, cache_k, cache_v, *, sinks: int = 0, starts=None,
+                       lengths=None) -> None:
+    """A prompt's keys and values into ring caches (the layout of
+    :func:`window_attention_step`): of the tokens given, those that lie among
+    the first ``sinks`` positions or among the last ``slots - sinks``.
+
+    Args:
+        k, v: Shape ``(batch, tokens, kv_heads, dim)``.
+        cache_k, cache_v: Shape ``(batch, slots, kv_heads, dim)``, updated in
+            place.
+        sinks: First positions that keep their slots.
+        starts: Position of each sequence's first token here, shape
+            ``(batch,)``; zero by default.
+        lengths: Tokens of each sequence here, all by default.
+    """
+    name = "window_cache_store"
+    sinks = operator.index(sinks)
+    device = default_torch_device()
+    k, v = _operand(k, device).detach(), _operand(v, device).detach()
+    cache_k, cache_v = _cache(name, cache_k, device), _cache(name, cache_v, device)
+    starts, lengths = _counts(starts, device), _counts(lengths, device)
+    _check_dtypes(name, k, v=v, cache_k=cache_k, cache_v=cache_v)
+    if starts is not None and lengths is not None and starts.dtype != lengths.dtype:
+        starts = starts.to(lengths.dtype)
+    _native.window_cache_store(k, v, cache_k, cache_v, starts, lengths, sinks)

@@ -1,0 +1,183 @@
+"""Distillation from a teacher's top logits, which are a sparse matrix: row
+``i`` of a ``CSRArray`` of shape ``(tokens, vocabulary)`` holds the logits
+that the teacher kept for token ``i``, an empty row is a token without a
+target.
+
+With ``q`` the softmax of a student's row over the temperature ``T`` and
+``p`` the softmax of the kept logits over ``T``:
+
+    loss = T^2 sum_r p_r (ln p_r - ln q_r)      (r over the kept columns)
+    gradient in the student's logits = weight T (q - p)
+
+- :func:`distill_loss`: the rows' losses, differentiable in the logits;
+- :func:`distill_value_and_grad`: losses and gradient in one call, which reads
+  the logits from memory once where the derivative of :func:`distill_loss`
+  reads them again.
+"""
+
+from __future__ import annotations
+
+import inspect
+import math
+
+import torch
+from torch.autograd import forward_ad
+
+import mlx_sparse._native as _native
+from mlx_sparse._autograd import _call
+from mlx_sparse._csr import CSRArray
+from mlx_sparse._device import default_torch_device
+from mlx_sparse._validation import ensure_array
+
+_REAL = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _prepared(name: str, logits, teacher: CSRArray, temperature: float):
+    """The logits as rows, the teacher's buffers beside them, T."""
+    if not isinstance(teacher, CSRArray):
+        raise TypeError(f"{name} expects a CSRArray teacher, got {type(teacher).__name__}.")
+    device = default_torch_device()
+    logits = ensure_array(logits, device=device)
+    if logits.dtype not in _REAL:
+        raise TypeError(f"{name} supports float32, float16 and bfloat16 logits, got "
+                        f"{logits.dtype}.")
+    if teacher.dtype not in _REAL:
+        raise TypeError(f"{name} supports float32, float16 and bfloat16 teachers, got "
+                        f"{teacher.dtype}.")
+    if logits.ndim < 2:
+        raise ValueError(f"{name} expects logits of shape (..., tokens, vocabulary), got "
+                         f"{tuple(logits.shape)}.")
+    rows = math.prod(logits.shape[:-1])
+    if teacher.shape != (rows, logits.shape[-1]):
+        raise ValueError(f"{name} expects a teacher of shape {(rows, logits.shape[-1])}, got "
+                         f"{teacher.shape}.")
+    if teacher.data.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} has no derivative in the teacher: detach its values.")
+    temperature = float(temperature)
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"{name} temperature must be positive and finite, got {temperature}.")
+    return logits, teacher.buffers(device), temperature
+
+
+def _rows(logits: torch.Tensor) -> torch.Tensor:
+    """(rows, vocabulary) with adjacent columns, in place where they are."""
+    z = logits if logits.ndim == 2 else logits.reshape(-1, logits.shape[-1])
+    if z.is_neg():
+        z = z.resolve_neg()
+    usable = (z.shape[1] < 2 or z.stride(1) == 1) and (z.shape[0] < 2 or z.stride(0) >= z.shape[1])
+    return z if usable else z.contiguous()
+
+
+class _DistillLoss(torch.autograd.Function):
+    """``(losses, lse)`` of rows of logits."""
+
+    @staticmethod
+    def forward(z, data, indices, indptr, temperature):
+        return _native.distill_loss(z, data, indices, indptr, temperature, True)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        z, data, indices, indptr, temperature = inputs
+        ctx.temperature = temperature
+        ctx.mark_non_differentiable(output[1])
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(z, data, indices, indptr, output[1])
+
+    @staticmethod
+    def backward(ctx, grad, _lse):
+        if grad is None or not ctx.needs_input_grad[0]:
+            return (None,) * 5
+        z, data, indices, indptr, lse = ctx.saved_tensors
+        return (_call(_DistillGradient, z, data, indices, indptr, grad, lse, ctx.temperature),
+                None, None, None, None)
+
+
+class _DistillGradient(torch.autograd.Function):
+    """The gradient in the logits; no derivative of its own."""
+
+    @staticmethod
+    def forward(z, data, indices, indptr, grad, lse, temperature):
+        return _native.distill_grad(z, data, indices, indptr, grad.resolve_neg(), lse, temperature)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError("second-order derivatives of distill_loss are not supported.")
+
+
+for _function in (_DistillLoss, _DistillGradient):
+    _function.forward.__signature__ = inspect.signature(_function.forward)
+
+
+def distill_loss(logits, teacher: CSRArray, *, temperature: float = 1.0) -> torch.Tensor:
+    """Per-token divergence of a student from a teacher's kept logits.
+
+    Args:
+        logits: The student's logits, shape ``(..., vocabulary)``, float32,
+            float16 or bfloat16.
+        teacher: ``CSRArray`` of shape ``(tokens, vocabulary)``, ``tokens`` the
+            product of the leading dimensions: the teacher's kept logits (of
+            any of the three dtypes), columns in any order.
+        temperature: Divides both sides' logits.
+
+    Returns:
+        float32 losses of shape ``logits.shape[:-1]``, ``temperature**2`` times
+        the divergence; differentiable once in ``logits``.  A row without a
+        kept logit (none stored, all ``-inf``) has loss and gradient zero
+        whatever its logits are; so has the gradient of a row whose upstream
+        gradient is zero.
+
+    Raises:
+        TypeError: ``teacher`` is not a CSRArray or a dtype is unsupported.
+        ValueError: shapes or ``temperature`` do not fit.
+    """
+    logits, (data, indices, indptr), temperature = _prepared("distill_loss", logits, teacher,
+                                                             temperature)
+    z = _rows(logits)
+    if (torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
+            or (torch.is_grad_enabled() and z.requires_grad)):
+        losses = _DistillLoss.apply(z, data, indices, indptr, temperature)[0]
+    else:
+        losses = _native.distill_loss(z, data, indices, indptr, temperature, False)[0]
+    return losses if logits.ndim == 2 else losses.reshape(logits.shape[:-1])
+
+
+def distill_value_and_grad(logits, teacher: CSRArray, weights=None, *,
+                           temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows' losses and the gradient of their weighted sum, in one call.
+
+    ``logits.backward(gradient)`` continues the derivative from here.
+
+    Args:
+        logits, teacher, temperature: As in :func:`distill_loss`.
+        weights: Weight of each token, shape ``logits.shape[:-1]`` (a number
+            for one of all); ones by default.  A row of weight zero has
+            gradient zero whatever its logits are.
+
+    Returns:
+        ``(losses, gradient)``: float32 losses as :func:`distill_loss` returns
+        them (not weighted), and the gradient of ``(weights * losses).sum()``,
+        shaped as ``logits`` and of their dtype.
+    """
+    name = "distill_value_and_grad"
+    logits, (data, indices, indptr), temperature = _prepared(name, logits, teacher, temperature)
+    lead = logits.shape[:-1]
+    if weights is not None:
+        if not isinstance(weights, torch.Tensor):
+            weights = torch.as_tensor(weights, dtype=torch.float32)
+        weights = weights.detach().to(device=logits.device, dtype=torch.float32).resolve_neg()
+        if weights.ndim == 0:
+            weights = weights.expand(lead)
+        if weights.shape != lead:
+            raise ValueError(f"{name} weights must have shape {tuple(lead)}, got "
+                             f"{tuple(weights.shape)}.")
+        if weights.ndim != 1:
+            weights = weights.reshape(-1)
+    losses, grad = _native.distill_loss_grad(_rows(logits.detach()), data, indices, indptr, weights,
+                                             temperature)
+    if logits.ndim == 2:
+        return losses, grad
+    return losses.reshape(lead), grad.reshape(logits.shape)

@@ -156,3 +156,42 @@ def csr_plan(indptr, n_rows: int, nnz: int, block_nnz: int = 0, *, data=None, in
     wait where only many products repay their build)."""
     return extension().csr_plan(indptr, n_rows, nnz, block_nnz, data=data, indices=indices,
                                 n_cols=n_cols, slice_mode=slice_mode, defer=defer)
+
+
+def window_attention(q, k, v, lengths, window: int, sinks: int, scale: float, with_lse: bool):
+    """(out, lse or None) of attention over a band and sink columns."""
+    return extension().window_attention(q, k, v, lengths, window, sinks, scale, with_lse)
+
+
+def window_attention_backward(q, k, v, lengths, out, lse, grad, window: int, sinks: int,
+                              scale: float):
+    """(dq, dk, dv) of window_attention."""
+    return extension().window_attention_backward(q, k, v, lengths, out, lse, grad, window, sinks,
+                                                 scale)
+
+
+def window_attention_step(q, k, v, cache_k, cache_v, lengths, window: int, sinks: int,
+                          scale: float) -> torch.Tensor:
+    """One token of every sequence against its ring cache (updated in place)."""
+    return extension().window_attention_step(q, k, v, cache_k, cache_v, lengths, window, sinks,
+                                             scale)
+
+
+def window_cache_store(k, v, cache_k, cache_v, starts, lengths, sinks: int) -> None:
+    """A prompt's keys and values into ring caches, in place."""
+    extension().window_cache_store(k, v, cache_k, cache_v, starts, lengths, sinks)
+
+
+def distill_loss(logits, data, indices, indptr, temperature: float, with_lse: bool):
+    """(losses, lse or None) against a CSR teacher's kept logits."""
+    return extension().distill_loss(logits, data, indices, indptr, temperature, with_lse)
+
+
+def distill_grad(logits, data, indices, indptr, weights, lse, temperature: float) -> torch.Tensor:
+    """Gradient of the weighted losses in the logits."""
+    return extension().distill_grad(logits, data, indices, indptr, weights, lse, temperature)
+
+
+def distill_loss_grad(logits, data, indices, indptr, weights, temperature: float):
+    """(losses, gradient of the weighted losses)."""
+    return extension().distill_loss_grad(logits, data, indices, indptr, weights, temperature)

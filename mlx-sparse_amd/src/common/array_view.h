@@ -16,17 +16,18 @@ struct ArrayView {
   void *ptr = nullptr;
   DType dtype = DType::Other;
   std::string dtype_name;  // framework spelling, for error texts
-  int ndim = 0;                     // the layer handles ranks 0..3
-  int64_t shape[3] = {0, 0, 0};
-  int64_t strides[3] = {1, 1, 1};  // in elements
+  int ndim = 0;                        // the layer handles ranks 0..4
+  int64_t shape[4] = {0, 0, 0, 0};
+  int64_t strides[4] = {1, 1, 1, 1};  // in elements
   int device = -1;                 // -1: host memory; >= 0: HIP device ordinal
 
   int64_t size() const {
     int64_t s = 1;
-    for (int i = 0; i < ndim && i < 3; ++i) s *= shape[i];
+    for (int i = 0; i < ndim && i < 4; ++i) s *= shape[i];
     return ndim == 0 ? 1 : s;
   }
   bool contiguous() const {
+    if (size() == 0) return true;
     int64_t expect = 1;
     for (int i = ndim - 1; i >= 0; --i) {
       if (shape[i] > 1 && strides[i] != expect) return false;
