@@ -60,4 +60,8 @@ struct Seen {
   __device__ inline int32_t key(int32_t c) const { return c < far ? c : near + c - far; }
 };
 
+// window_forward.hip: operands that takes_tiles (window_attention.hip) admits.
+msx_status launch_window_forward(msx_vtype vt, const WindowArgs &a, void *out, float *lse,
+                                 hipStream_t stream);
+
 }  // namespace msx

@@ -361,6 +361,22 @@ WindowArgs args_of(const msx_window_attention_desc &d) {
   return a;
 }
 
+// Whether the tiles' kernels can read the operands: sixteen-byte rows at
+// sixteen-byte strides, a head of at most 128 values, and a scale that a
+// masked score survives.
+bool rows_aligned(size_t size, const void *p, const int64_t *strides, int n) {
+  bool ok = reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  for (int i = 0; i < n; ++i) ok = ok && strides[i] * static_cast<int64_t>(size) % 16 == 0;
+  return ok;
+}
+
+bool takes_tiles(const msx_window_attention_desc &d) {
+  const size_t size = value_bytes(static_cast<msx_vtype>(d.vtype));
+  return d.dim <= 128 && d.dim * size % 16 == 0 && d.scale != 0.0 &&
+         rows_aligned(size, d.q, d.q_strides, 3) && rows_aligned(size, d.k, d.k_strides, 3) &&
+         rows_aligned(size, d.v, d.v_strides, 3);
+}
+
 // Workgroups of `waves` waves for `rows` waves; fails beyond one grid.
 msx_status grid_for(const char *op, int64_t rows, unsigned *blocks) {
   const int64_t n = (rows + kRowWaves - 1) / kRowWaves;
@@ -395,6 +411,9 @@ extern "C" msx_status msx_window_attention(const msx_window_attention_desc *desc
   if (desc->batch == 0 || desc->lq == 0) return MSX_OK;
   if (out == nullptr) return fail(MSX_EINVAL, "window_attention out is NULL.");
   const WindowArgs a = args_of(*desc);
+  if (takes_tiles(*desc) && reinterpret_cast<uintptr_t>(out) % 16 == 0)
+    return launch_window_forward(static_cast<msx_vtype>(desc->vtype), a, out, lse,
+                                 static_cast<hipStream_t>(stream));
   const int64_t rows = a.batch * a.lq * a.heads;
   unsigned blocks = 0;
   if (msx_status st = grid_for("window_attention", rows, &blocks); st != MSX_OK) return st;

@@ -1,0 +1,316 @@
+// window_forward.hip - window attention's forward product on the matrix
+// cores: float32, float16 and bfloat16, head dimensions up to 128 whose rows
+// are sixteen-byte aligned.
+//
+// A wave takes 32 queries of one head, a workgroup kWaves such units that
+// follow each other over (32 positions, head of the group): with four heads a
+// kv head, its waves share one span of keys.  Keys are numbered through: the
+// sinks before the span, then the span, so that a few sinks cost no tile of
+// their own.  Per tile of keys: S^T = K Q^T from LDS, the running maximum and
+// sum, O^T += V^T P^T; the next tile's rows are in flight meanwhile.
+#include <hip/hip_runtime.h>
+
+#include "msx_internal.h"
+#include "msx_window.h"
+#include "msx_window_mfma.h"
+
+#pragma clang fp contract(fast)
+
+namespace msx {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kRows = 32;  // queries a wave
+
+template <class V, int DP>
+struct ForwardShape {
+  using T = TileShape<V, DP>;
+  static constexpr int kSub = T::kSize == 2 ? 2 : 1;  // 32-key parts of a tile
+  static constexpr int kKeys = 32 * kSub;
+  static constexpr int kTile = kKeys * T::kPitch;
+  static constexpr int kPerThread = (kKeys * T::kUsed + kThreads - 1) / kThreads;
+  static constexpr int kLds = 4 * kTile;  // K and V, twice
+  // workgroups a CU: two hide each other's waits; wide float32 heads need the
+  // registers of one (76 spilled with two at 128)
+  static constexpr int kBlocks = T::kRowBytes > 256 ? 1 : 2;
+};
+
+// A query row by its definition, one wave: keys over the lanes for the
+// scores, head values over the lanes for the sum.  Taken where a tile's
+// product is not finite, which a masked key's own infinity or NaN does too.
+template <class V>
+__device__ void forward_row(const WindowArgs &a, int64_t b, int32_t i, int32_t h, int32_t p,
+                            float *q_lds, typename V::Storage *out) {
+  using S = typename V::Storage;
+  const int lane = threadIdx.x % kWave;
+  const S *q = static_cast<const S *>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
+  const S *k = static_cast<const S *>(a.k) + b * a.ks[0] + (h / a.group) * a.ks[2];
+  const S *v = static_cast<const S *>(a.v) + b * a.vs[0] + (h / a.group) * a.vs[2];
+  __builtin_amdgcn_wave_barrier();
+  for (int d = lane; d < a.dim; d += kWave) q_lds[d] = V::widen(q[d]);
+  __builtin_amdgcn_wave_barrier();
+  const Seen seen(p, a.window, a.sinks);
+  const int32_t n = seen.count(p);
+  float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int32_t c0 = 0; c0 < n; c0 += kWave) {
+    const S *row = k + seen.key(min(c0 + lane, n - 1)) * a.ks[1];
+    float s = 0.0f;
+    for (int d = 0; d < a.dim; ++d) s += q_lds[d] * V::widen(row[d]);
+    s = c0 + lane < n ? s * a.scale : -INFINITY;
+    const float top = fmaxf(m, wave_max(s)), base = top == -INFINITY ? 0.0f : top;
+    const float e = exp2_fast(s - base), keep = exp2_fast(m - base);
+    l = l * keep + wave_sum(e);
+    m = top;
+    o0 *= keep;
+    o1 *= keep;
+    const int32_t here = min(kWave, n - c0);
+    for (int32_t t = 0; t < here; ++t) {
+      const float w = __shfl(e, t);
+      const S *from = v + seen.key(c0 + t) * a.vs[1];
+      if (lane < a.dim) o0 += w * V::widen(from[lane]);
+      if (lane + kWave < a.dim) o1 += w * V::widen(from[lane + kWave]);
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  S *to = out + ((b * a.lq + i) * a.heads + h) * a.dim;
+  if (lane < a.dim) to[lane] = V::narrow(o0 * inv);
+  if (lane + kWave < a.dim) to[lane + kWave] = V::narrow(o1 * inv);
+}
+
+template <class V, int DP>
+__global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forward_tiles(WindowArgs a, int32_t units_per_bh,
+                                                             int64_t blocks_per_bh, int64_t blocks,
+                                                             typename V::Storage *out, float *lse) {
+  using S = typename V::Storage;
+  using T = TileShape<V, DP>;
+  using F = ForwardShape<V, DP>;
+  using Frag = typename Mfma<V>::Frag;
+  constexpr int kSteps = DP / Mfma<V>::kDepth;
+  __shared__ __attribute__((aligned(16))) char lds[F::kLds];
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, half = lane / 32;
+  const int64_t id = xcd_order(blockIdx.x, blocks);
+  const int64_t bh = id / blocks_per_bh;
+  const int32_t first_unit = static_cast<int32_t>(id % blocks_per_bh) * kWaves;
+  const int64_t b = bh / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
+  const int32_t n = a.length(b), offset = a.lk - a.lq;
+
+  // this wave's queries
+  const int32_t unit = first_unit + wave;
+  const bool live = unit < units_per_bh;
+  const int32_t i0 = live ? unit / a.group * kRows : 0;
+  const int32_t h = kvh * a.group + (live ? unit % a.group : 0);
+  const int32_t i = i0 + lane % 32;
+  int32_t p = i + offset;
+  if (!live || i >= a.lq || p < 0 || p >= n) p = -1;
+  // positions of the wave's queries that see anything: [p_first, p_last]
+  const int32_t p_first = max(i0 + offset, 0);
+  const int32_t p_last = live ? min(min(i0 + kRows, a.lq) + offset, n) - 1 : -1;
+
+  // the workgroup's keys: sinks [0, far), then [near, end)
+  const int32_t last_unit = min(first_unit + kWaves, units_per_bh) - 1;
+  const int32_t g_first = max(first_unit / a.group * kRows + offset, 0);
+  const int32_t end = min(min((last_unit / a.group + 1) * kRows, a.lq) + offset, n);
+  const int32_t near = max(g_first - a.window + 1, 0);
+  const int32_t far = min(a.sinks, near);
+  const int32_t count = end > g_first ? far + end - near : 0;
+  const int32_t skip = near - far;  // key = c < far ? c : c + skip
+
+  const S *k_base = static_cast<const S *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
+  const S *v_base = static_cast<const S *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
+
+  // queries stay in registers; a negative scale moves its sign here, so that
+  // the largest product is the largest score
+  const float scale = fabsf(a.scale);
+  Frag qf[kSteps];
+  {
+    const S *q = static_cast<const S *>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      v4u w = {0, 0, 0, 0};
+      const int chunk = 2 * s + half;
+      if (p >= 0 && chunk * 16 < a.dim * T::kSize)
+        w = *reinterpret_cast<const v4u *>(reinterpret_cast<const char *>(q) + chunk * 16);
+      if (a.scale < 0.0f) w ^= Mfma<V>::kSign;
+      qf[s] = __builtin_bit_cast(Frag, w);
+    }
+  }
+
+  v4u k_next[F::kPerThread], v_next[F::kPerThread];
+  const auto fetch = [&](int32_t c0) {
+#pragma unroll
+    for (int r = 0; r < F::kPerThread; ++r) {
+      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
+      const int32_t c = c0 + row;
+      v4u kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
+      if (row < F::kKeys && c < count && chunk * 16 < a.dim * T::kSize) {
+        const int64_t key = c < far ? c : c + skip;
+        kw = *reinterpret_cast<const v4u *>(
+            reinterpret_cast<const char *>(k_base + key * a.ks[1]) + chunk * 16);
+        vw = *reinterpret_cast<const v4u *>(
+            reinterpret_cast<const char *>(v_base + key * a.vs[1]) + chunk * 16);
+      }
+      k_next[r] = kw;
+      v_next[r] = vw;
+    }
+  };
+  const auto keep = [&](int buffer) {
+    char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
+#pragma unroll
+    for (int r = 0; r < F::kPerThread; ++r) {
+      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
+      if (row < F::kKeys) {
+        *reinterpret_cast<v4u *>(kt + T::across(row, chunk)) = k_next[r];
+        *reinterpret_cast<v4u *>(vt + T::along(row, chunk)) = v_next[r];
+      }
+    }
+  };
+
+  v16f o[DP / 32];
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+  float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
+
+  fetch(0);
+  keep(0);
+  __syncthreads();
+  for (int32_t c0 = 0, buffer = 0; c0 < count; c0 += F::kKeys, buffer ^= 1) {
+    const bool more = c0 + F::kKeys < count;
+    if (more) fetch(c0 + F::kKeys);
+    const char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
+
+    // keys of the tile: sinks, and [k_first, k_last] of the span
+    const int32_t k_first = max(c0, far) + skip, k_last = min(c0 + F::kKeys, count) - 1 + skip;
+    const bool any = p_last >= p_first &&
+                     (c0 < far || (k_first <= p_last && (p_first - k_last < a.window || k_first < a.sinks)));
+    if (any) {
+      v16f s[F::kSub];
+#pragma unroll
+      for (int t = 0; t < F::kSub; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st)
+          s[t] = Mfma<V>::mul(read_across<V, DP>(kt, 32 * t + lane % 32, st), qf[st], s[t]);
+      }
+      // all of the tile's keys seen by all of the wave's queries: no mask
+      const bool whole = c0 + F::kKeys <= count && k_last <= p_first &&
+                         (p_last - k_first < a.window || k_last < a.sinks) &&
+                         p_last - p_first == kRows - 1;
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < F::kSub; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
+            const int32_t key = c < far ? c : c + skip;
+            const bool seen = c < count && key <= p && (p - key < a.window || key < a.sinks);
+            s[t][r] = seen ? s[t][r] : -INFINITY;
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int t = 0; t < F::kSub; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+      top = fmaxf(top, other_half(top)) * scale;
+      // The maximum is moved only where it has grown by more than 2^8: until
+      // then exponentials up to 2^8 stand beside sums of their own scale.
+      if (__any(top > m + 8.0f)) {
+        const float grown = fmaxf(m, top);
+        const float shrink = grown == -INFINITY ? 1.0f : exp2_fast(m - grown);
+        m = grown;
+        l *= shrink;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= shrink;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int t = 0; t < F::kSub; ++t) {
+        float e[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          e[r] = exp2_fast(s[t][r] * scale - base);
+          l += e[r];
+        }
+        mul_transposed<V, DP>(vt, 32 * t, e, o);
+      }
+    }
+    if (more) keep(buffer ^ 1);
+    __syncthreads();
+  }
+
+  l += other_half(l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  bool odd = false;  // something is not finite: the row is computed anew
+  if (live && i < a.lq) {
+    S *to = out + ((b * a.lq + i) * a.heads + h) * a.dim;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = dt * 32 + 2 * r + 4 * half;
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = o[dt][r + j] * inv;
+          odd = odd || !(fabsf(x[j]) < INFINITY);
+        }
+        if (d < a.dim) {
+          if constexpr (T::kSize == 2)
+            *reinterpret_cast<v2u *>(to + d) =
+                v2u{Mfma<V>::pack(x[0], x[1]), Mfma<V>::pack(x[2], x[3])};
+          else
+            *reinterpret_cast<v4f *>(to + d) = v4f{x[0], x[1], x[2], x[3]};
+        }
+      }
+    if (lse != nullptr && half == 0)
+      lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
+  }
+  uint64_t anew = __ballot(odd && p >= 0);
+  anew = (anew | anew >> 32) & 0xffffffffu;
+  while (anew != 0) {  // the tiles in LDS are done with: all waves left the loop
+    const int r = __builtin_ctzll(anew);
+    anew &= anew - 1;
+    forward_row<V>(a, b, i0 + r, h, i0 + r + offset, reinterpret_cast<float *>(lds) + wave * DP, out);
+  }
+}
+
+template <class V, int DP>
+msx_status run(const WindowArgs &a, void *out, float *lse, hipStream_t stream) {
+  const int64_t units = (static_cast<int64_t>(a.lq) + kRows - 1) / kRows * a.group;
+  const int64_t per_bh = (units + kWaves - 1) / kWaves, blocks = per_bh * a.batch * a.kv_heads;
+  if (units > 0x7fffffff || blocks > 0x7fffffff)
+    return fail(MSX_EINVAL, "window_attention has more rows than a grid holds.");
+  forward_tiles<V, DP><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+      a, static_cast<int32_t>(units), per_bh, blocks, static_cast<typename V::Storage *>(out), lse);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MSX_OK : hip_fail(e, "window_attention");
+}
+
+template <class V>
+msx_status by_dim(const WindowArgs &a, void *out, float *lse, hipStream_t stream) {
+  if (a.dim <= 32) return run<V, 32>(a, out, lse, stream);
+  if (a.dim <= 64) return run<V, 64>(a, out, lse, stream);
+  if (a.dim <= 96) return run<V, 96>(a, out, lse, stream);
+  return run<V, 128>(a, out, lse, stream);
+}
+
+}  // namespace
+
+msx_status launch_window_forward(msx_vtype vt, const WindowArgs &a, void *out, float *lse,
+                                 hipStream_t stream) {
+  switch (vt) {
+  case MSX_F32: return by_dim<F32>(a, out, lse, stream);
+  case MSX_F16: return by_dim<F16>(a, out, lse, stream);
+  default: return by_dim<BF16>(a, out, lse, stream);
+  }
+}
+
+}  // namespace msx
