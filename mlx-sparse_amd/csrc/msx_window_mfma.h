@@ -30,7 +30,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
 // A tile of rows in LDS: rows of `kPitch` bytes, their 16-byte chunks
-// permuted by row so that the reads below spread over the 64 banks.
+// permuted by row so that the reads below spread over the banks.
 template <class V, int DP>
 struct TileShape {
   static constexpr int kSize = sizeof(typename V::Storage);
@@ -40,13 +40,8 @@ struct TileShape {
   static constexpr int kUsed = kRowBytes / 16;
   static constexpr int kRowsPerLine = kPitch >= 256 ? 1 : 256 / kPitch;  // rows over all banks
 
-  // Rows read across keys (a lane a row, sixteen bytes): neighbouring rows
-  // get different chunks.
-  __device__ static inline int across(int row, int chunk) {
-    return row * kPitch + ((chunk ^ ((row / kRowsPerLine) & (kChunks - 1))) * 16);
-  }
-  // Rows read by the transposing read (four rows by 32 bytes at once): the
-  // 32-byte pairs are permuted.
+  // The 32-byte pairs of chunks are permuted by row: the transposing read
+  // takes four rows by 32 bytes at once, a row read sixteen bytes of eight.
   __device__ static inline int along(int row, int chunk) {
     return row * kPitch + ((chunk ^ (((row / kRowsPerLine) * 2) & (kChunks - 1))) * 16);
   }
@@ -98,10 +93,10 @@ struct Mfma<F32> {
 // Sixteen bytes of a row for step `s` of a product over the head dimension:
 // chunk 2 s + lane / 32 in either type.
 template <class V, int DP>
-__device__ inline typename Mfma<V>::Frag read_across(const char *tile, int row, int s) {
+__device__ inline typename Mfma<V>::Frag read_rows(const char *tile, int row, int s) {
   const int half = (threadIdx.x % kWave) / 32;
   return *reinterpret_cast<const typename Mfma<V>::Frag *>(
-      tile + TileShape<V, DP>::across(row, 2 * s + half));
+      tile + TileShape<V, DP>::along(row, 2 * s + half));
 }
 
 __device__ inline v4s read_transposed(const char *p) {

@@ -377,6 +377,11 @@ bool takes_tiles(const msx_window_attention_desc &d) {
          rows_aligned(size, d.v, d.v_strides, 3);
 }
 
+// delta, before the tiles' sums (which need sixteen-byte addresses).
+size_t delta_bytes(const msx_window_attention_desc &d) {
+  return (sizeof(float) * static_cast<size_t>(d.batch * d.heads * d.lq) + 255) / 256 * 256;
+}
+
 // Workgroups of `waves` waves for `rows` waves; fails beyond one grid.
 msx_status grid_for(const char *op, int64_t rows, unsigned *blocks) {
   const int64_t n = (rows + kRowWaves - 1) / kRowWaves;
@@ -426,8 +431,10 @@ extern "C" msx_status msx_window_attention(const msx_window_attention_desc *desc
 }
 
 extern "C" size_t msx_window_attention_backward_scratch(const msx_window_attention_desc *desc) {
-  if (desc == nullptr || desc->batch <= 0 || desc->heads <= 0 || desc->lq <= 0) return 0;
-  return sizeof(float) * static_cast<size_t>(desc->batch * desc->heads * desc->lq);
+  if (check_window_attention("window_attention_backward", desc) != MSX_OK || desc->batch == 0)
+    return 0;
+  const size_t tiles = takes_tiles(*desc) ? window_backward_scratch(args_of(*desc)) : 0;
+  return delta_bytes(*desc) + tiles;
 }
 
 extern "C" msx_status msx_window_attention_backward(const msx_window_attention_desc *desc,
@@ -448,6 +455,14 @@ extern "C" msx_status msx_window_attention_backward(const msx_window_attention_d
   if (scratch_bytes < msx_window_attention_backward_scratch(desc) || (queries && scratch == nullptr))
     return fail(MSX_EINVAL, "window_attention_backward scratch is too small.");
   const WindowArgs a = args_of(*desc);
+  const size_t size = value_bytes(static_cast<msx_vtype>(desc->vtype));
+  const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  if (queries && keys && takes_tiles(*desc) && rows_aligned(size, grad, grad_strides, 3) &&
+      aligned(out) && aligned(dq) && aligned(dk) && aligned(dv) && aligned(scratch))
+    return launch_window_backward(static_cast<msx_vtype>(desc->vtype), a, out, lse, grad,
+                                  grad_strides, static_cast<float *>(scratch), dq, dk, dv,
+                                  static_cast<char *>(scratch) + delta_bytes(*desc),
+                                  static_cast<hipStream_t>(stream));
   const int64_t q_rows = a.batch * a.lq * a.heads, k_rows = a.batch * a.lk * a.kv_heads;
   unsigned q_blocks = 0, k_blocks = 0;
   if (msx_status st = grid_for(op, q_rows, &q_blocks); st != MSX_OK) return st;

@@ -1,0 +1,635 @@
+// window_backward.hip - window attention's gradients on the matrix cores, for
+// the operands the forward tiles take.
+//
+// Two sums over the same products, each in a fixed order and without atomics:
+//
+//   queries (dq): a wave takes 32 queries, as in the forward pass, and goes
+//     through their keys: S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T;
+//   keys (dk, dv): a wave takes 32 keys, its workgroup 128, and goes through
+//     the queries that see them, of every head of the group: S = Q K^T,
+//     dP = dO V^T (rows are queries now), dV^T += dO^T P, dK^T += Q^T dS.
+//
+// The products of scores are made twice, seven in all where five would do with
+// dq added atomically in float32; the rounding order would then change from
+// run to run, and dq would pass through memory in 32 bits.
+//
+// Sinks are seen by all later queries, L of them where another key has
+// `window`: the queries beyond a key block's own span are a pass of their own
+// (the far pass), whose four waves take different queries for the same 32
+// keys; its parts and the blocks' own sums are joined in order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "msx_internal.h"
+#include "msx_window.h"
+#include "msx_window_mfma.h"
+
+#pragma clang fp contract(fast)
+
+namespace msx {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kBlockKeys = 32 * kWaves;
+
+struct Upstream {
+  const void *grad;
+  int64_t gs[3];
+  const void *out;
+  const float *lse;
+  float *delta;
+};
+
+template <class V, int DP>
+struct BackwardShape {
+  using T = TileShape<V, DP>;
+  static constexpr int kSub = T::kSize == 2 ? 2 : 1;
+  static constexpr int kTokens = 32 * kSub;  // tokens of a tile
+  static constexpr int kTile = kTokens * T::kPitch;
+  static constexpr int kPerThread = (kTokens * T::kUsed + kThreads - 1) / kThreads;
+};
+
+// Sixteen bytes of a row, zeros beyond the head.
+template <class V>
+__device__ inline v4u load_chunk(const typename V::Storage *row, int chunk, int dim) {
+  if (chunk * 16 >= dim * static_cast<int>(sizeof(typename V::Storage))) return v4u{0, 0, 0, 0};
+  return *reinterpret_cast<const v4u *>(reinterpret_cast<const char *>(row) + chunk * 16);
+}
+
+// Sum of products of two sixteen-byte pieces.
+template <class V>
+__device__ inline float dot_chunk(v4u x, v4u y) {
+  float acc = 0.0f;
+  if constexpr (sizeof(typename V::Storage) == 4) {
+    const auto a = __builtin_bit_cast(v4f, x), b = __builtin_bit_cast(v4f, y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc += a[j] * b[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      acc += V::widen(static_cast<uint16_t>(x[j])) * V::widen(static_cast<uint16_t>(y[j]));
+      acc += V::widen(static_cast<uint16_t>(x[j] >> 16)) * V::widen(static_cast<uint16_t>(y[j] >> 16));
+    }
+  }
+  return acc;
+}
+
+// A lane's column of a transposed result: row `to` gets acc * factor.
+template <class V, int DP>
+__device__ inline void store_column(const v16f (&acc)[DP / 32], float factor, int dim,
+                                    typename V::Storage *to) {
+  const int half = (threadIdx.x % kWave) / 32;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = dt * 32 + 2 * r + 4 * half;
+      if (d >= dim) continue;
+      const float x0 = acc[dt][r] * factor, x1 = acc[dt][r + 1] * factor;
+      const float x2 = acc[dt][r + 2] * factor, x3 = acc[dt][r + 3] * factor;
+      if constexpr (sizeof(typename V::Storage) == 2)
+        *reinterpret_cast<v2u *>(to + d) = v2u{Mfma<V>::pack(x0, x1), Mfma<V>::pack(x2, x3)};
+      else
+        *reinterpret_cast<v4f *>(to + d) = v4f{x0, x1, x2, x3};
+    }
+}
+
+template <int DP>
+__device__ inline void zero(v16f (&acc)[DP / 32]) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
+}
+
+// ---------------------------------------------------------------------------
+// dq, and delta for the keys' pass.
+
+template <class V, int DP>
+__global__ __launch_bounds__(kThreads, (sizeof(typename V::Storage) == 4 && DP > 64 ? 1 : 2)) void
+backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks_per_bh,
+                 int64_t blocks, typename V::Storage *dq) {
+  using S = typename V::Storage;
+  using T = TileShape<V, DP>;
+  using F = BackwardShape<V, DP>;
+  using Frag = typename Mfma<V>::Frag;
+  constexpr int kSteps = DP / Mfma<V>::kDepth;
+  __shared__ __attribute__((aligned(16))) char lds[4 * F::kTile];
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, half = lane / 32;
+  const int64_t id = xcd_order(blockIdx.x, blocks);
+  const int64_t bh = id / blocks_per_bh;
+  const int32_t first_unit = static_cast<int32_t>(id % blocks_per_bh) * kWaves;
+  const int64_t b = bh / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
+  const int32_t n = a.length(b), offset = a.lk - a.lq;
+
+  // units, spans and numbering of keys as in the forward pass
+  const int32_t unit = first_unit + wave;
+  const bool live = unit < units_per_bh;
+  const int32_t i0 = live ? unit / a.group * 32 : 0;
+  const int32_t h = kvh * a.group + (live ? unit % a.group : 0);
+  const int32_t i = i0 + lane % 32;
+  int32_t p = i + offset;
+  if (!live || i >= a.lq || p < 0 || p >= n) p = -1;
+  const int32_t p_first = max(i0 + offset, 0);
+  const int32_t p_last = live ? min(min(i0 + 32, a.lq) + offset, n) - 1 : -1;
+  const int32_t last_unit = min(first_unit + kWaves, units_per_bh) - 1;
+  const int32_t g_first = max(first_unit / a.group * 32 + offset, 0);
+  const int32_t end = min(min((last_unit / a.group + 1) * 32, a.lq) + offset, n);
+  const int32_t near = max(g_first - a.window + 1, 0);
+  const int32_t far = min(a.sinks, near);
+  const int32_t count = end > g_first ? far + end - near : 0;
+  const int32_t skip = near - far;
+
+  const S *k_base = static_cast<const S *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
+  const S *v_base = static_cast<const S *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
+  Frag qf[kSteps], gf[kSteps];
+  float delta = 0.0f, lse = INFINITY;
+  {
+    const S *q = static_cast<const S *>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
+    const S *g = static_cast<const S *>(up.grad) + b * up.gs[0] + i * up.gs[1] + h * up.gs[2];
+    const S *o = static_cast<const S *>(up.out) + ((b * a.lq + i) * a.heads + h) * a.dim;
+    if (p >= 0) lse = up.lse[(b * a.heads + h) * a.lq + i];
+    if (lse == INFINITY) p = -1;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      v4u qw = {0, 0, 0, 0}, gw = {0, 0, 0, 0};
+      if (p >= 0) {
+        qw = load_chunk<V>(q, 2 * s + half, a.dim);
+        gw = load_chunk<V>(g, 2 * s + half, a.dim);
+        delta += dot_chunk<V>(gw, load_chunk<V>(o, 2 * s + half, a.dim));
+      }
+      qf[s] = __builtin_bit_cast(Frag, qw);
+      gf[s] = __builtin_bit_cast(Frag, gw);
+    }
+    delta += other_half(delta);
+    if (live && i < a.lq && half == 0) up.delta[(b * a.heads + h) * a.lq + i] = delta;
+  }
+
+  v4u k_next[F::kPerThread], v_next[F::kPerThread];
+  const auto fetch = [&](int32_t c0) {
+#pragma unroll
+    for (int r = 0; r < F::kPerThread; ++r) {
+      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
+      const int32_t c = c0 + row;
+      k_next[r] = v_next[r] = v4u{0, 0, 0, 0};
+      if (row < F::kTokens && c < count) {
+        const int64_t key = c < far ? c : c + skip;
+        k_next[r] = load_chunk<V>(k_base + key * a.ks[1], chunk, a.dim);
+        v_next[r] = load_chunk<V>(v_base + key * a.vs[1], chunk, a.dim);
+      }
+    }
+  };
+  const auto keep = [&](int buffer) {
+    char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
+#pragma unroll
+    for (int r = 0; r < F::kPerThread; ++r) {
+      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
+      if (row < F::kTokens) {
+        *reinterpret_cast<v4u *>(kt + T::along(row, chunk)) = k_next[r];
+        *reinterpret_cast<v4u *>(vt + T::along(row, chunk)) = v_next[r];
+      }
+    }
+  };
+
+  v16f acc[DP / 32];
+  zero<DP>(acc);
+  fetch(0);
+  keep(0);
+  __syncthreads();
+  for (int32_t c0 = 0, buffer = 0; c0 < count; c0 += F::kTokens, buffer ^= 1) {
+    const bool more = c0 + F::kTokens < count;
+    if (more) fetch(c0 + F::kTokens);
+    const char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
+    const int32_t k_first = max(c0, far) + skip, k_last = min(c0 + F::kTokens, count) - 1 + skip;
+    const bool any = p_last >= p_first &&
+                     (c0 < far || (k_first <= p_last && (p_first - k_last < a.window || k_first < a.sinks)));
+    if (any) {
+      const bool whole = c0 + F::kTokens <= count && k_last <= p_first &&
+                         (p_last - k_first < a.window || k_last < a.sinks) && p_last - p_first == 31;
+#pragma unroll
+      for (int t = 0; t < F::kSub; ++t) {
+        v16f s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          s = Mfma<V>::mul(read_rows<V, DP>(kt, 32 * t + lane % 32, st), qf[st], s);
+          dp = Mfma<V>::mul(read_rows<V, DP>(vt, 32 * t + lane % 32, st), gf[st], dp);
+        }
+        float ds[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(s[r] * a.scale - lse) * (dp[r] - delta);
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
+            const int32_t key = c < far ? c : c + skip;
+            const bool seen = c < count && key <= p && (p - key < a.window || key < a.sinks);
+            ds[r] = seen ? ds[r] : 0.0f;
+          }
+        }
+        mul_transposed<V, DP>(kt, 32 * t, ds, acc);
+      }
+    }
+    if (more) keep(buffer ^ 1);
+    __syncthreads();
+  }
+  if (live && i < a.lq)
+    store_column<V, DP>(acc, a.grad_scale, a.dim, dq + ((b * a.lq + i) * a.heads + h) * a.dim);
+}
+
+// ---------------------------------------------------------------------------
+// dk and dv.
+
+// The keys of one wave and their sums.
+template <class V, int DP>
+struct KeyWave {
+  static constexpr int kSteps = DP / Mfma<V>::kDepth;
+  typename Mfma<V>::Frag kf[kSteps], vf[kSteps];
+  v16f dk[DP / 32], dv[DP / 32];
+
+  __device__ inline void start(const WindowArgs &a, int64_t b, int32_t kvh, int32_t key, bool live) {
+    using S = typename V::Storage;
+    const int half = (threadIdx.x % kWave) / 32;
+    const S *k = static_cast<const S *>(a.k) + b * a.ks[0] + key * a.ks[1] + kvh * a.ks[2];
+    const S *v = static_cast<const S *>(a.v) + b * a.vs[0] + key * a.vs[1] + kvh * a.vs[2];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      v4u kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
+      if (live) {
+        kw = load_chunk<V>(k, 2 * s + half, a.dim);
+        vw = load_chunk<V>(v, 2 * s + half, a.dim);
+      }
+      kf[s] = __builtin_bit_cast(typename Mfma<V>::Frag, kw);
+      vf[s] = __builtin_bit_cast(typename Mfma<V>::Frag, vw);
+    }
+    zero<DP>(dk);
+    zero<DP>(dv);
+  }
+
+  // 32 queries from row `row0` of the tiles, at positions p0 .. p0 + 31;
+  // `masked`: the lane's key is not seen by all of them.
+  __device__ inline void add(const WindowArgs &a, const char *q_tile, const char *g_tile,
+                             const float *lse, const float *delta, int row0, int32_t p0,
+                             int32_t key, bool masked) {
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    v16f s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      s = Mfma<V>::mul(read_rows<V, DP>(q_tile, row0 + lane % 32, st), kf[st], s);
+      dp = Mfma<V>::mul(read_rows<V, DP>(g_tile, row0 + lane % 32, st), vf[st], dp);
+    }
+    float p[16], ds[16];
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int row = row0 + 2 * r + 4 * half;
+      const v4f l = *reinterpret_cast<const v4f *>(lse + row);
+      const v4f d = *reinterpret_cast<const v4f *>(delta + row);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[r + j] = exp2_fast(s[r + j] * a.scale - l[j]);
+        ds[r + j] = p[r + j] * (dp[r + j] - d[j]);
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int32_t at = p0 + 8 * (r / 4) + 4 * half + r % 4;
+        const bool seen = at >= key && (at - key < a.window || key < a.sinks);
+        p[r] = seen ? p[r] : 0.0f;
+        ds[r] = seen ? ds[r] : 0.0f;
+      }
+    }
+    mul_transposed<V, DP>(g_tile, row0, p, dv);
+    mul_transposed<V, DP>(q_tile, row0, ds, dk);
+  }
+};
+
+// The next queries of the walk, on their way through registers into LDS.
+// A query beyond the sequence is zeros with lse = +inf: its P is zero.
+template <class V, int DP, int kTokens>
+struct QueryTile {
+  using T = TileShape<V, DP>;
+  static constexpr int kTile = kTokens * T::kPitch;
+  static constexpr int kBytes = 2 * kTile + 2 * kTokens * 4;
+  static constexpr int kPerThread = (kTokens * T::kUsed + kThreads - 1) / kThreads;
+  v4u q[kPerThread], g[kPerThread];
+  float stat;
+
+  __device__ inline void fetch(const WindowArgs &a, const Upstream &up, int64_t b, int32_t h,
+                               int32_t p0, int32_t last, int32_t offset) {
+    using S = typename V::Storage;
+    const S *q_base = static_cast<const S *>(a.q) + b * a.qs[0] + h * a.qs[2];
+    const S *g_base = static_cast<const S *>(up.grad) + b * up.gs[0] + h * up.gs[2];
+#pragma unroll
+    for (int r = 0; r < kPerThread; ++r) {
+      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
+      q[r] = g[r] = v4u{0, 0, 0, 0};
+      if (row < kTokens && p0 + row <= last) {
+        const int64_t i = p0 + row - offset;
+        q[r] = load_chunk<V>(q_base + i * a.qs[1], chunk, a.dim);
+        g[r] = load_chunk<V>(g_base + i * up.gs[1], chunk, a.dim);
+      }
+    }
+    // the first kTokens threads take lse, the next as many delta
+    static_assert(2 * kTokens <= kThreads, "a thread a statistic");
+    const int row = threadIdx.x % kTokens;
+    const bool is_lse = threadIdx.x < kTokens;
+    stat = is_lse ? INFINITY : 0.0f;
+    if (threadIdx.x < 2 * kTokens && p0 + row <= last) {
+      const int64_t at = (b * a.heads + h) * a.lq + p0 + row - offset;
+      stat = is_lse ? up.lse[at] : up.delta[at];
+    }
+  }
+  __device__ inline void keep(char *to) const {
+#pragma unroll
+    for (int r = 0; r < kPerThread; ++r) {
+      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
+      if (row < kTokens) {
+        *reinterpret_cast<v4u *>(to + T::along(row, chunk)) = q[r];
+        *reinterpret_cast<v4u *>(to + kTile + T::along(row, chunk)) = g[r];
+      }
+    }
+    if (threadIdx.x < 2 * kTokens)
+      reinterpret_cast<float *>(to + 2 * kTile)[threadIdx.x] = stat;
+  }
+};
+
+// How the keys' work is cut: blocks of kBlockKeys keys, each in `parts`; and
+// the far units, 32 sink keys each, in `far_parts`.
+struct KeyPlan {
+  int32_t blocks, parts;
+  int32_t joined;  // blocks whose sums go through scratch, from the first on
+  int32_t far_units, far_parts;
+  float *near_sums, *far_sums;
+};
+
+// Sums of one lane's key: dk then dv, `dim` floats each.
+template <int DP>
+__device__ inline void store_sums(const v16f (&dk)[DP / 32], const v16f (&dv)[DP / 32], int dim,
+                                  float *to) {
+  const int half = (threadIdx.x % kWave) / 32;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = dt * 32 + 2 * r + 4 * half;
+      if (d >= dim) continue;
+      *reinterpret_cast<v4f *>(to + d) = v4f{dk[dt][r], dk[dt][r + 1], dk[dt][r + 2], dk[dt][r + 3]};
+      *reinterpret_cast<v4f *>(to + dim + d) =
+          v4f{dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]};
+    }
+}
+
+// Queries within reach of a block's window: positions first .. last; the rest
+// of a sink's queries are the far pass's.
+__device__ inline int32_t near_last(const WindowArgs &a, int32_t block, int32_t n) {
+  const int64_t last = static_cast<int64_t>(block) * kBlockKeys + kBlockKeys + a.window - 2;
+  return last < n - 1 ? static_cast<int32_t>(last) : n - 1;
+}
+
+template <class V, int DP>
+__global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, Upstream up,
+                                                                  KeyPlan plan, int64_t blocks,
+                                                                  typename V::Storage *dk,
+                                                                  typename V::Storage *dv) {
+  constexpr int kSub = BackwardShape<V, DP>::kSub, kTokens = 32 * kSub;
+  using Tile = QueryTile<V, DP, kTokens>;
+  __shared__ __attribute__((aligned(16))) char lds[2 * Tile::kBytes];
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t id = xcd_order(blockIdx.x, blocks);
+  const int32_t part = static_cast<int32_t>(id % plan.parts);
+  const int32_t block = static_cast<int32_t>(id / plan.parts % plan.blocks);
+  const int64_t bh = id / plan.parts / plan.blocks;
+  const int64_t b = bh / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
+  const int32_t n = a.length(b), offset = a.lk - a.lq;
+  const int32_t w_first = block * kBlockKeys + wave * 32, w_last = w_first + 31;
+  const int32_t key = w_first + lane % 32;
+
+  KeyWave<V, DP> keys;
+  keys.start(a, b, kvh, key, key < n);
+
+  const int32_t first = max(block * kBlockKeys, offset), last = near_last(a, block, n);
+  const int32_t tiles = last >= first ? (last - first) / kTokens + 1 : 0;
+  const int64_t total = static_cast<int64_t>(tiles) * a.group;
+  const int32_t begin = static_cast<int32_t>(total * part / plan.parts);
+  const int32_t end = static_cast<int32_t>(total * (part + 1) / plan.parts);
+
+  Tile next;
+  const auto fetch = [&](int32_t step) {
+    next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset);
+  };
+  if (begin < end) {
+    fetch(begin);
+    next.keep(lds);
+  }
+  __syncthreads();
+  for (int32_t step = begin, buffer = 0; step < end; ++step, buffer ^= 1) {
+    const bool more = step + 1 < end;
+    if (more) fetch(step + 1);
+    const char *tile = lds + buffer * Tile::kBytes;
+    const float *stat = reinterpret_cast<const float *>(tile + 2 * Tile::kTile);
+#pragma unroll
+    for (int t = 0; t < kSub; ++t) {
+      const int32_t p0 = first + step % tiles * kTokens + 32 * t, p1 = p0 + 31;
+      const bool any = p1 >= w_first && p0 <= last && (p0 - w_last < a.window || w_first < a.sinks);
+      const bool whole = p0 >= w_last && (p1 - w_first < a.window || w_last < a.sinks);
+      if (any)
+        keys.add(a, tile, tile + Tile::kTile, stat, stat + kTokens, 32 * t, p0, key, !whole);
+    }
+    if (more) next.keep(lds + (buffer ^ 1) * Tile::kBytes);
+    __syncthreads();
+  }
+
+  if (key >= a.lk) return;
+  if (block < plan.joined) {
+    const int64_t slot = ((bh * plan.joined + block) * plan.parts + part) * kBlockKeys + wave * 32 + lane % 32;
+    store_sums<DP>(keys.dk, keys.dv, a.dim, plan.near_sums + slot * 2 * a.dim);
+  } else {
+    const int64_t row = (b * a.lk + key) * a.kv_heads + kvh;
+    store_column<V, DP>(keys.dk, a.grad_scale, a.dim, dk + row * a.dim);
+    store_column<V, DP>(keys.dv, 1.0f, a.dim, dv + row * a.dim);
+  }
+}
+
+// Sinks and the queries beyond their block's span: a wave takes every fourth
+// 32 queries.
+template <class V, int DP>
+__global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, Upstream up,
+                                                                 KeyPlan plan, int64_t blocks) {
+  constexpr int kTokens = 32 * kWaves;
+  using Tile = QueryTile<V, DP, kTokens>;
+  extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
+  char *lds = dynamic_lds;
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t id = xcd_order(blockIdx.x, blocks);
+  const int32_t part = static_cast<int32_t>(id % plan.far_parts);
+  const int32_t unit = static_cast<int32_t>(id / plan.far_parts % plan.far_units);
+  const int64_t bh = id / plan.far_parts / plan.far_units;
+  const int64_t b = bh / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
+  const int32_t n = a.length(b), offset = a.lk - a.lq;
+  const int32_t key = unit * 32 + lane % 32;
+  const bool live = key < a.sinks && key < n;
+
+  KeyWave<V, DP> keys;
+  keys.start(a, b, kvh, key, live);
+
+  const int32_t first = max(near_last(a, unit * 32 / kBlockKeys, n) + 1, offset), last = n - 1;
+  const int32_t tiles = last >= first ? (last - first) / kTokens + 1 : 0;
+  const int64_t total = static_cast<int64_t>(tiles) * a.group;
+  const int32_t begin = static_cast<int32_t>(total * part / plan.far_parts);
+  const int32_t end = static_cast<int32_t>(total * (part + 1) / plan.far_parts);
+
+  Tile next;
+  const auto fetch = [&](int32_t step) {
+    next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset);
+  };
+  if (begin < end) fetch(begin);
+  for (int32_t step = begin; step < end; ++step) {
+    next.keep(lds);
+    __syncthreads();
+    if (step + 1 < end) fetch(step + 1);
+    const float *stat = reinterpret_cast<const float *>(lds + 2 * Tile::kTile);
+    // all of these queries see the sinks; a key that is none is not stored
+    keys.add(a, lds, lds + Tile::kTile, stat, stat + kTokens, 32 * wave, 0, key, false);
+    __syncthreads();
+  }
+  if (key >= a.sinks || key >= a.lk) return;
+  const int64_t slot = ((bh * plan.far_units + unit) * plan.far_parts + part) * kWaves + wave;
+  store_sums<DP>(keys.dk, keys.dv, a.dim, plan.far_sums + (slot * 32 + lane % 32) * 2 * a.dim);
+}
+
+// dk and dv of the joined blocks: a block's parts, then the far parts, in order.
+template <class V>
+__global__ __launch_bounds__(256) void join_keys(WindowArgs a, KeyPlan plan, int64_t total,
+                                                 typename V::Storage *dk, typename V::Storage *dv) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= total) return;
+  const int64_t dims = 2 * a.dim;
+  const int32_t d = static_cast<int32_t>(at % dims);
+  const int32_t key = static_cast<int32_t>(at / dims % (static_cast<int64_t>(plan.joined) * kBlockKeys));
+  const int64_t bh = at / dims / (static_cast<int64_t>(plan.joined) * kBlockKeys);
+  if (key >= a.lk) return;
+  const int32_t block = key / kBlockKeys;
+  float sum = 0.0f;
+  for (int32_t part = 0; part < plan.parts; ++part)
+    sum += plan.near_sums[((((bh * plan.joined + block) * plan.parts + part) * kBlockKeys) + key % kBlockKeys) * dims + d];
+  if (key < a.sinks && key / 32 < plan.far_units)
+    for (int32_t part = 0; part < plan.far_parts * kWaves; ++part)
+      sum += plan.far_sums[((((bh * plan.far_units + key / 32) * plan.far_parts * kWaves + part) * 32) + key % 32) * dims + d];
+  const int64_t row = (bh / a.kv_heads * a.lk + key) * a.kv_heads + bh % a.kv_heads;
+  if (d < a.dim)
+    dk[row * a.dim + d] = V::narrow(sum * a.grad_scale);
+  else
+    dv[row * a.dim + d - a.dim] = V::narrow(sum);
+}
+
+// The cut depends on sizes alone.  One workgroup runs on a CU; with fewer
+// blocks than CUs each is cut until there are about two a CU, of eight tiles
+// of 32 queries at least.  The far pass goes by the same two numbers.
+KeyPlan plan_keys(const WindowArgs &a) {
+  constexpr int64_t kCus = 256;
+  KeyPlan p{};
+  const int64_t bh = a.batch * a.kv_heads;
+  p.blocks = (a.lk + kBlockKeys - 1) / kBlockKeys;
+  const int64_t span = std::min<int64_t>(a.lq, static_cast<int64_t>(a.window) + kBlockKeys - 1);
+  const int64_t work = std::max<int64_t>(1, (span + 31) / 32 * a.group / 8);
+  p.parts = static_cast<int32_t>(
+      bh * p.blocks >= kCus ? 1 : std::min<int64_t>(work, 2 * kCus / std::max<int64_t>(1, bh * p.blocks)));
+  // queries that see sinks from beyond the first block's span
+  const int64_t beyond =
+      std::min<int64_t>(a.lq, static_cast<int64_t>(a.lk) - kBlockKeys - a.window + 1);
+  if (beyond > 0 && a.sinks > 0) {
+    p.far_units = (a.sinks + 31) / 32;
+    const int64_t steps = std::max<int64_t>(1, (beyond + 127) / 128 * a.group / 4);
+    p.far_parts = static_cast<int32_t>(
+        std::min<int64_t>(steps, std::max<int64_t>(1, 2 * kCus / (bh * p.far_units))));
+  }
+  p.joined = p.parts > 1 ? p.blocks : (p.far_units * 32 + kBlockKeys - 1) / kBlockKeys;
+  p.joined = std::min(p.joined, p.blocks);
+  return p;
+}
+
+size_t near_floats(const WindowArgs &a, const KeyPlan &p) {
+  return static_cast<size_t>(a.batch) * a.kv_heads * p.joined * p.parts * kBlockKeys * 2 * a.dim;
+}
+size_t far_floats(const WindowArgs &a, const KeyPlan &p) {
+  return static_cast<size_t>(a.batch) * a.kv_heads * p.far_units * p.far_parts * kWaves * 32 * 2 * a.dim;
+}
+
+template <class V, int DP>
+msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, void *dk, void *dv,
+               hipStream_t stream) {
+  using S = typename V::Storage;
+  const int64_t bh = a.batch * a.kv_heads;
+  const int64_t units = (static_cast<int64_t>(a.lq) + 31) / 32 * a.group;
+  const int64_t per_bh = (units + kWaves - 1) / kWaves, q_blocks = per_bh * bh;
+  const int64_t k_blocks = bh * plan.blocks * plan.parts, f_blocks = bh * plan.far_units * plan.far_parts;
+  const int64_t joined = bh * plan.joined * kBlockKeys * 2 * a.dim;
+  for (int64_t blocks : {units, q_blocks, k_blocks, f_blocks, joined / 256})
+    if (blocks >= 0x7fffffff)
+      return fail(MSX_EINVAL, "window_attention_backward has more rows than a grid holds.");
+  if (q_blocks > 0)
+    backward_queries<V, DP><<<static_cast<unsigned>(q_blocks), kThreads, 0, stream>>>(
+        a, up, static_cast<int32_t>(units), per_bh, q_blocks, static_cast<S *>(dq));
+  if (k_blocks > 0)
+    backward_keys_near<V, DP><<<static_cast<unsigned>(k_blocks), kThreads, 0, stream>>>(
+        a, up, plan, k_blocks, static_cast<S *>(dk), static_cast<S *>(dv));
+  if (f_blocks > 0) {
+    constexpr int lds = QueryTile<V, DP, 32 * kWaves>::kBytes;
+    if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(backward_keys_far<V, DP>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        e != hipSuccess)
+      return hip_fail(e, "window_attention_backward");
+    backward_keys_far<V, DP><<<static_cast<unsigned>(f_blocks), kThreads, lds, stream>>>(
+        a, up, plan, f_blocks);
+  }
+  if (joined > 0)
+    join_keys<V><<<static_cast<unsigned>((joined + 255) / 256), 256, 0, stream>>>(
+        a, plan, joined, static_cast<S *>(dk), static_cast<S *>(dv));
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MSX_OK : hip_fail(e, "window_attention_backward");
+}
+
+template <class V>
+msx_status by_dim(const WindowArgs &a, const Upstream &up, const KeyPlan &plan, void *dq, void *dk,
+                  void *dv, hipStream_t stream) {
+  if (a.dim <= 32) return run<V, 32>(a, up, plan, dq, dk, dv, stream);
+  if (a.dim <= 64) return run<V, 64>(a, up, plan, dq, dk, dv, stream);
+  if (a.dim <= 96) return run<V, 96>(a, up, plan, dq, dk, dv, stream);
+  return run<V, 128>(a, up, plan, dq, dk, dv, stream);
+}
+
+}  // namespace
+
+size_t window_backward_scratch(const WindowArgs &a) {
+  const KeyPlan p = plan_keys(a);
+  return sizeof(float) * (near_floats(a, p) + far_floats(a, p));
+}
+
+msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void *out,
+                                  const float *lse, const void *grad, const int64_t *grad_strides,
+                                  float *delta, void *dq, void *dk, void *dv, void *scratch,
+                                  hipStream_t stream) {
+  Upstream up{grad, {grad_strides[0], grad_strides[1], grad_strides[2]}, out, lse, delta};
+  KeyPlan plan = plan_keys(a);
+  plan.near_sums = static_cast<float *>(scratch);
+  plan.far_sums = plan.near_sums + near_floats(a, plan);
+  switch (vt) {
+  case MSX_F32: return by_dim<F32>(a, up, plan, dq, dk, dv, stream);
+  case MSX_F16: return by_dim<F16>(a, up, plan, dq, dk, dv, stream);
+  default: return by_dim<BF16>(a, up, plan, dq, dk, dv, stream);
+  }
+}
+
+}  // namespace msx

@@ -162,7 +162,7 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
     for (int r = 0; r < F::kPerThread; ++r) {
       const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
       if (row < F::kKeys) {
-        *reinterpret_cast<v4u *>(kt + T::across(row, chunk)) = k_next[r];
+        *reinterpret_cast<v4u *>(kt + T::along(row, chunk)) = k_next[r];
         *reinterpret_cast<v4u *>(vt + T::along(row, chunk)) = v_next[r];
       }
     }
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
         for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
 #pragma unroll
         for (int st = 0; st < kSteps; ++st)
-          s[t] = Mfma<V>::mul(read_across<V, DP>(kt, 32 * t + lane % 32, st), qf[st], s[t]);
+          s[t] = Mfma<V>::mul(read_rows<V, DP>(kt, 32 * t + lane % 32, st), qf[st], s[t]);
       }
       // all of the tile's keys seen by all of the wave's queries: no mask
       const bool whole = c0 + F::kKeys <= count && k_last <= p_first &&
