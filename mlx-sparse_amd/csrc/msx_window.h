@@ -60,6 +60,27 @@ struct Seen {
   __device__ inline int32_t key(int32_t c) const { return c < far ? c : near + c - far; }
 };
 
+// Operands of a single-token step.
+struct StepArgs {
+  int64_t batch;
+  int32_t heads, kv_heads, group, dim, slots, window, sinks;
+  float scale;
+  const void *lengths;
+  int32_t lengths64;
+  const void *q, *k, *v;
+  int64_t qs[2], ks[2], vs[2];
+  void *ck, *cv;
+  int64_t cks[3], cvs[3];
+
+  __device__ inline int64_t length(int64_t b) const {
+    return lengths64 ? static_cast<const int64_t *>(lengths)[b]
+                     : static_cast<const int32_t *>(lengths)[b];
+  }
+  __device__ inline int32_t slot(int64_t j) const {
+    return static_cast<int32_t>(j < sinks ? j : sinks + (j - sinks) % (slots - sinks));
+  }
+};
+
 // window_forward.hip: operands that takes_tiles (window_attention.hip) admits.
 msx_status launch_window_forward(msx_vtype vt, const WindowArgs &a, void *out, float *lse,
                                  hipStream_t stream);
@@ -71,5 +92,11 @@ msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void 
                                   const float *lse, const void *grad, const int64_t *grad_strides,
                                   float *delta, void *dq, void *dk, void *dv, void *scratch,
                                   hipStream_t stream);
+
+// window_step.hip: rows and caches at sixteen-byte addresses and strides.
+// `scratch`: window_step_scratch bytes.
+size_t window_step_scratch(msx_vtype vt, const StepArgs &a);
+msx_status launch_window_step(msx_vtype vt, const StepArgs &a, void *out, void *scratch,
+                              hipStream_t stream);
 
 }  // namespace msx

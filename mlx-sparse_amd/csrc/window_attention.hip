@@ -213,26 +213,6 @@ __global__ __launch_bounds__(kRowWaves * kWave) void backward_keys(
 // ---------------------------------------------------------------------------
 // Single-token step.
 
-struct StepArgs {
-  int64_t batch;
-  int32_t heads, kv_heads, group, dim, slots, window, sinks;
-  float scale;
-  const void *lengths;
-  int32_t lengths64;
-  const void *q, *k, *v;
-  int64_t qs[2], ks[2], vs[2];
-  void *ck, *cv;
-  int64_t cks[3], cvs[3];
-
-  __device__ inline int64_t length(int64_t b) const {
-    return lengths64 ? static_cast<const int64_t *>(lengths)[b]
-                     : static_cast<const int32_t *>(lengths)[b];
-  }
-  __device__ inline int32_t slot(int64_t j) const {
-    return static_cast<int32_t>(j < sinks ? j : sinks + (j - sinks) % (slots - sinks));
-  }
-};
-
 // One workgroup a (sequence, kv head): the token's row is written first, then
 // a wave takes a query head of the group after the other.
 template <class V>
@@ -377,6 +357,40 @@ bool takes_tiles(const msx_window_attention_desc &d) {
          rows_aligned(size, d.v, d.v_strides, 3);
 }
 
+StepArgs args_of(const msx_window_step_desc &d) {
+  StepArgs a{};
+  a.batch = d.batch;
+  a.heads = static_cast<int32_t>(d.heads);
+  a.kv_heads = static_cast<int32_t>(d.kv_heads);
+  a.group = a.heads / a.kv_heads;
+  a.dim = static_cast<int32_t>(d.dim);
+  a.slots = static_cast<int32_t>(d.slots);
+  a.window = static_cast<int32_t>(d.window);
+  a.sinks = static_cast<int32_t>(d.sinks);
+  a.scale = static_cast<float>(d.scale * 1.44269504088896340736);
+  a.lengths = d.lengths;
+  a.lengths64 = d.lengths_itype == MSX_I64;
+  a.q = d.q;
+  a.k = d.k;
+  a.v = d.v;
+  a.ck = d.cache_k;
+  a.cv = d.cache_v;
+  std::copy(d.q_strides, d.q_strides + 2, a.qs);
+  std::copy(d.k_strides, d.k_strides + 2, a.ks);
+  std::copy(d.v_strides, d.v_strides + 2, a.vs);
+  std::copy(d.cache_k_strides, d.cache_k_strides + 3, a.cks);
+  std::copy(d.cache_v_strides, d.cache_v_strides + 3, a.cvs);
+  return a;
+}
+
+bool takes_tiles(const msx_window_step_desc &d) {
+  const size_t size = value_bytes(static_cast<msx_vtype>(d.vtype));
+  return d.dim * size % 16 == 0 && rows_aligned(size, d.q, d.q_strides, 2) &&
+         rows_aligned(size, d.k, d.k_strides, 2) && rows_aligned(size, d.v, d.v_strides, 2) &&
+         rows_aligned(size, d.cache_k, d.cache_k_strides, 3) &&
+         rows_aligned(size, d.cache_v, d.cache_v_strides, 3);
+}
+
 // delta, before the tiles' sums (which need sixteen-byte addresses).
 size_t delta_bytes(const msx_window_attention_desc &d) {
   return (sizeof(float) * static_cast<size_t>(d.batch * d.heads * d.lq) + 255) / 256 * 256;
@@ -486,10 +500,16 @@ extern "C" msx_status msx_window_attention_backward(const msx_window_attention_d
   });
 }
 
-extern "C" size_t msx_window_attention_step_scratch(const msx_window_step_desc *) { return 0; }
+extern "C" size_t msx_window_attention_step_scratch(const msx_window_step_desc *desc) {
+  if (check_window_step("window_attention_step", desc) != MSX_OK || desc->batch == 0) return 0;
+  return takes_tiles(*desc)
+             ? window_step_scratch(static_cast<msx_vtype>(desc->vtype), args_of(*desc))
+             : 0;
+}
 
 extern "C" msx_status msx_window_attention_step(const msx_window_step_desc *desc, void *out,
-                                                void *, size_t, void *stream) {
+                                                void *scratch, size_t scratch_bytes,
+                                                void *stream) {
   clear_error();
   const char *op = "window_attention_step";
   if (msx_status st = check_window_step(op, desc); st != MSX_OK) return st;
@@ -498,28 +518,14 @@ extern "C" msx_status msx_window_attention_step(const msx_window_step_desc *desc
   if (out == nullptr) return fail(MSX_EINVAL, "window_attention_step out is NULL.");
   if (d.batch * d.kv_heads > kWindowIntMax)
     return fail(MSX_EINVAL, "window_attention_step has more rows than a grid holds.");
-  StepArgs a{};
-  a.batch = d.batch;
-  a.heads = static_cast<int32_t>(d.heads);
-  a.kv_heads = static_cast<int32_t>(d.kv_heads);
-  a.group = a.heads / a.kv_heads;
-  a.dim = static_cast<int32_t>(d.dim);
-  a.slots = static_cast<int32_t>(d.slots);
-  a.window = static_cast<int32_t>(d.window);
-  a.sinks = static_cast<int32_t>(d.sinks);
-  a.scale = static_cast<float>(d.scale * 1.44269504088896340736);
-  a.lengths = d.lengths;
-  a.lengths64 = d.lengths_itype == MSX_I64;
-  a.q = d.q;
-  a.k = d.k;
-  a.v = d.v;
-  a.ck = d.cache_k;
-  a.cv = d.cache_v;
-  std::copy(d.q_strides, d.q_strides + 2, a.qs);
-  std::copy(d.k_strides, d.k_strides + 2, a.ks);
-  std::copy(d.v_strides, d.v_strides + 2, a.vs);
-  std::copy(d.cache_k_strides, d.cache_k_strides + 3, a.cks);
-  std::copy(d.cache_v_strides, d.cache_v_strides + 3, a.cvs);
+  const StepArgs a = args_of(d);
+  const msx_vtype vt = static_cast<msx_vtype>(d.vtype);
+  if (takes_tiles(d)) {
+    const size_t need = window_step_scratch(vt, a);
+    if (scratch_bytes < need || (need > 0 && scratch == nullptr))
+      return fail(MSX_EINVAL, "window_attention_step scratch is too small.");
+    return launch_window_step(vt, a, out, scratch, static_cast<hipStream_t>(stream));
+  }
   return by_vtype(d.vtype, [&](auto v) {
     using V = decltype(v);
     step_rows<V><<<static_cast<unsigned>(a.batch * a.kv_heads), kRowWaves * kWave, 0,
