@@ -16,14 +16,12 @@
 #include "msx_internal.h"
 #include "msx_window.h"
 #include "msx_window_check.h"
+#include "msx_window_mfma.h"
 
 #pragma clang fp contract(fast)
 
 namespace msx {
 namespace {
-
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 
 struct DistillArgs {
   int64_t n_cols, ld, ld_grad, nnz;
@@ -61,11 +59,19 @@ struct DistillArgs {
 struct Stat {
   float top, sum;
   __device__ inline float base() const { return top == -INFINITY ? 0.0f : top; }
-  __device__ inline void add(float x) {
-    const float t = fmaxf(top, x);
-    const float b = t == -INFINITY ? 0.0f : t;
-    sum = sum * exp2_fast(top - b) + exp2_fast(x - b);
-    top = t;
+  __device__ inline float log_sum() const { return base() + log2_fast(sum); }
+  template <int N>
+  __device__ inline void add(const float (&x)[N]) {
+    float t = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) t = fmaxf(t, x[j]);
+    if (t > top) {
+      sum *= exp2_fast(top - t);
+      top = t;
+    }
+    const float b = base();
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum += exp2_fast(x[j] - b);
   }
   __device__ inline void merge(Stat o) {
     const float t = fmaxf(top, o.top);
@@ -73,107 +79,222 @@ struct Stat {
     sum = sum * exp2_fast(top - b) + o.sum * exp2_fast(o.top - b);
     top = t;
   }
+  __device__ inline void merge_wave() {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) merge({__shfl_xor(top, d), __shfl_xor(sum, d)});
+  }
 };
 
-__device__ inline Stat block_merge(Stat s, Stat *lds) {
+// A row as sixteen-byte pieces at sixteen-byte addresses, and up to seven
+// values before and after them, one a thread.
+template <class V>
+struct RowPieces {
+  using S = typename V::Storage;
+  static constexpr int kPer = 16 / sizeof(S);
+  int64_t n;
+  int32_t head;
+  int64_t pieces;
+  __device__ inline RowPieces(const S *row, int64_t columns) : n(columns) {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(S));
+    const int lead = off == 0 ? 0 : kPer - off;
+    head = static_cast<int32_t>(lead < n ? lead : n);
+    pieces = (n - head) / kPer;
+  }
+  // The column of this thread's single value, or -1.
+  __device__ inline int64_t single() const {
+    const int64_t tail = head + pieces * kPer, t = threadIdx.x;
+    if (t < head) return t;
+    return tail + (t - head) < n ? tail + (t - head) : -1;
+  }
+  __device__ static inline void widen(v4u piece, float scale, float (&x)[kPer]) {
+    const v4f values = __builtin_bit_cast(v4f, piece);
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) s.merge({__shfl_xor(s.top, d), __shfl_xor(s.sum, d)});
-  const int wave = threadIdx.x / kWave;
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) lds[wave] = s;
-  __syncthreads();
-  s = lds[0];
-  for (int w = 1; w < kWaves; ++w) s.merge(lds[w]);
-  return s;
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kPer == 4) {
+        x[j] = values[j] * scale;
+      } else {
+        x[2 * j] = V::widen(static_cast<uint16_t>(piece[j])) * scale;
+        x[2 * j + 1] = V::widen(static_cast<uint16_t>(piece[j] >> 16)) * scale;
+      }
+    }
+  }
+};
+
+// q factor of a piece, rounded.
+template <class V>
+__device__ inline v4u softmax_piece(v4u piece, float scale, float total, float factor) {
+  constexpr int kPer = RowPieces<V>::kPer;
+  float x[kPer];
+  RowPieces<V>::widen(piece, scale, x);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) x[j] = exp2_fast(x[j] - total) * factor;
+  v4u out;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (kPer == 4)
+      out[j] = __builtin_bit_cast(uint32_t, x[j]);
+    else
+      out[j] = Mfma<V>::pack(x[2 * j], x[2 * j + 1]);
+  }
+  return out;
 }
 
-__device__ inline float block_sum(float v, float *lds) {
-  v = wave_sum(v);
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  v = lds[0];
-  for (int w = 1; w < kWaves; ++w) v += lds[w];
-  return v;
+// A piece to where the gradient's rows lie, which may start elsewhere in
+// their sixteen bytes than the logits'.  It is not read again here.
+template <class S>
+__device__ inline void store_piece(v4u piece, S *to) {
+  if (reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+    __builtin_nontemporal_store(piece, reinterpret_cast<v4u *>(to));
+  } else {
+    S v[16 / sizeof(S)];
+    __builtin_memcpy(v, &piece, 16);
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(16 / sizeof(S)); ++j) to[j] = v[j];
+  }
 }
 
 // kLoss: losses (and lse where asked); kGrad: the gradient, from `lse_in` or
 // from the row's own pass.
-template <class V, bool kLoss, bool kGrad>
-__global__ __launch_bounds__(kThreads) void distill_rows(DistillArgs a, float *losses, float *lse,
+template <class V, bool kLoss, bool kGrad, int kThreads>
+__global__ __launch_bounds__(kThreads, 8) void distill_rows(DistillArgs a, float *losses, float *lse,
                                                          const float *lse_in,
                                                          typename V::Storage *grad) {
   using S = typename V::Storage;
-  __shared__ Stat stat_lds[kWaves];
-  __shared__ float sum_lds[kWaves];
+  using Row = RowPieces<V>;
+  constexpr int kPer = Row::kPer, kWaves = kThreads / kWave, kAhead = 4;
+  __shared__ Stat kept_lds[kWaves], stat_lds[kWaves];
+  __shared__ float part_lds[kWaves];
+  __shared__ int ascending_lds[kWaves];
+  const int wave = threadIdx.x / kWave;
   const int64_t row = blockIdx.x;
   const S *z = static_cast<const S *>(a.logits) + row * a.ld;
   S *g = kGrad ? grad + row * a.ld_grad : nullptr;
   const int64_t begin = a.offset(row), end = a.offset(row + 1);
   const float weight = kGrad ? a.weight(row) : 0.0f;
 
-  // the teacher's distribution; ascending: no column is there twice
+  // the thread's first kept logit stays at hand; ascending: none is there twice
   Stat kept{-INFINITY, 0.0f};
+  int64_t column = -1;
+  float mine = -INFINITY, mine_z = 0.0f;
   int ascending = 1;
   for (int64_t e = begin + threadIdx.x; e < end; e += kThreads) {
     const int64_t c = a.column(e);
-    if (c >= 0) kept.add(a.kept(e));
+    const float t = c >= 0 ? a.kept(e) : -INFINITY;
+    kept.add<1>({t});
     if (e + 1 < end && a.column(e + 1) <= c) ascending = 0;
-  }
-  kept = block_merge(kept, stat_lds);
-  ascending = __syncthreads_and(ascending);
-  const bool target = !(kept.sum == 0.0f);
-
-  if (!target) {
-    if (kLoss && threadIdx.x == 0) {
-      losses[row] = 0.0f;
-      if (lse != nullptr) lse[row] = 0.0f;
+    if (e == begin + threadIdx.x && c >= 0) {
+      column = c;
+      mine = t;
+      mine_z = V::widen(z[c]) * a.scale;
     }
   }
+  kept.merge_wave();
+  ascending = __all(ascending);
+
+  const Row r(z, a.n_cols);
+  const v4u *pieces = reinterpret_cast<const v4u *>(z + r.head);
+  const int64_t single = r.single();
+  Stat s{-INFINITY, 0.0f};
+  if (kLoss && begin < end) {
+    int64_t c = threadIdx.x;
+    for (; c + (kAhead - 1) * kThreads < r.pieces; c += kAhead * kThreads) {
+      v4u w[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) w[k] = pieces[c + k * kThreads];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        float x[kPer];
+        Row::widen(w[k], a.scale, x);
+        s.add<kPer>(x);
+      }
+    }
+    for (; c < r.pieces; c += kThreads) {
+      float x[kPer];
+      Row::widen(pieces[c], a.scale, x);
+      s.add<kPer>(x);
+    }
+    if (single >= 0) s.add<1>({V::widen(z[single]) * a.scale});
+    s.merge_wave();
+  }
+  if (threadIdx.x % kWave == 0) {
+    kept_lds[wave] = kept;
+    stat_lds[wave] = s;
+    ascending_lds[wave] = ascending;
+  }
+  __syncthreads();
+  kept = kept_lds[0];
+  s = stat_lds[0];
+  ascending = ascending_lds[0];
+  for (int w = 1; w < kWaves; ++w) {
+    kept.merge(kept_lds[w]);
+    if (kLoss) s.merge(stat_lds[w]);
+    ascending &= ascending_lds[w];
+  }
+
+  const bool target = !(kept.sum == 0.0f);  // NaN is one
   const bool wanted = kGrad && target && weight != 0.0f;
-  if (kGrad && !wanted)
-    for (int64_t c = threadIdx.x; c < a.n_cols; c += kThreads) g[c] = 0;
-  if (!target || !(kLoss || wanted)) return;
-
-  const float kept_base = kept.base(), kept_inv = 1.0f / kept.sum;
-  const float kept_lse = kept_base + log2_fast(kept.sum);
-  float total;
+  const float kept_base = kept.base(), kept_inv = 1.0f / kept.sum, kept_lse = kept.log_sum();
+  const float total = !kLoss ? (wanted ? lse_in[row] : 0.0f) : s.log_sum();
   if (kLoss) {
-    Stat s{-INFINITY, 0.0f};
-    for (int64_t c = threadIdx.x; c < a.n_cols; c += kThreads) s.add(V::widen(z[c]) * a.scale);
-    s = block_merge(s, stat_lds);
-    total = s.base() + log2_fast(s.sum);
     float part = 0.0f;
-    for (int64_t e = begin + threadIdx.x; e < end; e += kThreads) {
-      const int64_t c = a.column(e);
-      if (c < 0) continue;
-      const float t = a.kept(e), p = exp2_fast(t - kept_base) * kept_inv;
-      if (p != 0.0f) part += p * ((t - kept_lse) - (V::widen(z[c]) * a.scale - total));
-    }
-    part = block_sum(part, sum_lds);
-    if (threadIdx.x == 0) {
-      losses[row] = part * kLn2 * a.temperature * a.temperature;
-      if (lse != nullptr) lse[row] = total;
-    }
-    if (!wanted) return;
-  } else {
-    total = lse_in[row];
+    if (target)
+      for (int64_t e = begin + threadIdx.x; e < end; e += kThreads) {
+        const bool first = e == begin + threadIdx.x;
+        const int64_t c = first ? column : a.column(e);
+        if (c < 0) continue;
+        const float t = first ? mine : a.kept(e);
+        const float x = first ? mine_z : V::widen(z[c]) * a.scale;
+        const float p = exp2_fast(t - kept_base) * kept_inv;
+        if (p != 0.0f) part += p * ((t - kept_lse) - (x - total));
+      }
+    part = wave_sum(part);
+    if (threadIdx.x % kWave == 0) part_lds[wave] = part;
   }
   if (kGrad) {
+    if (wanted) {
+      const float factor = weight * a.temperature;
+      int64_t c = threadIdx.x;
+      for (; c + (kAhead - 1) * kThreads < r.pieces; c += kAhead * kThreads) {
+        v4u w[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) w[k] = pieces[c + k * kThreads];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          store_piece(softmax_piece<V>(w[k], a.scale, total, factor),
+                      g + r.head + (c + k * kThreads) * kPer);
+      }
+      for (; c < r.pieces; c += kThreads)
+        store_piece(softmax_piece<V>(pieces[c], a.scale, total, factor), g + r.head + c * kPer);
+      if (single >= 0)
+        g[single] = V::narrow(exp2_fast(V::widen(z[single]) * a.scale - total) * factor);
+    } else {
+      const v4u none = {0, 0, 0, 0};
+      for (int64_t c = threadIdx.x; c < r.pieces; c += kThreads)
+        store_piece(none, g + r.head + c * kPer);
+      if (single >= 0) g[single] = 0;
+    }
+  }
+  if (kLoss || wanted) __syncthreads();
+  if (kLoss && threadIdx.x == 0) {
+    float part = part_lds[0];
+    for (int w = 1; w < kWaves; ++w) part += part_lds[w];
+    losses[row] = target ? part * kLn2 * a.temperature * a.temperature : 0.0f;
+    if (lse != nullptr) lse[row] = target ? total : 0.0f;
+  }
+  if (wanted) {
     const float factor = weight * a.temperature;
-    for (int64_t c = threadIdx.x; c < a.n_cols; c += kThreads)
-      g[c] = V::narrow(exp2_fast(V::widen(z[c]) * a.scale - total) * factor);
-    __syncthreads();
     for (int64_t e = begin + threadIdx.x; e < end; e += kThreads) {
-      const int64_t c = a.column(e);
+      const bool first = e == begin + threadIdx.x;
+      const int64_t c = first ? column : a.column(e);
       if (c < 0) continue;
-      float p = exp2_fast(a.kept(e) - kept_base) * kept_inv;
+      float p = exp2_fast((first ? mine : a.kept(e)) - kept_base) * kept_inv;
       if (!ascending) {
         p = 0.0f;
         for (int64_t o = begin; o < end; ++o)
           if (a.column(o) == c) p += exp2_fast(a.kept(o) - kept_base) * kept_inv;
       }
-      g[c] = V::narrow((exp2_fast(V::widen(z[c]) * a.scale - total) - p) * factor);
+      const float x = first ? mine_z : V::widen(z[c]) * a.scale;
+      g[c] = V::narrow((exp2_fast(x - total) - p) * factor);
     }
   }
 }
@@ -197,15 +318,27 @@ DistillArgs args_of(const msx_distill_desc &d, int64_t ld_grad) {
   return a;
 }
 
+// Row sizes up to which a row has a wave, and four.
+constexpr int64_t kWaveRow = 4 << 10;
+constexpr int64_t kQuarterRow = 64 << 10;
+
 template <bool kLoss, bool kGrad>
 msx_status launch(const msx_distill_desc &d, float *losses, float *lse, const float *lse_in,
                   void *grad, int64_t ld_grad, void *stream) {
   const DistillArgs a = args_of(d, ld_grad);
   const auto run = [&](auto v) {
     using V = decltype(v);
-    distill_rows<V, kLoss, kGrad>
-        <<<static_cast<unsigned>(d.n_rows), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            a, losses, lse, lse_in, static_cast<typename V::Storage *>(grad));
+    using S = typename V::Storage;
+    const auto blocks = static_cast<unsigned>(d.n_rows);
+    const auto st = static_cast<hipStream_t>(stream);
+    S *g = static_cast<S *>(grad);
+    const int64_t bytes = d.n_cols * static_cast<int64_t>(sizeof(S));
+    if (bytes <= kWaveRow)
+      distill_rows<V, kLoss, kGrad, 64><<<blocks, 64, 0, st>>>(a, losses, lse, lse_in, g);
+    else if (bytes <= kQuarterRow)
+      distill_rows<V, kLoss, kGrad, 256><<<blocks, 256, 0, st>>>(a, losses, lse, lse_in, g);
+    else
+      distill_rows<V, kLoss, kGrad, 1024><<<blocks, 1024, 0, st>>>(a, losses, lse, lse_in, g);
   };
   switch (d.vtype) {
   case MSX_F32: run(F32{}); break;

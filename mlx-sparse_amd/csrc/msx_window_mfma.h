@@ -154,7 +154,8 @@ __device__ inline void mul_transposed(const char *tile, int row0, const float (&
 __device__ inline float other_half(float v) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __builtin_bit_cast(float, (threadIdx.x % kWave) < 32 ? r[1] : r[0]);
+  const uint32_t other = (threadIdx.x % kWave) < 32 ? r[1] : r[0];
+  return __builtin_bit_cast(float, other);
 }
 
 // Workgroups go to the 8 XCDs in turn; this gives each XCD one contiguous
