@@ -961,9 +961,12 @@ typedef struct msx_window_attention_desc {
  * Forward product: `out` is batch x lq x heads x dim, contiguous.  `lse`
  * (NULL, or batch x heads x lq floats) gets what the backward pass needs of
  * the softmax: the base-2 logarithm of its sum, +inf for a row without one.
+ * `scratch` holds msx_window_attention_scratch bytes (mostly none) at a
+ * sixteen-byte address.
  */
+size_t msx_window_attention_scratch(const msx_window_attention_desc *desc);
 msx_status msx_window_attention(const msx_window_attention_desc *desc, void *out,
-                                float *lse, void *stream);
+                                float *lse, void *scratch, size_t scratch_bytes, void *stream);
 
 /*
  * Gradients of the product: `grad` is the gradient of `out`, with strides as

@@ -82,8 +82,10 @@ struct StepArgs {
 };
 
 // window_forward.hip: operands that takes_tiles (window_attention.hip) admits.
+// `scratch`: window_forward_scratch bytes at a sixteen-byte address.
+size_t window_forward_scratch(msx_vtype vt, const WindowArgs &a);
 msx_status launch_window_forward(msx_vtype vt, const WindowArgs &a, void *out, float *lse,
-                                 hipStream_t stream);
+                                 void *scratch, hipStream_t stream);
 
 // window_backward.hip: the same operands; `grad` aligned as they are.
 // `delta`: batch x heads x lq floats, `scratch`: window_backward_scratch bytes.

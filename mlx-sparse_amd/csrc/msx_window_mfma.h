@@ -165,4 +165,50 @@ __device__ inline int64_t xcd_order(int64_t id, int64_t n) {
   return x * per + (x < rest ? x : rest) + at;
 }
 
+// How equal blocks of work are cut over `slots` workgroups that run at once:
+// the first `whole` run as they are, each of the rest in `parts`, so that the
+// last round does not leave most of the chip waiting for a few blocks.
+struct TailCut {
+  int64_t whole, rest;
+  int32_t parts;
+  __host__ __device__ inline int64_t items() const { return whole + rest * parts; }
+};
+
+// A part costs what kPartCost of a block does, in writing and joining sums.
+inline TailCut cut_tail(int64_t blocks, int64_t slots, int64_t most_parts) {
+  constexpr double kPartCost = 0.04;
+  const int64_t rest = blocks % slots;
+  TailCut cut{blocks, 0, 1};
+  double best = rest > 0 ? 1.0 : 0.0;
+  for (int64_t p = 2; p <= most_parts && p <= 16 && rest > 0; ++p) {
+    const double rounds = static_cast<double>((rest * p + slots - 1) / slots) / p;
+    const double cost = rounds + kPartCost * (1 + rest * p / static_cast<double>(slots));
+    if (cost < best) {
+      best = cost;
+      cut = TailCut{blocks - rest, rest, static_cast<int32_t>(p)};
+    }
+  }
+  return cut;
+}
+
+// Which block and part of it a workgroup takes; the whole ones in XCD order.
+struct CutItem {
+  int64_t block;
+  int32_t part, parts;
+  int64_t slot;  // of its sums in scratch, -1 for a whole block
+  __device__ inline CutItem(const TailCut &cut, int64_t id) {
+    if (id < cut.whole) {
+      block = xcd_order(id, cut.whole);
+      part = 0;
+      parts = 1;
+      slot = -1;
+    } else {
+      slot = id - cut.whole;
+      block = cut.whole + slot / cut.parts;
+      part = static_cast<int32_t>(slot % cut.parts);
+      parts = cut.parts;
+    }
+  }
+};
+
 }  // namespace msx

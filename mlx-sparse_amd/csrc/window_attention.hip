@@ -423,16 +423,29 @@ msx_status launched(const char *what) {
 
 using namespace msx;
 
+extern "C" size_t msx_window_attention_scratch(const msx_window_attention_desc *desc) {
+  if (check_window_attention("window_attention", desc) != MSX_OK || desc->batch == 0 ||
+      desc->lq == 0 || !takes_tiles(*desc))
+    return 0;
+  return window_forward_scratch(static_cast<msx_vtype>(desc->vtype), args_of(*desc));
+}
+
 extern "C" msx_status msx_window_attention(const msx_window_attention_desc *desc, void *out,
-                                           float *lse, void *stream) {
+                                           float *lse, void *scratch, size_t scratch_bytes,
+                                           void *stream) {
   clear_error();
   if (msx_status st = check_window_attention("window_attention", desc); st != MSX_OK) return st;
   if (desc->batch == 0 || desc->lq == 0) return MSX_OK;
   if (out == nullptr) return fail(MSX_EINVAL, "window_attention out is NULL.");
   const WindowArgs a = args_of(*desc);
-  if (takes_tiles(*desc) && reinterpret_cast<uintptr_t>(out) % 16 == 0)
-    return launch_window_forward(static_cast<msx_vtype>(desc->vtype), a, out, lse,
-                                 static_cast<hipStream_t>(stream));
+  if (takes_tiles(*desc) && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    const auto vt = static_cast<msx_vtype>(desc->vtype);
+    const size_t need = window_forward_scratch(vt, a);
+    if (scratch_bytes < need || (need > 0 && (scratch == nullptr ||
+                                              reinterpret_cast<uintptr_t>(scratch) % 16 != 0)))
+      return fail(MSX_EINVAL, "window_attention scratch is too small or not aligned.");
+    return launch_window_forward(vt, a, out, lse, scratch, static_cast<hipStream_t>(stream));
+  }
   const int64_t rows = a.batch * a.lq * a.heads;
   unsigned blocks = 0;
   if (msx_status st = grid_for("window_attention", rows, &blocks); st != MSX_OK) return st;

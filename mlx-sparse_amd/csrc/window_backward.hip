@@ -509,24 +509,35 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
   store_sums<DP>(keys.dk, keys.dv, a.dim, plan.far_sums + (slot * 32 + lane % 32) * 2 * a.dim);
 }
 
-// dk and dv of the joined blocks: a block's parts, then the far parts, in order.
+// dk and dv of the joined blocks.  Sixteen sums a wave, four lanes a sum: each
+// takes every fourth part, and they are added in order.
 template <class V>
 __global__ __launch_bounds__(256) void join_keys(WindowArgs a, KeyPlan plan, int64_t total,
                                                  typename V::Storage *dk, typename V::Storage *dv) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= total) return;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x / kWave * 16 + threadIdx.x % 16;
+  const int quarter = threadIdx.x % kWave / 16;
   const int64_t dims = 2 * a.dim;
   const int32_t d = static_cast<int32_t>(at % dims);
   const int32_t key = static_cast<int32_t>(at / dims % (static_cast<int64_t>(plan.joined) * kBlockKeys));
   const int64_t bh = at / dims / (static_cast<int64_t>(plan.joined) * kBlockKeys);
-  if (key >= a.lk) return;
+  const bool live = at < total && key < a.lk;
   const int32_t block = key / kBlockKeys;
   float sum = 0.0f;
-  for (int32_t part = 0; part < plan.parts; ++part)
-    sum += plan.near_sums[((((bh * plan.joined + block) * plan.parts + part) * kBlockKeys) + key % kBlockKeys) * dims + d];
-  if (key < a.sinks && key / 32 < plan.far_units)
-    for (int32_t part = 0; part < plan.far_parts * kWaves; ++part)
-      sum += plan.far_sums[((((bh * plan.far_units + key / 32) * plan.far_parts * kWaves + part) * 32) + key % 32) * dims + d];
+  if (live) {
+    const float *near = plan.near_sums +
+        ((bh * plan.joined + block) * plan.parts * kBlockKeys + key % kBlockKeys) * dims + d;
+    for (int32_t part = quarter; part < plan.parts; part += 4) sum += near[part * kBlockKeys * dims];
+    if (key < a.sinks && key / 32 < plan.far_units) {
+      const int32_t parts = plan.far_parts * kWaves;
+      const float *far = plan.far_sums +
+          ((bh * plan.far_units + key / 32) * parts * 32 + key % 32) * dims + d;
+#pragma unroll 8
+      for (int32_t part = quarter; part < parts; part += 4) sum += far[part * 32 * dims];
+    }
+  }
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if (!live || quarter != 0) return;
   const int64_t row = (bh / a.kv_heads * a.lk + key) * a.kv_heads + bh % a.kv_heads;
   if (d < a.dim)
     dk[row * a.dim + d] = V::narrow(sum * a.grad_scale);
@@ -576,7 +587,7 @@ msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, 
   const int64_t per_bh = (units + kWaves - 1) / kWaves, q_blocks = per_bh * bh;
   const int64_t k_blocks = bh * plan.blocks * plan.parts, f_blocks = bh * plan.far_units * plan.far_parts;
   const int64_t joined = bh * plan.joined * kBlockKeys * 2 * a.dim;
-  for (int64_t blocks : {units, q_blocks, k_blocks, f_blocks, joined / 256})
+  for (int64_t blocks : {units, q_blocks, k_blocks, f_blocks, joined / 64})
     if (blocks >= 0x7fffffff)
       return fail(MSX_EINVAL, "window_attention_backward has more rows than a grid holds.");
   if (q_blocks > 0)
@@ -595,7 +606,7 @@ msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, 
         a, up, plan, f_blocks);
   }
   if (joined > 0)
-    join_keys<V><<<static_cast<unsigned>((joined + 255) / 256), 256, 0, stream>>>(
+    join_keys<V><<<static_cast<unsigned>((joined + 63) / 64), 256, 0, stream>>>(
         a, plan, joined, static_cast<S *>(dk), static_cast<S *>(dv));
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "window_attention_backward");

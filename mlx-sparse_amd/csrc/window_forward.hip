@@ -10,6 +10,8 @@
 // sum, O^T += V^T P^T; the next tile's rows are in flight meanwhile.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "msx_internal.h"
 #include "msx_window.h"
 #include "msx_window_mfma.h"
@@ -34,6 +36,7 @@ struct ForwardShape {
   // workgroups a CU: two hide each other's waits; wide float32 heads need the
   // registers of one (76 spilled with two at 128)
   static constexpr int kBlocks = T::kRowBytes > 256 ? 1 : 2;
+  static constexpr int kStride = DP + 4;  // of a row's sums, m and l in scratch
 };
 
 // A query row by its definition, one wave: keys over the lanes for the
@@ -80,8 +83,9 @@ __device__ void forward_row(const WindowArgs &a, int64_t b, int32_t i, int32_t h
 
 template <class V, int DP>
 __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forward_tiles(WindowArgs a, int32_t units_per_bh,
-                                                             int64_t blocks_per_bh, int64_t blocks,
-                                                             typename V::Storage *out, float *lse) {
+                                                             int64_t blocks_per_bh, TailCut cut,
+                                                             typename V::Storage *out, float *lse,
+                                                             float *sums) {
   using S = typename V::Storage;
   using T = TileShape<V, DP>;
   using F = ForwardShape<V, DP>;
@@ -90,9 +94,9 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   __shared__ __attribute__((aligned(16))) char lds[F::kLds];
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, half = lane / 32;
-  const int64_t id = xcd_order(blockIdx.x, blocks);
-  const int64_t bh = id / blocks_per_bh;
-  const int32_t first_unit = static_cast<int32_t>(id % blocks_per_bh) * kWaves;
+  const CutItem item(cut, blockIdx.x);
+  const int64_t bh = item.block / blocks_per_bh;
+  const int32_t first_unit = static_cast<int32_t>(item.block % blocks_per_bh) * kWaves;
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
   const int32_t n = a.length(b), offset = a.lk - a.lq;
@@ -175,11 +179,14 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
 
-  fetch(0);
+  const int32_t tiles = (count + F::kKeys - 1) / F::kKeys;
+  const int32_t c_begin = static_cast<int32_t>(static_cast<int64_t>(tiles) * item.part / item.parts) * F::kKeys;
+  const int32_t c_end = static_cast<int32_t>(static_cast<int64_t>(tiles) * (item.part + 1) / item.parts) * F::kKeys;
+  fetch(c_begin);
   keep(0);
   __syncthreads();
-  for (int32_t c0 = 0, buffer = 0; c0 < count; c0 += F::kKeys, buffer ^= 1) {
-    const bool more = c0 + F::kKeys < count;
+  for (int32_t c0 = c_begin, buffer = 0; c0 < c_end; c0 += F::kKeys, buffer ^= 1) {
+    const bool more = c0 + F::kKeys < c_end;
     if (more) fetch(c0 + F::kKeys);
     const char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
 
@@ -247,6 +254,20 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   }
 
   l += other_half(l);
+  if (item.slot >= 0) {  // a part: its sums as they are, joined by forward_join
+    float *to = sums + ((item.slot * kWaves + wave) * kRows + lane % 32) * F::kStride;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<v4f *>(to + dt * 32 + 2 * r + 4 * half) =
+            v4f{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]};
+    if (half == 0) {
+      to[DP] = m;
+      to[DP + 1] = l;
+    }
+    return;
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   bool odd = false;  // something is not finite: the row is computed anew
   if (live && i < a.lq) {
@@ -282,35 +303,118 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   }
 }
 
+// A wave a query row of the blocks that ran in parts.
 template <class V, int DP>
-msx_status run(const WindowArgs &a, void *out, float *lse, hipStream_t stream) {
-  const int64_t units = (static_cast<int64_t>(a.lq) + kRows - 1) / kRows * a.group;
-  const int64_t per_bh = (units + kWaves - 1) / kWaves, blocks = per_bh * a.batch * a.kv_heads;
-  if (units > 0x7fffffff || blocks > 0x7fffffff)
+__global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t units_per_bh,
+                                                         int64_t blocks_per_bh, TailCut cut,
+                                                         const float *sums,
+                                                         typename V::Storage *out, float *lse) {
+  constexpr int kStride = ForwardShape<V, DP>::kStride;
+  __shared__ float q_lds[kWaves][DP];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + wave;  // (block, wave, row)
+  const int64_t rest = at / (kWaves * kRows), block = cut.whole + rest, bh = block / blocks_per_bh;
+  const int32_t in_block = static_cast<int32_t>(at % (kWaves * kRows));
+  const int64_t unit = block % blocks_per_bh * kWaves + in_block / kRows;
+  const int64_t b = bh / a.kv_heads;
+  const int32_t i = static_cast<int32_t>(unit / a.group) * kRows + in_block % kRows;
+  if (rest >= cut.rest || unit >= units_per_bh || i >= a.lq) return;
+  const int32_t h = static_cast<int32_t>(bh % a.kv_heads) * a.group + static_cast<int32_t>(unit % a.group);
+  const int32_t p = i + a.lk - a.lq;
+  const float *first = sums + (rest * cut.parts * kWaves * kRows + in_block) * kStride;
+  constexpr int64_t part_stride = static_cast<int64_t>(kWaves) * kRows * kStride;
+  float m = -INFINITY, l = 0.0f, o[(DP + kWave - 1) / kWave] = {};
+  for (int32_t part = 0; part < cut.parts; ++part) m = fmaxf(m, first[part * part_stride + DP]);
+  const float base = m == -INFINITY ? 0.0f : m;
+  for (int32_t part = 0; part < cut.parts; ++part) {
+    const float *from = first + part * part_stride;
+    const float f = exp2_fast(from[DP] - base);
+    l += from[DP + 1] * f;
+#pragma unroll
+    for (int r = 0; r < (DP + kWave - 1) / kWave; ++r)
+      if (lane + kWave * r < DP) o[r] += from[lane + kWave * r] * f;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  bool odd = false;
+#pragma unroll
+  for (int r = 0; r < (DP + kWave - 1) / kWave; ++r) {
+    const int d = lane + kWave * r;
+    if (d >= a.dim) continue;
+    odd = odd || !(fabsf(o[r] * inv) < INFINITY);
+    out[((b * a.lq + i) * a.heads + h) * a.dim + d] = V::narrow(o[r] * inv);
+  }
+  if (lse != nullptr && lane == 0)
+    lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
+  if (__any(odd) && p >= 0 && p < a.length(b)) forward_row<V>(a, b, i, h, p, q_lds[wave], out);
+}
+
+// Blocks of queries and how they are cut: into parts of eight tiles at least.
+struct Grid {
+  int64_t units, per_bh;
+  TailCut cut;
+};
+
+template <class V, int DP>
+Grid grid_of(const WindowArgs &a) {
+  using F = ForwardShape<V, DP>;
+  Grid g;
+  g.units = (static_cast<int64_t>(a.lq) + kRows - 1) / kRows * a.group;
+  g.per_bh = (g.units + kWaves - 1) / kWaves;
+  const int64_t keys = std::min<int64_t>(a.lk, static_cast<int64_t>(a.window) + a.sinks + kRows);
+  g.cut = cut_tail(g.per_bh * a.batch * a.kv_heads, 256 * F::kBlocks, keys / (8 * F::kKeys));
+  return g;
+}
+
+template <class V, int DP>
+msx_status run(const WindowArgs &a, void *out, float *lse, float *sums, size_t *bytes,
+               hipStream_t stream) {
+  const Grid g = grid_of<V, DP>(a);
+  const int64_t rows = g.cut.rest * kWaves * kRows;
+  if (bytes != nullptr) {
+    *bytes = sizeof(float) * static_cast<size_t>(rows * g.cut.parts) * ForwardShape<V, DP>::kStride;
+    return MSX_OK;
+  }
+  if (g.units > 0x7fffffff || g.cut.items() > 0x7fffffff)
     return fail(MSX_EINVAL, "window_attention has more rows than a grid holds.");
-  forward_tiles<V, DP><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-      a, static_cast<int32_t>(units), per_bh, blocks, static_cast<typename V::Storage *>(out), lse);
+  auto *to = static_cast<typename V::Storage *>(out);
+  forward_tiles<V, DP><<<static_cast<unsigned>(g.cut.items()), kThreads, 0, stream>>>(
+      a, static_cast<int32_t>(g.units), g.per_bh, g.cut, to, lse, sums);
+  if (rows > 0)
+    forward_join<V, DP><<<static_cast<unsigned>(rows / kWaves), kThreads, 0, stream>>>(
+        a, static_cast<int32_t>(g.units), g.per_bh, g.cut, sums, to, lse);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "window_attention");
 }
 
 template <class V>
-msx_status by_dim(const WindowArgs &a, void *out, float *lse, hipStream_t stream) {
-  if (a.dim <= 32) return run<V, 32>(a, out, lse, stream);
-  if (a.dim <= 64) return run<V, 64>(a, out, lse, stream);
-  if (a.dim <= 96) return run<V, 96>(a, out, lse, stream);
-  return run<V, 128>(a, out, lse, stream);
+msx_status by_dim(const WindowArgs &a, void *out, float *lse, float *sums, size_t *bytes,
+                  hipStream_t stream) {
+  if (a.dim <= 32) return run<V, 32>(a, out, lse, sums, bytes, stream);
+  if (a.dim <= 64) return run<V, 64>(a, out, lse, sums, bytes, stream);
+  if (a.dim <= 96) return run<V, 96>(a, out, lse, sums, bytes, stream);
+  return run<V, 128>(a, out, lse, sums, bytes, stream);
+}
+
+msx_status by_type(msx_vtype vt, const WindowArgs &a, void *out, float *lse, float *sums,
+                   size_t *bytes, hipStream_t stream) {
+  switch (vt) {
+  case MSX_F32: return by_dim<F32>(a, out, lse, sums, bytes, stream);
+  case MSX_F16: return by_dim<F16>(a, out, lse, sums, bytes, stream);
+  default: return by_dim<BF16>(a, out, lse, sums, bytes, stream);
+  }
 }
 
 }  // namespace
 
+size_t window_forward_scratch(msx_vtype vt, const WindowArgs &a) {
+  size_t bytes = 0;
+  by_type(vt, a, nullptr, nullptr, nullptr, &bytes, nullptr);
+  return bytes;
+}
+
 msx_status launch_window_forward(msx_vtype vt, const WindowArgs &a, void *out, float *lse,
-                                 hipStream_t stream) {
-  switch (vt) {
-  case MSX_F32: return by_dim<F32>(a, out, lse, stream);
-  case MSX_F16: return by_dim<F16>(a, out, lse, stream);
-  default: return by_dim<BF16>(a, out, lse, stream);
-  }
+                                 void *scratch, hipStream_t stream) {
+  return by_type(vt, a, out, lse, static_cast<float *>(scratch), nullptr, stream);
 }
 
 }  // namespace msx

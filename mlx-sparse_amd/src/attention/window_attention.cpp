@@ -97,7 +97,7 @@ msx_window_attention_desc window_attention_desc(const ArrayView &q, const ArrayV
 void window_attention(const msx_window_attention_desc &desc, const ArrayView &out, float *lse,
                       const ExecContext &ctx) {
   require_contiguous(out, "window_attention output");
-  check_status(out.device >= 0 ? msx_window_attention(&desc, out.ptr, lse, ctx.stream)
+  check_status(out.device >= 0 ? msx_window_attention(&desc, out.ptr, lse, ctx.scratch, ctx.scratch_bytes, ctx.stream)
                                : msx_window_attention_cpu(&desc, out.ptr, lse, ctx.n_threads),
                "window_attention");
 }

@@ -852,7 +852,9 @@ py::tuple window_attention(py::handle q_o, py::handle k_o, py::handle v_o, py::h
   if (with_lse) lse = new_tensor(q_o, {desc.batch, desc.heads, desc.lq}, at::kFloat);
   const ArrayView vo = view_of(out);
   float *l = with_lse ? lse.data_ptr<float>() : nullptr;
-  const msx::ExecContext ctx = context_for(q, n_threads);
+  msx::ExecContext ctx = context_for(q, n_threads);
+  at::Tensor scratch;
+  if (q.device >= 0) scratch = scratch_for(ctx, q_o, msx_window_attention_scratch(&desc));
   run_op(q, [&] { msx::window_attention(desc, vo, l, ctx); });
   return py::make_tuple(wrap(out), with_lse ? wrap(lse) : py::object(py::none()));
 }

@@ -157,11 +157,11 @@ def test_c_entry_points_refuse():
     """Status codes, before any HIP call."""
     L = _capi.lib()
     desc = (ctypes.c_char * 512)()
-    assert L.msx_window_attention(None, None, None, None) == _capi.EINVAL
+    assert L.msx_window_attention(None, None, None, None, ctypes.c_size_t(0), None) == _capi.EINVAL
     head = ctypes.cast(desc, ctypes.POINTER(ctypes.c_int32))
     head[0] = 3  # complex values
-    assert L.msx_window_attention(desc, None, None, None) == _capi.ETYPE
+    assert L.msx_window_attention(desc, None, None, None, ctypes.c_size_t(0), None) == _capi.ETYPE
     assert L.msx_window_attention_step(desc, None, None, ctypes.c_size_t(0), None) == _capi.ETYPE
     head[0] = 0
-    assert L.msx_window_attention(desc, None, None, None) == _capi.EINVAL  # no heads
+    assert L.msx_window_attention(desc, None, None, None, ctypes.c_size_t(0), None) == _capi.EINVAL  # no heads
     assert "heads" in _capi.last_error()

@@ -119,6 +119,22 @@ def test_tokens_out_of_sight(gpu, dtype, bad):
                 assert not torch.isfinite(out[0, sees, 1]).any()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lq,window,sinks,heads,kv_heads,dim", [
+    (1, 5000, 0, 4, 2, 64), (5, 4096, 20, 3, 1, 128), (40, 3000, 2, 2, 2, 32), (3, 2048, 0, 8, 1, 96)])
+def test_few_queries_over_long_windows(gpu, dtype, lq, window, sinks, heads, kv_heads, dim):
+    """Too few rows for the chip: the keys are cut, and the parts joined."""
+    q, k, v, g = operands(lq, 1, lq, 6001, heads, kv_heads, dim, dtype, "cuda")
+    forward_and_gradients(gpu, q, k, v, g, f"{lq} over {window}", window=window, sinks=sinks)
+    lengths = torch.tensor([6000], device="cuda")
+    forward_and_gradients(gpu, q, k, v, g, f"{lq} over {window}, cut", window=window, sinks=sinks,
+                          lengths=lengths)
+    if lq > 1:  # the newest key is the last query's alone
+        v[0, 6000] = NAN
+        out = gpu.window_attention(q, k, v, window=window, sinks=sinks)
+        assert torch.isfinite(out[0, :-1]).all() and torch.isnan(out[0, -1]).all()
+
+
 def test_rows_repeat(gpu):
     """The same inputs give the same bits, gradients among them."""
     q, k, v, g = operands(9, 2, 700, 700, 8, 2, 128, BF16, "cuda")
