@@ -38,12 +38,13 @@ struct TileShape {
   static constexpr int kPitch = kRowBytes <= 64 ? 64 : kRowBytes <= 128 ? 128 : kRowBytes <= 256 ? 256 : 512;
   static constexpr int kChunks = kPitch / 16;      // of which kRowBytes / 16 are used
   static constexpr int kUsed = kRowBytes / 16;
-  static constexpr int kRowsPerLine = kPitch >= 256 ? 1 : 256 / kPitch;  // rows over all banks
 
-  // The 32-byte pairs of chunks are permuted by row: the transposing read
-  // takes four rows by 32 bytes at once, a row read sixteen bytes of eight.
+  // Sixteen rows read at one chunk (a lane a row) fall into sixteen chunks of
+  // the 256 bytes that the banks span, and so do the four rows by four chunks
+  // that half a wave's transposing read takes.
   __device__ static inline int along(int row, int chunk) {
-    return row * kPitch + ((chunk ^ (((row / kRowsPerLine) * 2) & (kChunks - 1))) * 16);
+    const int low = kPitch >= 256 ? (row & 3) << 2 : kPitch == 128 ? (row & 2) << 1 : 0;
+    return row * kPitch + ((chunk ^ (low | ((row >> 2) & 3))) * 16);
   }
 };
 
@@ -149,6 +150,50 @@ __device__ inline void mul_transposed(const char *tile, int row0, const float (&
     }
   }
 }
+
+// A span of keys numbered through (sinks before it, then itself), and which of
+// them a position sees: those no further back than `window`, any of the first
+// `free` numbers.
+struct Numbering {
+  int32_t far, skip, free, window;
+  __device__ inline Numbering(const WindowArgs &a, int32_t near)
+      : far(min(a.sinks, near)), skip(near - far), free(skip == 0 ? a.sinks : far), window(a.window) {}
+  __device__ inline int32_t key(int32_t c) const { return c < far ? c : c + skip; }
+  // p = -1 sees nothing.
+  __device__ inline bool seen(int32_t p, int32_t c) const {
+    const uint32_t back = static_cast<uint32_t>(p - key(c));
+    return back < static_cast<uint32_t>(c < free ? 0x7fffffff : window);
+  }
+};
+
+// A workgroup's share of a tile's rows on its way from memory to LDS, sixteen
+// bytes a piece.  Rows that follow each other in memory are read from one
+// uniform address by 32-bit offsets that stay: with an address worked out for
+// every piece the forward tiles spent half of their vector instructions on it.
+template <class V, int DP, int kTokens, int kThreads>
+struct RowLoader {
+  using T = TileShape<V, DP>;
+  static constexpr int kPer = (kTokens * T::kUsed + kThreads - 1) / kThreads;
+  static constexpr bool kEven = kThreads % T::kUsed == 0 && kTokens * T::kUsed % kThreads == 0;
+  uint32_t offset;   // of the thread's first piece
+  int64_t step;      // bytes between rows
+  bool plain;        // whole rows within 2 GB of each other (uniform)
+
+  __device__ inline void start(int64_t stride, int dim) {
+    step = stride * T::kSize;
+    plain = kEven && dim == DP && step >= 0 && step * kTokens < (int64_t{1} << 31);
+    offset = static_cast<uint32_t>(threadIdx.x / T::kUsed) * static_cast<uint32_t>(step) +
+             threadIdx.x % T::kUsed * 16;
+  }
+  // kTokens rows from `first` on, all there.
+  __device__ inline void load(const void *first, v4u (&to)[kPer]) const {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const char *base = static_cast<const char *>(first) + r * (kThreads / T::kUsed) * step;
+      to[r] = *reinterpret_cast<const v4u *>(base + offset);
+    }
+  }
+};
 
 // The lane 32 away.
 __device__ inline float other_half(float v) {

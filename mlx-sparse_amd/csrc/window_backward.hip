@@ -118,13 +118,14 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
   constexpr int kSteps = DP / Mfma<V>::kDepth;
   __shared__ __attribute__((aligned(16))) char lds[4 * F::kTile];
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, half = lane / 32;
+  const int lane = threadIdx.x % kWave, half = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t id = xcd_order(blockIdx.x, blocks);
   const int64_t bh = id / blocks_per_bh;
   const int32_t first_unit = static_cast<int32_t>(id % blocks_per_bh) * kWaves;
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
-  const int32_t n = a.length(b), offset = a.lk - a.lq;
+  const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
 
   // units, spans and numbering of keys as in the forward pass
   const int32_t unit = first_unit + wave;
@@ -140,9 +141,9 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
   const int32_t g_first = max(first_unit / a.group * 32 + offset, 0);
   const int32_t end = min(min((last_unit / a.group + 1) * 32, a.lq) + offset, n);
   const int32_t near = max(g_first - a.window + 1, 0);
-  const int32_t far = min(a.sinks, near);
+  const Numbering number(a, near);
+  const int32_t far = number.far, skip = number.skip;
   const int32_t count = end > g_first ? far + end - near : 0;
-  const int32_t skip = near - far;
 
   const S *k_base = static_cast<const S *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const S *v_base = static_cast<const S *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
@@ -170,14 +171,23 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
   }
 
   v4u k_next[F::kPerThread], v_next[F::kPerThread];
+  RowLoader<V, DP, F::kTokens, kThreads> k_rows, v_rows;
+  k_rows.start(a.ks[1], a.dim);
+  v_rows.start(a.vs[1], a.dim);
   const auto fetch = [&](int32_t c0) {
+    if (k_rows.plain && v_rows.plain && c0 >= far && c0 + F::kTokens <= count) {
+      const int64_t key = c0 + skip;
+      k_rows.load(k_base + key * a.ks[1], k_next);
+      v_rows.load(v_base + key * a.vs[1], v_next);
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < F::kPerThread; ++r) {
       const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
       const int32_t c = c0 + row;
       k_next[r] = v_next[r] = v4u{0, 0, 0, 0};
       if (row < F::kTokens && c < count) {
-        const int64_t key = c < far ? c : c + skip;
+        const int64_t key = number.key(c);
         k_next[r] = load_chunk<V>(k_base + key * a.ks[1], chunk, a.dim);
         v_next[r] = load_chunk<V>(v_base + key * a.vs[1], chunk, a.dim);
       }
@@ -223,13 +233,11 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
         float ds[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(s[r] * a.scale - lse) * (dp[r] - delta);
-        if (!whole) {
+        if (__builtin_amdgcn_readfirstlane(!whole)) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-            const int32_t key = c < far ? c : c + skip;
-            const bool seen = c < count && key <= p && (p - key < a.window || key < a.sinks);
-            ds[r] = seen ? ds[r] : 0.0f;
+            ds[r] = number.seen(p, c) ? ds[r] : 0.0f;
           }
         }
         mul_transposed<V, DP>(kt, 32 * t, ds, acc);
@@ -298,12 +306,12 @@ struct KeyWave {
       }
     }
     if (masked) {
+      const uint32_t limit = key < a.sinks ? 0x7fffffff : a.window;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int32_t at = p0 + 8 * (r / 4) + 4 * half + r % 4;
-        const bool seen = at >= key && (at - key < a.window || key < a.sinks);
-        p[r] = seen ? p[r] : 0.0f;
-        ds[r] = seen ? ds[r] : 0.0f;
+        const uint32_t back = static_cast<uint32_t>(p0 + 8 * (r / 4) + 4 * half + r % 4 - key);
+        p[r] = back < limit ? p[r] : 0.0f;
+        ds[r] = back < limit ? ds[r] : 0.0f;
       }
     }
     mul_transposed<V, DP>(g_tile, row0, p, dv);
@@ -321,20 +329,32 @@ struct QueryTile {
   static constexpr int kPerThread = (kTokens * T::kUsed + kThreads - 1) / kThreads;
   v4u q[kPerThread], g[kPerThread];
   float stat;
+  RowLoader<V, DP, kTokens, kThreads> q_rows, g_rows;
+
+  __device__ inline void start(const WindowArgs &a, const Upstream &up) {
+    q_rows.start(a.qs[1], a.dim);
+    g_rows.start(up.gs[1], a.dim);
+  }
 
   __device__ inline void fetch(const WindowArgs &a, const Upstream &up, int64_t b, int32_t h,
                                int32_t p0, int32_t last, int32_t offset) {
     using S = typename V::Storage;
     const S *q_base = static_cast<const S *>(a.q) + b * a.qs[0] + h * a.qs[2];
     const S *g_base = static_cast<const S *>(up.grad) + b * up.gs[0] + h * up.gs[2];
+    if (q_rows.plain && g_rows.plain && p0 + kTokens - 1 <= last) {
+      const int64_t i = p0 - offset;
+      q_rows.load(q_base + i * a.qs[1], q);
+      g_rows.load(g_base + i * up.gs[1], g);
+    } else {
 #pragma unroll
-    for (int r = 0; r < kPerThread; ++r) {
-      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
-      q[r] = g[r] = v4u{0, 0, 0, 0};
-      if (row < kTokens && p0 + row <= last) {
-        const int64_t i = p0 + row - offset;
-        q[r] = load_chunk<V>(q_base + i * a.qs[1], chunk, a.dim);
-        g[r] = load_chunk<V>(g_base + i * up.gs[1], chunk, a.dim);
+      for (int r = 0; r < kPerThread; ++r) {
+        const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
+        q[r] = g[r] = v4u{0, 0, 0, 0};
+        if (row < kTokens && p0 + row <= last) {
+          const int64_t i = p0 + row - offset;
+          q[r] = load_chunk<V>(q_base + i * a.qs[1], chunk, a.dim);
+          g[r] = load_chunk<V>(g_base + i * up.gs[1], chunk, a.dim);
+        }
       }
     }
     // the first kTokens threads take lse, the next as many delta
@@ -403,14 +423,15 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, 
   using Tile = QueryTile<V, DP, kTokens>;
   __shared__ __attribute__((aligned(16))) char lds[2 * Tile::kBytes];
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t id = xcd_order(blockIdx.x, blocks);
   const int32_t part = static_cast<int32_t>(id % plan.parts);
   const int32_t block = static_cast<int32_t>(id / plan.parts % plan.blocks);
   const int64_t bh = id / plan.parts / plan.blocks;
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
-  const int32_t n = a.length(b), offset = a.lk - a.lq;
+  const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
   const int32_t w_first = block * kBlockKeys + wave * 32, w_last = w_first + 31;
   const int32_t key = w_first + lane % 32;
 
@@ -424,6 +445,7 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, 
   const int32_t end = static_cast<int32_t>(total * (part + 1) / plan.parts);
 
   Tile next;
+  next.start(a, up);
   const auto fetch = [&](int32_t step) {
     next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset);
   };
@@ -443,7 +465,8 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, 
       const bool any = p1 >= w_first && p0 <= last && (p0 - w_last < a.window || w_first < a.sinks);
       const bool whole = p0 >= w_last && (p1 - w_first < a.window || w_last < a.sinks);
       if (any)
-        keys.add(a, tile, tile + Tile::kTile, stat, stat + kTokens, 32 * t, p0, key, !whole);
+        keys.add(a, tile, tile + Tile::kTile, stat, stat + kTokens, 32 * t, p0, key,
+                 __builtin_amdgcn_readfirstlane(!whole));
     }
     if (more) next.keep(lds + (buffer ^ 1) * Tile::kBytes);
     __syncthreads();
@@ -470,14 +493,15 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
   extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
   char *lds = dynamic_lds;
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t id = xcd_order(blockIdx.x, blocks);
   const int32_t part = static_cast<int32_t>(id % plan.far_parts);
   const int32_t unit = static_cast<int32_t>(id / plan.far_parts % plan.far_units);
   const int64_t bh = id / plan.far_parts / plan.far_units;
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
-  const int32_t n = a.length(b), offset = a.lk - a.lq;
+  const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
   const int32_t key = unit * 32 + lane % 32;
   const bool live = key < a.sinks && key < n;
 
@@ -491,6 +515,7 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
   const int32_t end = static_cast<int32_t>(total * (part + 1) / plan.far_parts);
 
   Tile next;
+  next.start(a, up);
   const auto fetch = [&](int32_t step) {
     next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset);
   };

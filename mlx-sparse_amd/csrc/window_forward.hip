@@ -93,13 +93,14 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   constexpr int kSteps = DP / Mfma<V>::kDepth;
   __shared__ __attribute__((aligned(16))) char lds[F::kLds];
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, half = lane / 32;
+  const int lane = threadIdx.x % kWave, half = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const CutItem item(cut, blockIdx.x);
   const int64_t bh = item.block / blocks_per_bh;
   const int32_t first_unit = static_cast<int32_t>(item.block % blocks_per_bh) * kWaves;
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
-  const int32_t n = a.length(b), offset = a.lk - a.lq;
+  const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
 
   // this wave's queries
   const int32_t unit = first_unit + wave;
@@ -118,9 +119,9 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   const int32_t g_first = max(first_unit / a.group * kRows + offset, 0);
   const int32_t end = min(min((last_unit / a.group + 1) * kRows, a.lq) + offset, n);
   const int32_t near = max(g_first - a.window + 1, 0);
-  const int32_t far = min(a.sinks, near);
+  const Numbering number(a, near);
+  const int32_t far = number.far, skip = number.skip;
   const int32_t count = end > g_first ? far + end - near : 0;
-  const int32_t skip = near - far;  // key = c < far ? c : c + skip
 
   const S *k_base = static_cast<const S *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const S *v_base = static_cast<const S *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
@@ -143,14 +144,23 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   }
 
   v4u k_next[F::kPerThread], v_next[F::kPerThread];
+  RowLoader<V, DP, F::kKeys, kThreads> k_rows, v_rows;
+  k_rows.start(a.ks[1], a.dim);
+  v_rows.start(a.vs[1], a.dim);
   const auto fetch = [&](int32_t c0) {
+    if (k_rows.plain && v_rows.plain && c0 >= far && c0 + F::kKeys <= count) {
+      const int64_t key = c0 + skip;
+      k_rows.load(k_base + key * a.ks[1], k_next);
+      v_rows.load(v_base + key * a.vs[1], v_next);
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < F::kPerThread; ++r) {
       const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
       const int32_t c = c0 + row;
       v4u kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
       if (row < F::kKeys && c < count && chunk * 16 < a.dim * T::kSize) {
-        const int64_t key = c < far ? c : c + skip;
+        const int64_t key = number.key(c);
         kw = *reinterpret_cast<const v4u *>(
             reinterpret_cast<const char *>(k_base + key * a.ks[1]) + chunk * 16);
         vw = *reinterpret_cast<const v4u *>(
@@ -208,15 +218,13 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
       const bool whole = c0 + F::kKeys <= count && k_last <= p_first &&
                          (p_last - k_first < a.window || k_last < a.sinks) &&
                          p_last - p_first == kRows - 1;
-      if (!whole) {
+      if (__builtin_amdgcn_readfirstlane(!whole)) {
 #pragma unroll
         for (int t = 0; t < F::kSub; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-            const int32_t key = c < far ? c : c + skip;
-            const bool seen = c < count && key <= p && (p - key < a.window || key < a.sinks);
-            s[t][r] = seen ? s[t][r] : -INFINITY;
+            s[t][r] = number.seen(p, c) ? s[t][r] : -INFINITY;
           }
       }
       float top = s[0][0];
