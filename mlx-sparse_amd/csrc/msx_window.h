@@ -89,7 +89,7 @@ msx_status launch_window_forward(msx_vtype vt, const WindowArgs &a, void *out, f
 
 // window_backward.hip: the same operands; `grad` aligned as they are.
 // `delta`: batch x heads x lq floats, `scratch`: window_backward_scratch bytes.
-size_t window_backward_scratch(const WindowArgs &a);
+size_t window_backward_scratch(msx_vtype vt, const WindowArgs &a);
 msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void *out,
                                   const float *lse, const void *grad, const int64_t *grad_strides,
                                   float *delta, void *dq, void *dk, void *dv, void *scratch,

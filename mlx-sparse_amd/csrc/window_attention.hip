@@ -460,7 +460,7 @@ extern "C" msx_status msx_window_attention(const msx_window_attention_desc *desc
 extern "C" size_t msx_window_attention_backward_scratch(const msx_window_attention_desc *desc) {
   if (check_window_attention("window_attention_backward", desc) != MSX_OK || desc->batch == 0)
     return 0;
-  const size_t tiles = takes_tiles(*desc) ? window_backward_scratch(args_of(*desc)) : 0;
+  const size_t tiles = takes_tiles(*desc) ? window_backward_scratch(static_cast<msx_vtype>(desc->vtype), args_of(*desc)) : 0;
   return delta_bytes(*desc) + tiles;
 }
 

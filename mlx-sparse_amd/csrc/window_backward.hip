@@ -253,30 +253,44 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
 // ---------------------------------------------------------------------------
 // dk and dv.
 
-// The keys of one wave and their sums.
-template <class V, int DP>
+// The sums of one wave's 32 keys.  Its keys and values stay in registers, or
+// (kInLds) in LDS at the tiles' layout, where registers are short.
+template <class V, int DP, bool kInLds>
 struct KeyWave {
+  using Frag = typename Mfma<V>::Frag;
   static constexpr int kSteps = DP / Mfma<V>::kDepth;
-  typename Mfma<V>::Frag kf[kSteps], vf[kSteps];
+  Frag kf[kInLds ? 1 : kSteps], vf[kInLds ? 1 : kSteps];
+  const char *k_tile, *v_tile;  // with kInLds
+  int key_row;
   v16f dk[DP / 32], dv[DP / 32];
 
   __device__ inline void start(const WindowArgs &a, int64_t b, int32_t kvh, int32_t key, bool live) {
     using S = typename V::Storage;
     const int half = (threadIdx.x % kWave) / 32;
-    const S *k = static_cast<const S *>(a.k) + b * a.ks[0] + key * a.ks[1] + kvh * a.ks[2];
-    const S *v = static_cast<const S *>(a.v) + b * a.vs[0] + key * a.vs[1] + kvh * a.vs[2];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      v4u kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
-      if (live) {
-        kw = load_chunk<V>(k, 2 * s + half, a.dim);
-        vw = load_chunk<V>(v, 2 * s + half, a.dim);
-      }
-      kf[s] = __builtin_bit_cast(typename Mfma<V>::Frag, kw);
-      vf[s] = __builtin_bit_cast(typename Mfma<V>::Frag, vw);
-    }
     zero<DP>(dk);
     zero<DP>(dv);
+    if constexpr (!kInLds) {
+      const S *k = static_cast<const S *>(a.k) + b * a.ks[0] + key * a.ks[1] + kvh * a.ks[2];
+      const S *v = static_cast<const S *>(a.v) + b * a.vs[0] + key * a.vs[1] + kvh * a.vs[2];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        v4u kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
+        if (live) {
+          kw = load_chunk<V>(k, 2 * s + half, a.dim);
+          vw = load_chunk<V>(v, 2 * s + half, a.dim);
+        }
+        kf[s] = __builtin_bit_cast(Frag, kw);
+        vf[s] = __builtin_bit_cast(Frag, vw);
+      }
+    }
+  }
+  __device__ inline Frag key_frag(int s) const {
+    if constexpr (kInLds) return read_rows<V, DP>(k_tile, key_row, s);
+    else return kf[s];
+  }
+  __device__ inline Frag value_frag(int s) const {
+    if constexpr (kInLds) return read_rows<V, DP>(v_tile, key_row, s);
+    else return vf[s];
   }
 
   // 32 queries from row `row0` of the tiles, at positions p0 .. p0 + 31;
@@ -290,8 +304,8 @@ struct KeyWave {
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
-      s = Mfma<V>::mul(read_rows<V, DP>(q_tile, row0 + lane % 32, st), kf[st], s);
-      dp = Mfma<V>::mul(read_rows<V, DP>(g_tile, row0 + lane % 32, st), vf[st], dp);
+      s = Mfma<V>::mul(read_rows<V, DP>(q_tile, row0 + lane % 32, st), key_frag(st), s);
+      dp = Mfma<V>::mul(read_rows<V, DP>(g_tile, row0 + lane % 32, st), value_frag(st), dp);
     }
     float p[16], ds[16];
 #pragma unroll
@@ -321,7 +335,7 @@ struct KeyWave {
 
 // The next queries of the walk, on their way through registers into LDS.
 // A query beyond the sequence is zeros with lse = +inf: its P is zero.
-template <class V, int DP, int kTokens>
+template <class V, int DP, int kTokens, int kThreads>
 struct QueryTile {
   using T = TileShape<V, DP>;
   static constexpr int kTile = kTokens * T::kPitch;
@@ -385,7 +399,7 @@ struct QueryTile {
 // the far units, 32 sink keys each, in `far_parts`.
 struct KeyPlan {
   int32_t blocks, parts;
-  int32_t joined;  // blocks whose sums go through scratch, from the first on
+  int32_t joined;  // 32-key units whose sums go through scratch, from the first on
   int32_t far_units, far_parts;
   float *near_sums, *far_sums;
 };
@@ -414,17 +428,38 @@ __device__ inline int32_t near_last(const WindowArgs &a, int32_t block, int32_t 
   return last < n - 1 ? static_cast<int32_t>(last) : n - 1;
 }
 
+// The near pass's workgroup.  Sums of 128 values a key leave room for one wave
+// a SIMD if keys and values stay in registers too (476 us of a step of 16,384
+// tokens, waiting on LDS and products in turn): 16-bit heads above 64 keep
+// them in LDS, and eight waves, two for the same keys, take alternate halves
+// of a tile.
 template <class V, int DP>
-__global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, Upstream up,
-                                                                  KeyPlan plan, int64_t blocks,
-                                                                  typename V::Storage *dk,
-                                                                  typename V::Storage *dv) {
-  constexpr int kSub = BackwardShape<V, DP>::kSub, kTokens = 32 * kSub;
-  using Tile = QueryTile<V, DP, kTokens>;
-  __shared__ __attribute__((aligned(16))) char lds[2 * Tile::kBytes];
+struct NearShape {
+  using T = TileShape<V, DP>;
+  static constexpr bool kInLds = T::kSize == 2 && DP > 64;
+  static constexpr int kGroups = kInLds ? 2 : 1;  // waves of the same keys
+  static constexpr int kThreads = kGroups * kWaves * kWave;
+  static constexpr int kSub = T::kSize == 2 ? 2 : 1, kTokens = 32 * kSub;
+  using Tile = QueryTile<V, DP, kTokens, kThreads>;
+  static constexpr int kKeyBytes = kInLds ? 2 * kBlockKeys * T::kPitch : 0;
+  static constexpr int kSums = kInLds ? kWaves * kWave * DP / 2 * 4 : 0;  // of four waves, dk or dv
+  static constexpr int kLds = std::max(kKeyBytes + 2 * Tile::kBytes, kSums);
+};
+
+template <class V, int DP>
+__global__ __launch_bounds__((NearShape<V, DP>::kThreads), (NearShape<V, DP>::kGroups)) void
+backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
+                   typename V::Storage *dk, typename V::Storage *dv) {
+  using S = typename V::Storage;
+  using N = NearShape<V, DP>;
+  using T = TileShape<V, DP>;
+  using Tile = typename N::Tile;
+  constexpr int kSub = N::kSub, kTokens = N::kTokens;
+  __shared__ __attribute__((aligned(16))) char lds[N::kLds];
 
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int keys_of = wave % kWaves, group = wave / kWaves;
   const int64_t id = xcd_order(blockIdx.x, blocks);
   const int32_t part = static_cast<int32_t>(id % plan.parts);
   const int32_t block = static_cast<int32_t>(id / plan.parts % plan.blocks);
@@ -432,11 +467,30 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, 
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
   const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
-  const int32_t w_first = block * kBlockKeys + wave * 32, w_last = w_first + 31;
+  const int32_t w_first = block * kBlockKeys + keys_of * 32, w_last = w_first + 31;
   const int32_t key = w_first + lane % 32;
+  char *tiles_lds = lds + N::kKeyBytes;
 
-  KeyWave<V, DP> keys;
+  KeyWave<V, DP, N::kInLds> keys;
   keys.start(a, b, kvh, key, key < n);
+  if constexpr (N::kInLds) {
+    keys.k_tile = lds;
+    keys.v_tile = lds + kBlockKeys * T::kPitch;
+    keys.key_row = keys_of * 32 + lane % 32;
+    const S *k = static_cast<const S *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
+    const S *v = static_cast<const S *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
+    for (int at = threadIdx.x; at < kBlockKeys * T::kUsed; at += N::kThreads) {
+      const int row = at / T::kUsed, chunk = at % T::kUsed;
+      const int64_t j = block * kBlockKeys + row;
+      v4u kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
+      if (j < n) {
+        kw = load_chunk<V>(k + j * a.ks[1], chunk, a.dim);
+        vw = load_chunk<V>(v + j * a.vs[1], chunk, a.dim);
+      }
+      *reinterpret_cast<v4u *>(lds + T::along(row, chunk)) = kw;
+      *reinterpret_cast<v4u *>(lds + kBlockKeys * T::kPitch + T::along(row, chunk)) = vw;
+    }
+  }
 
   const int32_t first = max(block * kBlockKeys, offset), last = near_last(a, block, n);
   const int32_t tiles = last >= first ? (last - first) / kTokens + 1 : 0;
@@ -451,16 +505,17 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, 
   };
   if (begin < end) {
     fetch(begin);
-    next.keep(lds);
+    next.keep(tiles_lds);
   }
   __syncthreads();
   for (int32_t step = begin, buffer = 0; step < end; ++step, buffer ^= 1) {
     const bool more = step + 1 < end;
     if (more) fetch(step + 1);
-    const char *tile = lds + buffer * Tile::kBytes;
+    const char *tile = tiles_lds + buffer * Tile::kBytes;
     const float *stat = reinterpret_cast<const float *>(tile + 2 * Tile::kTile);
 #pragma unroll
-    for (int t = 0; t < kSub; ++t) {
+    for (int t0 = 0; t0 < kSub; t0 += N::kGroups) {
+      const int t = t0 + group;
       const int32_t p0 = first + step % tiles * kTokens + 32 * t, p1 = p0 + 31;
       const bool any = p1 >= w_first && p0 <= last && (p0 - w_last < a.window || w_first < a.sinks);
       const bool whole = p0 >= w_last && (p1 - w_first < a.window || w_last < a.sinks);
@@ -468,13 +523,40 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_near(WindowArgs a, 
         keys.add(a, tile, tile + Tile::kTile, stat, stat + kTokens, 32 * t, p0, key,
                  __builtin_amdgcn_readfirstlane(!whole));
     }
-    if (more) next.keep(lds + (buffer ^ 1) * Tile::kBytes);
+    if (more) next.keep(tiles_lds + (buffer ^ 1) * Tile::kBytes);
     __syncthreads();
   }
 
+  if constexpr (N::kGroups == 2) {  // the second wave's sums to the first: dk, then dv
+    float *sums = reinterpret_cast<float *>(lds) + (keys_of * kWave + lane) * 4;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      v16f(&mine)[DP / 32] = which == 0 ? keys.dk : keys.dv;
+      if (which == 1) __syncthreads();
+      if (group == 1) {
+#pragma unroll
+        for (int r = 0; r < DP / 2; r += 4)
+          *reinterpret_cast<v4f *>(sums + r * kWaves * kWave) =
+              v4f{mine[r / 16][r % 16], mine[r / 16][r % 16 + 1], mine[r / 16][r % 16 + 2],
+                  mine[r / 16][r % 16 + 3]};
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int r = 0; r < DP / 2; r += 4) {
+          const v4f other = *reinterpret_cast<const v4f *>(sums + r * kWaves * kWave);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mine[r / 16][r % 16 + j] += other[j];
+        }
+      }
+    }
+    if (group == 1) return;
+  }
+
   if (key >= a.lk) return;
-  if (block < plan.joined) {
-    const int64_t slot = ((bh * plan.joined + block) * plan.parts + part) * kBlockKeys + wave * 32 + lane % 32;
+  const int32_t unit = block * kWaves + keys_of;
+  if (unit < plan.joined) {
+    const int64_t slot = ((bh * plan.joined + unit) * plan.parts + part) * 32 + lane % 32;
     store_sums<DP>(keys.dk, keys.dv, a.dim, plan.near_sums + slot * 2 * a.dim);
   } else {
     const int64_t row = (b * a.lk + key) * a.kv_heads + kvh;
@@ -489,7 +571,7 @@ template <class V, int DP>
 __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, Upstream up,
                                                                  KeyPlan plan, int64_t blocks) {
   constexpr int kTokens = 32 * kWaves;
-  using Tile = QueryTile<V, DP, kTokens>;
+  using Tile = QueryTile<V, DP, kTokens, kThreads>;
   extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
   char *lds = dynamic_lds;
 
@@ -505,7 +587,7 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
   const int32_t key = unit * 32 + lane % 32;
   const bool live = key < a.sinks && key < n;
 
-  KeyWave<V, DP> keys;
+  KeyWave<V, DP, false> keys;
   keys.start(a, b, kvh, key, live);
 
   const int32_t first = max(near_last(a, unit * 32 / kBlockKeys, n) + 1, offset), last = n - 1;
@@ -534,24 +616,24 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
   store_sums<DP>(keys.dk, keys.dv, a.dim, plan.far_sums + (slot * 32 + lane % 32) * 2 * a.dim);
 }
 
-// dk and dv of the joined blocks.  Sixteen sums a wave, four lanes a sum: each
+// dk and dv of the joined units.  Sixteen sums a wave, four lanes a sum: each
 // takes every fourth part, and they are added in order.
 template <class V>
 __global__ __launch_bounds__(256) void join_keys(WindowArgs a, KeyPlan plan, int64_t total,
                                                  typename V::Storage *dk, typename V::Storage *dv) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x / kWave * 16 + threadIdx.x % 16;
   const int quarter = threadIdx.x % kWave / 16;
-  const int64_t dims = 2 * a.dim;
+  const int64_t dims = 2 * a.dim, keys = static_cast<int64_t>(plan.joined) * 32;
   const int32_t d = static_cast<int32_t>(at % dims);
-  const int32_t key = static_cast<int32_t>(at / dims % (static_cast<int64_t>(plan.joined) * kBlockKeys));
-  const int64_t bh = at / dims / (static_cast<int64_t>(plan.joined) * kBlockKeys);
+  const int32_t key = static_cast<int32_t>(at / dims % keys);
+  const int64_t bh = at / dims / keys;
   const bool live = at < total && key < a.lk;
-  const int32_t block = key / kBlockKeys;
   float sum = 0.0f;
   if (live) {
     const float *near = plan.near_sums +
-        ((bh * plan.joined + block) * plan.parts * kBlockKeys + key % kBlockKeys) * dims + d;
-    for (int32_t part = quarter; part < plan.parts; part += 4) sum += near[part * kBlockKeys * dims];
+        ((bh * plan.joined + key / 32) * plan.parts * 32 + key % 32) * dims + d;
+#pragma unroll 4
+    for (int32_t part = quarter; part < plan.parts; part += 4) sum += near[part * 32 * dims];
     if (key < a.sinks && key / 32 < plan.far_units) {
       const int32_t parts = plan.far_parts * kWaves;
       const float *far = plan.far_sums +
@@ -570,16 +652,17 @@ __global__ __launch_bounds__(256) void join_keys(WindowArgs a, KeyPlan plan, int
     dv[row * a.dim + d - a.dim] = V::narrow(sum);
 }
 
-// The cut depends on sizes alone.  One workgroup runs on a CU; with fewer
-// blocks than CUs each is cut until there are about two a CU, of eight tiles
-// of 32 queries at least.  The far pass goes by the same two numbers.
-KeyPlan plan_keys(const WindowArgs &a) {
+// The cut depends on sizes alone.  One workgroup runs on a CU (two of float32's
+// and the small heads').  With fewer blocks than CUs each is cut until there
+// are about two a CU, of two tiles at least.  The far pass goes by the same
+// number, of four tiles at least.
+KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
   constexpr int64_t kCus = 256;
   KeyPlan p{};
   const int64_t bh = a.batch * a.kv_heads;
   p.blocks = (a.lk + kBlockKeys - 1) / kBlockKeys;
   const int64_t span = std::min<int64_t>(a.lq, static_cast<int64_t>(a.window) + kBlockKeys - 1);
-  const int64_t work = std::max<int64_t>(1, (span + 31) / 32 * a.group / 8);
+  const int64_t work = std::max<int64_t>(1, (span + tile - 1) / tile * a.group / 2);
   p.parts = static_cast<int32_t>(
       bh * p.blocks >= kCus ? 1 : std::min<int64_t>(work, 2 * kCus / std::max<int64_t>(1, bh * p.blocks)));
   // queries that see sinks from beyond the first block's span
@@ -591,13 +674,12 @@ KeyPlan plan_keys(const WindowArgs &a) {
     p.far_parts = static_cast<int32_t>(
         std::min<int64_t>(steps, std::max<int64_t>(1, 2 * kCus / (bh * p.far_units))));
   }
-  p.joined = p.parts > 1 ? p.blocks : (p.far_units * 32 + kBlockKeys - 1) / kBlockKeys;
-  p.joined = std::min(p.joined, p.blocks);
+  p.joined = p.parts > 1 ? (a.lk + 31) / 32 : p.far_units;
   return p;
 }
 
 size_t near_floats(const WindowArgs &a, const KeyPlan &p) {
-  return static_cast<size_t>(a.batch) * a.kv_heads * p.joined * p.parts * kBlockKeys * 2 * a.dim;
+  return static_cast<size_t>(a.batch) * a.kv_heads * p.joined * p.parts * 32 * 2 * a.dim;
 }
 size_t far_floats(const WindowArgs &a, const KeyPlan &p) {
   return static_cast<size_t>(a.batch) * a.kv_heads * p.far_units * p.far_parts * kWaves * 32 * 2 * a.dim;
@@ -611,7 +693,7 @@ msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, 
   const int64_t units = (static_cast<int64_t>(a.lq) + 31) / 32 * a.group;
   const int64_t per_bh = (units + kWaves - 1) / kWaves, q_blocks = per_bh * bh;
   const int64_t k_blocks = bh * plan.blocks * plan.parts, f_blocks = bh * plan.far_units * plan.far_parts;
-  const int64_t joined = bh * plan.joined * kBlockKeys * 2 * a.dim;
+  const int64_t joined = bh * plan.joined * 32 * 2 * a.dim;
   for (int64_t blocks : {units, q_blocks, k_blocks, f_blocks, joined / 64})
     if (blocks >= 0x7fffffff)
       return fail(MSX_EINVAL, "window_attention_backward has more rows than a grid holds.");
@@ -619,10 +701,10 @@ msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, 
     backward_queries<V, DP><<<static_cast<unsigned>(q_blocks), kThreads, 0, stream>>>(
         a, up, static_cast<int32_t>(units), per_bh, q_blocks, static_cast<S *>(dq));
   if (k_blocks > 0)
-    backward_keys_near<V, DP><<<static_cast<unsigned>(k_blocks), kThreads, 0, stream>>>(
+    backward_keys_near<V, DP><<<static_cast<unsigned>(k_blocks), NearShape<V, DP>::kThreads, 0, stream>>>(
         a, up, plan, k_blocks, static_cast<S *>(dk), static_cast<S *>(dv));
   if (f_blocks > 0) {
-    constexpr int lds = QueryTile<V, DP, 32 * kWaves>::kBytes;
+    constexpr int lds = QueryTile<V, DP, 32 * kWaves, kThreads>::kBytes;
     if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(backward_keys_far<V, DP>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         e != hipSuccess)
@@ -646,10 +728,13 @@ msx_status by_dim(const WindowArgs &a, const Upstream &up, const KeyPlan &plan, 
   return run<V, 128>(a, up, plan, dq, dk, dv, stream);
 }
 
+// Queries of a tile of the near pass (BackwardShape::kTokens).
+int32_t tile_of(msx_vtype vt) { return vt == MSX_F32 ? 32 : 64; }
+
 }  // namespace
 
-size_t window_backward_scratch(const WindowArgs &a) {
-  const KeyPlan p = plan_keys(a);
+size_t window_backward_scratch(msx_vtype vt, const WindowArgs &a) {
+  const KeyPlan p = plan_keys(a, tile_of(vt));
   return sizeof(float) * (near_floats(a, p) + far_floats(a, p));
 }
 
@@ -658,7 +743,7 @@ msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void 
                                   float *delta, void *dq, void *dk, void *dv, void *scratch,
                                   hipStream_t stream) {
   Upstream up{grad, {grad_strides[0], grad_strides[1], grad_strides[2]}, out, lse, delta};
-  KeyPlan plan = plan_keys(a);
+  KeyPlan plan = plan_keys(a, tile_of(vt));
   plan.near_sums = static_cast<float *>(scratch);
   plan.far_sums = plan.near_sums + near_floats(a, plan);
   switch (vt) {
