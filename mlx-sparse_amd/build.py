@@ -31,6 +31,7 @@ BUILD = PKG_ROOT / "_build"
 
 ARCH = os.environ.get("MSX_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
+ROCM = Path(HIPCC).resolve().parent.parent
 
 # Device code: -ffp-contract=off keeps products and sums separately rounded
 # (the reference CPU arithmetic); packed fp32 instructions are disabled.
@@ -81,11 +82,13 @@ def build(verbose: bool = True) -> Path:
     import torch  # noqa: PLC0415 - its headers and libraries, for the binding
 
     torch_dir = Path(torch.__file__).resolve().parent
-    torch_flags = [f"-I{torch_dir / 'include'}",
+    # (its HIP headers, for the current stream, are those of this ROCm)
+    torch_flags = ["-D__HIP_PLATFORM_AMD__", f"-I{ROCM / 'include'}", f"-I{torch_dir / 'include'}",
                    f"-I{torch_dir / 'include/torch/csrc/api/include'}",
                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
     py_inc = sysconfig.get_paths()["include"]
-    bind_srcs = [SRC / "bindings.cpp", SRC / "common" / "validate.cpp",
+    bind_srcs = [SRC / "bindings.cpp", SRC / "bindings_operators.cpp",
+                 SRC / "common" / "validate.cpp",
                  SRC / "sparse" / "csr_matvec" / "csr_matvec.cpp",
                  SRC / "sparse" / "csr_matmul" / "csr_matmul.cpp",
                  SRC / "sparse" / "csr_batched_matvec" / "csr_batched_matvec.cpp",
@@ -98,7 +101,7 @@ def build(verbose: bool = True) -> Path:
         o = BUILD / ("bind_" + s.stem + ".o")
         bind_objs.append(o)
         # torch's headers are not warning-free under -Wextra
-        extra = [*torch_flags, "-Wno-extra"] if s.name == "bindings.cpp" else []
+        extra = [*torch_flags, "-Wno-extra"] if s.parent == SRC else []
         jobs.append(["g++", *CXX_FLAGS, "-fvisibility=hidden", f"-I{pybind11.get_include()}",
                      f"-I{py_inc}", *extra, "-c", str(s), "-o", str(o)])
 
@@ -116,7 +119,7 @@ def build(verbose: bool = True) -> Path:
     tmp = ext.with_suffix(".tmp")
     _run(["g++", "-shared", "-fPIC", "-o", str(tmp), *map(str, bind_objs),
           f"-L{OUT_DIR}", "-lmsx_sparse", "-Wl,-rpath,$ORIGIN", f"-L{torch_dir / 'lib'}",
-          "-ltorch_python", "-ltorch_cpu", "-lc10"])
+          "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"])
     os.replace(tmp, ext)
     if verbose:
         print(f"built {lib.relative_to(REPO)} and {ext.relative_to(REPO)}")

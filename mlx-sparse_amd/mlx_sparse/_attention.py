@@ -24,7 +24,8 @@ from torch.autograd import forward_ad
 
 import mlx_sparse._native as _native
 from mlx_sparse._autograd import _call
-from mlx_sparse._device import default_torch_device
+from mlx_sparse._device import default_device_index, default_torch_device
+from mlx_sparse._ext_loader import extension
 from mlx_sparse._validation import ensure_array
 
 _REAL = (torch.float32, torch.float16, torch.bfloat16)
@@ -75,14 +76,15 @@ def _scale(scale, dim: int) -> float:
     return dim ** -0.5 if scale is None else float(scale)
 
 
-def _tracked(*tensors: torch.Tensor) -> bool:
-    if torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0:
-        return True
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+def _transformed() -> bool:
+    """A torch.func transform or a forward-mode level is active."""
+    return torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
 
 
 class _WindowAttention(torch.autograd.Function):
-    """``(out, lse)``; ``lse`` is the backward pass's and has no derivative."""
+    """``(out, lse)``; ``lse`` is the backward pass's and has no derivative.
+    Takes the calls under a transform; others have a node of the native
+    module's, whose backward pass does not enter the interpreter."""
 
     @staticmethod
     def forward(q, k, v, lengths, window, sinks, scale):
@@ -181,6 +183,12 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale: float | Non
         TypeError: dtypes differ or are unsupported.
         ValueError: shapes, ``window`` or ``sinks`` are out of range.
     """
+    transformed = _transformed()
+    if not transformed:
+        out = extension().window_attention_plain(q, k, v, lengths, window, sinks, scale,
+                                                 default_device_index())
+        if out is not None:
+            return out
     window, sinks = _span("window_attention", window, sinks)
     device = default_torch_device()
     q, k, v = _operand(q, device), _operand(k, device), _operand(v, device)
@@ -195,9 +203,13 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale: float | Non
                          f"{tuple(q.shape)} and {tuple(k.shape)}.")
     _check_heads("window_attention", q.shape[2], k.shape[2], q.shape[3])
     scale = _scale(scale, q.shape[3])
-    if _tracked(q, k, v):
+    if transformed:
         return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)[0]
-    return _native.window_attention(q, k, v, lengths, window, sinks, scale, False)[0]
+    out = extension().window_attention_plain(q, k, v, lengths, window, sinks, scale,
+                                             default_device_index())
+    if out is None:  # an operand that no rule above names: let the native checks name it
+        out = _native.window_attention(q, k, v, lengths, window, sinks, scale, False)[0]
+    return out
 
 
 def _cache(name: str, cache, device) -> torch.Tensor:
@@ -237,6 +249,10 @@ def window_attention_step(q, k, v, cache_k, cache_v, lengths, *, window: int, si
         differentiable.
     """
     name = "window_attention_step"
+    out = extension().window_attention_step_plain(q, k, v, cache_k, cache_v, lengths, window,
+                                                  sinks, scale, default_device_index())
+    if out is not None:
+        return out
     window, sinks = _span(name, window, sinks)
     device = default_torch_device()
     q, k, v = (_operand(t, device).detach() for t in (q, k, v))
@@ -253,9 +269,8 @@ def window_attention_step(q, k, v, cache_k, cache_v, lengths, *, window: int, si
     if cache_k.ndim == 4 and sinks + window > cache_k.shape[1]:
         raise ValueError(f"{name} cache needs at least sinks + window = {sinks + window} slots, "
                          f"got {cache_k.shape[1]}.")
-    out = _native.window_attention_step(q, k, v, cache_k, cache_v, lengths, window, sinks,
-                                        _scale(scale, q.shape[2]))
-    return out
+    return _native.window_attention_step(q, k, v, cache_k, cache_v, lengths, window, sinks,
+                                         _scale(scale, q.shape[2]))
 
 
 def window_cache_store(k, v, cache_k, cache_v, *, sinks: int = 0, starts=None,

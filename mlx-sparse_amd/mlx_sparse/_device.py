@@ -30,6 +30,15 @@ def default_torch_device() -> torch.device:
     return _DEFAULT
 
 
+def default_device_index() -> int:
+    """``default_torch_device`` as the native module numbers devices: the HIP
+    device's ordinal, -1 for the host."""
+    device = default_torch_device()
+    if device.type == "cpu":
+        return -1
+    return device.index if device.index is not None else torch.cuda.current_device()
+
+
 def _set(device: torch.device) -> torch.device:
     global _DEFAULT, _CHOSEN
     _DEFAULT = device

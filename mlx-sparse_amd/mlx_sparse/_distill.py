@@ -26,7 +26,8 @@ from torch.autograd import forward_ad
 import mlx_sparse._native as _native
 from mlx_sparse._autograd import _call
 from mlx_sparse._csr import CSRArray
-from mlx_sparse._device import default_torch_device
+from mlx_sparse._device import default_device_index, default_torch_device
+from mlx_sparse._ext_loader import extension
 from mlx_sparse._validation import ensure_array
 
 _REAL = (torch.float32, torch.float16, torch.bfloat16)
@@ -69,7 +70,8 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
 
 
 class _DistillLoss(torch.autograd.Function):
-    """``(losses, lse)`` of rows of logits."""
+    """``(losses, lse)`` of rows of logits, under a transform; other calls
+    have a node of the native module's."""
 
     @staticmethod
     def forward(z, data, indices, indptr, temperature):
@@ -134,14 +136,23 @@ def distill_loss(logits, teacher: CSRArray, *, temperature: float = 1.0) -> torc
         TypeError: ``teacher`` is not a CSRArray or a dtype is unsupported.
         ValueError: shapes or ``temperature`` do not fit.
     """
+    transformed = torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
+    if not transformed and type(teacher) is CSRArray:
+        losses = extension().distill_loss_plain(logits, teacher.data, teacher.indices,
+                                                teacher.indptr, *teacher.shape, temperature,
+                                                default_device_index())
+        if losses is not None:
+            return losses
     logits, (data, indices, indptr), temperature = _prepared("distill_loss", logits, teacher,
                                                              temperature)
     z = _rows(logits)
-    if (torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
-            or (torch.is_grad_enabled() and z.requires_grad)):
+    if transformed:
         losses = _DistillLoss.apply(z, data, indices, indptr, temperature)[0]
     else:
-        losses = _native.distill_loss(z, data, indices, indptr, temperature, False)[0]
+        losses = extension().distill_loss_plain(z, data, indices, indptr, *teacher.shape,
+                                                temperature, default_device_index())
+        if losses is None:  # an operand that no rule above names: let the native checks name it
+            losses = _native.distill_loss(z, data, indices, indptr, temperature, False)[0]
     return losses if logits.ndim == 2 else losses.reshape(logits.shape[:-1])
 
 
@@ -163,6 +174,12 @@ def distill_value_and_grad(logits, teacher: CSRArray, weights=None, *,
         shaped as ``logits`` and of their dtype.
     """
     name = "distill_value_and_grad"
+    if type(teacher) is CSRArray:
+        both = extension().distill_loss_grad_plain(logits, teacher.data, teacher.indices,
+                                                   teacher.indptr, weights, *teacher.shape,
+                                                   temperature, default_device_index())
+        if both is not None:
+            return both
     logits, (data, indices, indptr), temperature = _prepared(name, logits, teacher, temperature)
     lead = logits.shape[:-1]
     if weights is not None:

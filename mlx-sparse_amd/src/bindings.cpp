@@ -16,11 +16,6 @@
 // output is allocated with torch.empty on the inputs' device, device work is
 // ordered on torch's current stream for that device, and errors surface as
 // ValueError (std::invalid_argument), RuntimeError or MemoryError.
-#include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/autograd/python_variable.h>
-
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
@@ -28,13 +23,13 @@
 #include <string>
 #include <vector>
 
-#include "attention/window_attention.h"
+#include "bindings_operators.h"
 #include "common/array_view.h"
+#include "common/torch_view.h"
 #include "common/validate.h"
 #include "msx_sparse.h"
 #include "linalg/csr_cg.h"
 #include "linalg/csr_krylov.h"
-#include "loss/distill.h"
 #include "sparse/csr_adjoint/csr_adjoint.h"
 #include "sparse/csr_batched_matmul/csr_batched_matmul.h"
 #include "sparse/csr_batched_matvec/csr_batched_matvec.h"
@@ -43,7 +38,15 @@
 
 namespace py = pybind11;
 using msx::ArrayView;
+using msx::context_for;
+using msx::device_index;
 using msx::DType;
+using msx::dtype_name;
+using msx::dtype_of;
+using msx::scratch_for;
+using msx::stream_for;
+using msx::tensor_of;
+using msx::view_of;
 
 namespace {
 
@@ -54,78 +57,6 @@ py::module_ &torch() {
   return *mod;
 }
 
-DType dtype_of(at::ScalarType t) {
-  switch (t) {
-  case at::kFloat: return DType::Float32;
-  case at::kHalf: return DType::Float16;
-  case at::kBFloat16: return DType::BFloat16;
-  case at::kComplexFloat: return DType::Complex64;
-  case at::kInt: return DType::Int32;
-  case at::kLong: return DType::Int64;
-  default: return DType::Other;
-  }
-}
-
-// torch's spelling of a dtype, for error texts.
-std::string dtype_name(at::ScalarType t) {
-  switch (t) {
-  case at::kFloat: return "float32";
-  case at::kHalf: return "float16";
-  case at::kBFloat16: return "bfloat16";
-  case at::kComplexFloat: return "complex64";
-  case at::kInt: return "int32";
-  case at::kLong: return "int64";
-  case at::kShort: return "int16";
-  case at::kDouble: return "float64";
-  case at::kComplexDouble: return "complex128";
-  case at::kBool: return "bool";
-  case at::kByte: return "uint8";
-  case at::kChar: return "int8";
-  default: return c10::toString(t);
-  }
-}
-
-DType dtype_of(py::handle dtype) {
-  if (!THPDtype_Check(dtype.ptr())) return DType::Other;
-  return dtype_of(reinterpret_cast<THPDtype *>(dtype.ptr())->scalar_type);
-}
-
-const at::Tensor &tensor_of(py::handle t) {
-  if (!THPVariable_Check(t.ptr())) throw py::type_error("mlx_sparse expects a torch tensor.");
-  return THPVariable_Unpack(t.ptr());
-}
-
-int current_device() {
-  static auto *f = new py::object(torch().attr("_C").attr("_cuda_getDevice"));
-  return (*f)().cast<int>();
-}
-
-int device_index(const at::Tensor &t) {
-  const at::Device d = t.device();
-  if (d.is_cpu()) return -1;
-  if (!d.is_cuda())
-    throw std::invalid_argument("mlx_sparse supports cpu and HIP (cuda) tensors only, got " +
-                                c10::DeviceTypeName(d.type(), true) + ".");
-  return d.has_index() ? d.index() : current_device();
-}
-
-ArrayView view_of(const at::Tensor &t) {
-  ArrayView v;
-  v.dtype_name = dtype_name(t.scalar_type());
-  v.dtype = dtype_of(t.scalar_type());
-  v.ndim = static_cast<int>(t.dim());
-  if (v.ndim <= 4) {
-    for (int i = 0; i < v.ndim; ++i) {
-      v.shape[i] = t.size(i);
-      v.strides[i] = t.stride(i);
-    }
-  }
-  v.device = device_index(t);
-  v.ptr = t.data_ptr();
-  return v;
-}
-
-ArrayView view_of(py::handle t) { return view_of(tensor_of(t)); }
 
 py::object as_tensor(py::handle obj) {
   if (THPVariable_Check(obj.ptr())) return py::reinterpret_borrow<py::object>(obj);
@@ -141,17 +72,6 @@ py::object contiguous(py::handle obj) {
     if (a.is_contiguous() && !a.is_conj() && !a.is_neg()) return t;
   }
   return t.attr("resolve_conj")().attr("resolve_neg")().attr("contiguous")();
-}
-
-// The stream torch's current stream of `device` wraps.
-void *stream_for(int device) {
-  if (device < 0) return nullptr;
-  const int current = current_device();
-  if (current != device)
-    throw std::invalid_argument("mlx_sparse: GPU operands must be on the current device (cuda:" +
-                                std::to_string(current) + "), got cuda:" + std::to_string(device) + ".");
-  static auto *f = new py::object(torch().attr("_C").attr("_cuda_getCurrentRawStream"));
-  return reinterpret_cast<void *>((*f)(device).cast<uintptr_t>());
 }
 
 // Owner of a device plan; destroyed with the Python object.
@@ -246,26 +166,13 @@ py::object empty_like_out(const ArrayView &, py::handle like, py::tuple shape) {
       THPVariable_Wrap(at::empty(dims, tensor_of(like).options().requires_grad(false))));
 }
 
-// Device scratch of one call from torch's caching allocator (the stream-ordered
-// one of the C ABI gives its memory back at every synchronisation and maps it
-// anew: 40 us a call), kept until the call's kernels are enqueued; torch
-// orders its reuse on the current stream.
-at::Tensor scratch_for(msx::ExecContext &ctx, py::handle like, size_t bytes) {
-  if (ctx.stream == nullptr && tensor_of(like).is_cpu()) return {};
-  if (bytes == 0) return {};
-  at::Tensor t = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(tensor_of(like).device()));
-  ctx.scratch = t.data_ptr();
-  ctx.scratch_bytes = bytes;
-  return t;
-}
-
 // The same for a plan; none where torch has no room for it: the library then
 // asks the stream-ordered allocator or does without the plan's copy.
 at::Tensor plan_scratch_for(msx::ExecContext &ctx, py::handle like, const msx_csr_plan *plan) {
   const size_t bytes = msx_csr_plan_scratch(plan);
   if (bytes == 0) return {};
   try {
-    return scratch_for(ctx, like, bytes);
+    return scratch_for(ctx, tensor_of(like), bytes);
   } catch (const c10::OutOfMemoryError &) {
     return {};
   }
@@ -357,7 +264,7 @@ py::object csr_batched_matvec(py::handle data_o, py::handle indices_o, py::handl
   ctx.stream = vd.device >= 0 ? stream_for(vd.device) : nullptr;
   if (vd.device >= 0) {
     const at::Tensor scratch = scratch_for(
-        ctx, data, msx::is_value_dtype(vd.dtype)
+        ctx, tensor_of(data), msx::is_value_dtype(vd.dtype)
                        ? msx_csr_batched_spmv_scratch(msx::to_vtype(vd.dtype), n_rows, n_cols, vr.shape[0])
                        : 0);
     msx::csr_batched_matvec(vd, vi, vp, vr, vo, n_rows, n_cols, ctx);
@@ -388,13 +295,6 @@ py::object csr_batched_matmul(py::handle data_o, py::handle indices_o, py::handl
     msx::csr_batched_matmul(vd, vi, vp, vr, vo, n_rows, n_cols, ctx);
   }
   return out;
-}
-
-msx::ExecContext context_for(const ArrayView &v, int n_threads) {
-  msx::ExecContext ctx;
-  ctx.n_threads = n_threads;
-  ctx.stream = v.device >= 0 ? stream_for(v.device) : nullptr;
-  return ctx;
 }
 
 py::tuple csr_transpose(py::handle data_o, py::handle indices_o, py::handle indptr_o,
@@ -806,168 +706,6 @@ py::dict compiled_capabilities() {
   return info;
 }
 
-// ---------------------------------------------------------------------------
-// Window attention and distillation.  Strided operands are read in place.
-
-struct OptionalView {
-  ArrayView view;
-  const ArrayView *get = nullptr;
-  explicit OptionalView(py::handle o) {
-    if (o.is_none()) return;
-    view = view_of(o);
-    get = &view;
-  }
-  OptionalView(const OptionalView &) = delete;
-  OptionalView &operator=(const OptionalView &) = delete;
-};
-
-at::Tensor new_tensor(py::handle like, std::initializer_list<int64_t> shape,
-                      at::ScalarType dtype) {
-  return at::empty(at::IntArrayRef(shape), at::TensorOptions().dtype(dtype).device(tensor_of(like).device()));
-}
-
-py::object wrap(const at::Tensor &t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
-
-// Runs `fn`; without the interpreter lock where it works on the host.
-template <class Fn>
-void run_op(const ArrayView &v, Fn &&fn) {
-  if (v.device >= 0) {
-    fn();
-  } else {
-    py::gil_scoped_release nogil;
-    fn();
-  }
-}
-
-// (out, lse); lse is None unless asked for.
-py::tuple window_attention(py::handle q_o, py::handle k_o, py::handle v_o, py::handle lengths_o,
-                           int64_t window, int64_t sinks, double scale, bool with_lse,
-                           int n_threads) {
-  const ArrayView q = view_of(q_o), k = view_of(k_o), v = view_of(v_o);
-  const OptionalView lengths(lengths_o);
-  const auto desc = msx::window_attention_desc(q, k, v, lengths.get, window, sinks, scale);
-  const at::Tensor out = new_tensor(q_o, {desc.batch, desc.lq, desc.heads, desc.dim},
-                                    tensor_of(q_o).scalar_type());
-  at::Tensor lse;
-  if (with_lse) lse = new_tensor(q_o, {desc.batch, desc.heads, desc.lq}, at::kFloat);
-  const ArrayView vo = view_of(out);
-  float *l = with_lse ? lse.data_ptr<float>() : nullptr;
-  msx::ExecContext ctx = context_for(q, n_threads);
-  at::Tensor scratch;
-  if (q.device >= 0) scratch = scratch_for(ctx, q_o, msx_window_attention_scratch(&desc));
-  run_op(q, [&] { msx::window_attention(desc, vo, l, ctx); });
-  return py::make_tuple(wrap(out), with_lse ? wrap(lse) : py::object(py::none()));
-}
-
-py::tuple window_attention_backward(py::handle q_o, py::handle k_o, py::handle v_o,
-                                    py::handle lengths_o, py::handle out_o, py::handle lse_o,
-                                    py::handle grad_o, int64_t window, int64_t sinks, double scale,
-                                    int n_threads) {
-  const ArrayView q = view_of(q_o), k = view_of(k_o), v = view_of(v_o), out = view_of(out_o),
-                  lse = view_of(lse_o), grad = view_of(grad_o);
-  const OptionalView lengths(lengths_o);
-  const auto desc = msx::window_attention_desc(q, k, v, lengths.get, window, sinks, scale);
-  if (lse.dtype != DType::Float32)
-    throw std::invalid_argument("window_attention_backward lse must have dtype float32.");
-  msx::require_size(lse, desc.batch * desc.heads * desc.lq, "window_attention_backward lse");
-  msx::require_contiguous(lse, "window_attention_backward lse");
-  msx::require_same_device({&q, &out, &lse, &grad}, "window_attention_backward");
-  const at::ScalarType type = tensor_of(q_o).scalar_type();
-  const at::Tensor dq = new_tensor(q_o, {desc.batch, desc.lq, desc.heads, desc.dim}, type);
-  const at::Tensor dk = new_tensor(q_o, {desc.batch, desc.lk, desc.kv_heads, desc.dim}, type);
-  const at::Tensor dv = new_tensor(q_o, {desc.batch, desc.lk, desc.kv_heads, desc.dim}, type);
-  const ArrayView vq = view_of(dq), vk = view_of(dk), vv = view_of(dv);
-  msx::ExecContext ctx = context_for(q, n_threads);
-  at::Tensor scratch;
-  if (q.device >= 0)
-    scratch = scratch_for(ctx, q_o, msx_window_attention_backward_scratch(&desc));
-  run_op(q, [&] {
-    msx::window_attention_backward(desc, out, static_cast<const float *>(lse.ptr), grad, vq, vk,
-                                   vv, ctx);
-  });
-  return py::make_tuple(wrap(dq), wrap(dk), wrap(dv));
-}
-
-py::object window_attention_step(py::handle q_o, py::handle k_o, py::handle v_o,
-                                 py::handle cache_k_o, py::handle cache_v_o, py::handle lengths_o,
-                                 int64_t window, int64_t sinks, double scale, int n_threads) {
-  const ArrayView q = view_of(q_o), k = view_of(k_o), v = view_of(v_o), ck = view_of(cache_k_o),
-                  cv = view_of(cache_v_o), lengths = view_of(lengths_o);
-  const auto desc = msx::window_step_desc(q, k, v, ck, cv, lengths, window, sinks, scale);
-  const at::Tensor out =
-      new_tensor(q_o, {desc.batch, desc.heads, desc.dim}, tensor_of(q_o).scalar_type());
-  const ArrayView vo = view_of(out);
-  msx::ExecContext ctx = context_for(q, n_threads);
-  at::Tensor scratch;
-  if (q.device >= 0) scratch = scratch_for(ctx, q_o, msx_window_attention_step_scratch(&desc));
-  run_op(q, [&] { msx::window_attention_step(desc, vo, ctx); });
-  return wrap(out);
-}
-
-void window_cache_store(py::handle k_o, py::handle v_o, py::handle cache_k_o, py::handle cache_v_o,
-                        py::handle starts_o, py::handle lengths_o, int64_t sinks) {
-  const ArrayView k = view_of(k_o), v = view_of(v_o), ck = view_of(cache_k_o),
-                  cv = view_of(cache_v_o);
-  const OptionalView starts(starts_o), lengths(lengths_o);
-  const msx::ExecContext ctx = context_for(k, 0);
-  run_op(k, [&] { msx::window_cache_store(k, v, ck, cv, starts.get, lengths.get, sinks, ctx); });
-}
-
-// (losses, lse); lse is None unless asked for.
-py::tuple distill_loss(py::handle logits_o, py::handle data_o, py::handle indices_o,
-                       py::handle indptr_o, double temperature, bool with_lse, int n_threads) {
-  const ArrayView logits = view_of(logits_o), data = view_of(data_o), indices = view_of(indices_o),
-                  indptr = view_of(indptr_o);
-  const auto desc = msx::distill_desc(logits, data, indices, indptr, nullptr, temperature);
-  const at::Tensor losses = new_tensor(logits_o, {desc.n_rows}, at::kFloat);
-  at::Tensor lse;
-  if (with_lse) lse = new_tensor(logits_o, {desc.n_rows}, at::kFloat);
-  const ArrayView vl = view_of(losses);
-  float *l = with_lse ? lse.data_ptr<float>() : nullptr;
-  const msx::ExecContext ctx = context_for(logits, n_threads);
-  run_op(logits, [&] { msx::distill_loss(desc, vl, l, ctx); });
-  return py::make_tuple(wrap(losses), with_lse ? wrap(lse) : py::object(py::none()));
-}
-
-py::object distill_grad(py::handle logits_o, py::handle data_o, py::handle indices_o,
-                        py::handle indptr_o, py::handle weights_o, py::handle lse_o,
-                        double temperature, int n_threads) {
-  const ArrayView logits = view_of(logits_o), data = view_of(data_o), indices = view_of(indices_o),
-                  indptr = view_of(indptr_o), lse = view_of(lse_o);
-  const OptionalView weights(weights_o);
-  const auto desc = msx::distill_desc(logits, data, indices, indptr, weights.get, temperature);
-  if (lse.dtype != DType::Float32)
-    throw std::invalid_argument("distill_grad lse must have dtype float32.");
-  msx::require_size(lse, desc.n_rows, "distill_grad lse");
-  msx::require_contiguous(lse, "distill_grad lse");
-  msx::require_same_device({&logits, &lse}, "distill_grad");
-  const at::Tensor grad =
-      new_tensor(logits_o, {desc.n_rows, desc.n_cols}, tensor_of(logits_o).scalar_type());
-  const ArrayView vg = view_of(grad);
-  const msx::ExecContext ctx = context_for(logits, n_threads);
-  run_op(logits, [&] { msx::distill_grad(desc, static_cast<const float *>(lse.ptr), vg, ctx); });
-  return wrap(grad);
-}
-
-py::tuple distill_loss_grad(py::handle logits_o, py::handle data_o, py::handle indices_o,
-                            py::handle indptr_o, py::handle weights_o, double temperature,
-                            int n_threads) {
-  const ArrayView logits = view_of(logits_o), data = view_of(data_o), indices = view_of(indices_o),
-                  indptr = view_of(indptr_o);
-  const OptionalView weights(weights_o);
-  const auto desc = msx::distill_desc(logits, data, indices, indptr, weights.get, temperature);
-  const at::Tensor losses = new_tensor(logits_o, {desc.n_rows}, at::kFloat);
-  const at::Tensor grad =
-      new_tensor(logits_o, {desc.n_rows, desc.n_cols}, tensor_of(logits_o).scalar_type());
-  at::Tensor lse;
-  if (logits.device < 0) lse = new_tensor(logits_o, {desc.n_rows}, at::kFloat);
-  const ArrayView vl = view_of(losses), vg = view_of(grad);
-  float *l = logits.device < 0 ? lse.data_ptr<float>() : nullptr;
-  const msx::ExecContext ctx = context_for(logits, n_threads);
-  run_op(logits, [&] { msx::distill_loss_grad(desc, vl, l, vg, ctx); });
-  return py::make_tuple(wrap(losses), wrap(grad));
-}
-
 }  // namespace
 
 PYBIND11_MODULE(_ext, m) {
@@ -1000,30 +738,7 @@ PYBIND11_MODULE(_ext, m) {
         "Build a row-block plan from a GPU indptr; with data/indices, a plan bound to the "
         "matrix (slice_mode 0 auto, 1 off, 2 column slices per XCD, 3 LDS column panels; "
         "defer: auto's panels wait where only many products repay them).");
-  m.def("window_attention", &window_attention, py::arg("q"), py::arg("k"), py::arg("v"),
-        py::arg("lengths"), py::arg("window"), py::arg("sinks"), py::arg("scale"),
-        py::arg("with_lse"), py::arg("n_threads") = 0,
-        "(out, lse) of attention over the last window and the first sinks keys.");
-  m.def("window_attention_backward", &window_attention_backward, py::arg("q"), py::arg("k"),
-        py::arg("v"), py::arg("lengths"), py::arg("out"), py::arg("lse"), py::arg("grad"),
-        py::arg("window"), py::arg("sinks"), py::arg("scale"), py::arg("n_threads") = 0,
-        "(dq, dk, dv) of window_attention.");
-  m.def("window_attention_step", &window_attention_step, py::arg("q"), py::arg("k"), py::arg("v"),
-        py::arg("cache_k"), py::arg("cache_v"), py::arg("lengths"), py::arg("window"),
-        py::arg("sinks"), py::arg("scale"), py::arg("n_threads") = 0,
-        "One token of every sequence: into its ring cache, and its attention over it.");
-  m.def("window_cache_store", &window_cache_store, py::arg("k"), py::arg("v"), py::arg("cache_k"),
-        py::arg("cache_v"), py::arg("starts"), py::arg("lengths"), py::arg("sinks"),
-        "A prompt's keys and values into ring caches.");
-  m.def("distill_loss", &distill_loss, py::arg("logits"), py::arg("data"), py::arg("indices"),
-        py::arg("indptr"), py::arg("temperature"), py::arg("with_lse"), py::arg("n_threads") = 0,
-        "(losses, lse) of distillation from a CSR teacher's logits.");
-  m.def("distill_grad", &distill_grad, py::arg("logits"), py::arg("data"), py::arg("indices"),
-        py::arg("indptr"), py::arg("weights"), py::arg("lse"), py::arg("temperature"),
-        py::arg("n_threads") = 0, "Gradient of the weighted losses in the logits.");
-  m.def("distill_loss_grad", &distill_loss_grad, py::arg("logits"), py::arg("data"),
-        py::arg("indices"), py::arg("indptr"), py::arg("weights"), py::arg("temperature"),
-        py::arg("n_threads") = 0, "(losses, gradient of the weighted losses) in one call.");
+  bind_operators(m);
   m.def("csr_matvec", &csr_matvec, py::arg("data"), py::arg("indices"), py::arg("indptr"),
         py::arg("x"), py::arg("n_rows"), py::arg("n_cols"), py::arg("plan") = py::none(),
         py::arg("n_threads") = 0, "Multiply CSR buffers by a dense vector.");
