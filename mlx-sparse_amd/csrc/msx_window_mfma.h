@@ -42,9 +42,13 @@ struct TileShape {
   // Sixteen rows read at one chunk (a lane a row) fall into sixteen chunks of
   // the 256 bytes that the banks span, and so do the four rows by four chunks
   // that half a wave's transposing read takes.
-  __device__ static inline int along(int row, int chunk) {
+  __device__ static __forceinline__ int along(int row, int chunk) {
+    return row * kPitch + logical(row, chunk) * 16;
+  }
+  // The chunk at a place of the row, and the place of a chunk.
+  __device__ static __forceinline__ int logical(int row, int chunk) {
     const int low = kPitch >= 256 ? (row & 3) << 2 : kPitch == 128 ? (row & 2) << 1 : 0;
-    return row * kPitch + ((chunk ^ (low | ((row >> 2) & 3))) * 16);
+    return chunk ^ (low | ((row >> 2) & 3));
   }
 };
 
@@ -57,10 +61,10 @@ template <>
 struct Mfma<BF16> {
   using Frag = v8bf;
   static constexpr int kDepth = 16;
-  __device__ static inline v16f mul(Frag a, Frag b, v16f c) {
+  __device__ static __forceinline__ v16f mul(Frag a, Frag b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  __device__ static inline uint32_t pack(float lo, float hi) {
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{lo, hi}), v2bf));
   }
   static constexpr uint32_t kSign = 0x80008000u;
@@ -69,10 +73,10 @@ template <>
 struct Mfma<F16> {
   using Frag = v8h;
   static constexpr int kDepth = 16;
-  __device__ static inline v16f mul(Frag a, Frag b, v16f c) {
+  __device__ static __forceinline__ v16f mul(Frag a, Frag b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  __device__ static inline uint32_t pack(float lo, float hi) {
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{lo, hi}), v2h));
   }
   static constexpr uint32_t kSign = 0x80008000u;
@@ -83,7 +87,7 @@ template <>
 struct Mfma<F32> {
   using Frag = v4f;
   static constexpr int kDepth = 8;
-  __device__ static inline v16f mul(Frag a, Frag b, v16f c) {
+  __device__ static __forceinline__ v16f mul(Frag a, Frag b, v16f c) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
     return c;
@@ -91,30 +95,97 @@ struct Mfma<F32> {
   static constexpr uint32_t kSign = 0x80000000u;
 };
 
-// Sixteen bytes of a row for step `s` of a product over the head dimension:
-// chunk 2 s + lane / 32 in either type.
-template <class V, int DP>
-__device__ inline typename Mfma<V>::Frag read_rows(const char *tile, int row, int s) {
-  const int half = (threadIdx.x % kWave) / 32;
-  return *reinterpret_cast<const typename Mfma<V>::Frag *>(
-      tile + TileShape<V, DP>::along(row, 2 * s + half));
+using LdsPtr = const __attribute__((address_space(3))) char *;
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsPtr)(p)));
 }
 
-__device__ inline v4s read_transposed(const char *p) {
-  // the builtin takes an LDS pointer
-  auto *lds = (__attribute__((address_space(3))) v4s *)(p);
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds);
-}
-
-// acc[dt] += X^T P over 32 rows of the tile from `row0` on: p the lane's
-// sixteen values in the order above, X read along its columns.
+// Where a lane reads tiles in LDS.  TileShape's permutation is linear over the
+// bits of row and chunk, and what varies by lane and what is known when
+// compiling lie in different bits of both: an address is the lane's part, an
+// exclusive or with a constant, and the instruction's own offset.  (Worked out
+// from row and chunk each, the addresses of a tile took forty registers.)
 template <class V, int DP>
-__device__ inline void mul_transposed(const char *tile, int row0, const float (&p)[16],
-                                      v16f (&acc)[DP / 32]) {
+struct TileLanes {
   using T = TileShape<V, DP>;
-  const int lane = threadIdx.x % kWave, half = lane / 32;
-  if constexpr (T::kSize == 2) {
-    typename Mfma<V>::Frag b[2];
+  uint32_t rows;     // a row a lane: row lane % 32, chunk lane / 32
+  uint32_t columns;  // see mul_transposed
+
+  __device__ __forceinline__ explicit TileLanes(const char *lds) {
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const uint32_t base = lds_address(lds);
+    rows = base + T::along(lane % 32, half);
+    if constexpr (T::kSize == 2) {
+      const int i = lane % 16, place = ((lane / 16) % 2) * 16 + (i % 4) * 4;
+      columns = base + T::along(4 * half + i / 4, place / 8) + (place % 8) * 2;
+    } else {
+      columns = base + T::along(4 * half, (lane % 32) / 4) + (lane % 4) * 4;
+    }
+  }
+  // Of the tile at byte `tile` of LDS, row row0 + lane % 32, chunk 2 step + half.
+  __device__ __forceinline__ const char *row_at(uint32_t tile, int row0, int step) const {
+    return at(rows, tile + row0 * T::kPitch, 0, 2 * step);
+  }
+  // The lane's place of the columns from 32 dt on, `row` rows below row0.
+  __device__ __forceinline__ const char *column_at(uint32_t tile, int row0, int row, int dt) const {
+    return at(columns, tile + row0 * T::kPitch, row, dt * (32 * T::kSize / 16));
+  }
+
+ private:
+  __device__ static __forceinline__ const char *at(uint32_t lane, uint32_t tile, int row, int chunk) {
+    return (const char *)(LdsPtr)(static_cast<uintptr_t>(
+        (lane ^ static_cast<uint32_t>(T::logical(row, chunk) * 16)) + tile + row * T::kPitch));
+  }
+};
+
+// The same addresses worked out from row and chunk each, of an array that the
+// compiler knows: it then moves reads past what is written elsewhere.
+template <class V, int DP>
+struct TilePlaces {
+  using T = TileShape<V, DP>;
+  const char *base;
+  __device__ __forceinline__ explicit TilePlaces(const char *lds) : base(lds) {}
+  __device__ __forceinline__ const char *row_at(uint32_t tile, int row0, int step) const {
+    const int lane = threadIdx.x % kWave;
+    return base + tile + T::along(row0 + lane % 32, 2 * step + lane / 32);
+  }
+  __device__ __forceinline__ const char *column_at(uint32_t tile, int row0, int row, int dt) const {
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    if constexpr (T::kSize == 2) {
+      const int i = lane % 16, d = dt * 32 + ((lane / 16) % 2) * 16 + (i % 4) * 4;
+      return base + tile + T::along(row0 + row + 4 * half + i / 4, d / 8) + (d % 8) * 2;
+    } else {
+      const int d = dt * 32 + lane % 32;
+      return base + tile + T::along(row0 + row + 4 * half, d / 4) + (d % 4) * 4;
+    }
+  }
+};
+
+template <class X>
+__device__ __forceinline__ X read_lds(const char *at) {
+  return *reinterpret_cast<const X *>(at);
+}
+
+// Sixteen bytes of a row for step `s` of a product over the head dimension:
+// chunk 2 s + lane / 32 in either type, of row row0 + lane % 32 (row0 a
+// multiple of 32: the permutation starts anew there).
+template <class V, class Lanes>
+__device__ __forceinline__ typename Mfma<V>::Frag read_rows(const Lanes &lanes, uint32_t tile,
+                                                            int row0, int s) {
+  return read_lds<typename Mfma<V>::Frag>(lanes.row_at(tile, row0, s));
+}
+
+__device__ __forceinline__ v4s read_transposed(const char *at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) v4s *)(static_cast<uintptr_t>(lds_address(at))));
+}
+
+// A lane's sixteen values in the order above as the second operand of a
+// product: rounded to 16 bits, or as they are.
+template <class V>
+struct Column {
+  typename Mfma<V>::Frag b[2];
+  __device__ __forceinline__ explicit Column(const float (&p)[16]) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       v4u w;
@@ -122,32 +193,43 @@ __device__ inline void mul_transposed(const char *tile, int row0, const float (&
       for (int j = 0; j < 4; ++j) w[j] = Mfma<V>::pack(p[8 * k + 2 * j], p[8 * k + 2 * j + 1]);
       b[k] = __builtin_bit_cast(typename Mfma<V>::Frag, w);
     }
-    const int i = lane % 16, column = ((lane / 16) % 2) * 16 + (i % 4) * 4;
+  }
+};
+template <>
+struct Column<F32> {
+  float p[16];
+  __device__ __forceinline__ explicit Column(const float (&from)[16]) {
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int r = 0; r < 16; ++r) p[r] = from[r];
+  }
+};
+
+// acc[dt] += X^T P over 32 rows of the tile from `row0` on (a multiple of 32), X
+// read along its columns.
+template <class V, class Lanes, int kBlocks>
+__device__ __forceinline__ void mul_transposed(const Lanes &lanes, uint32_t tile, int row0,
+                                               const Column<V> &column, v16f (&acc)[kBlocks]) {
+  if constexpr (sizeof(typename V::Storage) == 2) {
+#pragma unroll
+    for (int dt = 0; dt < kBlocks; ++dt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         v4s part[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int row = row0 + 16 * k + 8 * t + 4 * half + i / 4, d = dt * 32 + column;
-          part[t] = read_transposed(tile + T::along(row, d / 8) + (d % 8) * 2);
-        }
+        for (int t = 0; t < 2; ++t)
+          part[t] = read_transposed(lanes.column_at(tile, row0, 16 * k + 8 * t, dt));
         const auto lo = __builtin_bit_cast(v2u, part[0]), hi = __builtin_bit_cast(v2u, part[1]);
         const auto a = __builtin_bit_cast(typename Mfma<V>::Frag, (v4u{lo[0], lo[1], hi[0], hi[1]}));
-        acc[dt] = Mfma<V>::mul(a, b[k], acc[dt]);
+        acc[dt] = Mfma<V>::mul(a, column.b[k], acc[dt]);
       }
   } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = row0 + 8 * (r / 4) + 4 * half + r % 4;
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
-        const int d = dt * 32 + lane % 32;
-        const float a = *reinterpret_cast<const float *>(tile + T::along(row, d / 4) + (d % 4) * 4);
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
+      for (int dt = 0; dt < kBlocks; ++dt) {
+        const float a = read_lds<float>(lanes.column_at(tile, row0, 8 * (r / 4) + r % 4, dt));
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, column.p[r], acc[dt], 0, 0, 0);
       }
-    }
   }
 }
 
@@ -156,47 +238,83 @@ __device__ inline void mul_transposed(const char *tile, int row0, const float (&
 // `free` numbers.
 struct Numbering {
   int32_t far, skip, free, window;
-  __device__ inline Numbering(const WindowArgs &a, int32_t near)
+  __device__ __forceinline__ Numbering(const WindowArgs &a, int32_t near)
       : far(min(a.sinks, near)), skip(near - far), free(skip == 0 ? a.sinks : far), window(a.window) {}
-  __device__ inline int32_t key(int32_t c) const { return c < far ? c : c + skip; }
+  __device__ __forceinline__ int32_t key(int32_t c) const { return c < far ? c : c + skip; }
   // p = -1 sees nothing.
-  __device__ inline bool seen(int32_t p, int32_t c) const {
+  __device__ __forceinline__ bool seen(int32_t p, int32_t c) const {
     const uint32_t back = static_cast<uint32_t>(p - key(c));
     return back < static_cast<uint32_t>(c < free ? 0x7fffffff : window);
   }
 };
 
-// A workgroup's share of a tile's rows on its way from memory to LDS, sixteen
-// bytes a piece.  Rows that follow each other in memory are read from one
-// uniform address by 32-bit offsets that stay: with an address worked out for
-// every piece the forward tiles spent half of their vector instructions on it.
+// A workgroup's share of a tile's rows, from memory to LDS, sixteen bytes a
+// piece.  Whole tiles go there directly: no registers on the way, and the
+// address of a tile is uniform, so that a piece costs one instruction (a prompt
+// of 8,192 tokens: 198 us with an address a piece, 180 through registers with
+// a uniform one, 171 directly).
+//
+// A direct load puts lane i's piece at sixteen i bytes: the piece at place c
+// of a row is the row's chunk c ^ f(row), the permutation of TileShape::along.
 template <class V, int DP, int kTokens, int kThreads>
 struct RowLoader {
   using T = TileShape<V, DP>;
-  static constexpr int kPer = (kTokens * T::kUsed + kThreads - 1) / kThreads;
-  static constexpr bool kEven = kThreads % T::kUsed == 0 && kTokens * T::kUsed % kThreads == 0;
-  uint32_t offset;   // of the thread's first piece
+  static constexpr int kPieces = kTokens * T::kChunks;
+  static constexpr int kPer = (kPieces + kThreads - 1) / kThreads;
+  static constexpr int kRows = kThreads / T::kChunks;  // between a thread's pieces
+  static constexpr bool kEven = T::kUsed == T::kChunks && kPieces % kThreads == 0;
+  // the permutation repeats after sixteen rows
+  static constexpr int kKinds = kRows % 16 == 0 ? 1 : 2;
+  static_assert(!kEven || kRows * kKinds % 16 == 0, "a thread's pieces are of one or two kinds");
+  uint32_t offset[kKinds];  // of the thread's pieces from the first row it has of a kind
   int64_t step;      // bytes between rows
   bool plain;        // whole rows within 2 GB of each other (uniform)
 
-  __device__ inline void start(int64_t stride, int dim) {
+  __device__ __forceinline__ void start(int64_t stride, int dim) {
     step = stride * T::kSize;
     plain = kEven && dim == DP && step >= 0 && step * kTokens < (int64_t{1} << 31);
-    offset = static_cast<uint32_t>(threadIdx.x / T::kUsed) * static_cast<uint32_t>(step) +
-             threadIdx.x % T::kUsed * 16;
+    const int row = threadIdx.x / T::kChunks;
+#pragma unroll
+    for (int kind = 0; kind < kKinds; ++kind)
+      offset[kind] = static_cast<uint32_t>(row) * static_cast<uint32_t>(step) +
+                     T::logical(row + kind * kRows, threadIdx.x % T::kChunks) * 16;
   }
-  // kTokens rows from `first` on, all there.
-  __device__ inline void load(const void *first, v4u (&to)[kPer]) const {
+  // kTokens rows from `first` on, all there, to `tile`: done when the loads
+  // in flight are.
+  __device__ __forceinline__ void direct(const void *first, char *tile) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const char *base = static_cast<const char *>(first) + r * (kThreads / T::kUsed) * step;
-      to[r] = *reinterpret_cast<const v4u *>(base + offset);
+      const char *from = static_cast<const char *>(first) + r * kRows * step + offset[r % kKinds];
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)(from),
+          (__attribute__((address_space(3))) void *)(tile + (r * kThreads + wave * kWave) * 16), 16, 0, 0);
+    }
+  }
+  // Rows one by one: `row_at(row)` gives a row's address, null for zeros.
+  template <class RowAt>
+  __device__ __forceinline__ void each(const RowAt &row_at, int dim, char *tile) const {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const int at = threadIdx.x + r * kThreads, row = at / T::kChunks, chunk = at % T::kChunks;
+      if (row >= kTokens || chunk >= T::kUsed) continue;
+      const void *from = row_at(row);
+      v4u piece = {0, 0, 0, 0};
+      if (from != nullptr && chunk * 16 < dim * T::kSize)
+        piece = *reinterpret_cast<const v4u *>(static_cast<const char *>(from) + chunk * 16);
+      *reinterpret_cast<v4u *>(tile + T::along(row, chunk)) = piece;
     }
   }
 };
 
+// A barrier after which every wave's direct loads are in LDS.
+__device__ __forceinline__ void sync_tiles() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0); the other counters as they are
+  __syncthreads();
+}
+
 // The lane 32 away.
-__device__ inline float other_half(float v) {
+__device__ __forceinline__ float other_half(float v) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   const uint32_t other = (threadIdx.x % kWave) < 32 ? r[1] : r[0];
@@ -205,7 +323,7 @@ __device__ inline float other_half(float v) {
 
 // Workgroups go to the 8 XCDs in turn; this gives each XCD one contiguous
 // part of the work, whose neighbours share what they read through its L2.
-__device__ inline int64_t xcd_order(int64_t id, int64_t n) {
+__device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t n) {
   const int64_t per = n / 8, rest = n % 8, x = id % 8, at = id / 8;
   return x * per + (x < rest ? x : rest) + at;
 }
@@ -216,7 +334,7 @@ __device__ inline int64_t xcd_order(int64_t id, int64_t n) {
 struct TailCut {
   int64_t whole, rest;
   int32_t parts;
-  __host__ __device__ inline int64_t items() const { return whole + rest * parts; }
+  __host__ __device__ __forceinline__ int64_t items() const { return whole + rest * parts; }
 };
 
 // A part costs what kPartCost of a block does, in writing and joining sums.
@@ -241,7 +359,7 @@ struct CutItem {
   int64_t block;
   int32_t part, parts;
   int64_t slot;  // of its sums in scratch, -1 for a whole block
-  __device__ inline CutItem(const TailCut &cut, int64_t id) {
+  __device__ __forceinline__ CutItem(const TailCut &cut, int64_t id) {
     if (id < cut.whole) {
       block = xcd_order(id, cut.whole);
       part = 0;

@@ -48,19 +48,18 @@ struct BackwardShape {
   static constexpr int kSub = T::kSize == 2 ? 2 : 1;
   static constexpr int kTokens = 32 * kSub;  // tokens of a tile
   static constexpr int kTile = kTokens * T::kPitch;
-  static constexpr int kPerThread = (kTokens * T::kUsed + kThreads - 1) / kThreads;
 };
 
 // Sixteen bytes of a row, zeros beyond the head.
 template <class V>
-__device__ inline v4u load_chunk(const typename V::Storage *row, int chunk, int dim) {
+__device__ __forceinline__ v4u load_chunk(const typename V::Storage *row, int chunk, int dim) {
   if (chunk * 16 >= dim * static_cast<int>(sizeof(typename V::Storage))) return v4u{0, 0, 0, 0};
   return *reinterpret_cast<const v4u *>(reinterpret_cast<const char *>(row) + chunk * 16);
 }
 
 // Sum of products of two sixteen-byte pieces.
 template <class V>
-__device__ inline float dot_chunk(v4u x, v4u y) {
+__device__ __forceinline__ float dot_chunk(v4u x, v4u y) {
   float acc = 0.0f;
   if constexpr (sizeof(typename V::Storage) == 4) {
     const auto a = __builtin_bit_cast(v4f, x), b = __builtin_bit_cast(v4f, y);
@@ -78,7 +77,7 @@ __device__ inline float dot_chunk(v4u x, v4u y) {
 
 // A lane's column of a transposed result: row `to` gets acc * factor.
 template <class V, int DP>
-__device__ inline void store_column(const v16f (&acc)[DP / 32], float factor, int dim,
+__device__ __forceinline__ void store_column(const v16f (&acc)[DP / 32], float factor, int dim,
                                     typename V::Storage *to) {
   const int half = (threadIdx.x % kWave) / 32;
 #pragma unroll
@@ -97,7 +96,7 @@ __device__ inline void store_column(const v16f (&acc)[DP / 32], float factor, in
 }
 
 template <int DP>
-__device__ inline void zero(v16f (&acc)[DP / 32]) {
+__device__ __forceinline__ void zero(v16f (&acc)[DP / 32]) {
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -116,7 +115,8 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
   using F = BackwardShape<V, DP>;
   using Frag = typename Mfma<V>::Frag;
   constexpr int kSteps = DP / Mfma<V>::kDepth;
-  __shared__ __attribute__((aligned(16))) char lds[4 * F::kTile];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * F::kTile];
+  const TileLanes<V, DP> lanes(lds);
 
   const int lane = threadIdx.x % kWave, half = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -170,50 +170,31 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
     if (live && i < a.lq && half == 0) up.delta[(b * a.heads + h) * a.lq + i] = delta;
   }
 
-  v4u k_next[F::kPerThread], v_next[F::kPerThread];
   RowLoader<V, DP, F::kTokens, kThreads> k_rows, v_rows;
   k_rows.start(a.ks[1], a.dim);
   v_rows.start(a.vs[1], a.dim);
-  const auto fetch = [&](int32_t c0) {
-    if (k_rows.plain && v_rows.plain && c0 >= far && c0 + F::kTokens <= count) {
-      const int64_t key = c0 + skip;
-      k_rows.load(k_base + key * a.ks[1], k_next);
-      v_rows.load(v_base + key * a.vs[1], v_next);
-      return;
-    }
-#pragma unroll
-    for (int r = 0; r < F::kPerThread; ++r) {
-      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
-      const int32_t c = c0 + row;
-      k_next[r] = v_next[r] = v4u{0, 0, 0, 0};
-      if (row < F::kTokens && c < count) {
-        const int64_t key = number.key(c);
-        k_next[r] = load_chunk<V>(k_base + key * a.ks[1], chunk, a.dim);
-        v_next[r] = load_chunk<V>(v_base + key * a.vs[1], chunk, a.dim);
-      }
-    }
+  const auto fetch = [&](const S *base, int64_t stride, const auto &rows, int32_t c0, uint32_t to) {
+    if (rows.plain && c0 >= far && c0 + F::kTokens <= count)
+      rows.direct(base + (c0 + skip) * stride, lds + to);
+    else
+      rows.each([&](int row) -> const void * {
+        const int32_t c = c0 + row;
+        return c < count ? base + number.key(c) * stride : nullptr;
+      }, a.dim, lds + to);
   };
-  const auto keep = [&](int buffer) {
-    char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
-#pragma unroll
-    for (int r = 0; r < F::kPerThread; ++r) {
-      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
-      if (row < F::kTokens) {
-        *reinterpret_cast<v4u *>(kt + T::along(row, chunk)) = k_next[r];
-        *reinterpret_cast<v4u *>(vt + T::along(row, chunk)) = v_next[r];
-      }
-    }
-  };
+  const auto k_tile = [](int parity) { return static_cast<uint32_t>(parity * F::kTile); };
+  const auto v_tile = [](int parity) { return static_cast<uint32_t>((2 + parity) * F::kTile); };
 
   v16f acc[DP / 32];
   zero<DP>(acc);
-  fetch(0);
-  keep(0);
-  __syncthreads();
-  for (int32_t c0 = 0, buffer = 0; c0 < count; c0 += F::kTokens, buffer ^= 1) {
-    const bool more = c0 + F::kTokens < count;
-    if (more) fetch(c0 + F::kTokens);
-    const char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
+  fetch(k_base, a.ks[1], k_rows, 0, k_tile(0));
+  fetch(v_base, a.vs[1], v_rows, 0, v_tile(0));
+  sync_tiles();
+  const auto tile = [&](int32_t c0, int parity) __attribute__((always_inline)) {
+    if (c0 + F::kTokens < count) {  // into the other tiles, which all waves are past
+      fetch(k_base, a.ks[1], k_rows, c0 + F::kTokens, k_tile(parity ^ 1));
+      fetch(v_base, a.vs[1], v_rows, c0 + F::kTokens, v_tile(parity ^ 1));
+    }
     const int32_t k_first = max(c0, far) + skip, k_last = min(c0 + F::kTokens, count) - 1 + skip;
     const bool any = p_last >= p_first &&
                      (c0 < far || (k_first <= p_last && (p_first - k_last < a.window || k_first < a.sinks)));
@@ -227,8 +208,8 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
         for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
-          s = Mfma<V>::mul(read_rows<V, DP>(kt, 32 * t + lane % 32, st), qf[st], s);
-          dp = Mfma<V>::mul(read_rows<V, DP>(vt, 32 * t + lane % 32, st), gf[st], dp);
+          s = Mfma<V>::mul(read_rows<V>(lanes, k_tile(parity), 32 * t, st), qf[st], s);
+          dp = Mfma<V>::mul(read_rows<V>(lanes, v_tile(parity), 32 * t, st), gf[st], dp);
         }
         float ds[16];
 #pragma unroll
@@ -240,11 +221,14 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
             ds[r] = number.seen(p, c) ? ds[r] : 0.0f;
           }
         }
-        mul_transposed<V, DP>(kt, 32 * t, ds, acc);
+        mul_transposed<V>(lanes, k_tile(parity), 32 * t, Column<V>(ds), acc);
       }
     }
-    if (more) keep(buffer ^ 1);
-    __syncthreads();
+    sync_tiles();
+  };
+  for (int32_t c0 = 0; c0 < count; c0 += 2 * F::kTokens) {
+    tile(c0, 0);
+    if (c0 + F::kTokens < count) tile(c0 + F::kTokens, 1);
   }
   if (live && i < a.lq)
     store_column<V, DP>(acc, a.grad_scale, a.dim, dq + ((b * a.lq + i) * a.heads + h) * a.dim);
@@ -260,11 +244,11 @@ struct KeyWave {
   using Frag = typename Mfma<V>::Frag;
   static constexpr int kSteps = DP / Mfma<V>::kDepth;
   Frag kf[kInLds ? 1 : kSteps], vf[kInLds ? 1 : kSteps];
-  const char *k_tile, *v_tile;  // with kInLds
-  int key_row;
+  uint32_t k_tile, v_tile;  // with kInLds
+  int key_row;               // of the tiles, the wave's first
   v16f dk[DP / 32], dv[DP / 32];
 
-  __device__ inline void start(const WindowArgs &a, int64_t b, int32_t kvh, int32_t key, bool live) {
+  __device__ __forceinline__ void start(const WindowArgs &a, int64_t b, int32_t kvh, int32_t key, bool live) {
     using S = typename V::Storage;
     const int half = (threadIdx.x % kWave) / 32;
     zero<DP>(dk);
@@ -284,28 +268,28 @@ struct KeyWave {
       }
     }
   }
-  __device__ inline Frag key_frag(int s) const {
-    if constexpr (kInLds) return read_rows<V, DP>(k_tile, key_row, s);
+  __device__ __forceinline__ Frag key_frag(const TilePlaces<V, DP> &lanes, int s) const {
+    if constexpr (kInLds) return read_rows<V>(lanes, k_tile, key_row, s);
     else return kf[s];
   }
-  __device__ inline Frag value_frag(int s) const {
-    if constexpr (kInLds) return read_rows<V, DP>(v_tile, key_row, s);
+  __device__ __forceinline__ Frag value_frag(const TilePlaces<V, DP> &lanes, int s) const {
+    if constexpr (kInLds) return read_rows<V>(lanes, v_tile, key_row, s);
     else return vf[s];
   }
 
   // 32 queries from row `row0` of the tiles, at positions p0 .. p0 + 31;
   // `masked`: the lane's key is not seen by all of them.
-  __device__ inline void add(const WindowArgs &a, const char *q_tile, const char *g_tile,
-                             const float *lse, const float *delta, int row0, int32_t p0,
-                             int32_t key, bool masked) {
+  __device__ __forceinline__ void add(const WindowArgs &a, const TilePlaces<V, DP> &lanes, uint32_t q_tile,
+                             uint32_t g_tile, const float *lse, const float *delta, int row0,
+                             int32_t p0, int32_t key, bool masked) {
     const int lane = threadIdx.x % kWave, half = lane / 32;
     v16f s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
-      s = Mfma<V>::mul(read_rows<V, DP>(q_tile, row0 + lane % 32, st), key_frag(st), s);
-      dp = Mfma<V>::mul(read_rows<V, DP>(g_tile, row0 + lane % 32, st), value_frag(st), dp);
+      s = Mfma<V>::mul(read_rows<V>(lanes, q_tile, row0, st), key_frag(lanes, st), s);
+      dp = Mfma<V>::mul(read_rows<V>(lanes, g_tile, row0, st), value_frag(lanes, st), dp);
     }
     float p[16], ds[16];
 #pragma unroll
@@ -328,48 +312,42 @@ struct KeyWave {
         ds[r] = back < limit ? ds[r] : 0.0f;
       }
     }
-    mul_transposed<V, DP>(g_tile, row0, p, dv);
-    mul_transposed<V, DP>(q_tile, row0, ds, dk);
+    mul_transposed<V>(lanes, g_tile, row0, Column<V>(p), dv);
+    mul_transposed<V>(lanes, q_tile, row0, Column<V>(ds), dk);
   }
 };
 
-// The next queries of the walk, on their way through registers into LDS.
-// A query beyond the sequence is zeros with lse = +inf: its P is zero.
+// Queries of the walk in LDS: q, the upstream gradient, lse and delta.  A query
+// beyond the sequence is zeros with lse = +inf: its P is zero.
 template <class V, int DP, int kTokens, int kThreads>
 struct QueryTile {
   using T = TileShape<V, DP>;
   static constexpr int kTile = kTokens * T::kPitch;
   static constexpr int kBytes = 2 * kTile + 2 * kTokens * 4;
-  static constexpr int kPerThread = (kTokens * T::kUsed + kThreads - 1) / kThreads;
-  v4u q[kPerThread], g[kPerThread];
   float stat;
   RowLoader<V, DP, kTokens, kThreads> q_rows, g_rows;
 
-  __device__ inline void start(const WindowArgs &a, const Upstream &up) {
+  __device__ __forceinline__ void start(const WindowArgs &a, const Upstream &up) {
     q_rows.start(a.qs[1], a.dim);
     g_rows.start(up.gs[1], a.dim);
   }
-
-  __device__ inline void fetch(const WindowArgs &a, const Upstream &up, int64_t b, int32_t h,
-                               int32_t p0, int32_t last, int32_t offset) {
+  // The rows are on their way to `to`; the statistics wait for keep.
+  __device__ __forceinline__ void fetch(const WindowArgs &a, const Upstream &up, int64_t b, int32_t h,
+                               int32_t p0, int32_t last, int32_t offset, char *to) {
     using S = typename V::Storage;
-    const S *q_base = static_cast<const S *>(a.q) + b * a.qs[0] + h * a.qs[2];
-    const S *g_base = static_cast<const S *>(up.grad) + b * up.gs[0] + h * up.gs[2];
+    const S *q = static_cast<const S *>(a.q) + b * a.qs[0] + h * a.qs[2];
+    const S *g = static_cast<const S *>(up.grad) + b * up.gs[0] + h * up.gs[2];
+    const int64_t first = p0 - offset;
     if (q_rows.plain && g_rows.plain && p0 + kTokens - 1 <= last) {
-      const int64_t i = p0 - offset;
-      q_rows.load(q_base + i * a.qs[1], q);
-      g_rows.load(g_base + i * up.gs[1], g);
+      q_rows.direct(q + first * a.qs[1], to);
+      g_rows.direct(g + first * up.gs[1], to + kTile);
     } else {
-#pragma unroll
-      for (int r = 0; r < kPerThread; ++r) {
-        const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
-        q[r] = g[r] = v4u{0, 0, 0, 0};
-        if (row < kTokens && p0 + row <= last) {
-          const int64_t i = p0 + row - offset;
-          q[r] = load_chunk<V>(q_base + i * a.qs[1], chunk, a.dim);
-          g[r] = load_chunk<V>(g_base + i * up.gs[1], chunk, a.dim);
-        }
-      }
+      q_rows.each([&](int row) -> const void * {
+        return p0 + row <= last ? q + (first + row) * a.qs[1] : nullptr;
+      }, a.dim, to);
+      g_rows.each([&](int row) -> const void * {
+        return p0 + row <= last ? g + (first + row) * up.gs[1] : nullptr;
+      }, a.dim, to + kTile);
     }
     // the first kTokens threads take lse, the next as many delta
     static_assert(2 * kTokens <= kThreads, "a thread a statistic");
@@ -377,19 +355,11 @@ struct QueryTile {
     const bool is_lse = threadIdx.x < kTokens;
     stat = is_lse ? INFINITY : 0.0f;
     if (threadIdx.x < 2 * kTokens && p0 + row <= last) {
-      const int64_t at = (b * a.heads + h) * a.lq + p0 + row - offset;
+      const int64_t at = (b * a.heads + h) * a.lq + first + row;
       stat = is_lse ? up.lse[at] : up.delta[at];
     }
   }
-  __device__ inline void keep(char *to) const {
-#pragma unroll
-    for (int r = 0; r < kPerThread; ++r) {
-      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
-      if (row < kTokens) {
-        *reinterpret_cast<v4u *>(to + T::along(row, chunk)) = q[r];
-        *reinterpret_cast<v4u *>(to + kTile + T::along(row, chunk)) = g[r];
-      }
-    }
+  __device__ __forceinline__ void keep(char *to) const {
     if (threadIdx.x < 2 * kTokens)
       reinterpret_cast<float *>(to + 2 * kTile)[threadIdx.x] = stat;
   }
@@ -406,7 +376,7 @@ struct KeyPlan {
 
 // Sums of one lane's key: dk then dv, `dim` floats each.
 template <int DP>
-__device__ inline void store_sums(const v16f (&dk)[DP / 32], const v16f (&dv)[DP / 32], int dim,
+__device__ __forceinline__ void store_sums(const v16f (&dk)[DP / 32], const v16f (&dv)[DP / 32], int dim,
                                   float *to) {
   const int half = (threadIdx.x % kWave) / 32;
 #pragma unroll
@@ -423,16 +393,17 @@ __device__ inline void store_sums(const v16f (&dk)[DP / 32], const v16f (&dv)[DP
 
 // Queries within reach of a block's window: positions first .. last; the rest
 // of a sink's queries are the far pass's.
-__device__ inline int32_t near_last(const WindowArgs &a, int32_t block, int32_t n) {
+__device__ __forceinline__ int32_t near_last(const WindowArgs &a, int32_t block, int32_t n) {
   const int64_t last = static_cast<int64_t>(block) * kBlockKeys + kBlockKeys + a.window - 2;
   return last < n - 1 ? static_cast<int32_t>(last) : n - 1;
 }
 
 // The near pass's workgroup.  Sums of 128 values a key leave room for one wave
-// a SIMD if keys and values stay in registers too (476 us of a step of 16,384
-// tokens, waiting on LDS and products in turn): 16-bit heads above 64 keep
-// them in LDS, and eight waves, two for the same keys, take alternate halves
-// of a tile.
+// a SIMD if keys and values stay in registers too, which waits on LDS and
+// products in turn: 16-bit heads above 64 keep them in LDS, and eight waves,
+// two for the same keys, take alternate halves of a tile (16,384 tokens of 16
+// heads of 128, a window of 1,024: 476 us with one wave a SIMD, 384 with two;
+// 421 with TileLanes' addresses, which leave fewer registers to reads).
 template <class V, int DP>
 struct NearShape {
   using T = TileShape<V, DP>;
@@ -455,7 +426,8 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
   using T = TileShape<V, DP>;
   using Tile = typename N::Tile;
   constexpr int kSub = N::kSub, kTokens = N::kTokens;
-  __shared__ __attribute__((aligned(16))) char lds[N::kLds];
+  __shared__ __attribute__((aligned(1024))) char lds[N::kLds];
+  const TilePlaces<V, DP> lanes(lds);
 
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -469,14 +441,13 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
   const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
   const int32_t w_first = block * kBlockKeys + keys_of * 32, w_last = w_first + 31;
   const int32_t key = w_first + lane % 32;
-  char *tiles_lds = lds + N::kKeyBytes;
 
   KeyWave<V, DP, N::kInLds> keys;
   keys.start(a, b, kvh, key, key < n);
   if constexpr (N::kInLds) {
-    keys.k_tile = lds;
-    keys.v_tile = lds + kBlockKeys * T::kPitch;
-    keys.key_row = keys_of * 32 + lane % 32;
+    keys.k_tile = 0;
+    keys.v_tile = kBlockKeys * T::kPitch;
+    keys.key_row = keys_of * 32;
     const S *k = static_cast<const S *>(a.k) + b * a.ks[0] + kvh * a.ks[2];
     const S *v = static_cast<const S *>(a.v) + b * a.vs[0] + kvh * a.vs[2];
     for (int at = threadIdx.x; at < kBlockKeys * T::kUsed; at += N::kThreads) {
@@ -500,19 +471,21 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
 
   Tile next;
   next.start(a, up);
-  const auto fetch = [&](int32_t step) {
-    next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset);
+  const auto tile_at = [](int parity) { return static_cast<uint32_t>(N::kKeyBytes + parity * Tile::kBytes); };
+  const auto fetch = [&](int32_t step, int parity) {
+    next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset,
+               lds + tile_at(parity));
   };
   if (begin < end) {
-    fetch(begin);
-    next.keep(tiles_lds);
+    fetch(begin, 0);
+    next.keep(lds + tile_at(0));
   }
-  __syncthreads();
-  for (int32_t step = begin, buffer = 0; step < end; ++step, buffer ^= 1) {
+  sync_tiles();
+  const auto walk = [&](int32_t step, int parity) __attribute__((always_inline)) {
     const bool more = step + 1 < end;
-    if (more) fetch(step + 1);
-    const char *tile = tiles_lds + buffer * Tile::kBytes;
-    const float *stat = reinterpret_cast<const float *>(tile + 2 * Tile::kTile);
+    if (more) fetch(step + 1, parity ^ 1);  // into the other tile, which all waves are past
+    const uint32_t tile = tile_at(parity);
+    const float *stat = reinterpret_cast<const float *>(lds + tile + 2 * Tile::kTile);
 #pragma unroll
     for (int t0 = 0; t0 < kSub; t0 += N::kGroups) {
       const int t = t0 + group;
@@ -520,19 +493,21 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
       const bool any = p1 >= w_first && p0 <= last && (p0 - w_last < a.window || w_first < a.sinks);
       const bool whole = p0 >= w_last && (p1 - w_first < a.window || w_last < a.sinks);
       if (any)
-        keys.add(a, tile, tile + Tile::kTile, stat, stat + kTokens, 32 * t, p0, key,
+        keys.add(a, lanes, tile, tile + Tile::kTile, stat, stat + kTokens, 32 * t, p0, key,
                  __builtin_amdgcn_readfirstlane(!whole));
     }
-    if (more) next.keep(tiles_lds + (buffer ^ 1) * Tile::kBytes);
-    __syncthreads();
-  }
+    if (more) next.keep(lds + tile_at(parity ^ 1));
+    sync_tiles();
+  };
+#pragma unroll 1
+  for (int32_t step = begin; step < end; ++step) walk(step, (step - begin) & 1);
 
   if constexpr (N::kGroups == 2) {  // the second wave's sums to the first: dk, then dv
     float *sums = reinterpret_cast<float *>(lds) + (keys_of * kWave + lane) * 4;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       v16f(&mine)[DP / 32] = which == 0 ? keys.dk : keys.dv;
-      if (which == 1) __syncthreads();
+      if (which == 1) sync_tiles();
       if (group == 1) {
 #pragma unroll
         for (int r = 0; r < DP / 2; r += 4)
@@ -540,7 +515,7 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
               v4f{mine[r / 16][r % 16], mine[r / 16][r % 16 + 1], mine[r / 16][r % 16 + 2],
                   mine[r / 16][r % 16 + 3]};
       }
-      __syncthreads();
+      sync_tiles();
       if (group == 0) {
 #pragma unroll
         for (int r = 0; r < DP / 2; r += 4) {
@@ -565,6 +540,13 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
   }
 }
 
+// Two tiles of 128 queries where the LDS of a CU holds them (all but wide
+// float32 heads).
+template <class V, int DP>
+constexpr int far_buffers() {
+  return 2 * QueryTile<V, DP, 32 * kWaves, kThreads>::kBytes <= 160 * 1024 ? 2 : 1;
+}
+
 // Sinks and the queries beyond their block's span: a wave takes every fourth
 // 32 queries.
 template <class V, int DP>
@@ -572,8 +554,9 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
                                                                  KeyPlan plan, int64_t blocks) {
   constexpr int kTokens = 32 * kWaves;
   using Tile = QueryTile<V, DP, kTokens, kThreads>;
-  extern __shared__ __attribute__((aligned(16))) char dynamic_lds[];
-  char *lds = dynamic_lds;
+  constexpr int kBuffers = far_buffers<V, DP>();
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const TilePlaces<V, DP> lanes(lds);
 
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -598,18 +581,29 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
 
   Tile next;
   next.start(a, up);
-  const auto fetch = [&](int32_t step) {
-    next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset);
+  const auto fetch = [&](int32_t step, uint32_t to) {
+    next.fetch(a, up, b, kvh * a.group + step / tiles, first + step % tiles * kTokens, last, offset,
+               lds + to);
   };
-  if (begin < end) fetch(begin);
-  for (int32_t step = begin; step < end; ++step) {
+  if (begin < end) {
+    fetch(begin, 0);
     next.keep(lds);
-    __syncthreads();
-    if (step + 1 < end) fetch(step + 1);
-    const float *stat = reinterpret_cast<const float *>(lds + 2 * Tile::kTile);
+  }
+  sync_tiles();
+  for (int32_t step = begin; step < end; ++step) {
+    const bool more = step + 1 < end;
+    const uint32_t tile = kBuffers == 2 ? (step - begin) % 2 * Tile::kBytes : 0;
+    const uint32_t other = kBuffers == 2 ? Tile::kBytes - tile : 0;
+    if (kBuffers == 2 && more) fetch(step + 1, other);
+    const float *stat = reinterpret_cast<const float *>(lds + tile + 2 * Tile::kTile);
     // all of these queries see the sinks; a key that is none is not stored
-    keys.add(a, lds, lds + Tile::kTile, stat, stat + kTokens, 32 * wave, 0, key, false);
-    __syncthreads();
+    keys.add(a, lanes, tile, tile + Tile::kTile, stat, stat + kTokens, 32 * wave, 0, key, false);
+    if (kBuffers == 1) {
+      sync_tiles();
+      if (more) fetch(step + 1, 0);
+    }
+    if (more) next.keep(lds + other);
+    sync_tiles();
   }
   if (key >= a.sinks || key >= a.lk) return;
   const int64_t slot = ((bh * plan.far_units + unit) * plan.far_parts + part) * kWaves + wave;
@@ -704,7 +698,7 @@ msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, 
     backward_keys_near<V, DP><<<static_cast<unsigned>(k_blocks), NearShape<V, DP>::kThreads, 0, stream>>>(
         a, up, plan, k_blocks, static_cast<S *>(dk), static_cast<S *>(dv));
   if (f_blocks > 0) {
-    constexpr int lds = QueryTile<V, DP, 32 * kWaves, kThreads>::kBytes;
+    constexpr int lds = far_buffers<V, DP>() * QueryTile<V, DP, 32 * kWaves, kThreads>::kBytes;
     if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(backward_keys_far<V, DP>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         e != hipSuccess)

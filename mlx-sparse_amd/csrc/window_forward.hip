@@ -7,7 +7,7 @@
 // kv head, its waves share one span of keys.  Keys are numbered through: the
 // sinks before the span, then the span, so that a few sinks cost no tile of
 // their own.  Per tile of keys: S^T = K Q^T from LDS, the running maximum and
-// sum, O^T += V^T P^T; the next tile's rows are in flight meanwhile.
+// sum, O^T += V^T P^T; the next tile's rows are on their way to LDS meanwhile.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,7 +31,6 @@ struct ForwardShape {
   static constexpr int kSub = T::kSize == 2 ? 2 : 1;  // 32-key parts of a tile
   static constexpr int kKeys = 32 * kSub;
   static constexpr int kTile = kKeys * T::kPitch;
-  static constexpr int kPerThread = (kKeys * T::kUsed + kThreads - 1) / kThreads;
   static constexpr int kLds = 4 * kTile;  // K and V, twice
   // workgroups a CU: two hide each other's waits; wide float32 heads need the
   // registers of one (76 spilled with two at 128)
@@ -91,7 +90,8 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   using F = ForwardShape<V, DP>;
   using Frag = typename Mfma<V>::Frag;
   constexpr int kSteps = DP / Mfma<V>::kDepth;
-  __shared__ __attribute__((aligned(16))) char lds[F::kLds];
+  __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
+  const TileLanes<V, DP> lanes(lds);
 
   const int lane = threadIdx.x % kWave, half = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -143,43 +143,29 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
     }
   }
 
-  v4u k_next[F::kPerThread], v_next[F::kPerThread];
   RowLoader<V, DP, F::kKeys, kThreads> k_rows, v_rows;
   k_rows.start(a.ks[1], a.dim);
   v_rows.start(a.vs[1], a.dim);
-  const auto fetch = [&](int32_t c0) {
-    if (k_rows.plain && v_rows.plain && c0 >= far && c0 + F::kKeys <= count) {
-      const int64_t key = c0 + skip;
-      k_rows.load(k_base + key * a.ks[1], k_next);
-      v_rows.load(v_base + key * a.vs[1], v_next);
-      return;
-    }
-#pragma unroll
-    for (int r = 0; r < F::kPerThread; ++r) {
-      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
-      const int32_t c = c0 + row;
-      v4u kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
-      if (row < F::kKeys && c < count && chunk * 16 < a.dim * T::kSize) {
-        const int64_t key = number.key(c);
-        kw = *reinterpret_cast<const v4u *>(
-            reinterpret_cast<const char *>(k_base + key * a.ks[1]) + chunk * 16);
-        vw = *reinterpret_cast<const v4u *>(
-            reinterpret_cast<const char *>(v_base + key * a.vs[1]) + chunk * 16);
-      }
-      k_next[r] = kw;
-      v_next[r] = vw;
-    }
+  // one operand's rows of the tile at c0, to LDS
+  const auto fetch = [&](const S *base, int64_t stride, const auto &rows, int32_t c0,
+                         uint32_t to) {
+    if (rows.plain && c0 >= far && c0 + F::kKeys <= count)
+      rows.direct(base + (c0 + skip) * stride, lds + to);
+    else
+      rows.each([&](int row) -> const void * {
+        const int32_t c = c0 + row;
+        return c < count ? base + number.key(c) * stride : nullptr;
+      }, a.dim, lds + to);
   };
-  const auto keep = [&](int buffer) {
-    char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
-#pragma unroll
-    for (int r = 0; r < F::kPerThread; ++r) {
-      const int at = threadIdx.x + r * kThreads, row = at / T::kUsed, chunk = at % T::kUsed;
-      if (row < F::kKeys) {
-        *reinterpret_cast<v4u *>(kt + T::along(row, chunk)) = k_next[r];
-        *reinterpret_cast<v4u *>(vt + T::along(row, chunk)) = v_next[r];
-      }
-    }
+  const auto k_tile = [](int parity) { return static_cast<uint32_t>(parity * F::kTile); };
+  const auto v_tile = [](int parity) { return static_cast<uint32_t>((2 + parity) * F::kTile); };
+
+  // whether the wave sees any key of the tile at c0: sinks, and [first, last]
+  // of the span
+  const auto sees = [&](int32_t c0) {
+    const int32_t first = max(c0, far) + skip, last = min(c0 + F::kKeys, count) - 1 + skip;
+    return c0 < count && p_last >= p_first &&
+           (c0 < far || (first <= p_last && (p_first - last < a.window || first < a.sinks)));
   };
 
   v16f o[DP / 32];
@@ -187,78 +173,87 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
-  float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
+  float m = -INFINITY, base = 0.0f, l = 0.0f;  // l: this lane's keys only
+
+  const auto scores = [&](uint32_t tile, int t, v16f &to) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) to[r] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+      to = Mfma<V>::mul(read_rows<V>(lanes, tile, 32 * t, st), qf[st], to);
+  };
+  const auto exponentials = [&](const v16f &from) {
+    float e[16], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      e[r] = exp2_fast(from[r] * scale - base);
+      sum[r % 2] += e[r];
+    }
+    l += sum[0] + sum[1];
+    return Column<V>(e);
+  };
+  // masks the scores of the tile at c0 and moves the maximum.  It is moved
+  // only where it has grown by more than 2^8: until then exponentials up to
+  // 2^8 stand beside sums of their own scale.
+  const auto settle = [&](int32_t c0, v16f (&x)[F::kSub]) {
+    // all of the tile's keys seen by all of the wave's queries: no mask
+    const int32_t first = max(c0, far) + skip, last = min(c0 + F::kKeys, count) - 1 + skip;
+    const bool whole = c0 + F::kKeys <= count && last <= p_first &&
+                       (p_last - first < a.window || last < a.sinks) && p_last - p_first == kRows - 1;
+    if (__builtin_amdgcn_readfirstlane(!whole)) {
+#pragma unroll
+      for (int t = 0; t < F::kSub; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
+          x[t][r] = number.seen(p, c) ? x[t][r] : -INFINITY;
+        }
+    }
+    float tops[2] = {x[0][0], x[0][1]};
+#pragma unroll
+    for (int t = 0; t < F::kSub; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) tops[r % 2] = fmaxf(tops[r % 2], x[t][r]);
+    float top = fmaxf(tops[0], tops[1]);
+    top = fmaxf(top, other_half(top)) * scale;
+    if (__any(top > m + 8.0f)) {
+      const float grown = fmaxf(m, top);
+      const float shrink = grown == -INFINITY ? 1.0f : exp2_fast(m - grown);
+      m = grown;
+      base = m == -INFINITY ? 0.0f : m;
+      l *= shrink;
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= shrink;
+    }
+  };
 
   const int32_t tiles = (count + F::kKeys - 1) / F::kKeys;
   const int32_t c_begin = static_cast<int32_t>(static_cast<int64_t>(tiles) * item.part / item.parts) * F::kKeys;
   const int32_t c_end = static_cast<int32_t>(static_cast<int64_t>(tiles) * (item.part + 1) / item.parts) * F::kKeys;
-  fetch(c_begin);
-  keep(0);
-  __syncthreads();
-  for (int32_t c0 = c_begin, buffer = 0; c0 < c_end; c0 += F::kKeys, buffer ^= 1) {
-    const bool more = c0 + F::kKeys < c_end;
-    if (more) fetch(c0 + F::kKeys);
-    const char *kt = lds + buffer * 2 * F::kTile, *vt = kt + F::kTile;
-
-    // keys of the tile: sinks, and [k_first, k_last] of the span
-    const int32_t k_first = max(c0, far) + skip, k_last = min(c0 + F::kKeys, count) - 1 + skip;
-    const bool any = p_last >= p_first &&
-                     (c0 < far || (k_first <= p_last && (p_first - k_last < a.window || k_first < a.sinks)));
-    if (any) {
+  fetch(k_base, a.ks[1], k_rows, c_begin, k_tile(0));
+  fetch(v_base, a.vs[1], v_rows, c_begin, v_tile(0));
+  sync_tiles();
+  const auto tile = [&](int32_t c0, int parity) __attribute__((always_inline)) {
+    if (c0 + F::kKeys < c_end) {  // into the other tiles, which all waves are past
+      fetch(k_base, a.ks[1], k_rows, c0 + F::kKeys, k_tile(parity ^ 1));
+      fetch(v_base, a.vs[1], v_rows, c0 + F::kKeys, v_tile(parity ^ 1));
+    }
+    if (sees(c0)) {
       v16f s[F::kSub];
 #pragma unroll
-      for (int t = 0; t < F::kSub; ++t) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-          s[t] = Mfma<V>::mul(read_rows<V, DP>(kt, 32 * t + lane % 32, st), qf[st], s[t]);
-      }
-      // all of the tile's keys seen by all of the wave's queries: no mask
-      const bool whole = c0 + F::kKeys <= count && k_last <= p_first &&
-                         (p_last - k_first < a.window || k_last < a.sinks) &&
-                         p_last - p_first == kRows - 1;
-      if (__builtin_amdgcn_readfirstlane(!whole)) {
-#pragma unroll
-        for (int t = 0; t < F::kSub; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-            s[t][r] = number.seen(p, c) ? s[t][r] : -INFINITY;
-          }
-      }
-      float top = s[0][0];
+      for (int t = 0; t < F::kSub; ++t) scores(k_tile(parity), t, s[t]);
+      settle(c0, s);
 #pragma unroll
       for (int t = 0; t < F::kSub; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-      top = fmaxf(top, other_half(top)) * scale;
-      // The maximum is moved only where it has grown by more than 2^8: until
-      // then exponentials up to 2^8 stand beside sums of their own scale.
-      if (__any(top > m + 8.0f)) {
-        const float grown = fmaxf(m, top);
-        const float shrink = grown == -INFINITY ? 1.0f : exp2_fast(m - grown);
-        m = grown;
-        l *= shrink;
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[dt][r] *= shrink;
-      }
-      const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int t = 0; t < F::kSub; ++t) {
-        float e[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          e[r] = exp2_fast(s[t][r] * scale - base);
-          l += e[r];
-        }
-        mul_transposed<V, DP>(vt, 32 * t, e, o);
-      }
+        mul_transposed<V>(lanes, v_tile(parity), 32 * t, exponentials(s[t]), o);
     }
-    if (more) keep(buffer ^ 1);
-    __syncthreads();
+    sync_tiles();
+  };
+  for (int32_t c0 = c_begin; c0 < c_end; c0 += 2 * F::kKeys) {
+    tile(c0, 0);
+    if (c0 + F::kKeys < c_end) tile(c0 + F::kKeys, 1);
   }
 
   l += other_half(l);
