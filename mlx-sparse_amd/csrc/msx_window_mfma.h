@@ -321,10 +321,11 @@ __device__ __forceinline__ float other_half(float v) {
   return __builtin_bit_cast(float, other);
 }
 
-// Workgroups go to the 8 XCDs in turn; this gives each XCD one contiguous
+// Workgroups (2^31 - 1 at most, as checked before a launch; divisions of 64 bits
+// would cost a short block a tenth) go to the 8 XCDs in turn; this gives each XCD one contiguous
 // part of the work, whose neighbours share what they read through its L2.
-__device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t n) {
-  const int64_t per = n / 8, rest = n % 8, x = id % 8, at = id / 8;
+__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t n) {
+  const uint32_t per = n / 8, rest = n % 8, x = id % 8, at = id / 8;
   return x * per + (x < rest ? x : rest) + at;
 }
 
@@ -337,15 +338,16 @@ struct TailCut {
   __host__ __device__ __forceinline__ int64_t items() const { return whole + rest * parts; }
 };
 
-// A part costs what kPartCost of a block does, in writing and joining sums.
-inline TailCut cut_tail(int64_t blocks, int64_t slots, int64_t most_parts) {
-  constexpr double kPartCost = 0.04;
+// Costs in tiles, of which a block has `tiles`: a part more for its start and
+// its sums, `join` for the launch that joins them; a part has two at least.
+inline TailCut cut_tail(int64_t blocks, int64_t slots, int64_t tiles, double join) {
+  constexpr double kPart = 0.75;
   const int64_t rest = blocks % slots;
   TailCut cut{blocks, 0, 1};
-  double best = rest > 0 ? 1.0 : 0.0;
-  for (int64_t p = 2; p <= most_parts && p <= 16 && rest > 0; ++p) {
-    const double rounds = static_cast<double>((rest * p + slots - 1) / slots) / p;
-    const double cost = rounds + kPartCost * (1 + rest * p / static_cast<double>(slots));
+  double best = static_cast<double>(tiles);
+  for (int64_t p = 2; 2 * p <= tiles && p <= 16 && rest > 0; ++p) {
+    const double rounds = static_cast<double>((rest * p + slots - 1) / slots);
+    const double cost = rounds * (static_cast<double>((tiles + p - 1) / p) + kPart) + join;
     if (cost < best) {
       best = cost;
       cut = TailCut{blocks - rest, rest, static_cast<int32_t>(p)};
@@ -356,21 +358,27 @@ inline TailCut cut_tail(int64_t blocks, int64_t slots, int64_t most_parts) {
 
 // Which block and part of it a workgroup takes; the whole ones in XCD order.
 struct CutItem {
-  int64_t block;
+  uint32_t block;
   int32_t part, parts;
   int64_t slot;  // of its sums in scratch, -1 for a whole block
-  __device__ __forceinline__ CutItem(const TailCut &cut, int64_t id) {
-    if (id < cut.whole) {
-      block = xcd_order(id, cut.whole);
+  __device__ __forceinline__ CutItem(const TailCut &cut, uint32_t id) {
+    const uint32_t whole = static_cast<uint32_t>(cut.whole);
+    if (id < whole) {
+      block = xcd_order(id, whole);
       part = 0;
       parts = 1;
       slot = -1;
     } else {
-      slot = id - cut.whole;
-      block = cut.whole + slot / cut.parts;
-      part = static_cast<int32_t>(slot % cut.parts);
+      const uint32_t at = id - whole, of = static_cast<uint32_t>(cut.parts);
+      slot = at;
+      block = whole + at / of;
+      part = static_cast<int32_t>(at % of);
       parts = cut.parts;
     }
+  }
+  // The part's first tile of `tiles` (2^26 at most, in 16 parts at most).
+  __device__ __forceinline__ int32_t first(int32_t tiles, int32_t more = 0) const {
+    return parts == 1 ? tiles * more : tiles * (part + more) / parts;
   }
 };
 

@@ -103,13 +103,33 @@ __device__ __forceinline__ void zero(v16f (&acc)[DP / 32]) {
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
 }
 
+// The same as sums in scratch.
+template <int DP>
+__device__ __forceinline__ void store_sums(const v16f (&acc)[DP / 32], int dim, float *to) {
+  const int half = (threadIdx.x % kWave) / 32;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = dt * 32 + 2 * r + 4 * half;
+      if (d < dim)
+        *reinterpret_cast<v4f *>(to + d) = v4f{acc[dt][r], acc[dt][r + 1], acc[dt][r + 2], acc[dt][r + 3]};
+    }
+}
+
 // ---------------------------------------------------------------------------
 // dq, and delta for the keys' pass.
 
+// Blocks of 4 x 32 query rows of one key-value head, and how they are cut.
+struct QueryPlan {
+  int64_t units, per_bh;
+  TailCut cut;
+  float *sums;  // of the parts
+};
+
 template <class V, int DP>
 __global__ __launch_bounds__(kThreads, (sizeof(typename V::Storage) == 4 && DP > 64 ? 1 : 2)) void
-backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks_per_bh,
-                 int64_t blocks, typename V::Storage *dq) {
+backward_queries(WindowArgs a, Upstream up, QueryPlan plan, typename V::Storage *dq) {
   using S = typename V::Storage;
   using T = TileShape<V, DP>;
   using F = BackwardShape<V, DP>;
@@ -120,9 +140,10 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
 
   const int lane = threadIdx.x % kWave, half = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t id = xcd_order(blockIdx.x, blocks);
-  const int64_t bh = id / blocks_per_bh;
-  const int32_t first_unit = static_cast<int32_t>(id % blocks_per_bh) * kWaves;
+  const CutItem item(plan.cut, blockIdx.x);
+  const int32_t units_per_bh = static_cast<int32_t>(plan.units);
+  const uint32_t per_bh = static_cast<uint32_t>(plan.per_bh), bh = item.block / per_bh;
+  const int32_t first_unit = static_cast<int32_t>(item.block % per_bh) * kWaves;
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
   const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
@@ -167,7 +188,7 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
       gf[s] = __builtin_bit_cast(Frag, gw);
     }
     delta += other_half(delta);
-    if (live && i < a.lq && half == 0) up.delta[(b * a.heads + h) * a.lq + i] = delta;
+    if (live && i < a.lq && half == 0 && item.part == 0) up.delta[(b * a.heads + h) * a.lq + i] = delta;
   }
 
   RowLoader<V, DP, F::kTokens, kThreads> k_rows, v_rows;
@@ -187,11 +208,13 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
 
   v16f acc[DP / 32];
   zero<DP>(acc);
-  fetch(k_base, a.ks[1], k_rows, 0, k_tile(0));
-  fetch(v_base, a.vs[1], v_rows, 0, v_tile(0));
+  const int32_t tiles = (count + F::kTokens - 1) / F::kTokens;
+  const int32_t c_begin = item.first(tiles) * F::kTokens, c_end = item.first(tiles, 1) * F::kTokens;
+  fetch(k_base, a.ks[1], k_rows, c_begin, k_tile(0));
+  fetch(v_base, a.vs[1], v_rows, c_begin, v_tile(0));
   sync_tiles();
   const auto tile = [&](int32_t c0, int parity) __attribute__((always_inline)) {
-    if (c0 + F::kTokens < count) {  // into the other tiles, which all waves are past
+    if (c0 + F::kTokens < c_end) {  // into the other tiles, which all waves are past
       fetch(k_base, a.ks[1], k_rows, c0 + F::kTokens, k_tile(parity ^ 1));
       fetch(v_base, a.vs[1], v_rows, c0 + F::kTokens, v_tile(parity ^ 1));
     }
@@ -226,11 +249,14 @@ backward_queries(WindowArgs a, Upstream up, int32_t units_per_bh, int64_t blocks
     }
     sync_tiles();
   };
-  for (int32_t c0 = 0; c0 < count; c0 += 2 * F::kTokens) {
+  for (int32_t c0 = c_begin; c0 < c_end; c0 += 2 * F::kTokens) {
     tile(c0, 0);
-    if (c0 + F::kTokens < count) tile(c0 + F::kTokens, 1);
+    if (c0 + F::kTokens < c_end) tile(c0 + F::kTokens, 1);
   }
-  if (live && i < a.lq)
+  if (!live || i >= a.lq) return;
+  if (item.slot >= 0)  // a part: its sums as they are, joined by join_sums
+    store_sums<DP>(acc, a.dim, plan.sums + ((item.slot * kWaves + wave) * 32 + lane % 32) * a.dim);
+  else
     store_column<V, DP>(acc, a.grad_scale, a.dim, dq + ((b * a.lq + i) * a.heads + h) * a.dim);
 }
 
@@ -374,23 +400,6 @@ struct KeyPlan {
   float *near_sums, *far_sums;
 };
 
-// Sums of one lane's key: dk then dv, `dim` floats each.
-template <int DP>
-__device__ __forceinline__ void store_sums(const v16f (&dk)[DP / 32], const v16f (&dv)[DP / 32], int dim,
-                                  float *to) {
-  const int half = (threadIdx.x % kWave) / 32;
-#pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int d = dt * 32 + 2 * r + 4 * half;
-      if (d >= dim) continue;
-      *reinterpret_cast<v4f *>(to + d) = v4f{dk[dt][r], dk[dt][r + 1], dk[dt][r + 2], dk[dt][r + 3]};
-      *reinterpret_cast<v4f *>(to + dim + d) =
-          v4f{dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]};
-    }
-}
-
 // Queries within reach of a block's window: positions first .. last; the rest
 // of a sink's queries are the far pass's.
 __device__ __forceinline__ int32_t near_last(const WindowArgs &a, int32_t block, int32_t n) {
@@ -419,7 +428,7 @@ struct NearShape {
 
 template <class V, int DP>
 __global__ __launch_bounds__((NearShape<V, DP>::kThreads), (NearShape<V, DP>::kGroups)) void
-backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
+backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, uint32_t blocks,
                    typename V::Storage *dk, typename V::Storage *dv) {
   using S = typename V::Storage;
   using N = NearShape<V, DP>;
@@ -432,12 +441,12 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int keys_of = wave % kWaves, group = wave / kWaves;
-  const int64_t id = xcd_order(blockIdx.x, blocks);
+  const uint32_t id = xcd_order(blockIdx.x, blocks);
   const int32_t part = static_cast<int32_t>(id % plan.parts);
   const int32_t block = static_cast<int32_t>(id / plan.parts % plan.blocks);
-  const int64_t bh = id / plan.parts / plan.blocks;
-  const int64_t b = bh / a.kv_heads;
-  const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
+  const uint32_t head = id / plan.parts / plan.blocks;
+  const int64_t bh = head, b = head / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(head % a.kv_heads);
   const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
   const int32_t w_first = block * kBlockKeys + keys_of * 32, w_last = w_first + 31;
   const int32_t key = w_first + lane % 32;
@@ -466,8 +475,8 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
   const int32_t first = max(block * kBlockKeys, offset), last = near_last(a, block, n);
   const int32_t tiles = last >= first ? (last - first) / kTokens + 1 : 0;
   const int64_t total = static_cast<int64_t>(tiles) * a.group;
-  const int32_t begin = static_cast<int32_t>(total * part / plan.parts);
-  const int32_t end = static_cast<int32_t>(total * (part + 1) / plan.parts);
+  const int32_t begin = plan.parts == 1 ? 0 : static_cast<int32_t>(total * part / plan.parts);
+  const int32_t end = static_cast<int32_t>(plan.parts == 1 ? total : total * (part + 1) / plan.parts);
 
   Tile next;
   next.start(a, up);
@@ -532,7 +541,9 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, int64_t blocks,
   const int32_t unit = block * kWaves + keys_of;
   if (unit < plan.joined) {
     const int64_t slot = ((bh * plan.joined + unit) * plan.parts + part) * 32 + lane % 32;
-    store_sums<DP>(keys.dk, keys.dv, a.dim, plan.near_sums + slot * 2 * a.dim);
+    float *to = plan.near_sums + slot * 2 * a.dim;
+    store_sums<DP>(keys.dk, a.dim, to);
+    store_sums<DP>(keys.dv, a.dim, to + a.dim);
   } else {
     const int64_t row = (b * a.lk + key) * a.kv_heads + kvh;
     store_column<V, DP>(keys.dk, a.grad_scale, a.dim, dk + row * a.dim);
@@ -551,7 +562,7 @@ constexpr int far_buffers() {
 // 32 queries.
 template <class V, int DP>
 __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, Upstream up,
-                                                                 KeyPlan plan, int64_t blocks) {
+                                                                 KeyPlan plan, uint32_t blocks) {
   constexpr int kTokens = 32 * kWaves;
   using Tile = QueryTile<V, DP, kTokens, kThreads>;
   constexpr int kBuffers = far_buffers<V, DP>();
@@ -560,12 +571,12 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
 
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t id = xcd_order(blockIdx.x, blocks);
+  const uint32_t id = xcd_order(blockIdx.x, blocks);
   const int32_t part = static_cast<int32_t>(id % plan.far_parts);
   const int32_t unit = static_cast<int32_t>(id / plan.far_parts % plan.far_units);
-  const int64_t bh = id / plan.far_parts / plan.far_units;
-  const int64_t b = bh / a.kv_heads;
-  const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
+  const uint32_t head = id / plan.far_parts / plan.far_units;
+  const int64_t bh = head, b = head / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(head % a.kv_heads);
   const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
   const int32_t key = unit * 32 + lane % 32;
   const bool live = key < a.sinks && key < n;
@@ -607,49 +618,103 @@ __global__ __launch_bounds__(kThreads, 1) void backward_keys_far(WindowArgs a, U
   }
   if (key >= a.sinks || key >= a.lk) return;
   const int64_t slot = ((bh * plan.far_units + unit) * plan.far_parts + part) * kWaves + wave;
-  store_sums<DP>(keys.dk, keys.dv, a.dim, plan.far_sums + (slot * 32 + lane % 32) * 2 * a.dim);
+  float *to = plan.far_sums + (slot * 32 + lane % 32) * 2 * a.dim;
+  store_sums<DP>(keys.dk, a.dim, to);
+  store_sums<DP>(keys.dv, a.dim, to + a.dim);
 }
 
-// dk and dv of the joined units.  Sixteen sums a wave, four lanes a sum: each
-// takes every fourth part, and they are added in order.
-template <class V>
-__global__ __launch_bounds__(256) void join_keys(WindowArgs a, KeyPlan plan, int64_t total,
-                                                 typename V::Storage *dk, typename V::Storage *dv) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x / kWave * 16 + threadIdx.x % 16;
-  const int quarter = threadIdx.x % kWave / 16;
-  const int64_t dims = 2 * a.dim, keys = static_cast<int64_t>(plan.joined) * 32;
-  const int32_t d = static_cast<int32_t>(at % dims);
-  const int32_t key = static_cast<int32_t>(at / dims % keys);
-  const int64_t bh = at / dims / keys;
-  const bool live = at < total && key < a.lk;
-  float sum = 0.0f;
-  if (live) {
-    const float *near = plan.near_sums +
-        ((bh * plan.joined + key / 32) * plan.parts * 32 + key % 32) * dims + d;
-#pragma unroll 4
-    for (int32_t part = quarter; part < plan.parts; part += 4) sum += near[part * 32 * dims];
-    if (key < a.sinks && key / 32 < plan.far_units) {
-      const int32_t parts = plan.far_parts * kWaves;
-      const float *far = plan.far_sums +
-          ((bh * plan.far_units + key / 32) * parts * 32 + key % 32) * dims + d;
+// dk and dv of the joined units, and dq of the blocks that ran in parts, a few
+// rows a workgroup.  Four values a lane, four lanes a sum: each takes every
+// fourth part, and the four are added in one order.
+constexpr int kJoinKeys = 2, kJoinQueries = 8;
+
+__device__ __forceinline__ void add_parts(const float *first, int32_t parts, int64_t stride, v4f &sum) {
 #pragma unroll 8
-      for (int32_t part = quarter; part < parts; part += 4) sum += far[part * 32 * dims];
+  for (int32_t part = threadIdx.x % kWave / 16; part < parts; part += 4) {
+    const v4f x = *reinterpret_cast<const v4f *>(first + part * stride);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] += x[j];
+  }
+}
+template <class V>
+__device__ __forceinline__ void store_joined(v4f sum, float factor, typename V::Storage *to) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    sum[j] += __shfl_xor(sum[j], 16);
+    sum[j] += __shfl_xor(sum[j], 32);
+    sum[j] *= factor;
+  }
+  if (threadIdx.x % kWave >= 16 || to == nullptr) return;
+  if constexpr (sizeof(typename V::Storage) == 2)
+    *reinterpret_cast<v2u *>(to) = v2u{Mfma<V>::pack(sum[0], sum[1]), Mfma<V>::pack(sum[2], sum[3])};
+  else
+    *reinterpret_cast<v4f *>(to) = sum;
+}
+
+template <class V>
+__global__ __launch_bounds__(256) void join_sums(WindowArgs a, KeyPlan keys, QueryPlan queries,
+                                                 int64_t of_keys, typename V::Storage *dq,
+                                                 typename V::Storage *dk, typename V::Storage *dv) {
+  const int first = threadIdx.x / kWave * 16 + threadIdx.x % 16;  // piece of the workgroup's
+  const int32_t pieces = a.dim / 4;
+  if (blockIdx.x < of_keys) {
+    constexpr int kPer = 32 / kJoinKeys;
+    const int32_t unit = static_cast<int32_t>(blockIdx.x / kPer % keys.joined);
+    const int32_t row0 = blockIdx.x % kPer * kJoinKeys;
+    const int64_t bh = blockIdx.x / kPer / keys.joined, b = bh / a.kv_heads;
+    const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads), dims = 2 * a.dim;
+    const float *near = keys.near_sums + (bh * keys.joined + unit) * keys.parts * 32 * dims;
+    const int32_t far_parts = unit < keys.far_units ? keys.far_parts * kWaves : 0;
+    const float *far = keys.far_sums + (bh * keys.far_units + unit) * far_parts * 32 * dims;
+    for (int at = first; at - first % 16 < kJoinKeys * 2 * pieces; at += 64) {
+      const int32_t row = row0 + at / (2 * pieces), d = at % (2 * pieces) * 4, key = unit * 32 + row;
+      v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      typename V::Storage *to = nullptr;
+      if (row < row0 + kJoinKeys && key < a.lk) {
+        add_parts(near + row * dims + d, keys.parts, 32 * dims, sum);
+        if (key < a.sinks) add_parts(far + row * dims + d, far_parts, 32 * dims, sum);
+        const int64_t at_row = ((b * a.lk + key) * a.kv_heads + kvh) * a.dim;
+        to = d < a.dim ? dk + at_row + d : dv + at_row + d - a.dim;
+      }
+      store_joined<V>(sum, d < a.dim ? a.grad_scale : 1.0f, to);
+    }
+  } else {
+    constexpr int kRows = kWaves * 32, kPer = kRows / kJoinQueries;
+    const int64_t id = blockIdx.x - of_keys, rest = id / kPer, block = queries.cut.whole + rest;
+    const int64_t bh = block / queries.per_bh, b = bh / a.kv_heads;
+    const int32_t row0 = static_cast<int32_t>(id % kPer) * kJoinQueries;
+    const int32_t unit = static_cast<int32_t>(block % queries.per_bh) * kWaves + row0 / 32;
+    if (unit >= queries.units) return;
+    const int32_t h = static_cast<int32_t>(bh % a.kv_heads) * a.group + unit % a.group;
+    const int32_t i0 = unit / a.group * 32 + row0 % 32;
+    const float *sums = queries.sums + (rest * queries.cut.parts * kRows + row0) * a.dim;
+    for (int at = first; at - first % 16 < kJoinQueries * pieces; at += 64) {
+      const int32_t row = at / pieces, d = at % pieces * 4;
+      v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      typename V::Storage *to = nullptr;
+      if (row < kJoinQueries && i0 + row < a.lq) {
+        add_parts(sums + row * a.dim + d, queries.cut.parts, static_cast<int64_t>(kRows) * a.dim, sum);
+        to = dq + ((b * a.lq + i0 + row) * a.heads + h) * a.dim + d;
+      }
+      store_joined<V>(sum, a.grad_scale, to);
     }
   }
-  sum += __shfl_xor(sum, 16);
-  sum += __shfl_xor(sum, 32);
-  if (!live || quarter != 0) return;
-  const int64_t row = (bh / a.kv_heads * a.lk + key) * a.kv_heads + bh % a.kv_heads;
-  if (d < a.dim)
-    dk[row * a.dim + d] = V::narrow(sum * a.grad_scale);
-  else
-    dv[row * a.dim + d - a.dim] = V::narrow(sum);
 }
 
-// The cut depends on sizes alone.  One workgroup runs on a CU (two of float32's
-// and the small heads').  With fewer blocks than CUs each is cut until there
-// are about two a CU, of two tiles at least.  The far pass goes by the same
-// number, of four tiles at least.
+// Queries are cut as in the forward pass.
+QueryPlan plan_queries(const WindowArgs &a, int32_t tile) {
+  QueryPlan p{};
+  p.units = (static_cast<int64_t>(a.lq) + 31) / 32 * a.group;
+  p.per_bh = (p.units + kWaves - 1) / kWaves;
+  const int64_t keys = std::min<int64_t>(a.lk, static_cast<int64_t>(a.window) + a.sinks + 32);
+  p.cut = cut_tail(p.per_bh * a.batch * a.kv_heads, 2 * 256, (keys + tile - 1) / tile, tile == 64 ? 6 : 2);
+  return p;
+}
+
+// The cut depends on sizes alone.  With fewer blocks than CUs each is cut until
+// there are about as many, of two tiles at least, and the far pass's units too,
+// of four (twice as many: 74 -> 77 us for 3 x 517 tokens of 6 float32 heads of 64, 94 ->
+// 102 for 2 x 1,000 of 8 bfloat16 heads of 128, in joining them).
 KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
   constexpr int64_t kCus = 256;
   KeyPlan p{};
@@ -658,7 +723,7 @@ KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
   const int64_t span = std::min<int64_t>(a.lq, static_cast<int64_t>(a.window) + kBlockKeys - 1);
   const int64_t work = std::max<int64_t>(1, (span + tile - 1) / tile * a.group / 2);
   p.parts = static_cast<int32_t>(
-      bh * p.blocks >= kCus ? 1 : std::min<int64_t>(work, 2 * kCus / std::max<int64_t>(1, bh * p.blocks)));
+      bh * p.blocks >= kCus ? 1 : std::min<int64_t>(work, kCus / std::max<int64_t>(1, bh * p.blocks)));
   // queries that see sinks from beyond the first block's span
   const int64_t beyond =
       std::min<int64_t>(a.lq, static_cast<int64_t>(a.lk) - kBlockKeys - a.window + 1);
@@ -666,7 +731,7 @@ KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
     p.far_units = (a.sinks + 31) / 32;
     const int64_t steps = std::max<int64_t>(1, (beyond + 127) / 128 * a.group / 4);
     p.far_parts = static_cast<int32_t>(
-        std::min<int64_t>(steps, std::max<int64_t>(1, 2 * kCus / (bh * p.far_units))));
+        std::min<int64_t>(steps, std::max<int64_t>(1, kCus / (bh * p.far_units))));
   }
   p.joined = p.parts > 1 ? (a.lk + 31) / 32 : p.far_units;
   return p;
@@ -675,28 +740,30 @@ KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
 size_t near_floats(const WindowArgs &a, const KeyPlan &p) {
   return static_cast<size_t>(a.batch) * a.kv_heads * p.joined * p.parts * 32 * 2 * a.dim;
 }
+size_t query_floats(const WindowArgs &a, const QueryPlan &p) {
+  return p.cut.parts > 1 ? static_cast<size_t>(p.cut.rest) * p.cut.parts * kWaves * 32 * a.dim : 0;
+}
 size_t far_floats(const WindowArgs &a, const KeyPlan &p) {
   return static_cast<size_t>(a.batch) * a.kv_heads * p.far_units * p.far_parts * kWaves * 32 * 2 * a.dim;
 }
 
 template <class V, int DP>
-msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, void *dk, void *dv,
+msx_status run(const WindowArgs &a, const Upstream &up, const QueryPlan &queries, const KeyPlan &plan, void *dq, void *dk, void *dv,
                hipStream_t stream) {
   using S = typename V::Storage;
-  const int64_t bh = a.batch * a.kv_heads;
-  const int64_t units = (static_cast<int64_t>(a.lq) + 31) / 32 * a.group;
-  const int64_t per_bh = (units + kWaves - 1) / kWaves, q_blocks = per_bh * bh;
+  const int64_t bh = a.batch * a.kv_heads, q_blocks = queries.cut.items();
   const int64_t k_blocks = bh * plan.blocks * plan.parts, f_blocks = bh * plan.far_units * plan.far_parts;
-  const int64_t joined = bh * plan.joined * 32 * 2 * a.dim;
-  for (int64_t blocks : {units, q_blocks, k_blocks, f_blocks, joined / 64})
+  const int64_t of_keys = bh * plan.joined * (32 / kJoinKeys);
+  const int64_t joined = of_keys + queries.cut.rest * (kWaves * 32 / kJoinQueries);
+  for (int64_t blocks : {queries.units, q_blocks, k_blocks, f_blocks, joined})
     if (blocks >= 0x7fffffff)
       return fail(MSX_EINVAL, "window_attention_backward has more rows than a grid holds.");
   if (q_blocks > 0)
     backward_queries<V, DP><<<static_cast<unsigned>(q_blocks), kThreads, 0, stream>>>(
-        a, up, static_cast<int32_t>(units), per_bh, q_blocks, static_cast<S *>(dq));
+        a, up, queries, static_cast<S *>(dq));
   if (k_blocks > 0)
     backward_keys_near<V, DP><<<static_cast<unsigned>(k_blocks), NearShape<V, DP>::kThreads, 0, stream>>>(
-        a, up, plan, k_blocks, static_cast<S *>(dk), static_cast<S *>(dv));
+        a, up, plan, static_cast<uint32_t>(k_blocks), static_cast<S *>(dk), static_cast<S *>(dv));
   if (f_blocks > 0) {
     constexpr int lds = far_buffers<V, DP>() * QueryTile<V, DP, 32 * kWaves, kThreads>::kBytes;
     if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(backward_keys_far<V, DP>),
@@ -704,22 +771,23 @@ msx_status run(const WindowArgs &a, const Upstream &up, KeyPlan plan, void *dq, 
         e != hipSuccess)
       return hip_fail(e, "window_attention_backward");
     backward_keys_far<V, DP><<<static_cast<unsigned>(f_blocks), kThreads, lds, stream>>>(
-        a, up, plan, f_blocks);
+        a, up, plan, static_cast<uint32_t>(f_blocks));
   }
   if (joined > 0)
-    join_keys<V><<<static_cast<unsigned>((joined + 63) / 64), 256, 0, stream>>>(
-        a, plan, joined, static_cast<S *>(dk), static_cast<S *>(dv));
+    join_sums<V><<<static_cast<unsigned>(joined), 256, 0, stream>>>(
+        a, plan, queries, of_keys, static_cast<S *>(dq), static_cast<S *>(dk),
+        static_cast<S *>(dv));
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "window_attention_backward");
 }
 
 template <class V>
-msx_status by_dim(const WindowArgs &a, const Upstream &up, const KeyPlan &plan, void *dq, void *dk,
-                  void *dv, hipStream_t stream) {
-  if (a.dim <= 32) return run<V, 32>(a, up, plan, dq, dk, dv, stream);
-  if (a.dim <= 64) return run<V, 64>(a, up, plan, dq, dk, dv, stream);
-  if (a.dim <= 96) return run<V, 96>(a, up, plan, dq, dk, dv, stream);
-  return run<V, 128>(a, up, plan, dq, dk, dv, stream);
+msx_status by_dim(const WindowArgs &a, const Upstream &up, const QueryPlan &queries, const KeyPlan &plan,
+                  void *dq, void *dk, void *dv, hipStream_t stream) {
+  if (a.dim <= 32) return run<V, 32>(a, up, queries, plan, dq, dk, dv, stream);
+  if (a.dim <= 64) return run<V, 64>(a, up, queries, plan, dq, dk, dv, stream);
+  if (a.dim <= 96) return run<V, 96>(a, up, queries, plan, dq, dk, dv, stream);
+  return run<V, 128>(a, up, queries, plan, dq, dk, dv, stream);
 }
 
 // Queries of a tile of the near pass (BackwardShape::kTokens).
@@ -729,7 +797,8 @@ int32_t tile_of(msx_vtype vt) { return vt == MSX_F32 ? 32 : 64; }
 
 size_t window_backward_scratch(msx_vtype vt, const WindowArgs &a) {
   const KeyPlan p = plan_keys(a, tile_of(vt));
-  return sizeof(float) * (near_floats(a, p) + far_floats(a, p));
+  return sizeof(float) *
+         (near_floats(a, p) + far_floats(a, p) + query_floats(a, plan_queries(a, tile_of(vt))));
 }
 
 msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void *out,
@@ -740,10 +809,12 @@ msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void 
   KeyPlan plan = plan_keys(a, tile_of(vt));
   plan.near_sums = static_cast<float *>(scratch);
   plan.far_sums = plan.near_sums + near_floats(a, plan);
+  QueryPlan queries = plan_queries(a, tile_of(vt));
+  queries.sums = plan.far_sums + far_floats(a, plan);
   switch (vt) {
-  case MSX_F32: return by_dim<F32>(a, up, plan, dq, dk, dv, stream);
-  case MSX_F16: return by_dim<F16>(a, up, plan, dq, dk, dv, stream);
-  default: return by_dim<BF16>(a, up, plan, dq, dk, dv, stream);
+  case MSX_F32: return by_dim<F32>(a, up, queries, plan, dq, dk, dv, stream);
+  case MSX_F16: return by_dim<F16>(a, up, queries, plan, dq, dk, dv, stream);
+  default: return by_dim<BF16>(a, up, queries, plan, dq, dk, dv, stream);
   }
 }
 

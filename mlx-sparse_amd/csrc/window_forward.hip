@@ -96,8 +96,8 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   const int lane = threadIdx.x % kWave, half = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const CutItem item(cut, blockIdx.x);
-  const int64_t bh = item.block / blocks_per_bh;
-  const int32_t first_unit = static_cast<int32_t>(item.block % blocks_per_bh) * kWaves;
+  const uint32_t per_bh = static_cast<uint32_t>(blocks_per_bh), bh = item.block / per_bh;
+  const int32_t first_unit = static_cast<int32_t>(item.block % per_bh) * kWaves;
   const int64_t b = bh / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads);
   const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
@@ -230,8 +230,7 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   };
 
   const int32_t tiles = (count + F::kKeys - 1) / F::kKeys;
-  const int32_t c_begin = static_cast<int32_t>(static_cast<int64_t>(tiles) * item.part / item.parts) * F::kKeys;
-  const int32_t c_end = static_cast<int32_t>(static_cast<int64_t>(tiles) * (item.part + 1) / item.parts) * F::kKeys;
+  const int32_t c_begin = item.first(tiles) * F::kKeys, c_end = item.first(tiles, 1) * F::kKeys;
   fetch(k_base, a.ks[1], k_rows, c_begin, k_tile(0));
   fetch(v_base, a.vs[1], v_rows, c_begin, v_tile(0));
   sync_tiles();
@@ -306,52 +305,72 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   }
 }
 
-// A wave a query row of the blocks that ran in parts.
+// The blocks that ran in parts: four values of a row a lane.
+template <class V, int DP>
+struct JoinShape {
+  static constexpr int kLanes = DP <= 32 ? 8 : DP <= 64 ? 16 : 32;  // of a row
+  static constexpr int kRows = kThreads / kLanes;                   // of a workgroup
+};
 template <class V, int DP>
 __global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t units_per_bh,
                                                          int64_t blocks_per_bh, TailCut cut,
                                                          const float *sums,
                                                          typename V::Storage *out, float *lse) {
-  constexpr int kStride = ForwardShape<V, DP>::kStride;
+  using J = JoinShape<V, DP>;
+  constexpr int kStride = ForwardShape<V, DP>::kStride, kPerBlock = kWaves * kRows / J::kRows;
+  constexpr int64_t kPart = static_cast<int64_t>(kWaves) * kRows * kStride;
   __shared__ float q_lds[kWaves][DP];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + wave;  // (block, wave, row)
-  const int64_t rest = at / (kWaves * kRows), block = cut.whole + rest, bh = block / blocks_per_bh;
-  const int32_t in_block = static_cast<int32_t>(at % (kWaves * kRows));
-  const int64_t unit = block % blocks_per_bh * kWaves + in_block / kRows;
+  const int64_t rest = blockIdx.x / kPerBlock, block = cut.whole + rest, bh = block / blocks_per_bh;
+  const int32_t in_block = static_cast<int32_t>(blockIdx.x % kPerBlock) * J::kRows + threadIdx.x / J::kLanes;
+  const int32_t unit = static_cast<int32_t>(block % blocks_per_bh) * kWaves + in_block / kRows;
   const int64_t b = bh / a.kv_heads;
-  const int32_t i = static_cast<int32_t>(unit / a.group) * kRows + in_block % kRows;
-  if (rest >= cut.rest || unit >= units_per_bh || i >= a.lq) return;
-  const int32_t h = static_cast<int32_t>(bh % a.kv_heads) * a.group + static_cast<int32_t>(unit % a.group);
-  const int32_t p = i + a.lk - a.lq;
-  const float *first = sums + (rest * cut.parts * kWaves * kRows + in_block) * kStride;
-  constexpr int64_t part_stride = static_cast<int64_t>(kWaves) * kRows * kStride;
-  float m = -INFINITY, l = 0.0f, o[(DP + kWave - 1) / kWave] = {};
-  for (int32_t part = 0; part < cut.parts; ++part) m = fmaxf(m, first[part * part_stride + DP]);
-  const float base = m == -INFINITY ? 0.0f : m;
-  for (int32_t part = 0; part < cut.parts; ++part) {
-    const float *from = first + part * part_stride;
-    const float f = exp2_fast(from[DP] - base);
-    l += from[DP + 1] * f;
-#pragma unroll
-    for (int r = 0; r < (DP + kWave - 1) / kWave; ++r)
-      if (lane + kWave * r < DP) o[r] += from[lane + kWave * r] * f;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int32_t i = unit / a.group * kRows + in_block % kRows;
+  const int32_t h = static_cast<int32_t>(bh % a.kv_heads) * a.group + unit % a.group;
+  const int32_t p = i + a.lk - a.lq, d = threadIdx.x % J::kLanes * 4;
+  const bool live = unit < units_per_bh && i < a.lq;
   bool odd = false;
+  if (live) {
+    const float *first = sums + rest * cut.parts * kPart + in_block * kStride;
+    float m = -INFINITY, l = 0.0f;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int32_t part = 0; part < cut.parts; ++part) m = fmaxf(m, first[part * kPart + DP]);
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+    for (int32_t part = 0; part < cut.parts; ++part) {
+      const float *from = first + part * kPart;
+      const float f = exp2_fast(from[DP] - base);
+      l += from[DP + 1] * f;
+      const v4f x = *reinterpret_cast<const v4f *>(from + min(d, DP - 4));
 #pragma unroll
-  for (int r = 0; r < (DP + kWave - 1) / kWave; ++r) {
-    const int d = lane + kWave * r;
-    if (d >= a.dim) continue;
-    odd = odd || !(fabsf(o[r] * inv) < INFINITY);
-    out[((b * a.lq + i) * a.heads + h) * a.dim + d] = V::narrow(o[r] * inv);
+      for (int j = 0; j < 4; ++j) o[j] += x[j] * f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[j] *= inv;
+      odd = odd || (d < a.dim && !(fabsf(o[j]) < INFINITY));
+    }
+    if (d < a.dim) {
+      auto *to = out + ((b * a.lq + i) * a.heads + h) * a.dim + d;
+      if constexpr (sizeof(typename V::Storage) == 2)
+        *reinterpret_cast<v2u *>(to) = v2u{Mfma<V>::pack(o[0], o[1]), Mfma<V>::pack(o[2], o[3])};
+      else
+        *reinterpret_cast<v4f *>(to) = o;
+    }
+    if (lse != nullptr && d == 0)
+      lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
   }
-  if (lse != nullptr && lane == 0)
-    lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
-  if (__any(odd) && p >= 0 && p < a.length(b)) forward_row<V>(a, b, i, h, p, q_lds[wave], out);
+  uint64_t anew = __ballot(odd && p >= 0 && p < a.length(b));
+  while (anew != 0) {
+    const int row = __builtin_ctzll(anew) / J::kLanes;  // of the wave's
+    anew &= ~(((uint64_t{1} << J::kLanes) - 1) << (row * J::kLanes));
+    const int at = row * J::kLanes;
+    forward_row<V>(a, b, __shfl(i, at), __shfl(h, at), __shfl(p, at), q_lds[threadIdx.x / kWave], out);
+  }
 }
 
-// Blocks of queries and how they are cut: into parts of eight tiles at least.
+// Blocks of queries and how they are cut.
 struct Grid {
   int64_t units, per_bh;
   TailCut cut;
@@ -364,7 +383,8 @@ Grid grid_of(const WindowArgs &a) {
   g.units = (static_cast<int64_t>(a.lq) + kRows - 1) / kRows * a.group;
   g.per_bh = (g.units + kWaves - 1) / kWaves;
   const int64_t keys = std::min<int64_t>(a.lk, static_cast<int64_t>(a.window) + a.sinks + kRows);
-  g.cut = cut_tail(g.per_bh * a.batch * a.kv_heads, 256 * F::kBlocks, keys / (8 * F::kKeys));
+  g.cut = cut_tail(g.per_bh * a.batch * a.kv_heads, 256 * F::kBlocks, (keys + F::kKeys - 1) / F::kKeys,
+                   F::T::kSize == 2 ? 6 : 2);
   return g;
 }
 
@@ -383,7 +403,7 @@ msx_status run(const WindowArgs &a, void *out, float *lse, float *sums, size_t *
   forward_tiles<V, DP><<<static_cast<unsigned>(g.cut.items()), kThreads, 0, stream>>>(
       a, static_cast<int32_t>(g.units), g.per_bh, g.cut, to, lse, sums);
   if (rows > 0)
-    forward_join<V, DP><<<static_cast<unsigned>(rows / kWaves), kThreads, 0, stream>>>(
+    forward_join<V, DP><<<static_cast<unsigned>(rows / JoinShape<V, DP>::kRows), kThreads, 0, stream>>>(
         a, static_cast<int32_t>(g.units), g.per_bh, g.cut, sums, to, lse);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "window_attention");
