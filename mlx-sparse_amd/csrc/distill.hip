@@ -6,8 +6,15 @@
 //   loss = T^2 sum_r p_r (ln p_r - ln q_r),  ln q_r = z_r - lse
 //   grad = weight T (q - p)
 // One workgroup a row: a pass over the row for its maximum and the sum of
-// exponentials, and for the gradient a second one.  The columns of kept logits
-// are written last, each by the thread that holds it, q - p rounded once.
+// exponentials, and for the gradient a second one, over what the first kept in
+// registers.  The columns of kept logits are written last, each by the thread
+// that holds it, q - p rounded once.
+//
+// Memory bounds it: the logits read and the gradient written once, 2.1 GB for
+// 4,096 rows of 131,072 bfloat16, take 425 us (5.05 TB/s, what a copy reaches;
+// 470 with the row read twice); 2,000 rows of 50,257 take 68 us (90), 65 of
+// 1,009 float32 5.6.  The loss alone reads 2,049 rows of 50,001 float16 in 40 us
+// (5.1 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -155,8 +162,9 @@ __device__ inline void store_piece(v4u piece, S *to) {
 
 // kLoss: losses (and lse where asked); kGrad: the gradient, from `lse_in` or
 // from the row's own pass.
-template <class V, bool kLoss, bool kGrad, int kThreads>
-__global__ __launch_bounds__(kThreads, 8) void distill_rows(DistillArgs a, float *losses, float *lse,
+// kHold: pieces a thread keeps in registers between the two passes.
+template <class V, bool kLoss, bool kGrad, int kThreads, int kHold>
+__global__ __launch_bounds__(kThreads, kHold > 0 ? 4 : 8) void distill_rows(DistillArgs a, float *losses, float *lse,
                                                          const float *lse_in,
                                                          typename V::Storage *grad) {
   using S = typename V::Storage;
@@ -195,8 +203,23 @@ __global__ __launch_bounds__(kThreads, 8) void distill_rows(DistillArgs a, float
   const v4u *pieces = reinterpret_cast<const v4u *>(z + r.head);
   const int64_t single = r.single();
   Stat s{-INFINITY, 0.0f};
+  v4u held[kHold > 0 ? kHold : 1];
   if (kLoss && begin < end) {
     int64_t c = threadIdx.x;
+    if constexpr (kHold > 0) {
+      if (r.pieces > 0) {
+#pragma unroll
+        for (int k = 0; k < kHold; ++k) held[k] = pieces[c + k * kThreads < r.pieces ? c + k * kThreads : r.pieces - 1];
+      }
+#pragma unroll
+      for (int k = 0; k < kHold; ++k)
+        if (c + k * kThreads < r.pieces) {
+          float x[kPer];
+          Row::widen(held[k], a.scale, x);
+          s.add<kPer>(x);
+        }
+      c += kHold * kThreads;
+    }
     for (; c + (kAhead - 1) * kThreads < r.pieces; c += kAhead * kThreads) {
       v4u w[kAhead];
 #pragma unroll
@@ -254,6 +277,14 @@ __global__ __launch_bounds__(kThreads, 8) void distill_rows(DistillArgs a, float
     if (wanted) {
       const float factor = weight * a.temperature;
       int64_t c = threadIdx.x;
+      if constexpr (kHold > 0) {
+#pragma unroll
+        for (int k = 0; k < kHold; ++k)
+          if (c + k * kThreads < r.pieces)
+            store_piece(softmax_piece<V>(held[k], a.scale, total, factor),
+                        g + r.head + (c + k * kThreads) * kPer);
+        c += kHold * kThreads;
+      }
       for (; c + (kAhead - 1) * kThreads < r.pieces; c += kAhead * kThreads) {
         v4u w[kAhead];
 #pragma unroll
@@ -318,10 +349,6 @@ DistillArgs args_of(const msx_distill_desc &d, int64_t ld_grad) {
   return a;
 }
 
-// Row sizes up to which a row has a wave, and four.
-constexpr int64_t kWaveRow = 4 << 10;
-constexpr int64_t kQuarterRow = 64 << 10;
-
 template <bool kLoss, bool kGrad>
 msx_status launch(const msx_distill_desc &d, float *losses, float *lse, const float *lse_in,
                   void *grad, int64_t ld_grad, void *stream) {
@@ -332,13 +359,30 @@ msx_status launch(const msx_distill_desc &d, float *losses, float *lse, const fl
     const auto blocks = static_cast<unsigned>(d.n_rows);
     const auto st = static_cast<hipStream_t>(stream);
     S *g = static_cast<S *>(grad);
-    const int64_t bytes = d.n_cols * static_cast<int64_t>(sizeof(S));
-    if (bytes <= kWaveRow)
-      distill_rows<V, kLoss, kGrad, 64><<<blocks, 64, 0, st>>>(a, losses, lse, lse_in, g);
-    else if (bytes <= kQuarterRow)
-      distill_rows<V, kLoss, kGrad, 256><<<blocks, 256, 0, st>>>(a, losses, lse, lse_in, g);
-    else
-      distill_rows<V, kLoss, kGrad, 1024><<<blocks, 1024, 0, st>>>(a, losses, lse, lse_in, g);
+    const int64_t kb = (d.n_cols * static_cast<int64_t>(sizeof(S)) + 1023) / 1024;
+    const auto with = [&](auto kernel, unsigned threads) {
+      kernel<<<blocks, threads, 0, st>>>(a, losses, lse, lse_in, g);
+    };
+    if constexpr (kLoss && kGrad) {
+      // 256 bytes of the row a thread, in its registers, so that it is read
+      // once; what is beyond 256 KB is read twice
+      if (kb <= 4) with(distill_rows<V, true, true, 64, 4>, 64);
+      else if (kb <= 16) with(distill_rows<V, true, true, 64, 16>, 64);
+      else if (kb <= 32) with(distill_rows<V, true, true, 128, 16>, 128);
+      else if (kb <= 64) with(distill_rows<V, true, true, 256, 16>, 256);
+      else if (kb <= 128) with(distill_rows<V, true, true, 512, 16>, 512);
+      else with(distill_rows<V, true, true, 1024, 16>, 1024);
+    } else if constexpr (kLoss) {
+      // small enough workgroups that one's start and end run beside others'
+      // passes (2,049 rows of 50,001 float16: 58 us with 1024, 40 with 512)
+      if (kb <= 4) with(distill_rows<V, true, false, 64, 0>, 64);
+      else if (kb <= 64) with(distill_rows<V, true, false, 256, 0>, 256);
+      else with(distill_rows<V, true, false, 512, 0>, 512);
+    } else {
+      if (kb <= 4) with(distill_rows<V, false, true, 64, 0>, 64);
+      else if (kb <= 64) with(distill_rows<V, false, true, 256, 0>, 256);
+      else with(distill_rows<V, false, true, 1024, 0>, 1024);
+    }
   };
   switch (d.vtype) {
   case MSX_F32: run(F32{}); break;
