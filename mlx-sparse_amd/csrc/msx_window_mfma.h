@@ -339,7 +339,8 @@ struct TailCut {
 };
 
 // Costs in tiles, of which a block has `tiles`: a part more for its start and
-// its sums, `join` for the launch that joins them; a part has two at least.
+// its sums, `join` for the launch that joins one part a slot (5 to 8 us, by tiles
+// of 1 to 3 us); a part has two at least.
 inline TailCut cut_tail(int64_t blocks, int64_t slots, int64_t tiles, double join) {
   constexpr double kPart = 0.75;
   const int64_t rest = blocks % slots;
@@ -347,7 +348,8 @@ inline TailCut cut_tail(int64_t blocks, int64_t slots, int64_t tiles, double joi
   double best = static_cast<double>(tiles);
   for (int64_t p = 2; 2 * p <= tiles && p <= 16 && rest > 0; ++p) {
     const double rounds = static_cast<double>((rest * p + slots - 1) / slots);
-    const double cost = rounds * (static_cast<double>((tiles + p - 1) / p) + kPart) + join;
+    const double cost = rounds * (static_cast<double>((tiles + p - 1) / p) + kPart) +
+                        join * (0.5 + 0.5 * static_cast<double>(rest * p) / slots);
     if (cost < best) {
       best = cost;
       cut = TailCut{blocks - rest, rest, static_cast<int32_t>(p)};

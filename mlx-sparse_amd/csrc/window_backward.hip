@@ -391,13 +391,14 @@ struct QueryTile {
   }
 };
 
-// How the keys' work is cut: blocks of kBlockKeys keys, each in `parts`; and
-// the far units, 32 sink keys each, in `far_parts`.
+// How the keys' work is cut: blocks of kBlockKeys keys as in the forward pass,
+// and the far units, 32 sink keys each, in `far_parts`.  The sums of blocks in
+// parts and those of far units go through scratch.
 struct KeyPlan {
-  int32_t blocks, parts;
-  int32_t joined;  // 32-key units whose sums go through scratch, from the first on
+  int32_t blocks;  // of a key-value head
+  TailCut cut;
   int32_t far_units, far_parts;
-  float *near_sums, *far_sums;
+  float *part_sums, *unit_sums, *far_sums;  // parts, far units of whole blocks, the far pass
 };
 
 // Queries within reach of a block's window: positions first .. last; the rest
@@ -428,8 +429,8 @@ struct NearShape {
 
 template <class V, int DP>
 __global__ __launch_bounds__((NearShape<V, DP>::kThreads), (NearShape<V, DP>::kGroups)) void
-backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, uint32_t blocks,
-                   typename V::Storage *dk, typename V::Storage *dv) {
+backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, typename V::Storage *dk,
+                   typename V::Storage *dv) {
   using S = typename V::Storage;
   using N = NearShape<V, DP>;
   using T = TileShape<V, DP>;
@@ -441,10 +442,9 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, uint32_t blocks,
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int keys_of = wave % kWaves, group = wave / kWaves;
-  const uint32_t id = xcd_order(blockIdx.x, blocks);
-  const int32_t part = static_cast<int32_t>(id % plan.parts);
-  const int32_t block = static_cast<int32_t>(id / plan.parts % plan.blocks);
-  const uint32_t head = id / plan.parts / plan.blocks;
+  const CutItem item(plan.cut, blockIdx.x);
+  const int32_t block = static_cast<int32_t>(item.block % plan.blocks);
+  const uint32_t head = item.block / plan.blocks;
   const int64_t bh = head, b = head / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(head % a.kv_heads);
   const int32_t n = __builtin_amdgcn_readfirstlane(a.length(b)), offset = a.lk - a.lq;
@@ -475,8 +475,8 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, uint32_t blocks,
   const int32_t first = max(block * kBlockKeys, offset), last = near_last(a, block, n);
   const int32_t tiles = last >= first ? (last - first) / kTokens + 1 : 0;
   const int64_t total = static_cast<int64_t>(tiles) * a.group;
-  const int32_t begin = plan.parts == 1 ? 0 : static_cast<int32_t>(total * part / plan.parts);
-  const int32_t end = static_cast<int32_t>(plan.parts == 1 ? total : total * (part + 1) / plan.parts);
+  const int32_t begin = static_cast<int32_t>(item.parts == 1 ? 0 : total * item.part / item.parts);
+  const int32_t end = static_cast<int32_t>(item.parts == 1 ? total : total * (item.part + 1) / item.parts);
 
   Tile next;
   next.start(a, up);
@@ -539,9 +539,9 @@ backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, uint32_t blocks,
 
   if (key >= a.lk) return;
   const int32_t unit = block * kWaves + keys_of;
-  if (unit < plan.joined) {
-    const int64_t slot = ((bh * plan.joined + unit) * plan.parts + part) * 32 + lane % 32;
-    float *to = plan.near_sums + slot * 2 * a.dim;
+  if (item.slot >= 0 || unit < plan.far_units) {
+    const int64_t slot = item.slot >= 0 ? item.slot * kWaves + keys_of : bh * plan.far_units + unit;
+    float *to = (item.slot >= 0 ? plan.part_sums : plan.unit_sums) + (slot * 32 + lane % 32) * 2 * a.dim;
     store_sums<DP>(keys.dk, a.dim, to);
     store_sums<DP>(keys.dv, a.dim, to + a.dim);
   } else {
@@ -658,20 +658,37 @@ __global__ __launch_bounds__(256) void join_sums(WindowArgs a, KeyPlan keys, Que
   const int first = threadIdx.x / kWave * 16 + threadIdx.x % 16;  // piece of the workgroup's
   const int32_t pieces = a.dim / 4;
   if (blockIdx.x < of_keys) {
-    constexpr int kPer = 32 / kJoinKeys;
-    const int32_t unit = static_cast<int32_t>(blockIdx.x / kPer % keys.joined);
-    const int32_t row0 = blockIdx.x % kPer * kJoinKeys;
-    const int64_t bh = blockIdx.x / kPer / keys.joined, b = bh / a.kv_heads;
-    const int32_t kvh = static_cast<int32_t>(bh % a.kv_heads), dims = 2 * a.dim;
-    const float *near = keys.near_sums + (bh * keys.joined + unit) * keys.parts * 32 * dims;
+    // rows of the blocks in parts, then of the other far units
+    constexpr int kPer = kBlockKeys / kJoinKeys, kPerUnit = 32 / kJoinKeys;
+    const uint32_t cut = static_cast<uint32_t>(keys.cut.rest) * kPer, whole = static_cast<uint32_t>(keys.cut.whole);
+    const bool in_parts = blockIdx.x < cut;
+    const uint32_t id = in_parts ? blockIdx.x : blockIdx.x - cut, rest = id / kPer;
+    uint32_t head;
+    int32_t unit, row0;
+    if (in_parts) {
+      head = (whole + rest) / keys.blocks;
+      row0 = static_cast<int32_t>(id % kPer * kJoinKeys);
+      unit = static_cast<int32_t>((whole + rest) % keys.blocks) * kWaves + row0 / 32;
+    } else {
+      head = id / kPerUnit / keys.far_units;
+      row0 = static_cast<int32_t>(id % kPerUnit * kJoinKeys);
+      unit = static_cast<int32_t>(id / kPerUnit % keys.far_units);
+      if (head * keys.blocks + unit / kWaves >= whole) return;
+    }
+    const int64_t bh = head, b = head / a.kv_heads;
+    const int32_t kvh = static_cast<int32_t>(head % a.kv_heads), dims = 2 * a.dim;
+    const int32_t near_parts = in_parts ? keys.cut.parts : 1, stride = (in_parts ? kBlockKeys : 32) * dims;
+    const float *near = in_parts ? keys.part_sums + static_cast<int64_t>(rest) * near_parts * stride + row0 / 32 * 32 * dims
+                                 : keys.unit_sums + (bh * keys.far_units + unit) * stride;
     const int32_t far_parts = unit < keys.far_units ? keys.far_parts * kWaves : 0;
     const float *far = keys.far_sums + (bh * keys.far_units + unit) * far_parts * 32 * dims;
+    row0 %= 32;
     for (int at = first; at - first % 16 < kJoinKeys * 2 * pieces; at += 64) {
       const int32_t row = row0 + at / (2 * pieces), d = at % (2 * pieces) * 4, key = unit * 32 + row;
       v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
       typename V::Storage *to = nullptr;
       if (row < row0 + kJoinKeys && key < a.lk) {
-        add_parts(near + row * dims + d, keys.parts, 32 * dims, sum);
+        add_parts(near + row * dims + d, near_parts, stride, sum);
         if (key < a.sinks) add_parts(far + row * dims + d, far_parts, 32 * dims, sum);
         const int64_t at_row = ((b * a.lk + key) * a.kv_heads + kvh) * a.dim;
         to = d < a.dim ? dk + at_row + d : dv + at_row + d - a.dim;
@@ -711,19 +728,15 @@ QueryPlan plan_queries(const WindowArgs &a, int32_t tile) {
   return p;
 }
 
-// The cut depends on sizes alone.  With fewer blocks than CUs each is cut until
-// there are about as many, of two tiles at least, and the far pass's units too,
-// of four (twice as many: 74 -> 77 us for 3 x 517 tokens of 6 float32 heads of 64, 94 ->
-// 102 for 2 x 1,000 of 8 bfloat16 heads of 128, in joining them).
+// The far pass's units are cut until there are about as many as CUs, of four
+// tiles at least (two a CU lose 12 us of 665 in joining them, for 16,384 tokens).
 KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
   constexpr int64_t kCus = 256;
   KeyPlan p{};
   const int64_t bh = a.batch * a.kv_heads;
   p.blocks = (a.lk + kBlockKeys - 1) / kBlockKeys;
   const int64_t span = std::min<int64_t>(a.lq, static_cast<int64_t>(a.window) + kBlockKeys - 1);
-  const int64_t work = std::max<int64_t>(1, (span + tile - 1) / tile * a.group / 2);
-  p.parts = static_cast<int32_t>(
-      bh * p.blocks >= kCus ? 1 : std::min<int64_t>(work, kCus / std::max<int64_t>(1, bh * p.blocks)));
+  p.cut = cut_tail(bh * p.blocks, kCus, (span + tile - 1) / tile * a.group, tile == 64 ? 6 : 2);
   // queries that see sinks from beyond the first block's span
   const int64_t beyond =
       std::min<int64_t>(a.lq, static_cast<int64_t>(a.lk) - kBlockKeys - a.window + 1);
@@ -731,14 +744,16 @@ KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
     p.far_units = (a.sinks + 31) / 32;
     const int64_t steps = std::max<int64_t>(1, (beyond + 127) / 128 * a.group / 4);
     p.far_parts = static_cast<int32_t>(
-        std::min<int64_t>(steps, std::max<int64_t>(1, kCus / (bh * p.far_units))));
+        std::min<int64_t>(steps, std::max<int64_t>(1, kCus / std::max<int64_t>(1, bh * p.far_units))));
   }
-  p.joined = p.parts > 1 ? (a.lk + 31) / 32 : p.far_units;
   return p;
 }
 
-size_t near_floats(const WindowArgs &a, const KeyPlan &p) {
-  return static_cast<size_t>(a.batch) * a.kv_heads * p.joined * p.parts * 32 * 2 * a.dim;
+size_t part_floats(const WindowArgs &a, const KeyPlan &p) {
+  return p.cut.parts > 1 ? static_cast<size_t>(p.cut.rest) * p.cut.parts * kBlockKeys * 2 * a.dim : 0;
+}
+size_t unit_floats(const WindowArgs &a, const KeyPlan &p) {
+  return static_cast<size_t>(a.batch) * a.kv_heads * p.far_units * 32 * 2 * a.dim;
 }
 size_t query_floats(const WindowArgs &a, const QueryPlan &p) {
   return p.cut.parts > 1 ? static_cast<size_t>(p.cut.rest) * p.cut.parts * kWaves * 32 * a.dim : 0;
@@ -748,12 +763,13 @@ size_t far_floats(const WindowArgs &a, const KeyPlan &p) {
 }
 
 template <class V, int DP>
-msx_status run(const WindowArgs &a, const Upstream &up, const QueryPlan &queries, const KeyPlan &plan, void *dq, void *dk, void *dv,
-               hipStream_t stream) {
+msx_status run(const WindowArgs &a, const Upstream &up, const QueryPlan &queries, const KeyPlan &plan,
+               void *dq, void *dk, void *dv, hipStream_t stream) {
   using S = typename V::Storage;
   const int64_t bh = a.batch * a.kv_heads, q_blocks = queries.cut.items();
-  const int64_t k_blocks = bh * plan.blocks * plan.parts, f_blocks = bh * plan.far_units * plan.far_parts;
-  const int64_t of_keys = bh * plan.joined * (32 / kJoinKeys);
+  const int64_t k_blocks = plan.cut.items(), f_blocks = bh * plan.far_units * plan.far_parts;
+  const int64_t of_keys =
+      plan.cut.rest * (kBlockKeys / kJoinKeys) + bh * plan.far_units * (32 / kJoinKeys);
   const int64_t joined = of_keys + queries.cut.rest * (kWaves * 32 / kJoinQueries);
   for (int64_t blocks : {queries.units, q_blocks, k_blocks, f_blocks, joined})
     if (blocks >= 0x7fffffff)
@@ -763,7 +779,7 @@ msx_status run(const WindowArgs &a, const Upstream &up, const QueryPlan &queries
         a, up, queries, static_cast<S *>(dq));
   if (k_blocks > 0)
     backward_keys_near<V, DP><<<static_cast<unsigned>(k_blocks), NearShape<V, DP>::kThreads, 0, stream>>>(
-        a, up, plan, static_cast<uint32_t>(k_blocks), static_cast<S *>(dk), static_cast<S *>(dv));
+        a, up, plan, static_cast<S *>(dk), static_cast<S *>(dv));
   if (f_blocks > 0) {
     constexpr int lds = far_buffers<V, DP>() * QueryTile<V, DP, 32 * kWaves, kThreads>::kBytes;
     if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(backward_keys_far<V, DP>),
@@ -798,7 +814,8 @@ int32_t tile_of(msx_vtype vt) { return vt == MSX_F32 ? 32 : 64; }
 size_t window_backward_scratch(msx_vtype vt, const WindowArgs &a) {
   const KeyPlan p = plan_keys(a, tile_of(vt));
   return sizeof(float) *
-         (near_floats(a, p) + far_floats(a, p) + query_floats(a, plan_queries(a, tile_of(vt))));
+         (part_floats(a, p) + unit_floats(a, p) + far_floats(a, p) +
+          query_floats(a, plan_queries(a, tile_of(vt))));
 }
 
 msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void *out,
@@ -807,8 +824,9 @@ msx_status launch_window_backward(msx_vtype vt, const WindowArgs &a, const void 
                                   hipStream_t stream) {
   Upstream up{grad, {grad_strides[0], grad_strides[1], grad_strides[2]}, out, lse, delta};
   KeyPlan plan = plan_keys(a, tile_of(vt));
-  plan.near_sums = static_cast<float *>(scratch);
-  plan.far_sums = plan.near_sums + near_floats(a, plan);
+  plan.part_sums = static_cast<float *>(scratch);
+  plan.unit_sums = plan.part_sums + part_floats(a, plan);
+  plan.far_sums = plan.unit_sums + unit_floats(a, plan);
   QueryPlan queries = plan_queries(a, tile_of(vt));
   queries.sums = plan.far_sums + far_floats(a, plan);
   switch (vt) {

@@ -135,6 +135,18 @@ def test_few_queries_over_long_windows(gpu, dtype, lq, window, sinks, heads, kv_
         assert torch.isfinite(out[0, :-1]).all() and torch.isnan(out[0, -1]).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch,lq,heads,kv_heads,dim,window,sinks", [
+    (5, 1000, 8, 8, 32, 300, 40), (1, 2111, 4, 2, 64, 900, 3), (9, 300, 16, 16, 128, 250, 0)])
+def test_uneven_rounds(gpu, dtype, batch, lq, heads, kv_heads, dim, window, sinks):
+    """Blocks beyond whole rounds of the chip: those are cut, with sinks in
+    them and in whole blocks, and lengths that leave parts empty."""
+    q, k, v, g = operands(lq, batch, lq, lq, heads, kv_heads, dim, dtype, "cuda")
+    lengths = torch.tensor([(lq - 100 * b) % (lq + 1) for b in range(batch)], device="cuda")
+    forward_and_gradients(gpu, q, k, v, g, f"{batch} x {lq}", window=window, sinks=sinks,
+                          lengths=lengths)
+
+
 def test_rows_repeat(gpu):
     """The same inputs give the same bits, gradients among them."""
     q, k, v, g = operands(9, 2, 700, 700, 8, 2, 128, BF16, "cuda")
