@@ -188,7 +188,6 @@ backward_queries(WindowArgs a, Upstream up, QueryPlan plan, typename V::Storage 
       gf[s] = __builtin_bit_cast(Frag, gw);
     }
     delta += other_half(delta);
-    if (live && i < a.lq && half == 0 && item.part == 0) up.delta[(b * a.heads + h) * a.lq + i] = delta;
   }
 
   RowLoader<V, DP, F::kTokens, kThreads> k_rows, v_rows;
@@ -210,30 +209,74 @@ backward_queries(WindowArgs a, Upstream up, QueryPlan plan, typename V::Storage 
   zero<DP>(acc);
   const int32_t tiles = (count + F::kTokens - 1) / F::kTokens;
   const int32_t c_begin = item.first(tiles) * F::kTokens, c_end = item.first(tiles, 1) * F::kTokens;
-  fetch(k_base, a.ks[1], k_rows, c_begin, k_tile(0));
-  fetch(v_base, a.vs[1], v_rows, c_begin, v_tile(0));
-  sync_tiles();
+  // whether the wave sees any key of the tile at c0, and whether all of its
+  // queries see all of them
+  const auto sees = [&](int32_t c0, bool &whole) {
+    const int32_t first = max(c0, far) + skip, last = min(c0 + F::kTokens, count) - 1 + skip;
+    whole = c0 + F::kTokens <= count && last <= p_first &&
+            (p_last - first < a.window || last < a.sinks) && p_last - p_first == 31;
+    return p_last >= p_first &&
+           (c0 < far || (first <= p_last && (p_first - last < a.window || first < a.sinks)));
+  };
+  const auto products = [&](int parity, int t, v16f &s, v16f &dp) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      s = Mfma<V>::mul(read_rows<V>(lanes, k_tile(parity), 32 * t, st), qf[st], s);
+      dp = Mfma<V>::mul(read_rows<V>(lanes, v_tile(parity), 32 * t, st), gf[st], dp);
+    }
+  };
+  // delta so far is of outputs rounded to 16 bits, whose errors a sum over few
+  // keys does not even out: a query that sees one key alone would get 2^-9 of
+  // its dP where the gradient is zero.  A span of one or two tiles is in LDS
+  // as a whole, and delta the sum of P dP over it.
+  int32_t held = -1;  // the tile in the first buffer
+  if (T::kSize == 2 && count <= 2 * F::kTokens) {
+    held = 0;
+    fetch(k_base, a.ks[1], k_rows, 0, k_tile(0));
+    fetch(v_base, a.vs[1], v_rows, 0, v_tile(0));
+    if (count > F::kTokens) {
+      fetch(k_base, a.ks[1], k_rows, F::kTokens, k_tile(1));
+      fetch(v_base, a.vs[1], v_rows, F::kTokens, v_tile(1));
+    }
+    sync_tiles();
+    delta = 0.0f;
+#pragma unroll 1
+    for (int at = 0; at * F::kTokens < count; ++at) {
+      bool whole;
+      if (!sees(at * F::kTokens, whole)) continue;
+#pragma unroll 1
+      for (int t = 0; t < F::kSub; ++t) {
+        v16f s, dp;
+        products(at, t, s, dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int32_t c = at * F::kTokens + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
+          delta += number.seen(p, c) ? exp2_fast(s[r] * a.scale - lse) * dp[r] : 0.0f;
+        }
+      }
+    }
+    delta += other_half(delta);
+    sync_tiles();
+  }
+  if (held != c_begin) {
+    fetch(k_base, a.ks[1], k_rows, c_begin, k_tile(0));
+    fetch(v_base, a.vs[1], v_rows, c_begin, v_tile(0));
+    sync_tiles();
+  }
+  if (live && i < a.lq && half == 0 && item.part == 0) up.delta[(b * a.heads + h) * a.lq + i] = delta;
   const auto tile = [&](int32_t c0, int parity) __attribute__((always_inline)) {
     if (c0 + F::kTokens < c_end) {  // into the other tiles, which all waves are past
       fetch(k_base, a.ks[1], k_rows, c0 + F::kTokens, k_tile(parity ^ 1));
       fetch(v_base, a.vs[1], v_rows, c0 + F::kTokens, v_tile(parity ^ 1));
     }
-    const int32_t k_first = max(c0, far) + skip, k_last = min(c0 + F::kTokens, count) - 1 + skip;
-    const bool any = p_last >= p_first &&
-                     (c0 < far || (k_first <= p_last && (p_first - k_last < a.window || k_first < a.sinks)));
-    if (any) {
-      const bool whole = c0 + F::kTokens <= count && k_last <= p_first &&
-                         (p_last - k_first < a.window || k_last < a.sinks) && p_last - p_first == 31;
+    bool whole;
+    if (sees(c0, whole)) {
 #pragma unroll
       for (int t = 0; t < F::kSub; ++t) {
         v16f s, dp;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          s = Mfma<V>::mul(read_rows<V>(lanes, k_tile(parity), 32 * t, st), qf[st], s);
-          dp = Mfma<V>::mul(read_rows<V>(lanes, v_tile(parity), 32 * t, st), gf[st], dp);
-        }
+        products(parity, t, s, dp);
         float ds[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(s[r] * a.scale - lse) * (dp[r] - delta);
