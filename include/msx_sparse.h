@@ -3,8 +3,10 @@
  *
  * This is the drop-in boundary for mlx-sparse's sparse x dense hot path:
  * CSR SpMV (y = A x) and CSR SpMM with a dense row-major right-hand side
- * (Y = A X).  Every entry point takes plain pointers and sizes; no C++ or
- * framework type crosses it.
+ * (Y = A X), with what stands next to it: solvers, the adjoint side, Matrix
+ * Market input, and two operators of language models over sparse patterns
+ * (window attention with sinks, distillation from a CSR teacher).  Every entry
+ * point takes plain pointers and sizes; no C++ or framework type crosses it.
  *
  * Conventions
  *   - The caller owns every buffer.  Outputs (y / Y) are allocated by the
@@ -973,7 +975,10 @@ msx_status msx_window_attention(const msx_window_attention_desc *desc, void *out
  * q's; dq, dk and dv are contiguous and shaped as q, k and v.  `out` and
  * `lse` come from the forward call.  `scratch` holds
  * msx_window_attention_backward_scratch bytes.  Every gradient is summed in a
- * fixed order (no atomics): the same inputs give the same bits.
+ * fixed order (no atomics): the same inputs give the same bits.  A visible token
+ * that is not finite reaches the gradients of tokens near it as well (those of
+ * its tiles), where the forward product gives it to the queries that see it
+ * alone.
  */
 size_t msx_window_attention_backward_scratch(const msx_window_attention_desc *desc);
 msx_status msx_window_attention_backward(const msx_window_attention_desc *desc, const void *out,

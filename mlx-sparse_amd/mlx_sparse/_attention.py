@@ -177,7 +177,8 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale: float | Non
     256; any strides with adjacent head values are read in place.  Scores,
     softmax and sums are float32; 16-bit operands round probabilities to their
     own type for the products with values, which costs no more than the
-    rounding of the result.
+    rounding of the result.  Gradients are summed in a fixed order; a visible
+    token that is not finite reaches those of tokens near it too.
 
     Raises:
         TypeError: dtypes differ or are unsupported.
