@@ -241,10 +241,19 @@ struct Numbering {
   __device__ __forceinline__ Numbering(const WindowArgs &a, int32_t near)
       : far(min(a.sinks, near)), skip(near - far), free(skip == 0 ? a.sinks : far), window(a.window) {}
   __device__ __forceinline__ int32_t key(int32_t c) const { return c < far ? c : c + skip; }
-  // p = -1 sees nothing.
-  __device__ __forceinline__ bool seen(int32_t p, int32_t c) const {
-    const uint32_t back = static_cast<uint32_t>(p - key(c));
-    return back < static_cast<uint32_t>(c < free ? 0x7fffffff : window);
+};
+
+// What the query at p (-1 sees nothing) sees of numbers c0 + e, e known when
+// compiling.  A sink before the span is never ahead of the span's queries, so that
+// one comparison serves sinks on both sides of it: not past p, not past the
+// sinks.
+struct SeenFrom {
+  int32_t back, ahead;
+  uint32_t window;
+  __device__ __forceinline__ SeenFrom(const Numbering &n, int32_t p, int32_t c0)
+      : back(p - n.skip - c0), ahead(min(p, n.free - 1) - c0), window(n.window) {}
+  __device__ __forceinline__ bool operator()(int32_t e) const {
+    return (static_cast<uint32_t>(back - e) < window) | (e <= ahead);
   }
 };
 

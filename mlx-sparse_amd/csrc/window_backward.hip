@@ -259,11 +259,10 @@ backward_queries(WindowArgs a, Upstream up, QueryPlan plan, typename V::Storage 
       for (int t = 0; t < F::kSub; ++t) {
         v16f s, dp;
         products(at, t, s, dp);
+        const SeenFrom seen(number, p, at * F::kTokens + 32 * t + 4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int32_t c = at * F::kTokens + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-          delta += number.seen(p, c) ? exp2_fast(s[r] * a.scale - lse) * dp[r] : 0.0f;
-        }
+        for (int r = 0; r < 16; ++r)
+          delta += seen(8 * (r / 4) + r % 4) ? exp2_fast(s[r] * a.scale - lse) * dp[r] : 0.0f;
       }
     }
     delta += other_half(delta);
@@ -290,11 +289,9 @@ backward_queries(WindowArgs a, Upstream up, QueryPlan plan, typename V::Storage 
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(s[r] * a.scale - lse) * (dp[r] - delta);
         if (__builtin_amdgcn_readfirstlane(!whole)) {
+          const SeenFrom seen(number, p, c0 + 32 * t + 4 * half);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-            ds[r] = number.seen(p, c) ? ds[r] : 0.0f;
-          }
+          for (int r = 0; r < 16; ++r) ds[r] = seen(8 * (r / 4) + r % 4) ? ds[r] : 0.0f;
         }
         mul_transposed<V>(lanes, k_tile(parity), 32 * t, Column<V>(ds), acc);
       }

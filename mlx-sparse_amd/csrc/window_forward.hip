@@ -213,13 +213,12 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
     const bool whole = c0 + F::kKeys <= count && last <= p_first &&
                        (p_last - first < a.window || last < a.sinks) && p_last - p_first == kRows - 1;
     if (__builtin_amdgcn_readfirstlane(!whole)) {
+      const SeenFrom seen(number, p, c0 + 4 * half);
 #pragma unroll
       for (int t = 0; t < F::kSub; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int32_t c = c0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-          x[t][r] = number.seen(p, c) ? x[t][r] : -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r)
+          x[t][r] = seen(32 * t + 8 * (r / 4) + r % 4) ? x[t][r] : -INFINITY;
     }
     float tops[2] = {x[0][0], x[0][1]};
 #pragma unroll
