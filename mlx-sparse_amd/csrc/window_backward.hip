@@ -469,6 +469,9 @@ struct NearShape {
   static constexpr bool kInLds = T::kSize == 2 && DP > 64;
   static constexpr int kGroups = kInLds ? 2 : 1;  // waves of the same keys
   static constexpr int kThreads = kGroups * kWaves * kWave;
+  // all but wide float32 heads fit twice (at 64: 3 to 7 % of a backward pass;
+  // a third wave spills, 145 us become 204)
+  static constexpr int kWavesASimd = kInLds || DP <= 64 ? 2 : 1;
   static constexpr int kSub = T::kSize == 2 ? 2 : 1, kTokens = 32 * kSub;
   using Tile = QueryTile<V, DP, kTokens, kThreads>;
   static constexpr int kKeyBytes = kInLds ? 2 * kBlockKeys * T::kPitch : 0;
@@ -477,7 +480,7 @@ struct NearShape {
 };
 
 template <class V, int DP>
-__global__ __launch_bounds__((NearShape<V, DP>::kThreads), (NearShape<V, DP>::kGroups)) void
+__global__ __launch_bounds__((NearShape<V, DP>::kThreads), (NearShape<V, DP>::kWavesASimd)) void
 backward_keys_near(WindowArgs a, Upstream up, KeyPlan plan, typename V::Storage *dk,
                    typename V::Storage *dv) {
   using S = typename V::Storage;
