@@ -24,7 +24,7 @@
 //
 // Bound like the forward pass by products, exponentials and LDS reads taking
 // turns; the products are under way 30 % of the time.  16,384 tokens of 16
-// heads of 128 on 8, a window of 1,024: queries 300 us, keys 380 (both about
+// heads of 128 on 8, a window of 1,024: queries 293 us, keys 384 (both about
 // 700 TFLOP/s), sinks 30, joining 9.
 #include <hip/hip_runtime.h>
 
