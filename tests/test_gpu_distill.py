@@ -128,3 +128,21 @@ def test_another_stream(gpu):
         got = gpu.distill_value_and_grad(logits, A)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_in_a_graph(gpu):
+    """Losses and gradient captured once; every replay against the eager call."""
+    z = student(9, 70, 5000, BF16)
+    data, indices, indptr = teacher_rows(9, 70, 5000, [20, 0, 3], F32, torch.int32)
+    teacher = gpu.csr_array((data.cuda(), indices.cuda(), indptr.cuda()), (70, 5000))
+    gpu.distill_value_and_grad(z, teacher)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = gpu.distill_value_and_grad(z, teacher)
+    for i in range(3):
+        z.copy_(student(30 + i, 70, 5000, BF16))
+        want = gpu.distill_value_and_grad(z, teacher)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -280,3 +280,33 @@ def test_caches_elsewhere_are_refused(gpu):
     cache = torch.zeros(1, 9, 1, 8)
     with pytest.raises(ValueError, match="caches must be on"):
         gpu.window_attention_step(q, k, k, cache, cache.clone(), torch.tensor([0]), window=4)
+
+
+def test_training_in_a_graph(gpu):
+    """Forward and gradients captured once, in parts and with sinks' far pass;
+    every replay against the eager call on the same inputs."""
+    q, k, v, g = operands(13, 3, 700, 700, 4, 2, 64, BF16, "cuda")
+    pattern = {"window": 128, "sinks": 4}
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def call():
+        out = gpu.window_attention(*leaves, **pattern)
+        return (out.detach(), *torch.autograd.grad(out, leaves, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(3):
+        with torch.no_grad():
+            q.copy_(operands(20 + i, 3, 700, 700, 4, 2, 64, BF16, "cuda")[0])
+        want = call()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
