@@ -347,9 +347,14 @@ struct TailCut {
   __host__ __device__ __forceinline__ int64_t items() const { return whole + rest * parts; }
 };
 
+// The launch that joins one part a slot takes 5 to 8 us, a tile 1 to 3, the most in
+// float32: 128 bfloat16 key blocks are not worth two parts each (2 x 1,000 tokens
+// of 8 heads of 128: 94 us, 84 whole), 45 float32 ones are worth five (3 x 517
+// tokens of 6 heads of 64: 89 us, 104 in eleven parts).
+inline double join_cost(bool float32) { return float32 ? 2.0 : 6.0; }
+
 // Costs in tiles, of which a block has `tiles`: a part more for its start and
-// its sums, `join` for the launch that joins one part a slot (5 to 8 us, by tiles
-// of 1 to 3 us); a part has two at least.
+// its sums, `join` as above by their number; a part has two at least.
 inline TailCut cut_tail(int64_t blocks, int64_t slots, int64_t tiles, double join) {
   constexpr double kPart = 0.75;
   const int64_t rest = blocks % slots;

@@ -776,7 +776,8 @@ QueryPlan plan_queries(const WindowArgs &a, int32_t tile) {
   p.units = (static_cast<int64_t>(a.lq) + 31) / 32 * a.group;
   p.per_bh = (p.units + kWaves - 1) / kWaves;
   const int64_t keys = std::min<int64_t>(a.lk, static_cast<int64_t>(a.window) + a.sinks + 32);
-  p.cut = cut_tail(p.per_bh * a.batch * a.kv_heads, 2 * 256, (keys + tile - 1) / tile, tile == 64 ? 6 : 2);
+  p.cut = cut_tail(p.per_bh * a.batch * a.kv_heads, 2 * 256, (keys + tile - 1) / tile,
+                   join_cost(tile == 32));
   return p;
 }
 
@@ -788,7 +789,8 @@ KeyPlan plan_keys(const WindowArgs &a, int32_t tile) {
   const int64_t bh = a.batch * a.kv_heads;
   p.blocks = (a.lk + kBlockKeys - 1) / kBlockKeys;
   const int64_t span = std::min<int64_t>(a.lq, static_cast<int64_t>(a.window) + kBlockKeys - 1);
-  p.cut = cut_tail(bh * p.blocks, kCus, (span + tile - 1) / tile * a.group, tile == 64 ? 6 : 2);
+  p.cut = cut_tail(bh * p.blocks, kCus, (span + tile - 1) / tile * a.group,
+                   join_cost(tile == 32));
   // queries that see sinks from beyond the first block's span
   const int64_t beyond =
       std::min<int64_t>(a.lq, static_cast<int64_t>(a.lk) - kBlockKeys - a.window + 1);

@@ -396,7 +396,7 @@ Grid grid_of(const WindowArgs &a) {
   g.per_bh = (g.units + kWaves - 1) / kWaves;
   const int64_t keys = std::min<int64_t>(a.lk, static_cast<int64_t>(a.window) + a.sinks + kRows);
   g.cut = cut_tail(g.per_bh * a.batch * a.kv_heads, 256 * F::kBlocks, (keys + F::kKeys - 1) / F::kKeys,
-                   F::T::kSize == 2 ? 6 : 2);
+                   join_cost(F::T::kSize == 4));
   return g;
 }
 
