@@ -957,6 +957,11 @@ typedef struct msx_window_attention_desc {
   const void *q, *k, *v;
   /* (sequence, token, head), in values; the values of a head are adjacent */
   int64_t q_strides[3], k_strides[3], v_strides[3];
+  /* NULL, or for 16-bit types room for batch x heads x (lq rounded up to a
+   * multiple of 32) x (dim rounded up to one of 8) values: what rounding out to
+   * 16 bits left of it, written by the forward call and read by the backward
+   * call in an order of their own */
+  void *out_low;
 } msx_window_attention_desc;
 
 /*
@@ -978,7 +983,9 @@ msx_status msx_window_attention(const msx_window_attention_desc *desc, void *out
  * fixed order (no atomics): the same inputs give the same bits.  A visible token
  * that is not finite reaches the gradients of tokens near it as well (those of
  * its tiles), where the forward product gives it to the queries that see it
- * alone.
+ * alone.  Scores' gradients are P (dP - grad.out): with 16-bit types both calls
+ * should have `out_low`, without which out's own rounding stays in them, large
+ * beside a difference that is small where attention is concentrated.
  */
 size_t msx_window_attention_backward_scratch(const msx_window_attention_desc *desc);
 msx_status msx_window_attention_backward(const msx_window_attention_desc *desc, const void *out,

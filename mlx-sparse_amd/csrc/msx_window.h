@@ -21,6 +21,14 @@ struct WindowArgs {
   int32_t lengths64;
   const void *q, *k, *v;
   int64_t qs[3], ks[3], vs[3];
+  void *low;  // the residues of out, see Residue; may be null
+
+  // Where the residue of out[b][i][h][d] lies: eight values of a row, then the
+  // rows of 32 queries, as the tiles' waves store and load them.
+  __host__ __device__ inline int64_t low_at(int64_t b, int32_t i, int32_t h, int32_t d) const {
+    const int64_t units = (lq + 31) / 32, chunks = (dim + 7) / 8;
+    return ((((b * heads + h) * units + i / 32) * chunks + d / 8) * 32 + i % 32) * 8 + d % 8;
+  }
 
   // Tokens of sequence b that exist: [0, lk].
   __device__ inline int32_t length(int64_t b) const {
@@ -38,6 +46,21 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+
+// What rounding a result to 16 bits leaves of it, in 16 bits more: kept for
+// delta = grad.out of the backward pass, which is subtracted from dP and has to
+// be good to a rounding of the difference, not of itself.  float16's is held
+// 2^11 larger, so that it is as far above the subnormals as the result.
+template <class V>
+struct Residue {
+  static constexpr float kUp = V::kType == MSX_F16 ? 2048.0f : 1.0f;
+  __device__ static inline typename V::Storage of(float x, typename V::Storage kept) {
+    return V::narrow((x - V::widen(kept)) * kUp);
+  }
+  __device__ static inline float value(typename V::Storage low) {
+    return V::widen(low) * (1.0f / kUp);
+  }
+};
 
 __device__ inline float wave_max(float v) {
 #pragma unroll

@@ -95,6 +95,27 @@ struct Mfma<F32> {
   static constexpr uint32_t kSign = 0x80000000u;
 };
 
+// The residues of a pair of results, rounded to `kept`.
+template <class V>
+__device__ __forceinline__ uint32_t residues(float x0, float x1, uint32_t kept) {
+  return Mfma<V>::pack((x0 - V::widen(static_cast<uint16_t>(kept))) * Residue<V>::kUp,
+                       (x1 - V::widen(static_cast<uint16_t>(kept >> 16))) * Residue<V>::kUp);
+}
+
+// Four results of a row in the operands' type, and their residues where asked for.
+template <class V>
+__device__ __forceinline__ void store_four(const float (&x)[4], typename V::Storage *out,
+                                           typename V::Storage *low) {
+  if constexpr (sizeof(typename V::Storage) == 2) {
+    const v2u w{Mfma<V>::pack(x[0], x[1]), Mfma<V>::pack(x[2], x[3])};
+    *reinterpret_cast<v2u *>(out) = w;
+    if (low != nullptr)
+      *reinterpret_cast<v2u *>(low) = v2u{residues<V>(x[0], x[1], w[0]), residues<V>(x[2], x[3], w[1])};
+  } else {
+    *reinterpret_cast<v4f *>(out) = v4f{x[0], x[1], x[2], x[3]};
+  }
+}
+
 using LdsPtr = const __attribute__((address_space(3))) char *;
 __device__ __forceinline__ uint32_t lds_address(const char *p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsPtr)(p)));
@@ -203,6 +224,38 @@ struct Column<F32> {
     for (int r = 0; r < 16; ++r) p[r] = from[r];
   }
 };
+
+// The sum of a column as the products take it: divided by this, probabilities
+// sum to one however they were rounded, and one that is nearly alone comes out
+// as one.
+__device__ __forceinline__ float rounded_sum(const Column<BF16> &c) {
+  constexpr v2bf kOnes = {1.0f, 1.0f};
+  float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const v4u w = __builtin_bit_cast(v4u, c.b[k]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t pair = w[j];
+      sum[j % 2] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pair), kOnes, sum[j % 2], false);
+    }
+  }
+  return sum[0] + sum[1];
+}
+__device__ __forceinline__ float rounded_sum(const Column<F16> &c) {
+  constexpr v2h kOnes = {1.0f, 1.0f};
+  float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const v4u w = __builtin_bit_cast(v4u, c.b[k]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t pair = w[j];
+      sum[j % 2] = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, pair), kOnes, sum[j % 2], false);
+    }
+  }
+  return sum[0] + sum[1];
+}
 
 // acc[dt] += X^T P over 32 rows of the tile from `row0` on (a multiple of 32), X
 // read along its columns.

@@ -88,7 +88,14 @@ __global__ __launch_bounds__(kRowWaves * kWave) void forward_rows(WindowArgs a, 
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int r = 0; r < kMaxPer; ++r)
-    if (lane + kWave * r < a.dim) out[row * a.dim + lane + kWave * r] = V::narrow(o[r] * inv);
+    if (lane + kWave * r < a.dim) {
+      const int64_t at = row * a.dim + lane + kWave * r;
+      out[at] = V::narrow(o[r] * inv);
+      if constexpr (sizeof(*out) == 2)
+        if (a.low != nullptr)
+          static_cast<typename V::Storage *>(a.low)[a.low_at(b, i, h, lane + kWave * r)] =
+              Residue<V>::of(o[r] * inv, out[at]);
+    }
   if (lse != nullptr && lane == 0)
     lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
 }
@@ -119,7 +126,11 @@ __global__ __launch_bounds__(kRowWaves * kWave) void backward_rows(
     for (int d = lane; d < a.dim; d += kWave) {
       ql[d] = V::widen(q[d]);
       gl[d] = V::widen(g[d]);
-      part += gl[d] * V::widen(out[row * a.dim + d]);
+      float o = V::widen(out[row * a.dim + d]);
+      if constexpr (sizeof(*out) == 2)
+        if (a.low != nullptr)
+          o += Residue<V>::value(static_cast<const typename V::Storage *>(a.low)[a.low_at(b, i, h, d)]);
+      part += gl[d] * o;
     }
     delta = wave_sum(part);
     __builtin_amdgcn_wave_barrier();
@@ -335,6 +346,7 @@ WindowArgs args_of(const msx_window_attention_desc &d) {
   a.q = d.q;
   a.k = d.k;
   a.v = d.v;
+  a.low = d.out_low;
   std::copy(d.q_strides, d.q_strides + 3, a.qs);
   std::copy(d.k_strides, d.k_strides + 3, a.ks);
   std::copy(d.v_strides, d.v_strides + 3, a.vs);
@@ -438,7 +450,8 @@ extern "C" msx_status msx_window_attention(const msx_window_attention_desc *desc
   if (desc->batch == 0 || desc->lq == 0) return MSX_OK;
   if (out == nullptr) return fail(MSX_EINVAL, "window_attention out is NULL.");
   const WindowArgs a = args_of(*desc);
-  if (takes_tiles(*desc) && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+  if (takes_tiles(*desc) && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+      reinterpret_cast<uintptr_t>(desc->out_low) % 16 == 0) {
     const auto vt = static_cast<msx_vtype>(desc->vtype);
     const size_t need = window_forward_scratch(vt, a);
     if (scratch_bytes < need || (need > 0 && (scratch == nullptr ||
@@ -485,7 +498,7 @@ extern "C" msx_status msx_window_attention_backward(const msx_window_attention_d
   const size_t size = value_bytes(static_cast<msx_vtype>(desc->vtype));
   const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   if (queries && keys && takes_tiles(*desc) && rows_aligned(size, grad, grad_strides, 3) &&
-      aligned(out) && aligned(dq) && aligned(dk) && aligned(dv) && aligned(scratch))
+      aligned(out) && aligned(desc->out_low) && aligned(dq) && aligned(dk) && aligned(dv) && aligned(scratch))
     return launch_window_backward(static_cast<msx_vtype>(desc->vtype), a, out, lse, grad,
                                   grad_strides, static_cast<float *>(scratch), dq, dk, dv,
                                   static_cast<char *>(scratch) + delta_bytes(*desc),

@@ -39,12 +39,20 @@ float dot(const typename V::Storage *x, const typename V::Storage *y, int64_t n)
   return acc;
 }
 
+// float16's residues are held 2^11 larger: see Residue in msx_window.h.
+template <class V>
+constexpr float kLowUp = 1.0f;
+template <>
+constexpr float kLowUp<F16> = 2048.0f;
+
 // Attention of one query over the listed rows; returns the base-2 logarithm
-// of the softmax's sum (+inf without one).
+// of the softmax's sum (+inf without one).  `low` (or null): what rounding
+// leaves of the output, as the device keeps it.
 template <class V>
 float attend(const typename V::Storage *q, const std::vector<const typename V::Storage *> &k,
              const std::vector<const typename V::Storage *> &v, int64_t dim, float scale,
-             std::vector<float> &s, std::vector<float> &o, typename V::Storage *out) {
+             std::vector<float> &s, std::vector<float> &o, typename V::Storage *out,
+             typename V::Storage *low = nullptr) {
   float top = -INFINITY, sum = 0.0f;
   s.resize(k.size());
   for (size_t j = 0; j < k.size(); ++j) {
@@ -58,7 +66,11 @@ float attend(const typename V::Storage *q, const std::vector<const typename V::S
     sum += e;
     for (int64_t x = 0; x < dim; ++x) o[x] += e * V::widen(v[j][x]);
   }
-  for (int64_t x = 0; x < dim; ++x) out[x] = V::narrow(sum == 0.0f ? 0.0f : o[x] / sum);
+  for (int64_t x = 0; x < dim; ++x) {
+    const float value = sum == 0.0f ? 0.0f : o[x] / sum;
+    out[x] = V::narrow(value);
+    if (low != nullptr) low[x] = V::narrow((value - V::widen(out[x])) * kLowUp<V>);
+  }
   return sum == 0.0f ? INFINITY : (base + std::log(sum)) * 1.44269504088896340736f;
 }
 
@@ -66,6 +78,7 @@ template <class V>
 void forward(const msx_window_attention_desc &d, void *out, float *lse, int n_threads) {
   using S = typename V::Storage;
   const int64_t group = d.heads / d.kv_heads;
+  S *low = sizeof(S) == 2 ? static_cast<S *>(d.out_low) : nullptr;
   split(d.batch * d.heads * d.lq, n_threads, [&](int64_t first, int64_t last) {
     std::vector<const S *> k, v;
     std::vector<float> s, o;
@@ -79,9 +92,10 @@ void forward(const msx_window_attention_desc &d, void *out, float *lse, int n_th
           k.push_back(at<V>(d.k, d.k_strides, b, j, h / group));
           v.push_back(at<V>(d.v, d.v_strides, b, j, h / group));
         });
+      const int64_t to = ((b * d.lq + i) * d.heads + h) * d.dim;
       const float l = attend<V>(at<V>(d.q, d.q_strides, b, i, h), k, v, d.dim,
-                                static_cast<float>(d.scale), s, o,
-                                static_cast<S *>(out) + ((b * d.lq + i) * d.heads + h) * d.dim);
+                                static_cast<float>(d.scale), s, o, static_cast<S *>(out) + to,
+                                low == nullptr ? nullptr : low + to);
       if (lse != nullptr) lse[r] = l;
     }
   });
@@ -95,6 +109,7 @@ void backward(const msx_window_attention_desc &d, const void *out, const float *
   using S = typename V::Storage;
   const int64_t group = d.heads / d.kv_heads, dim = d.dim;
   const float scale = static_cast<float>(d.scale);
+  const S *low = sizeof(S) == 2 ? static_cast<const S *>(d.out_low) : nullptr;
   split(d.batch * d.kv_heads, n_threads, [&](int64_t first, int64_t last) {
     std::vector<float> sum_k(static_cast<size_t>(d.lk * dim)), sum_v(sum_k.size()), sum_q(dim);
     for (int64_t r = first; r < last; ++r) {
@@ -108,7 +123,8 @@ void backward(const msx_window_attention_desc &d, const void *out, const float *
           std::fill(sum_q.begin(), sum_q.end(), 0.0f);
           if (p >= 0 && p < n && l != INFINITY) {
             const S *q = at<V>(d.q, d.q_strides, b, i, h), *g = at<V>(grad, gs, b, i, h);
-            const float delta = dot<V>(g, static_cast<const S *>(out) + at_out, dim);
+            float delta = dot<V>(g, static_cast<const S *>(out) + at_out, dim);
+            if (low != nullptr) delta += dot<V>(g, low + at_out, dim) / kLowUp<V>;
             each_seen(p, d.window, d.sinks, [&](int64_t j) {
               const S *k = at<V>(d.k, d.k_strides, b, j, kvh), *v = at<V>(d.v, d.v_strides, b, j, kvh);
               const float prob = std::exp2(dot<V>(q, k, dim) * scale * 1.44269504088896340736f - l);

@@ -11,8 +11,10 @@
 //
 // Probabilities are rounded to the operands' 16 bits for the second product,
 // unnormalised and at most 2^8, as the matrix instruction takes them: their errors are
-// independent and no larger than the output's own rounding.  Scores, maximum,
-// sum and output stay float32.
+// independent and no larger than the output's own rounding.  The output is
+// divided by the sum of the rounded ones, so that one that is nearly alone gives
+// its value row as it is (0 to 4 % of a prompt); lse takes the sum of the
+// exponentials themselves.  Scores, maximum, sums and output stay float32.
 //
 // Bound by how a wave's matrix instructions, exponentials and LDS reads take
 // turns: a tile of 64 keys costs a wave 1,024 cycles of products, some 950 of
@@ -48,7 +50,7 @@ struct ForwardShape {
   // workgroups a CU: two hide each other's waits; wide float32 heads need the
   // registers of one (76 spilled with two at 128)
   static constexpr int kBlocks = T::kRowBytes > 256 ? 1 : 2;
-  static constexpr int kStride = DP + 4;  // of a row's sums, m and l in scratch
+  static constexpr int kStride = DP + 4;  // of a row's sums, m, l and total in scratch
 };
 
 // A query row by its definition, one wave: keys over the lanes for the
@@ -88,9 +90,16 @@ __device__ void forward_row(const WindowArgs &a, int64_t b, int32_t i, int32_t h
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  S *to = out + ((b * a.lq + i) * a.heads + h) * a.dim;
-  if (lane < a.dim) to[lane] = V::narrow(o0 * inv);
-  if (lane + kWave < a.dim) to[lane + kWave] = V::narrow(o1 * inv);
+  const int64_t at = ((b * a.lq + i) * a.heads + h) * a.dim;
+  const auto store = [&](int d, float x) {
+    if (d >= a.dim) return;
+    const S kept = V::narrow(x);
+    out[at + d] = kept;
+    if constexpr (sizeof(S) == 2)
+      if (a.low != nullptr) static_cast<S *>(a.low)[a.low_at(b, i, h, d)] = Residue<V>::of(x, kept);
+  };
+  store(lane, o0 * inv);
+  store(lane + kWave, o1 * inv);
 }
 
 template <class V, int DP>
@@ -186,7 +195,9 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
-  float m = -INFINITY, base = 0.0f, l = 0.0f;  // l: this lane's keys only
+  // l, the sum of what the products take, and total, that of the exponentials
+  // themselves, for lse; of this lane's keys only
+  float m = -INFINITY, base = 0.0f, l = 0.0f, total = 0.0f;
 
   const auto scores = [&](uint32_t tile, int t, v16f &to) {
 #pragma unroll
@@ -202,8 +213,14 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
       e[r] = exp2_fast(from[r] * scale - base);
       sum[r % 2] += e[r];
     }
-    l += sum[0] + sum[1];
-    return Column<V>(e);
+    const Column<V> column(e);
+    if constexpr (T::kSize == 2) {
+      l += rounded_sum(column);
+      if (lse != nullptr) total += sum[0] + sum[1];
+    } else {
+      l += sum[0] + sum[1];
+    }
+    return column;
   };
   // masks the scores of the tile at c0 and moves the maximum.  It is moved
   // only where it has grown by more than 2^8: until then exponentials up to
@@ -234,6 +251,7 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
       m = grown;
       base = m == -INFINITY ? 0.0f : m;
       l *= shrink;
+      total *= shrink;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -268,6 +286,7 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   }
 
   l += other_half(l);
+  total = T::kSize == 2 ? total + other_half(total) : l;
   if (item.slot >= 0) {  // a part: its sums as they are, joined by forward_join
     float *to = sums + ((item.slot * kWaves + wave) * kRows + lane % 32) * F::kStride;
 #pragma unroll
@@ -279,13 +298,15 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
     if (half == 0) {
       to[DP] = m;
       to[DP + 1] = l;
+      to[DP + 2] = total;
     }
     return;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   bool odd = false;  // something is not finite: the row is computed anew
   if (live && i < a.lq) {
-    S *to = out + ((b * a.lq + i) * a.heads + h) * a.dim;
+    const int64_t at = ((b * a.lq + i) * a.heads + h) * a.dim;
+    S *low = a.low != nullptr ? static_cast<S *>(a.low) + a.low_at(b, i, h, 4 * half) : nullptr;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -297,16 +318,10 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
           x[j] = o[dt][r + j] * inv;
           odd = odd || !(fabsf(x[j]) < INFINITY);
         }
-        if (d < a.dim) {
-          if constexpr (T::kSize == 2)
-            *reinterpret_cast<v2u *>(to + d) =
-                v2u{Mfma<V>::pack(x[0], x[1]), Mfma<V>::pack(x[2], x[3])};
-          else
-            *reinterpret_cast<v4f *>(to + d) = v4f{x[0], x[1], x[2], x[3]};
-        }
+        if (d < a.dim) store_four<V>(x, out + at + d, low == nullptr ? nullptr : low + d / 8 * 256);
       }
     if (lse != nullptr && half == 0)
-      lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
+      lse[(b * a.heads + h) * a.lq + i] = total == 0.0f ? INFINITY : m + log2_fast(total);
   }
   uint64_t anew = __ballot(odd && p >= 0);
   anew = (anew | anew >> 32) & 0xffffffffu;
@@ -343,8 +358,7 @@ __global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t u
   bool odd = false;
   if (live) {
     const float *first = sums + rest * cut.parts * kPart + in_block * kStride;
-    float m = -INFINITY, l = 0.0f;
-    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f, total = 0.0f, o[4] = {};
 #pragma unroll 4
     for (int32_t part = 0; part < cut.parts; ++part) m = fmaxf(m, first[part * kPart + DP]);
     const float base = m == -INFINITY ? 0.0f : m;
@@ -353,6 +367,7 @@ __global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t u
       const float *from = first + part * kPart;
       const float f = exp2_fast(from[DP] - base);
       l += from[DP + 1] * f;
+      total += from[DP + 2] * f;
       const v4f x = *reinterpret_cast<const v4f *>(from + min(d, DP - 4));
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] += x[j] * f;
@@ -364,14 +379,11 @@ __global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t u
       odd = odd || (d < a.dim && !(fabsf(o[j]) < INFINITY));
     }
     if (d < a.dim) {
-      auto *to = out + ((b * a.lq + i) * a.heads + h) * a.dim + d;
-      if constexpr (sizeof(typename V::Storage) == 2)
-        *reinterpret_cast<v2u *>(to) = v2u{Mfma<V>::pack(o[0], o[1]), Mfma<V>::pack(o[2], o[3])};
-      else
-        *reinterpret_cast<v4f *>(to) = o;
+      const int64_t at = ((b * a.lq + i) * a.heads + h) * a.dim + d;
+      store_four<V>(o, out + at, a.low == nullptr ? nullptr : static_cast<typename V::Storage *>(a.low) + a.low_at(b, i, h, d));
     }
     if (lse != nullptr && d == 0)
-      lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
+      lse[(b * a.heads + h) * a.lq + i] = total == 0.0f ? INFINITY : m + log2_fast(total);
   }
   uint64_t anew = __ballot(odd && p >= 0 && p < a.length(b));
   while (anew != 0) {

@@ -82,7 +82,8 @@ def _transformed() -> bool:
 
 
 class _WindowAttention(torch.autograd.Function):
-    """``(out, lse)``; ``lse`` is the backward pass's and has no derivative.
+    """``(out, lse, low)``; the last two are the backward pass's and have no
+    derivative (``low``: what rounding left of a 16-bit ``out``, else None).
     Takes the calls under a transform; others have a node of the native
     module's, whose backward pass does not enter the interpreter."""
 
@@ -93,20 +94,17 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def setup_context(ctx, inputs, output):
         q, k, v, lengths, window, sinks, scale = inputs
-        out, lse = output
-        ctx.mark_non_differentiable(lse)
+        out, lse, low = output
+        ctx.mark_non_differentiable(*(t for t in (lse, low) if t is not None))
         ctx.set_materialize_grads(False)
         ctx.pattern = (window, sinks, scale)
-        ctx.has_lengths = lengths is not None
-        ctx.save_for_backward(q, k, v, out, lse, *((lengths,) if ctx.has_lengths else ()))
+        ctx.save_for_backward(q, k, v, lengths, out, lse, low)
 
     @staticmethod
-    def backward(ctx, grad, _lse):
+    def backward(ctx, grad, *_):
         if grad is None:
             return (None,) * 7
-        q, k, v, out, lse, *rest = ctx.saved_tensors
-        got = _call(_WindowGradients, q, k, v, rest[0] if ctx.has_lengths else None, out, lse,
-                    grad, *ctx.pattern)
+        got = _call(_WindowGradients, *ctx.saved_tensors, grad, *ctx.pattern)
         return (*(g if needed else None for g, needed in zip(got, ctx.needs_input_grad)),
                 None, None, None, None)
 
@@ -122,16 +120,17 @@ class _WindowAttention(torch.autograd.Function):
         q, k, v = (folded(t, d) for t, d in zip((q, k, v), in_dims))
         if lengths is not None:
             lengths = folded(lengths, in_dims[3]).contiguous()
-        out, lse = _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
-        return (out.reshape(n, -1, *out.shape[1:]), lse.reshape(n, -1, *lse.shape[1:])), (0, 0)
+        got = _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
+        return (tuple(t if t is None else t.reshape(n, -1, *t.shape[1:]) for t in got),
+                tuple(t if t is None else 0 for t in got))
 
 
 class _WindowGradients(torch.autograd.Function):
     """``(dq, dk, dv)``; no derivative of their own."""
 
     @staticmethod
-    def forward(q, k, v, lengths, out, lse, grad, window, sinks, scale):
-        return _native.window_attention_backward(q, k, v, lengths, out, lse,
+    def forward(q, k, v, lengths, out, lse, low, grad, window, sinks, scale):
+        return _native.window_attention_backward(q, k, v, lengths, out, lse, low,
                                                  _operand(grad, grad.device), window, sinks, scale)
 
     @staticmethod

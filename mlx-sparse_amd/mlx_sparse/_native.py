@@ -159,15 +159,17 @@ def csr_plan(indptr, n_rows: int, nnz: int, block_nnz: int = 0, *, data=None, in
 
 
 def window_attention(q, k, v, lengths, window: int, sinks: int, scale: float, with_lse: bool):
-    """(out, lse or None) of attention over a band and sink columns."""
+    """(out, lse, low) of attention over a band and sink columns; the last two,
+    with ``with_lse``, for the backward pass (``low``, of 16-bit outputs, what
+    rounding left of them)."""
     return extension().window_attention(q, k, v, lengths, window, sinks, scale, with_lse)
 
 
-def window_attention_backward(q, k, v, lengths, out, lse, grad, window: int, sinks: int,
+def window_attention_backward(q, k, v, lengths, out, lse, low, grad, window: int, sinks: int,
                               scale: float):
     """(dq, dk, dv) of window_attention."""
-    return extension().window_attention_backward(q, k, v, lengths, out, lse, grad, window, sinks,
-                                                 scale)
+    return extension().window_attention_backward(q, k, v, lengths, out, lse, low, grad, window,
+                                                 sinks, scale)
 
 
 def window_attention_step(q, k, v, cache_k, cache_v, lengths, window: int, sinks: int,

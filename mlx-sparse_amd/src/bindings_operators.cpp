@@ -77,31 +77,52 @@ struct Pattern {
   double scale;
 };
 
-std::tuple<Tensor, Tensor> attention(const Tensor &q_t, const Tensor &k_t, const Tensor &v_t,
+struct Attended {
+  Tensor out, lse, low;  // low: of 16-bit outputs, what rounding left of them
+};
+
+// With `with_lse` what the backward pass reads: lse and low.
+Attended attention(const Tensor &q_t, const Tensor &k_t, const Tensor &v_t,
                                      const Tensor &lengths_t, Pattern p, bool with_lse) {
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t);
   const OptionalView lengths(lengths_t);
-  const auto desc = msx::window_attention_desc(q, k, v, lengths.get, p.window, p.sinks, p.scale);
+  auto desc = msx::window_attention_desc(q, k, v, lengths.get, p.window, p.sinks, p.scale);
   const Tensor out = new_tensor(q_t, {desc.batch, desc.lq, desc.heads, desc.dim}, q_t.scalar_type());
-  Tensor lse;
+  Tensor lse, low;
   if (with_lse) lse = new_tensor(q_t, {desc.batch, desc.heads, desc.lq}, at::kFloat);
+  if (with_lse && q_t.scalar_type() != at::kFloat) {
+    low = new_tensor(q_t, {desc.batch, desc.heads, (desc.lq + 31) / 32 * 32, (desc.dim + 7) / 8 * 8},
+                     q_t.scalar_type());
+    desc.out_low = low.data_ptr();
+  }
   const ArrayView vo = view_of(out);
   float *l = with_lse ? lse.data_ptr<float>() : nullptr;
   msx::ExecContext ctx = msx::context_for(q, 0);
   Tensor scratch;
   if (q.device >= 0) scratch = msx::scratch_for(ctx, q_t, msx_window_attention_scratch(&desc));
   run_op(q, [&] { msx::window_attention(desc, vo, l, ctx); });
-  return {out, lse};
+  return {out, lse, low};
 }
 
 std::tuple<Tensor, Tensor, Tensor> attention_gradients(const Tensor &q_t, const Tensor &k_t,
                                                        const Tensor &v_t, const Tensor &lengths_t,
                                                        const Tensor &out_t, const Tensor &lse_t,
-                                                       const Tensor &grad_t, Pattern p) {
+                                                       const Tensor &low_t, const Tensor &grad_t,
+                                                       Pattern p) {
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t), out = view_of(out_t),
                   lse = view_of(lse_t), grad = view_of(grad_t);
   const OptionalView lengths(lengths_t);
-  const auto desc = msx::window_attention_desc(q, k, v, lengths.get, p.window, p.sinks, p.scale);
+  auto desc = msx::window_attention_desc(q, k, v, lengths.get, p.window, p.sinks, p.scale);
+  if (low_t.defined()) {
+    const ArrayView low = view_of(low_t);
+    msx::require_size(low, desc.batch * desc.heads * ((desc.lq + 31) / 32 * 32) * ((desc.dim + 7) / 8 * 8),
+                      "window_attention_backward low");
+    msx::require_contiguous(low, "window_attention_backward low");
+    msx::require_same_device({&q, &low}, "window_attention_backward");
+    if (low.dtype != q.dtype || q.dtype == DType::Float32)
+      throw std::invalid_argument("window_attention_backward low must have the queries' 16-bit dtype.");
+    desc.out_low = low.ptr;
+  }
   if (lse.dtype != DType::Float32)
     throw std::invalid_argument("window_attention_backward lse must have dtype float32.");
   msx::require_size(lse, desc.batch * desc.heads * desc.lq, "window_attention_backward lse");
@@ -134,9 +155,10 @@ using torch::autograd::variable_list;
 // derivatives, and an error where theirs are used.
 struct AttentionGradients : torch::autograd::Function<AttentionGradients> {
   static variable_list forward(AutogradContext *, Tensor q, Tensor k, Tensor v,
-                               std::optional<Tensor> lengths, Tensor out, Tensor lse, Tensor grad,
-                               int64_t window, int64_t sinks, double scale) {
-    const auto [dq, dk, dv] = attention_gradients(q, k, v, lengths.value_or(Tensor()), out, lse, grad, {window, sinks, scale});
+                               std::optional<Tensor> lengths, Tensor out, Tensor lse,
+                               std::optional<Tensor> low, Tensor grad, int64_t window, int64_t sinks, double scale) {
+    const auto [dq, dk, dv] = attention_gradients(q, k, v, lengths.value_or(Tensor()), out, lse,
+                                                  low.value_or(Tensor()), grad, {window, sinks, scale});
     return {dq, dk, dv};
   }
   static variable_list backward(AutogradContext *, variable_list) {
@@ -150,8 +172,8 @@ struct Attention : torch::autograd::Function<Attention> {
                         std::optional<Tensor> lengths_o, int64_t window, int64_t sinks,
                         double scale) {
     const Tensor lengths = lengths_o.value_or(Tensor());
-    const auto [out, lse] = attention(q, k, v, lengths, {window, sinks, scale}, true);
-    ctx->save_for_backward({q, k, v, lengths, out, lse});
+    const auto [out, lse, low] = attention(q, k, v, lengths, {window, sinks, scale}, true);
+    ctx->save_for_backward({q, k, v, lengths, out, lse, low});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
@@ -167,11 +189,11 @@ struct Attention : torch::autograd::Function<Attention> {
     const Tensor grad = made_direct(grads[0]);
     if (at::GradMode::is_enabled()) {
       const variable_list got = AttentionGradients::apply(s[0], s[1], s[2], present(s[3]), s[4],
-                                                          s[5], grad, p.window, p.sinks, p.scale);
+                                                          s[5], present(s[6]), grad, p.window, p.sinks, p.scale);
       std::copy(got.begin(), got.end(), result.begin());
     } else {
       std::tie(result[0], result[1], result[2]) =
-          attention_gradients(s[0], s[1], s[2], s[3], s[4], s[5], grad, p);
+          attention_gradients(s[0], s[1], s[2], s[3], s[4], s[5], s[6], grad, p);
     }
     return result;
   }
@@ -232,22 +254,23 @@ py::object window_attention_plain(py::handle q_o, py::handle k_o, py::handle v_o
     return py::none();
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return wrap(Attention::apply(q, k, v, present(lengths), p.window, p.sinks, p.scale));
-  return wrap(std::get<0>(attention(q, k, v, lengths, p, false)));
+  return wrap(attention(q, k, v, lengths, p, false).out);
 }
 
 py::tuple window_attention(py::handle q, py::handle k, py::handle v, py::handle lengths,
                            int64_t window, int64_t sinks, double scale, bool with_lse) {
-  const auto [out, lse] = attention(tensor_of(q), tensor_of(k), tensor_of(v),
-                                    optional_tensor(lengths), {window, sinks, scale}, with_lse);
-  return py::make_tuple(wrap(out), wrap(lse));
+  const auto [out, lse, low] = attention(tensor_of(q), tensor_of(k), tensor_of(v),
+                                         optional_tensor(lengths), {window, sinks, scale}, with_lse);
+  return py::make_tuple(wrap(out), wrap(lse), wrap(low));
 }
 
 py::tuple window_attention_backward(py::handle q, py::handle k, py::handle v, py::handle lengths,
-                                    py::handle out, py::handle lse, py::handle grad,
-                                    int64_t window, int64_t sinks, double scale) {
+                                    py::handle out, py::handle lse, py::handle low,
+                                    py::handle grad, int64_t window, int64_t sinks, double scale) {
   const auto [dq, dk, dv] =
       attention_gradients(tensor_of(q), tensor_of(k), tensor_of(v), optional_tensor(lengths),
-                          tensor_of(out), tensor_of(lse), tensor_of(grad), {window, sinks, scale});
+                          tensor_of(out), tensor_of(lse), optional_tensor(low), tensor_of(grad),
+                          {window, sinks, scale});
   return py::make_tuple(wrap(dq), wrap(dk), wrap(dv));
 }
 
@@ -490,9 +513,10 @@ void bind_operators(py::module_ &m) {
   m.def("window_attention", &window_attention, py::arg("q"), py::arg("k"), py::arg("v"),
         py::arg("lengths"), py::arg("window"), py::arg("sinks"), py::arg("scale"),
         py::arg("with_lse"),
-        "(out, lse) of attention over the last window and the first sinks keys.");
+        "(out, lse, low) of attention over the last window and the first sinks keys.");
   m.def("window_attention_backward", &window_attention_backward, py::arg("q"), py::arg("k"),
-        py::arg("v"), py::arg("lengths"), py::arg("out"), py::arg("lse"), py::arg("grad"),
+        py::arg("v"), py::arg("lengths"), py::arg("out"), py::arg("lse"), py::arg("low"),
+        py::arg("grad"),
         py::arg("window"), py::arg("sinks"), py::arg("scale"),
         "(dq, dk, dv) of window_attention.");
   m.def("window_attention_step_plain", &window_attention_step_plain, py::arg("q"), py::arg("k"),
