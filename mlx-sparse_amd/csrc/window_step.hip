@@ -12,8 +12,9 @@
 // us, 5.5 TB/s (a copy moves 5.1); 37 of up to 1,001 keys, 24 heads of 96 on
 // 8: 24 us, 3.4 TB/s, of which a third is the launch.
 //
-// Probabilities are rounded to 16 bits for their products as in the forward
-// pass.
+// A probability enters its products as two 16-bit values, rounded and what that
+// leaves: 16 bits would add half as much again to the error of rounding the
+// output, and the second product takes no time beside the memory.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -247,9 +248,14 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void step_tiles(StepArg
       l += x[j];
     }
     if constexpr (F::kSize == 2) {
-      v4u p;
+      v4u p, low;  // rounded, and what that leaves
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = Mfma<V>::pack(x[2 * j], x[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t pair = Mfma<V>::pack(x[2 * j], x[2 * j + 1]);
+        p[j] = pair;
+        low[j] = Mfma<V>::pack(x[2 * j] - V::widen(static_cast<uint16_t>(pair)),
+                               x[2 * j + 1] - V::widen(static_cast<uint16_t>(pair >> 16)));
+      }
       const int i = lane % 16;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
@@ -260,7 +266,9 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void step_tiles(StepArg
           part[t] = read_transposed(tile + F::at(row, column / 8) + (column % 8) * 2);
         }
         const auto lo = __builtin_bit_cast(v2u, part[0]), hi = __builtin_bit_cast(v2u, part[1]);
-        o[d] = Mfma16<V>::mul(v4u{lo[0], lo[1], hi[0], hi[1]}, p, o[d]);
+        const v4u values{lo[0], lo[1], hi[0], hi[1]};
+        o[d] = Mfma16<V>::mul(values, p, o[d]);
+        o[d] = Mfma16<V>::mul(values, low, o[d]);
       }
     } else {
 #pragma unroll
