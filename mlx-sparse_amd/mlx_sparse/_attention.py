@@ -203,13 +203,13 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale: float | Non
                          f"{tuple(q.shape)} and {tuple(k.shape)}.")
     _check_heads("window_attention", q.shape[2], k.shape[2], q.shape[3])
     scale = _scale(scale, q.shape[3])
-    if transformed:
-        return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)[0]
-    out = extension().window_attention_plain(q, k, v, lengths, window, sinks, scale,
-                                             default_device_index())
-    if out is None:  # an operand that no rule above names: let the native checks name it
-        out = _native.window_attention(q, k, v, lengths, window, sinks, scale, False)[0]
-    return out
+    if not transformed:
+        out = extension().window_attention_plain(q, k, v, lengths, window, sinks, scale,
+                                                 default_device_index())
+        if out is not None:
+            return out
+    # (an operand that no rule above names is named by the native checks)
+    return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)[0]
 
 
 def _cache(name: str, cache, device) -> torch.Tensor:

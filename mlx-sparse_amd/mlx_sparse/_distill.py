@@ -146,13 +146,12 @@ def distill_loss(logits, teacher: CSRArray, *, temperature: float = 1.0) -> torc
     logits, (data, indices, indptr), temperature = _prepared("distill_loss", logits, teacher,
                                                              temperature)
     z = _rows(logits)
-    if transformed:
-        losses = _DistillLoss.apply(z, data, indices, indptr, temperature)[0]
-    else:
+    losses = None
+    if not transformed:
         losses = extension().distill_loss_plain(z, data, indices, indptr, *teacher.shape,
                                                 temperature, default_device_index())
-        if losses is None:  # an operand that no rule above names: let the native checks name it
-            losses = _native.distill_loss(z, data, indices, indptr, temperature, False)[0]
+    if losses is None:  # (an operand that no rule above names is named by the native checks)
+        losses = _DistillLoss.apply(z, data, indices, indptr, temperature)[0]
     return losses if logits.ndim == 2 else losses.reshape(logits.shape[:-1])
 
 

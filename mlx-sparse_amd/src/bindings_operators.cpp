@@ -220,8 +220,9 @@ bool plain_span(py::handle window, py::handle sinks, Pattern &p) {
   int over_w = 0, over_s = 0;
   p.window = PyLong_AsLongLongAndOverflow(window.ptr(), &over_w);
   p.sinks = PyLong_AsLongLongAndOverflow(sinks.ptr(), &over_s);
-  return !over_w && !over_s && p.window >= 1 && p.sinks >= 0 && p.window < (int64_t{1} << 40) &&
-         p.sinks < (int64_t{1} << 40);
+  // 2^40 at most, to which the checks in Python lower wider ones
+  return !over_w && !over_s && p.window >= 1 && p.sinks >= 0 && p.window <= (int64_t{1} << 40) &&
+         p.sinks <= (int64_t{1} << 40);
 }
 
 bool plain_scale(py::handle scale, int64_t dim, Pattern &p) {
