@@ -29,6 +29,7 @@ from mlx_sparse._ext_loader import extension
 from mlx_sparse._validation import ensure_array
 
 _REAL = (torch.float32, torch.float16, torch.bfloat16)
+_INDEX = {torch.int32, torch.int64}
 
 
 def _span(name: str, window, sinks) -> tuple[int, int]:
@@ -295,6 +296,6 @@ def window_cache_store(k, v, cache_k, cache_v, *, sinks: int = 0, starts=None,
     cache_k, cache_v = _cache(name, cache_k, device), _cache(name, cache_v, device)
     starts, lengths = _counts(starts, device), _counts(lengths, device)
     _check_dtypes(name, k, v=v, cache_k=cache_k, cache_v=cache_v)
-    if starts is not None and lengths is not None and starts.dtype != lengths.dtype:
-        starts = starts.to(lengths.dtype)
+    if starts is not None and lengths is not None and {starts.dtype, lengths.dtype} == _INDEX:
+        starts, lengths = starts.long(), lengths.long()
     _native.window_cache_store(k, v, cache_k, cache_v, starts, lengths, sinks)
