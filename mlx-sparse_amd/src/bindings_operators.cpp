@@ -55,6 +55,12 @@ py::object wrap(const Tensor &t) {
   return py::reinterpret_steal<py::object>(THPVariable_Wrap(t));
 }
 
+// A write that torch did not make: a derivative that saved the tensor, or a view
+// of it, raises as after torch's own in-place operations.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Runs `fn`; without the interpreter lock where it works on the host.
 template <class Fn>
 void run_op(const ArrayView &v, Fn &&fn) {
@@ -289,6 +295,8 @@ Tensor step(const Tensor &q_t, const Tensor &k_t, const Tensor &v_t, const Tenso
   Tensor scratch;
   if (q.device >= 0) scratch = msx::scratch_for(ctx, q_t, msx_window_attention_step_scratch(&desc));
   run_op(q, [&] { msx::window_attention_step(desc, vo, ctx); });
+  written(ck_t);
+  written(cv_t);
   return out;
 }
 
@@ -329,6 +337,8 @@ void window_cache_store(py::handle k_o, py::handle v_o, py::handle cache_k_o, py
   const OptionalView starts(optional_tensor(starts_o)), lengths(optional_tensor(lengths_o));
   const msx::ExecContext ctx = msx::context_for(k, 0);
   run_op(k, [&] { msx::window_cache_store(k, v, ck, cv, starts.get, lengths.get, sinks, ctx); });
+  written(tensor_of(cache_k_o));
+  written(tensor_of(cache_v_o));
 }
 
 // ---------------------------------------------------------------------------
