@@ -55,6 +55,14 @@ py::object wrap(const Tensor &t) {
   return py::reinterpret_steal<py::object>(THPVariable_Wrap(t));
 }
 
+// What is written in place has a place for every value.
+void require_writable(const Tensor &t, const char *name) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0)
+      throw std::invalid_argument(std::string(name) +
+                                  " is written in place and cannot be an expanded tensor.");
+}
+
 // A write that torch did not make: a derivative that saved the tensor, or a view
 // of it, raises as after torch's own in-place operations.
 void written(const Tensor &t) {
@@ -288,6 +296,8 @@ Tensor step(const Tensor &q_t, const Tensor &k_t, const Tensor &v_t, const Tenso
             const Tensor &cv_t, const Tensor &lengths_t, Pattern p) {
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t), ck = view_of(ck_t),
                   cv = view_of(cv_t), lengths = view_of(lengths_t);
+  require_writable(ck_t, "window_attention_step cache_k");
+  require_writable(cv_t, "window_attention_step cache_v");
   const auto desc = msx::window_step_desc(q, k, v, ck, cv, lengths, p.window, p.sinks, p.scale);
   const Tensor out = new_tensor(q_t, {desc.batch, desc.heads, desc.dim}, q_t.scalar_type());
   const ArrayView vo = view_of(out);
@@ -335,6 +345,8 @@ void window_cache_store(py::handle k_o, py::handle v_o, py::handle cache_k_o, py
   const ArrayView k = view_of(k_o), v = view_of(v_o), ck = view_of(cache_k_o),
                   cv = view_of(cache_v_o);
   const OptionalView starts(optional_tensor(starts_o)), lengths(optional_tensor(lengths_o));
+  require_writable(tensor_of(cache_k_o), "window_cache_store cache_k");
+  require_writable(tensor_of(cache_v_o), "window_cache_store cache_v");
   const msx::ExecContext ctx = msx::context_for(k, 0);
   run_op(k, [&] { msx::window_cache_store(k, v, ck, cv, starts.get, lengths.get, sinks, ctx); });
   written(tensor_of(cache_k_o));
