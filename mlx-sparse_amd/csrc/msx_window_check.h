@@ -35,7 +35,9 @@ inline msx_status check_window_heads(const char *op, int vt, int it, int64_t bat
     return fail(MSX_EINVAL, name + " head dimension must be between 1 and 256.");
   if (window < 1) return fail(MSX_EINVAL, name + " window must be at least 1.");
   if (sinks < 0) return fail(MSX_EINVAL, name + " sinks must be non-negative.");
-  if (!std::isfinite(scale)) return fail(MSX_EINVAL, name + " scale must be finite.");
+  // scores are float32, in base 2
+  if (!std::isfinite(static_cast<float>(scale * 1.44269504088896340736)))
+    return fail(MSX_EINVAL, name + " scale must be finite in float32.");
   return MSX_OK;
 }
 

@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
+#include <limits>
 
 #include "msx_device.h"
 #include "msx_internal.h"
@@ -355,7 +357,7 @@ WindowArgs args_of(const msx_window_attention_desc &d) {
 
 // Whether the tiles' kernels can read the operands: sixteen-byte rows at
 // sixteen-byte strides, a head of at most 128 values, and a scale that a
-// masked score survives.
+// masked score (minus infinity times it) survives.
 bool rows_aligned(size_t size, const void *p, const int64_t *strides, int n) {
   bool ok = reinterpret_cast<uintptr_t>(p) % 16 == 0;
   for (int i = 0; i < n; ++i) ok = ok && strides[i] * static_cast<int64_t>(size) % 16 == 0;
@@ -364,7 +366,8 @@ bool rows_aligned(size_t size, const void *p, const int64_t *strides, int n) {
 
 bool takes_tiles(const msx_window_attention_desc &d) {
   const size_t size = value_bytes(static_cast<msx_vtype>(d.vtype));
-  return d.dim <= 128 && d.dim * size % 16 == 0 && d.scale != 0.0 &&
+  return d.dim <= 128 && d.dim * size % 16 == 0 &&
+         std::fabs(static_cast<float>(d.scale)) >= std::numeric_limits<float>::min() &&
          rows_aligned(size, d.q, d.q_strides, 3) && rows_aligned(size, d.k, d.k_strides, 3) &&
          rows_aligned(size, d.v, d.v_strides, 3);
 }
