@@ -1057,7 +1057,7 @@ typedef struct msx_distill_desc {
   int32_t itype;         /* of indices and indptr */
   int32_t reserved;
   int64_t n_rows, n_cols, nnz, ld;
-  double temperature;    /* > 0 */
+  double temperature;    /* > 0, its square a normal float32 */
   const void *logits;
   const void *data, *indices, *indptr;
   const float *weights;

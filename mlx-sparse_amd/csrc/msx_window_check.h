@@ -117,6 +117,9 @@ inline msx_status check_distill(const char *op, const msx_distill_desc *d) {
     return fail(MSX_EINVAL, name + " leading dimension must be at least the column count.");
   if (!(d->temperature > 0.0) || !std::isfinite(d->temperature))
     return fail(MSX_EINVAL, name + " temperature must be positive and finite.");
+  // losses take its square, and logits are divided by it, in float32
+  if (!std::isnormal(static_cast<float>(d->temperature * d->temperature)))
+    return fail(MSX_EINVAL, name + " temperature must have a square that float32 holds.");
   if (d->indptr == nullptr) return fail(MSX_EINVAL, name + " indptr is NULL.");
   if (d->nnz > 0 && (d->data == nullptr || d->indices == nullptr))
     return fail(MSX_EINVAL, name + " data and indices must be non-NULL when nnz > 0.");

@@ -57,6 +57,10 @@ def _prepared(name: str, logits, teacher: CSRArray, temperature: float):
     temperature = float(temperature)
     if not (temperature > 0.0 and math.isfinite(temperature)):
         raise ValueError(f"{name} temperature must be positive and finite, got {temperature}.")
+    tiny, largest = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
+    if not tiny**0.5 <= temperature <= largest**0.5:
+        raise ValueError(f"{name} temperature must have a square that float32 holds, got "
+                         f"{temperature}.")
     return logits, teacher.buffers(device), temperature
 
 
@@ -123,7 +127,8 @@ def distill_loss(logits, teacher: CSRArray, *, temperature: float = 1.0) -> torc
         teacher: ``CSRArray`` of shape ``(tokens, vocabulary)``, ``tokens`` the
             product of the leading dimensions: the teacher's kept logits (of
             any of the three dtypes), columns in any order.
-        temperature: Divides both sides' logits.
+        temperature: Divides both sides' logits; between 1.1e-19 and 1.8e19,
+            where float32 holds its square.
 
     Returns:
         float32 losses of shape ``logits.shape[:-1]``, ``temperature**2`` times

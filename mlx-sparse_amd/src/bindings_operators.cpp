@@ -469,7 +469,7 @@ bool plain_distill(py::handle logits_o, py::handle data_o, py::handle indices_o,
 bool plain_temperature(py::handle o, double &t) {
   if (!PyFloat_CheckExact(o.ptr())) return false;
   t = PyFloat_AS_DOUBLE(o.ptr());
-  return t > 0.0 && std::isfinite(t);
+  return t > 0.0 && std::isnormal(static_cast<float>(t * t));
 }
 
 py::object distill_loss_plain(py::handle logits, py::handle data, py::handle indices,
