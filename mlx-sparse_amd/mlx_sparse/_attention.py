@@ -82,6 +82,18 @@ def _transformed() -> bool:
     return torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
 
 
+def _refuse_transforms(name: str, *operands) -> None:
+    """For calls that write in place and have no derivative."""
+    for t in operands:
+        if not isinstance(t, torch.Tensor):
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise NotImplementedError(f"{name} does not support torch.func transforms of its "
+                                      "operands.")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative.")
+
+
 class _WindowAttention(torch.autograd.Function):
     """``(out, lse, low)``; the last two are the backward pass's and have no
     derivative (``low``: what rounding left of a 16-bit ``out``, else None).
@@ -250,6 +262,8 @@ def window_attention_step(q, k, v, cache_k, cache_v, lengths, *, window: int, si
         differentiable.
     """
     name = "window_attention_step"
+    if _transformed():
+        _refuse_transforms(name, q, k, v, cache_k, cache_v, lengths)
     out = extension().window_attention_step_plain(q, k, v, cache_k, cache_v, lengths, window,
                                                   sinks, scale, default_device_index())
     if out is not None:
@@ -290,6 +304,8 @@ def window_cache_store(k, v, cache_k, cache_v, *, sinks: int = 0, starts=None,
         lengths: Tokens of each sequence here, all by default.
     """
     name = "window_cache_store"
+    if _transformed():
+        _refuse_transforms(name, k, v, cache_k, cache_v, starts, lengths)
     sinks = operator.index(sinks)
     device = default_torch_device()
     k, v = _operand(k, device).detach(), _operand(v, device).detach()

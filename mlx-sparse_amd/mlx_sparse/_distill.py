@@ -114,8 +114,31 @@ class _DistillGradient(torch.autograd.Function):
         raise NotImplementedError("second-order derivatives of distill_loss are not supported.")
 
 
-for _function in (_DistillLoss, _DistillGradient):
+class _DistillBoth(torch.autograd.Function):
+    """``(losses, gradient)`` under a transform, which must not lose a
+    derivative: there is none."""
+
+    @staticmethod
+    def forward(z, data, indices, indptr, weights, temperature):
+        return _native.distill_loss_grad(z, data, indices, indptr, weights, temperature)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError("derivatives of distill_value_and_grad are not supported: "
+                                  "distill_loss has one.")
+
+
+for _function in (_DistillLoss, _DistillGradient, _DistillBoth):
     _function.forward.__signature__ = inspect.signature(_function.forward)
+
+
+def _transformed() -> bool:
+    """A torch.func transform or a forward-mode level is active."""
+    return torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
 
 
 def distill_loss(logits, teacher: CSRArray, *, temperature: float = 1.0) -> torch.Tensor:
@@ -141,7 +164,7 @@ def distill_loss(logits, teacher: CSRArray, *, temperature: float = 1.0) -> torc
         TypeError: ``teacher`` is not a CSRArray or a dtype is unsupported.
         ValueError: shapes or ``temperature`` do not fit.
     """
-    transformed = torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
+    transformed = _transformed()
     if not transformed and type(teacher) is CSRArray:
         losses = extension().distill_loss_plain(logits, teacher.data, teacher.indices,
                                                 teacher.indptr, *teacher.shape, temperature,
@@ -178,7 +201,8 @@ def distill_value_and_grad(logits, teacher: CSRArray, weights=None, *,
         shaped as ``logits`` and of their dtype.
     """
     name = "distill_value_and_grad"
-    if type(teacher) is CSRArray:
+    transformed = _transformed()
+    if not transformed and type(teacher) is CSRArray:
         both = extension().distill_loss_grad_plain(logits, teacher.data, teacher.indices,
                                                    teacher.indptr, weights, *teacher.shape,
                                                    temperature, default_device_index())
@@ -189,7 +213,9 @@ def distill_value_and_grad(logits, teacher: CSRArray, weights=None, *,
     if weights is not None:
         if not isinstance(weights, torch.Tensor):
             weights = torch.as_tensor(weights, dtype=torch.float32)
-        weights = weights.detach().to(device=logits.device, dtype=torch.float32).resolve_neg()
+        if not transformed:
+            weights = weights.detach()
+        weights = weights.to(device=logits.device, dtype=torch.float32).resolve_neg()
         if weights.ndim == 0:
             weights = weights.expand(lead)
         if weights.shape != lead:
@@ -197,8 +223,11 @@ def distill_value_and_grad(logits, teacher: CSRArray, weights=None, *,
                              f"{tuple(weights.shape)}.")
         if weights.ndim != 1:
             weights = weights.reshape(-1)
-    losses, grad = _native.distill_loss_grad(_rows(logits.detach()), data, indices, indptr, weights,
-                                             temperature)
+    if transformed:
+        losses, grad = _DistillBoth.apply(_rows(logits), data, indices, indptr, weights, temperature)
+    else:
+        losses, grad = _native.distill_loss_grad(_rows(logits.detach()), data, indices, indptr,
+                                                 weights, temperature)
     if logits.ndim == 2:
         return losses, grad
     return losses.reshape(lead), grad.reshape(logits.shape)
