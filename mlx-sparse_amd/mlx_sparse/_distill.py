@@ -73,6 +73,26 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
     return z if usable else z.contiguous()
 
 
+def _mapped(t: torch.Tensor, dim: int | None, n: int) -> torch.Tensor:
+    """``n`` of ``t`` one after the other along its first dimension."""
+    t = t.unsqueeze(0).expand(n, *t.shape) if dim is None else t.movedim(dim, 0)
+    return t.reshape(n * t.shape[1], *t.shape[2:])
+
+
+def _teachers(n: int, in_dims, data, indices, indptr):
+    """The CSR buffers of a teacher for ``n`` mapped students, its rows once for each."""
+    if any(d is not None for d in in_dims):
+        raise ValueError("distillation vmap supports batching only the logits and weights: the "
+                         "teacher must be unmapped.")
+    nnz = data.shape[0]
+    if indptr.dtype == torch.int32 and n * nnz > torch.iinfo(torch.int32).max:
+        indices, indptr = indices.long(), indptr.long()
+    first = torch.arange(n, dtype=indptr.dtype, device=indptr.device)[:, None] * nnz
+    # of a row that ends a student's, the next one's start is the same entry
+    starts = (first + indptr[:-1]).reshape(-1)
+    return data.repeat(n), indices.repeat(n), torch.cat([starts, indptr[-1:] + (n - 1) * nnz])
+
+
 class _DistillLoss(torch.autograd.Function):
     """``(losses, lse)`` of rows of logits, under a transform; other calls
     have a node of the native module's."""
@@ -97,6 +117,14 @@ class _DistillLoss(torch.autograd.Function):
         return (_call(_DistillGradient, z, data, indices, indptr, grad, lse, ctx.temperature),
                 None, None, None, None)
 
+    @staticmethod
+    def vmap(info, in_dims, z, data, indices, indptr, temperature):
+        """The mapped students' rows are rows of one matrix."""
+        n, rows = info.batch_size, indptr.shape[0] - 1
+        buffers = _teachers(n, in_dims[1:4], data, indices, indptr)
+        got = _DistillLoss.apply(_rows(_mapped(z, in_dims[0], n)), *buffers, temperature)
+        return tuple(t.reshape(n, rows) for t in got), (0, 0)
+
 
 class _DistillGradient(torch.autograd.Function):
     """The gradient in the logits; no derivative of its own."""
@@ -112,6 +140,15 @@ class _DistillGradient(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *_):
         raise NotImplementedError("second-order derivatives of distill_loss are not supported.")
+
+    @staticmethod
+    def vmap(info, in_dims, z, data, indices, indptr, grad, lse, temperature):
+        n, rows = info.batch_size, indptr.shape[0] - 1
+        buffers = _teachers(n, in_dims[1:4], data, indices, indptr)
+        z = _rows(_mapped(z, in_dims[0], n))
+        got = _DistillGradient.apply(z, *buffers, _mapped(grad, in_dims[4], n),
+                                     _mapped(lse, in_dims[5], n).contiguous(), temperature)
+        return got.reshape(n, rows, z.shape[1]), 0
 
 
 class _DistillBoth(torch.autograd.Function):
@@ -130,6 +167,15 @@ class _DistillBoth(torch.autograd.Function):
     def backward(ctx, *_):
         raise NotImplementedError("derivatives of distill_value_and_grad are not supported: "
                                   "distill_loss has one.")
+
+    @staticmethod
+    def vmap(info, in_dims, z, data, indices, indptr, weights, temperature):
+        n, rows = info.batch_size, indptr.shape[0] - 1
+        buffers = _teachers(n, in_dims[1:4], data, indices, indptr)
+        z = _rows(_mapped(z, in_dims[0], n))
+        weights = None if weights is None else _mapped(weights, in_dims[4], n)
+        losses, grad = _DistillBoth.apply(z, *buffers, weights, temperature)
+        return (losses.reshape(n, rows), grad.reshape(n, rows, z.shape[1])), (0, 0)
 
 
 for _function in (_DistillLoss, _DistillGradient, _DistillBoth):
