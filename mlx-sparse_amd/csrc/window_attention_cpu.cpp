@@ -45,6 +45,12 @@ constexpr float kLowUp = 1.0f;
 template <>
 constexpr float kLowUp<F16> = 2048.0f;
 
+// Where the residues of query i, head h lie: a sequence's after the other's as on
+// the device (a batch can be cut or joined), a sequence's in out's order.
+int64_t low_at(const msx_window_attention_desc &d, int64_t b, int64_t i, int64_t h) {
+  return b * d.heads * ((d.lq + 31) / 32 * 32) * ((d.dim + 7) / 8 * 8) + (i * d.heads + h) * d.dim;
+}
+
 // Attention of one query over the listed rows; returns the base-2 logarithm
 // of the softmax's sum (+inf without one).  `low` (or null): what rounding
 // leaves of the output, as the device keeps it.
@@ -95,7 +101,7 @@ void forward(const msx_window_attention_desc &d, void *out, float *lse, int n_th
       const int64_t to = ((b * d.lq + i) * d.heads + h) * d.dim;
       const float l = attend<V>(at<V>(d.q, d.q_strides, b, i, h), k, v, d.dim,
                                 static_cast<float>(d.scale), s, o, static_cast<S *>(out) + to,
-                                low == nullptr ? nullptr : low + to);
+                                low == nullptr ? nullptr : low + low_at(d, b, i, h));
       if (lse != nullptr) lse[r] = l;
     }
   });
@@ -124,7 +130,7 @@ void backward(const msx_window_attention_desc &d, const void *out, const float *
           if (p >= 0 && p < n && l != INFINITY) {
             const S *q = at<V>(d.q, d.q_strides, b, i, h), *g = at<V>(grad, gs, b, i, h);
             float delta = dot<V>(g, static_cast<const S *>(out) + at_out, dim);
-            if (low != nullptr) delta += dot<V>(g, low + at_out, dim) / kLowUp<V>;
+            if (low != nullptr) delta += dot<V>(g, low + low_at(d, b, i, h), dim) / kLowUp<V>;
             each_seen(p, d.window, d.sinks, [&](int64_t j) {
               const S *k = at<V>(d.k, d.k_strides, b, j, kvh), *v = at<V>(d.v, d.v_strides, b, j, kvh);
               const float prob = std::exp2(dot<V>(q, k, dim) * scale * 1.44269504088896340736f - l);

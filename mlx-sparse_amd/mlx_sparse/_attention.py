@@ -94,6 +94,16 @@ def _refuse_transforms(name: str, *operands) -> None:
             raise NotImplementedError(f"{name} has no forward-mode derivative.")
 
 
+def _folded(t: torch.Tensor, dim: int | None, n: int) -> torch.Tensor:
+    """The mapped axis joins the batch."""
+    t = t.unsqueeze(0).expand(n, *t.shape) if dim is None else t.movedim(dim, 0)
+    return t.reshape(n * t.shape[1], *t.shape[2:])
+
+
+def _unfolded(outputs, n: int) -> tuple:
+    return tuple(t if t is None else t.unflatten(0, (n, t.shape[0] // n)) for t in outputs)
+
+
 class _WindowAttention(torch.autograd.Function):
     """``(out, lse, low)``; the last two are the backward pass's and have no
     derivative (``low``: what rounding left of a 16-bit ``out``, else None).
@@ -123,19 +133,12 @@ class _WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def vmap(info, in_dims, q, k, v, lengths, window, sinks, scale):
-        """The mapped axis joins the batch."""
         n = info.batch_size
-
-        def folded(t, dim):
-            t = t.unsqueeze(0).expand(n, *t.shape) if dim is None else t.movedim(dim, 0)
-            return t.reshape(n * t.shape[1], *t.shape[2:])
-
-        q, k, v = (folded(t, d) for t, d in zip((q, k, v), in_dims))
+        q, k, v = (_folded(t, d, n) for t, d in zip((q, k, v), in_dims))
         if lengths is not None:
-            lengths = folded(lengths, in_dims[3]).contiguous()
+            lengths = _folded(lengths, in_dims[3], n).contiguous()
         got = _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
-        return (tuple(t if t is None else t.reshape(n, -1, *t.shape[1:]) for t in got),
-                tuple(t if t is None else 0 for t in got))
+        return _unfolded(got, n), tuple(t if t is None else 0 for t in got)
 
 
 class _WindowGradients(torch.autograd.Function):
@@ -153,6 +156,16 @@ class _WindowGradients(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *_):
         raise NotImplementedError("second-order derivatives of window_attention are not supported.")
+
+    @staticmethod
+    def vmap(info, in_dims, q, k, v, lengths, out, lse, low, grad, window, sinks, scale):
+        n = info.batch_size
+        q, k, v, grad = (_folded(t, d, n) for t, d in zip((q, k, v, grad), (*in_dims[:3], in_dims[7])))
+        lengths, out, lse, low = (
+            t if t is None else _folded(t, d, n).contiguous()
+            for t, d in zip((lengths, out, lse, low), in_dims[3:7]))
+        got = _WindowGradients.apply(q, k, v, lengths, out, lse, low, grad, window, sinks, scale)
+        return _unfolded(got, n), (0, 0, 0)
 
 
 for _function in (_WindowAttention, _WindowGradients):
