@@ -3,7 +3,6 @@
 // ctx.stream; host operands: the native CPU entry point).
 #include "attention/window_attention.h"
 
-#include <algorithm>
 #include <string>
 
 #include "common/validate.h"
@@ -37,6 +36,12 @@ void require_shape(const ArrayView &a, std::initializer_list<int64_t> shape,
   }
   if (!ok)
     throw std::invalid_argument(name + " must have shape (" + want + "), got (" + got + ").");
+}
+
+// Strides of the leading dimensions; one of a single place is never used, and
+// whatever it is says nothing about alignment.
+void copy_strides(const ArrayView &a, int64_t *to) {
+  for (int i = 0; i + 1 < a.ndim; ++i) to[i] = a.shape[i] > 1 ? a.strides[i] : 0;
 }
 
 // The values of a head lie side by side.
@@ -88,9 +93,9 @@ msx_window_attention_desc window_attention_desc(const ArrayView &q, const ArrayV
   d.q = q.ptr;
   d.k = k.ptr;
   d.v = v.ptr;
-  std::copy(q.strides, q.strides + 3, d.q_strides);
-  std::copy(k.strides, k.strides + 3, d.k_strides);
-  std::copy(v.strides, v.strides + 3, d.v_strides);
+  copy_strides(q, d.q_strides);
+  copy_strides(k, d.k_strides);
+  copy_strides(v, d.v_strides);
   return d;
 }
 
@@ -112,11 +117,13 @@ void window_attention_backward(const msx_window_attention_desc &desc, const Arra
   require_same_device({&out, &grad, &dq, &dk, &dv}, op.c_str());
   require_packed(grad, op + " grad");
   for (const ArrayView *a : {&out, &dq, &dk, &dv}) require_contiguous(*a, "window_attention_backward array");
+  int64_t grad_strides[3];
+  copy_strides(grad, grad_strides);
   check_status(out.device >= 0
-                   ? msx_window_attention_backward(&desc, out.ptr, lse, grad.ptr, grad.strides,
+                   ? msx_window_attention_backward(&desc, out.ptr, lse, grad.ptr, grad_strides,
                                                    dq.ptr, dk.ptr, dv.ptr, ctx.scratch,
                                                    ctx.scratch_bytes, ctx.stream)
-                   : msx_window_attention_backward_cpu(&desc, out.ptr, lse, grad.ptr, grad.strides,
+                   : msx_window_attention_backward_cpu(&desc, out.ptr, lse, grad.ptr, grad_strides,
                                                        dq.ptr, dk.ptr, dv.ptr, ctx.n_threads),
                op.c_str());
 }
@@ -155,11 +162,11 @@ msx_window_step_desc window_step_desc(const ArrayView &q, const ArrayView &k, co
   d.v = v.ptr;
   d.cache_k = cache_k.ptr;
   d.cache_v = cache_v.ptr;
-  std::copy(q.strides, q.strides + 2, d.q_strides);
-  std::copy(k.strides, k.strides + 2, d.k_strides);
-  std::copy(v.strides, v.strides + 2, d.v_strides);
-  std::copy(cache_k.strides, cache_k.strides + 3, d.cache_k_strides);
-  std::copy(cache_v.strides, cache_v.strides + 3, d.cache_v_strides);
+  copy_strides(q, d.q_strides);
+  copy_strides(k, d.k_strides);
+  copy_strides(v, d.v_strides);
+  copy_strides(cache_k, d.cache_k_strides);
+  copy_strides(cache_v, d.cache_v_strides);
   return d;
 }
 
@@ -203,8 +210,8 @@ void window_cache_store(const ArrayView &k, const ArrayView &v, const ArrayView 
   d.sinks = sinks;
   d.cache_k = cache_k.ptr;
   d.cache_v = cache_v.ptr;
-  std::copy(cache_k.strides, cache_k.strides + 3, d.cache_k_strides);
-  std::copy(cache_v.strides, cache_v.strides + 3, d.cache_v_strides);
+  copy_strides(cache_k, d.cache_k_strides);
+  copy_strides(cache_v, d.cache_v_strides);
   const msx_itype it = counts != nullptr ? to_itype(counts->dtype) : MSX_I32;
   const void *s = starts != nullptr ? starts->ptr : nullptr;
   const void *n = lengths != nullptr ? lengths->ptr : nullptr;

@@ -86,6 +86,27 @@ Tensor made_direct(const Tensor &t) {
   return (t.is_neg() ? t.resolve_neg() : t).contiguous();
 }
 
+// Rows at sixteen-byte addresses, as the matrix cores' kernels read them; a
+// dimension of one has no stride.
+bool aligned_rows(const Tensor &t) {
+  const auto size = static_cast<int64_t>(t.element_size());
+  bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) < 2 || t.stride(i) * size % 16 == 0);
+  return ok;
+}
+// A device operand whose layout alone would keep its call from those kernels, at
+// such addresses: copying it costs a pass over it, the kernels for any layout 80
+// times the others' and more (a slice of what `cat` was given, as its backward
+// pass hands on, is such an operand).
+Tensor for_tiles(const Tensor &t, int64_t most_dim) {
+  const int64_t dim = t.size(-1);
+  if (!t.is_cuda() || dim > most_dim || dim * static_cast<int64_t>(t.element_size()) % 16 != 0 ||
+      aligned_rows(t))
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+constexpr int64_t kTilesDim = 128, kStepDim = 256;
+
 struct Pattern {
   int64_t window, sinks;
   double scale;
@@ -96,8 +117,10 @@ struct Attended {
 };
 
 // With `with_lse` what the backward pass reads: lse and low.
-Attended attention(const Tensor &q_t, const Tensor &k_t, const Tensor &v_t,
-                                     const Tensor &lengths_t, Pattern p, bool with_lse) {
+Attended attention(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in,
+                   const Tensor &lengths_t, Pattern p, bool with_lse) {
+  const Tensor q_t = for_tiles(q_in, kTilesDim), k_t = for_tiles(k_in, kTilesDim),
+               v_t = for_tiles(v_in, kTilesDim);
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t);
   const OptionalView lengths(lengths_t);
   auto desc = msx::window_attention_desc(q, k, v, lengths.get, p.window, p.sinks, p.scale);
@@ -118,11 +141,13 @@ Attended attention(const Tensor &q_t, const Tensor &k_t, const Tensor &v_t,
   return {out, lse, low};
 }
 
-std::tuple<Tensor, Tensor, Tensor> attention_gradients(const Tensor &q_t, const Tensor &k_t,
-                                                       const Tensor &v_t, const Tensor &lengths_t,
+std::tuple<Tensor, Tensor, Tensor> attention_gradients(const Tensor &q_in, const Tensor &k_in,
+                                                       const Tensor &v_in, const Tensor &lengths_t,
                                                        const Tensor &out_t, const Tensor &lse_t,
-                                                       const Tensor &low_t, const Tensor &grad_t,
+                                                       const Tensor &low_t, const Tensor &grad_in,
                                                        Pattern p) {
+  const Tensor q_t = for_tiles(q_in, kTilesDim), k_t = for_tiles(k_in, kTilesDim),
+               v_t = for_tiles(v_in, kTilesDim), grad_t = for_tiles(grad_in, kTilesDim);
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t), out = view_of(out_t),
                   lse = view_of(lse_t), grad = view_of(grad_t);
   const OptionalView lengths(lengths_t);
@@ -292,8 +317,13 @@ py::tuple window_attention_backward(py::handle q, py::handle k, py::handle v, py
 // ---------------------------------------------------------------------------
 // Single-token step.
 
-Tensor step(const Tensor &q_t, const Tensor &k_t, const Tensor &v_t, const Tensor &ck_t,
+Tensor step(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, const Tensor &ck_t,
             const Tensor &cv_t, const Tensor &lengths_t, Pattern p) {
+  // (caches are written in place, so none is copied)
+  const bool caches = aligned_rows(ck_t) && aligned_rows(cv_t);
+  const Tensor q_t = caches ? for_tiles(q_in, kStepDim) : q_in,
+               k_t = caches ? for_tiles(k_in, kStepDim) : k_in,
+               v_t = caches ? for_tiles(v_in, kStepDim) : v_in;
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t), ck = view_of(ck_t),
                   cv = view_of(cv_t), lengths = view_of(lengths_t);
   require_writable(ck_t, "window_attention_step cache_k");
