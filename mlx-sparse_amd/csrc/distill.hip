@@ -17,6 +17,7 @@
 // (5.1 TB/s).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "msx_device.h"
@@ -193,7 +194,8 @@ struct Columns {
 // from the row's own pass.
 // kHold: pieces a thread keeps in registers between the two passes.
 template <class V, bool kLoss, bool kGrad, int kThreads, int kHold>
-__global__ __launch_bounds__(kThreads, kHold > 0 ? 4 : 8) void distill_rows(DistillArgs a, float *losses, float *lse,
+__global__ __launch_bounds__(kThreads, kHold > 0 ? 4 : 8) void distill_rows(DistillArgs a, int64_t first_row,
+                                                         float *losses, float *lse,
                                                          const float *lse_in,
                                                          typename V::Storage *grad) {
   using S = typename V::Storage;
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(kThreads, kHold > 0 ? 4 : 8) void distill_rows(Dist
   __shared__ int ascending_lds[kWaves];
   __shared__ Columns<kGrad ? kThreads : 1> columns_lds;
   const int wave = threadIdx.x / kWave;
-  const int64_t row = blockIdx.x;
+  const int64_t row = first_row + blockIdx.x;
   const S *z = static_cast<const S *>(a.logits) + row * a.ld;
   S *g = kGrad ? grad + row * a.ld_grad : nullptr;
   const int64_t begin = a.offset(row), end = a.offset(row + 1);
@@ -417,12 +419,13 @@ msx_status launch(const msx_distill_desc &d, float *losses, float *lse, const fl
   const auto run = [&](auto v) {
     using V = decltype(v);
     using S = typename V::Storage;
-    const auto blocks = static_cast<unsigned>(d.n_rows);
     const auto st = static_cast<hipStream_t>(stream);
-    S *g = static_cast<S *>(grad);
     const int64_t kb = (d.n_cols * static_cast<int64_t>(sizeof(S)) + 1023) / 1024;
     const auto with = [&](auto kernel, unsigned threads) {
-      kernel<<<blocks, threads, 0, st>>>(a, losses, lse, lse_in, g);
+      for (int64_t first = 0; first < d.n_rows; first += max_blocks(threads)) {
+        const auto blocks = static_cast<unsigned>(std::min(d.n_rows - first, max_blocks(threads)));
+        kernel<<<blocks, threads, 0, st>>>(a, first, losses, lse, lse_in, static_cast<S *>(grad));
+      }
     };
     if constexpr (kLoss && kGrad) {
       // 256 bytes of the row a thread, in its registers, so that it is read

@@ -39,6 +39,9 @@ struct WindowArgs {
   }
 };
 
+// Workgroups of `threads` that one launch holds: it counts its threads in 32 bits.
+constexpr int64_t max_blocks(int64_t threads) { return 0xffffffff / threads; }
+
 // Logarithms are base 2: exp2 is one instruction, and a score times log2(e)
 // costs nothing beside the scale.
 constexpr float kLog2e = 1.44269504088896340736f;

@@ -46,12 +46,12 @@ __device__ inline float dot_row(const float *lds, const typename V::Storage *row
 // One wave a query row; a lane takes a key of each 64 for the scores and
 // head values lane, lane + 64, ... for the sum over them.
 template <class V>
-__global__ __launch_bounds__(kRowWaves * kWave) void forward_rows(WindowArgs a, int64_t rows,
+__global__ __launch_bounds__(kRowWaves * kWave) void forward_rows(WindowArgs a, int64_t first, int64_t rows,
                                                                   typename V::Storage *out,
                                                                   float *lse) {
   __shared__ float q_lds[kRowWaves][kWindowMaxDim];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;  // (b, i, h)
+  const int64_t row = first + static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;  // (b, i, h)
   if (row >= rows) return;  // whole waves leave; there is no barrier below
   const int32_t h = static_cast<int32_t>(row % a.heads);
   const int32_t i = static_cast<int32_t>(row / a.heads % a.lq);
@@ -105,13 +105,13 @@ __global__ __launch_bounds__(kRowWaves * kWave) void forward_rows(WindowArgs a, 
 // dq by query row; also leaves delta for the keys' pass.
 template <class V>
 __global__ __launch_bounds__(kRowWaves * kWave) void backward_rows(
-    WindowArgs a, int64_t rows, const typename V::Storage *out, const float *lse,
+    WindowArgs a, int64_t first_row, int64_t rows, const typename V::Storage *out, const float *lse,
     const typename V::Storage *grad, int64_t g0, int64_t g1, int64_t g2, float *delta_out,
     typename V::Storage *dq) {
   __shared__ float q_lds[kRowWaves][kWindowMaxDim];
   __shared__ float g_lds[kRowWaves][kWindowMaxDim];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;
+  const int64_t row = first_row + static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;
   if (row >= rows) return;
   const int32_t h = static_cast<int32_t>(row % a.heads);
   const int32_t i = static_cast<int32_t>(row / a.heads % a.lq);
@@ -164,13 +164,13 @@ __global__ __launch_bounds__(kRowWaves * kWave) void backward_rows(
 // it, over the heads of its group.
 template <class V>
 __global__ __launch_bounds__(kRowWaves * kWave) void backward_keys(
-    WindowArgs a, int64_t rows, const float *lse, const typename V::Storage *grad, int64_t g0,
+    WindowArgs a, int64_t first_row, int64_t rows, const float *lse, const typename V::Storage *grad, int64_t g0,
     int64_t g1, int64_t g2, const float *delta, typename V::Storage *dk,
     typename V::Storage *dv) {
   __shared__ float k_lds[kRowWaves][kWindowMaxDim];
   __shared__ float v_lds[kRowWaves][kWindowMaxDim];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;  // (b, j, kv head)
+  const int64_t row = first_row + static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;  // (b, j, kv head)
   if (row >= rows) return;
   const int32_t kvh = static_cast<int32_t>(row % a.kv_heads);
   const int32_t j = static_cast<int32_t>(row / a.kv_heads % a.lk);
@@ -307,9 +307,9 @@ struct StoreArgs {
 
 // One wave a (sequence, token, kv head).
 template <class S>
-__global__ __launch_bounds__(kRowWaves * kWave) void store_rows(StoreArgs a, int64_t rows) {
+__global__ __launch_bounds__(kRowWaves * kWave) void store_rows(StoreArgs a, int64_t first, int64_t rows) {
   const int lane = threadIdx.x % kWave;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowWaves + threadIdx.x / kWave;
+  const int64_t row = first + static_cast<int64_t>(blockIdx.x) * kRowWaves + threadIdx.x / kWave;
   if (row >= rows) return;
   const int32_t h = static_cast<int32_t>(row % a.kv_heads);
   const int32_t t = static_cast<int32_t>(row / a.kv_heads % a.tokens);
@@ -411,12 +411,13 @@ size_t delta_bytes(const msx_window_attention_desc &d) {
   return (sizeof(float) * static_cast<size_t>(d.batch * d.heads * d.lq) + 255) / 256 * 256;
 }
 
-// Workgroups of `waves` waves for `rows` waves; fails beyond one grid.
-msx_status grid_for(const char *op, int64_t rows, unsigned *blocks) {
-  const int64_t n = (rows + kRowWaves - 1) / kRowWaves;
-  if (n > kWindowIntMax) return fail(MSX_EINVAL, std::string(op) + " has more rows than a grid holds.");
-  *blocks = static_cast<unsigned>(n);
-  return MSX_OK;
+// fn(first row, workgroups) over `rows` rows, a wave each: launches of as many as
+// one holds.
+template <class Fn>
+void each_launch(int64_t rows, Fn &&fn) {
+  constexpr int64_t kMost = max_blocks(kRowWaves * kWave) * kRowWaves;
+  for (int64_t first = 0; first < rows; first += kMost)
+    fn(first, static_cast<unsigned>((std::min(rows - first, kMost) + kRowWaves - 1) / kRowWaves));
 }
 
 template <class Fn>
@@ -463,12 +464,12 @@ extern "C" msx_status msx_window_attention(const msx_window_attention_desc *desc
     return launch_window_forward(vt, a, out, lse, scratch, static_cast<hipStream_t>(stream));
   }
   const int64_t rows = a.batch * a.lq * a.heads;
-  unsigned blocks = 0;
-  if (msx_status st = grid_for("window_attention", rows, &blocks); st != MSX_OK) return st;
   return by_vtype(desc->vtype, [&](auto v) {
     using V = decltype(v);
-    forward_rows<V><<<blocks, kRowWaves * kWave, 0, static_cast<hipStream_t>(stream)>>>(
-        a, rows, static_cast<typename V::Storage *>(out), lse);
+    each_launch(rows, [&](int64_t first, unsigned blocks) {
+      forward_rows<V><<<blocks, kRowWaves * kWave, 0, static_cast<hipStream_t>(stream)>>>(
+          a, first, rows, static_cast<typename V::Storage *>(out), lse);
+    });
     return launched("window_attention");
   });
 }
@@ -507,9 +508,6 @@ extern "C" msx_status msx_window_attention_backward(const msx_window_attention_d
                                   static_cast<char *>(scratch) + delta_bytes(*desc),
                                   static_cast<hipStream_t>(stream));
   const int64_t q_rows = a.batch * a.lq * a.heads, k_rows = a.batch * a.lk * a.kv_heads;
-  unsigned q_blocks = 0, k_blocks = 0;
-  if (msx_status st = grid_for(op, q_rows, &q_blocks); st != MSX_OK) return st;
-  if (msx_status st = grid_for(op, k_rows, &k_blocks); st != MSX_OK) return st;
   const int64_t gs[3] = {queries ? grad_strides[0] : 0, queries ? grad_strides[1] : 0,
                          queries ? grad_strides[2] : 0};
   return by_vtype(desc->vtype, [&](auto v) {
@@ -517,14 +515,16 @@ extern "C" msx_status msx_window_attention_backward(const msx_window_attention_d
     using S = typename V::Storage;
     const auto s = static_cast<hipStream_t>(stream);
     float *delta = static_cast<float *>(scratch);
-    if (queries)
-      backward_rows<V><<<q_blocks, kRowWaves * kWave, 0, s>>>(
-          a, q_rows, static_cast<const S *>(out), lse, static_cast<const S *>(grad), gs[0], gs[1],
-          gs[2], delta, static_cast<S *>(dq));
-    if (keys)
-      backward_keys<V><<<k_blocks, kRowWaves * kWave, 0, s>>>(
-          a, k_rows, lse, static_cast<const S *>(grad), gs[0], gs[1], gs[2], delta,
+    each_launch(q_rows, [&](int64_t first, unsigned blocks) {
+      backward_rows<V><<<blocks, kRowWaves * kWave, 0, s>>>(
+          a, first, q_rows, static_cast<const S *>(out), lse, static_cast<const S *>(grad), gs[0],
+          gs[1], gs[2], delta, static_cast<S *>(dq));
+    });
+    each_launch(k_rows, [&](int64_t first, unsigned blocks) {
+      backward_keys<V><<<blocks, kRowWaves * kWave, 0, s>>>(
+          a, first, k_rows, lse, static_cast<const S *>(grad), gs[0], gs[1], gs[2], delta,
           static_cast<S *>(dk), static_cast<S *>(dv));
+    });
     return launched("window_attention_backward");
   });
 }
@@ -545,7 +545,7 @@ extern "C" msx_status msx_window_attention_step(const msx_window_step_desc *desc
   const msx_window_step_desc &d = *desc;
   if (d.batch == 0) return MSX_OK;
   if (out == nullptr) return fail(MSX_EINVAL, "window_attention_step out is NULL.");
-  if (d.batch * d.kv_heads > kWindowIntMax)
+  if (d.batch * d.kv_heads > max_blocks(kRowWaves * kWave))
     return fail(MSX_EINVAL, "window_attention_step has more rows than a grid holds.");
   const StepArgs a = args_of(d);
   const msx_vtype vt = static_cast<msx_vtype>(d.vtype);
@@ -594,12 +594,12 @@ extern "C" msx_status msx_window_cache_store(const msx_window_step_desc *desc, i
   std::copy(d.cache_k_strides, d.cache_k_strides + 3, a.cks);
   std::copy(d.cache_v_strides, d.cache_v_strides + 3, a.cvs);
   const int64_t rows = a.batch * a.tokens * a.kv_heads;
-  unsigned blocks = 0;
-  if (msx_status st = grid_for(op, rows, &blocks); st != MSX_OK) return st;
   const auto s = static_cast<hipStream_t>(stream);
-  if (d.vtype == MSX_F32)
-    store_rows<uint32_t><<<blocks, kRowWaves * kWave, 0, s>>>(a, rows);
-  else
-    store_rows<uint16_t><<<blocks, kRowWaves * kWave, 0, s>>>(a, rows);
+  each_launch(rows, [&](int64_t first, unsigned blocks) {
+    if (d.vtype == MSX_F32)
+      store_rows<uint32_t><<<blocks, kRowWaves * kWave, 0, s>>>(a, first, rows);
+    else
+      store_rows<uint16_t><<<blocks, kRowWaves * kWave, 0, s>>>(a, first, rows);
+  });
   return launched("window_cache_store");
 }

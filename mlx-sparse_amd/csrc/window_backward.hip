@@ -916,8 +916,9 @@ msx_status run(const WindowArgs &a, const Upstream &up, const QueryPlan &queries
   const int64_t of_keys =
       plan.cut.rest * (kBlockKeys / kJoinKeys) + bh * plan.far_units * (32 / kJoinKeys);
   const int64_t joined = of_keys + queries.cut.rest * (kWaves * 32 / kJoinQueries);
-  for (int64_t blocks : {queries.units, q_blocks, k_blocks, f_blocks, joined})
-    if (blocks >= 0x7fffffff)
+  static_assert(kThreads <= NearShape<V, DP>::kThreads, "the keys' pass has the most threads");
+  for (int64_t blocks : {q_blocks, k_blocks, f_blocks, joined})
+    if (queries.units > 0x7fffffff || blocks > max_blocks(NearShape<V, DP>::kThreads))
       return fail(MSX_EINVAL, "window_attention_backward has more rows than a grid holds.");
   if (q_blocks > 0)
     backward_queries<V, DP><<<static_cast<unsigned>(q_blocks), kThreads, 0, stream>>>(

@@ -421,7 +421,7 @@ msx_status run(const WindowArgs &a, void *out, float *lse, float *sums, size_t *
     *bytes = sizeof(float) * static_cast<size_t>(rows * g.cut.parts) * ForwardShape<V, DP>::kStride;
     return MSX_OK;
   }
-  if (g.units > 0x7fffffff || g.cut.items() > 0x7fffffff)
+  if (g.units > 0x7fffffff || std::max(g.cut.items(), rows / JoinShape<V, DP>::kRows) > max_blocks(kThreads))
     return fail(MSX_EINVAL, "window_attention has more rows than a grid holds.");
   auto *to = static_cast<typename V::Storage *>(out);
   forward_tiles<V, DP><<<static_cast<unsigned>(g.cut.items()), kThreads, 0, stream>>>(

@@ -368,7 +368,7 @@ msx_status run(const StepArgs &a, void *out, float *parts, hipStream_t stream) {
   using S = typename V::Storage;
   const int32_t splits = splits_for(a, StepShape<V, DP>::kKeys);
   const int64_t blocks = a.batch * a.kv_heads * head_tiles(a) * splits;
-  if (blocks > 0x7fffffff)
+  if (std::max(blocks, (a.batch * a.heads + kWaves - 1) / kWaves) > max_blocks(kThreads))
     return fail(MSX_EINVAL, "window_attention_step has more rows than a grid holds.");
   step_tiles<V, DP><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
       a, head_tiles(a), splits, static_cast<S *>(out), parts);
