@@ -66,7 +66,7 @@ def _prepared(name: str, logits, teacher: CSRArray, temperature: float):
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     """(rows, vocabulary) with adjacent columns, in place where they are."""
-    z = logits if logits.ndim == 2 else logits.reshape(-1, logits.shape[-1])
+    z = logits if logits.ndim == 2 else logits.flatten(0, -2)
     if z.is_neg():
         z = z.resolve_neg()
     usable = (z.shape[1] < 2 or z.stride(1) == 1) and (z.shape[0] < 2 or z.stride(0) >= z.shape[1])
