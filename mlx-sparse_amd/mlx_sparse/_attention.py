@@ -319,7 +319,7 @@ def window_cache_store(k, v, cache_k, cache_v, *, sinks: int = 0, starts=None,
     name = "window_cache_store"
     if _transformed():
         _refuse_transforms(name, k, v, cache_k, cache_v, starts, lengths)
-    sinks = operator.index(sinks)
+    _, sinks = _span(name, 1, sinks)
     device = default_torch_device()
     k, v = _operand(k, device).detach(), _operand(v, device).detach()
     cache_k, cache_v = _cache(name, cache_k, device), _cache(name, cache_v, device)

@@ -259,6 +259,8 @@ def distill_value_and_grad(logits, teacher: CSRArray, weights=None, *,
     if weights is not None:
         if not isinstance(weights, torch.Tensor):
             weights = torch.as_tensor(weights, dtype=torch.float32)
+        if weights.is_complex():
+            raise TypeError(f"{name} weights must be real, got {weights.dtype}.")
         if not transformed:
             weights = weights.detach()
         weights = weights.to(device=logits.device, dtype=torch.float32).resolve_neg()
