@@ -50,13 +50,13 @@ constexpr float kLn2 = 0.69314718055994530942f;
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
-// What rounding a result to 16 bits leaves of it, in 16 bits more: kept for
-// delta = grad.out of the backward pass, which is subtracted from dP and has to
-// be good to a rounding of the difference, not of itself.  float16's is held
-// 2^11 larger, so that it is as far above the subnormals as the result.
+// What a result has beyond its 16 bits, in 16 bits more: kept for delta =
+// grad.out of the backward pass, which is subtracted from dP and has to be good to
+// a rounding of the difference, not of itself.  float16's is held 2^10 larger, so
+// that it is as far above the subnormals as the result.
 template <class V>
 struct Residue {
-  static constexpr float kUp = V::kType == MSX_F16 ? 2048.0f : 1.0f;
+  static constexpr float kUp = V::kType == MSX_F16 ? 1024.0f : 1.0f;
   __device__ static inline typename V::Storage of(float x, typename V::Storage kept) {
     return V::narrow((x - V::widen(kept)) * kUp);
   }

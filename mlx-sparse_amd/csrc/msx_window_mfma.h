@@ -95,22 +95,24 @@ struct Mfma<F32> {
   static constexpr uint32_t kSign = 0x80000000u;
 };
 
-// The residues of a pair of results, rounded to `kept`.
+// What a pair of results has beyond `kept`.
 template <class V>
 __device__ __forceinline__ uint32_t residues(float x0, float x1, uint32_t kept) {
   return Mfma<V>::pack((x0 - V::widen(static_cast<uint16_t>(kept))) * Residue<V>::kUp,
                        (x1 - V::widen(static_cast<uint16_t>(kept >> 16))) * Residue<V>::kUp);
 }
 
-// Four results of a row in the operands' type, and their residues where asked for.
+// Four results of a row in the operands' type, and where asked for what
+// `better` ones have beyond that.
 template <class V>
-__device__ __forceinline__ void store_four(const float (&x)[4], typename V::Storage *out,
-                                           typename V::Storage *low) {
+__device__ __forceinline__ void store_four(const float (&x)[4], const float (&better)[4],
+                                           typename V::Storage *out, typename V::Storage *low) {
   if constexpr (sizeof(typename V::Storage) == 2) {
     const v2u w{Mfma<V>::pack(x[0], x[1]), Mfma<V>::pack(x[2], x[3])};
     *reinterpret_cast<v2u *>(out) = w;
     if (low != nullptr)
-      *reinterpret_cast<v2u *>(low) = v2u{residues<V>(x[0], x[1], w[0]), residues<V>(x[2], x[3], w[1])};
+      *reinterpret_cast<v2u *>(low) = v2u{residues<V>(better[0], better[1], w[0]),
+                                          residues<V>(better[2], better[3], w[1])};
   } else {
     *reinterpret_cast<v4f *>(out) = v4f{x[0], x[1], x[2], x[3]};
   }
@@ -226,8 +228,7 @@ struct Column<F32> {
 };
 
 // The sum of a column as the products take it: divided by this, probabilities
-// sum to one however they were rounded, and one that is nearly alone comes out
-// as one.
+// sum to one however they were rounded.
 __device__ __forceinline__ float rounded_sum(const Column<BF16> &c) {
   constexpr v2bf kOnes = {1.0f, 1.0f};
   float sum[2] = {0.0f, 0.0f};

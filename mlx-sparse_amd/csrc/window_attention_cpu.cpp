@@ -39,11 +39,11 @@ float dot(const typename V::Storage *x, const typename V::Storage *y, int64_t n)
   return acc;
 }
 
-// float16's residues are held 2^11 larger: see Residue in msx_window.h.
+// float16's residues are held 2^10 larger: see Residue in msx_window.h.
 template <class V>
 constexpr float kLowUp = 1.0f;
 template <>
-constexpr float kLowUp<F16> = 2048.0f;
+constexpr float kLowUp<F16> = 1024.0f;
 
 // Where the residues of query i, head h lie: a sequence's after the other's as on
 // the device (a batch can be cut or joined), a sequence's in out's order.

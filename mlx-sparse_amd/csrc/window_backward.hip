@@ -23,9 +23,8 @@
 // rounded once.  dS = P (dP - delta) is small beside dP and delta where P is
 // nearly one, so delta = grad.out takes out with its residue, 32 bits in all
 // (with out as rounded alone, dq of a head that keeps 98 % of its attention on
-// one key was 39 % off in bfloat16, 5 % in float16; now 0.24 and 0.03 %).  Writing and
-// reading residues costs 5 % of a step of 4 x 2,048 tokens, 4 % of one of
-// 16,384.
+// one key was 39 % off in bfloat16, 5 % in float16; now 0.24 and 0.03 %).  Residues
+// cost a step of 4 x 2,048 tokens 6 %, one of 16,384 5 %.
 //
 // Bound like the forward pass by products, exponentials and LDS reads taking
 // turns; the products are under way 30 % of the time.  16,384 tokens of 16

@@ -11,10 +11,11 @@
 //
 // Probabilities are rounded to the operands' 16 bits for the second product,
 // unnormalised and at most 2^8, as the matrix instruction takes them: their errors are
-// independent and no larger than the output's own rounding.  The output is
-// divided by the sum of the rounded ones, so that one that is nearly alone gives
-// its value row as it is (0 to 4 % of a prompt); lse takes the sum of the
-// exponentials themselves.  Scores, maximum, sums and output stay float32.
+// independent and no larger than the output's own rounding.  The residue that a
+// call with gradients keeps is of the output divided by the sum of the rounded
+// ones: where two keys share a query 85 to 1 the rounding of one would be a factor of
+// delta, and dq 21 % off in bfloat16 (0.7 so).  Scores, maximum, sums and output stay
+// float32.
 //
 // Bound by how a wave's matrix instructions, exponentials and LDS reads take
 // turns: a tile of 64 keys costs a wave 1,024 cycles of products, some 950 of
@@ -50,7 +51,7 @@ struct ForwardShape {
   // workgroups a CU: two hide each other's waits; wide float32 heads need the
   // registers of one (76 spilled with two at 128)
   static constexpr int kBlocks = T::kRowBytes > 256 ? 1 : 2;
-  static constexpr int kStride = DP + 4;  // of a row's sums, m, l and total in scratch
+  static constexpr int kStride = DP + 4;  // of a row's sums, m, l and taken in scratch
 };
 
 // A query row by its definition, one wave: keys over the lanes for the
@@ -195,9 +196,9 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
-  // l, the sum of what the products take, and total, that of the exponentials
-  // themselves, for lse; of this lane's keys only
-  float m = -INFINITY, base = 0.0f, l = 0.0f, total = 0.0f;
+  // l: the sum of exponentials; taken: that of what the products take of them, for
+  // the residues; of this lane's keys only
+  float m = -INFINITY, base = 0.0f, l = 0.0f, taken = 0.0f;
 
   const auto scores = [&](uint32_t tile, int t, v16f &to) {
 #pragma unroll
@@ -214,12 +215,9 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
       sum[r % 2] += e[r];
     }
     const Column<V> column(e);
-    if constexpr (T::kSize == 2) {
-      l += rounded_sum(column);
-      if (lse != nullptr) total += sum[0] + sum[1];
-    } else {
-      l += sum[0] + sum[1];
-    }
+    l += sum[0] + sum[1];
+    if constexpr (T::kSize == 2)
+      if (a.low != nullptr) taken += rounded_sum(column);
     return column;
   };
   // masks the scores of the tile at c0 and moves the maximum.  It is moved
@@ -251,7 +249,7 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
       m = grown;
       base = m == -INFINITY ? 0.0f : m;
       l *= shrink;
-      total *= shrink;
+      taken *= shrink;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -286,7 +284,7 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
   }
 
   l += other_half(l);
-  total = T::kSize == 2 ? total + other_half(total) : l;
+  taken += other_half(taken);
   if (item.slot >= 0) {  // a part: its sums as they are, joined by forward_join
     float *to = sums + ((item.slot * kWaves + wave) * kRows + lane % 32) * F::kStride;
 #pragma unroll
@@ -298,11 +296,11 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
     if (half == 0) {
       to[DP] = m;
       to[DP + 1] = l;
-      to[DP + 2] = total;
+      to[DP + 2] = taken;
     }
     return;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l, better = taken == 0.0f ? 0.0f : 1.0f / taken;
   bool odd = false;  // something is not finite: the row is computed anew
   if (live && i < a.lq) {
     const int64_t at = ((b * a.lq + i) * a.heads + h) * a.dim;
@@ -312,16 +310,17 @@ __global__ __launch_bounds__(kThreads, (ForwardShape<V, DP>::kBlocks)) void forw
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int d = dt * 32 + 2 * r + 4 * half;
-        float x[4];
+        float x[4], y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           x[j] = o[dt][r + j] * inv;
+          y[j] = o[dt][r + j] * better;
           odd = odd || !(fabsf(x[j]) < INFINITY);
         }
-        if (d < a.dim) store_four<V>(x, out + at + d, low == nullptr ? nullptr : low + d / 8 * 256);
+        if (d < a.dim) store_four<V>(x, y, out + at + d, low == nullptr ? nullptr : low + d / 8 * 256);
       }
     if (lse != nullptr && half == 0)
-      lse[(b * a.heads + h) * a.lq + i] = total == 0.0f ? INFINITY : m + log2_fast(total);
+      lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
   }
   uint64_t anew = __ballot(odd && p >= 0);
   anew = (anew | anew >> 32) & 0xffffffffu;
@@ -358,7 +357,7 @@ __global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t u
   bool odd = false;
   if (live) {
     const float *first = sums + rest * cut.parts * kPart + in_block * kStride;
-    float m = -INFINITY, l = 0.0f, total = 0.0f, o[4] = {};
+    float m = -INFINITY, l = 0.0f, taken = 0.0f, o[4] = {}, better[4];
 #pragma unroll 4
     for (int32_t part = 0; part < cut.parts; ++part) m = fmaxf(m, first[part * kPart + DP]);
     const float base = m == -INFINITY ? 0.0f : m;
@@ -367,7 +366,7 @@ __global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t u
       const float *from = first + part * kPart;
       const float f = exp2_fast(from[DP] - base);
       l += from[DP + 1] * f;
-      total += from[DP + 2] * f;
+      taken += from[DP + 2] * f;
       const v4f x = *reinterpret_cast<const v4f *>(from + min(d, DP - 4));
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] += x[j] * f;
@@ -375,15 +374,16 @@ __global__ __launch_bounds__(kThreads) void forward_join(WindowArgs a, int32_t u
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      better[j] = taken == 0.0f ? 0.0f : o[j] / taken;
       o[j] *= inv;
       odd = odd || (d < a.dim && !(fabsf(o[j]) < INFINITY));
     }
     if (d < a.dim) {
       const int64_t at = ((b * a.lq + i) * a.heads + h) * a.dim + d;
-      store_four<V>(o, out + at, a.low == nullptr ? nullptr : static_cast<typename V::Storage *>(a.low) + a.low_at(b, i, h, d));
+      store_four<V>(o, better, out + at, a.low == nullptr ? nullptr : static_cast<typename V::Storage *>(a.low) + a.low_at(b, i, h, d));
     }
     if (lse != nullptr && d == 0)
-      lse[(b * a.heads + h) * a.lq + i] = total == 0.0f ? INFINITY : m + log2_fast(total);
+      lse[(b * a.heads + h) * a.lq + i] = l == 0.0f ? INFINITY : m + log2_fast(l);
   }
   uint64_t anew = __ballot(odd && p >= 0 && p < a.length(b));
   while (anew != 0) {
