@@ -98,6 +98,7 @@ bool aligned_rows(const Tensor &t) {
 // such addresses: copying it costs a pass over it, the kernels for any layout 80
 // times the others' and more (a slice of what `cat` was given, as its backward
 // pass hands on, is such an operand).
+constexpr int64_t kTilesDim = 128, kStepDim = 256;
 Tensor for_tiles(const Tensor &t, int64_t most_dim) {
   const int64_t dim = t.size(-1);
   if (!t.is_cuda() || dim > most_dim || dim * static_cast<int64_t>(t.element_size()) % 16 != 0 ||
@@ -105,7 +106,22 @@ Tensor for_tiles(const Tensor &t, int64_t most_dim) {
     return t;
   return t.clone(at::MemoryFormat::Contiguous);
 }
-constexpr int64_t kTilesDim = 128, kStepDim = 256;
+// The head dimension that those kernels take for `t`'s: whole sixteen bytes, as
+// long as zeros are a third of it at most.
+int64_t padded_dim(const Tensor &t) {
+  const int64_t dim = t.size(-1), per = 16 / static_cast<int64_t>(t.element_size());
+  const int64_t padded = (dim + per - 1) / per * per;
+  return t.is_cuda() && padded <= kTilesDim && 2 * padded <= 3 * dim ? padded : dim;
+}
+// An operand of attention, with zeros beyond its heads' values (scores and
+// gradients do not see them) or at an address where either is all it lacks.
+Tensor attention_operand(const Tensor &t, int64_t padded) {
+  return padded == t.size(-1) ? for_tiles(t, kTilesDim)
+                              : at::constant_pad_nd(t, {0, padded - t.size(-1)});
+}
+Tensor without_padding(const Tensor &t, int64_t dim) {
+  return t.size(-1) == dim ? t : t.narrow(-1, 0, dim).contiguous();
+}
 
 struct Pattern {
   int64_t window, sinks;
@@ -119,8 +135,9 @@ struct Attended {
 // With `with_lse` what the backward pass reads: lse and low.
 Attended attention(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in,
                    const Tensor &lengths_t, Pattern p, bool with_lse) {
-  const Tensor q_t = for_tiles(q_in, kTilesDim), k_t = for_tiles(k_in, kTilesDim),
-               v_t = for_tiles(v_in, kTilesDim);
+  const int64_t dim = padded_dim(q_in);
+  const Tensor q_t = attention_operand(q_in, dim), k_t = attention_operand(k_in, dim),
+               v_t = attention_operand(v_in, dim);
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t);
   const OptionalView lengths(lengths_t);
   auto desc = msx::window_attention_desc(q, k, v, lengths.get, p.window, p.sinks, p.scale);
@@ -138,16 +155,18 @@ Attended attention(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in,
   Tensor scratch;
   if (q.device >= 0) scratch = msx::scratch_for(ctx, q_t, msx_window_attention_scratch(&desc));
   run_op(q, [&] { msx::window_attention(desc, vo, l, ctx); });
-  return {out, lse, low};
+  return {without_padding(out, q_in.size(-1)), lse, low};
 }
 
 std::tuple<Tensor, Tensor, Tensor> attention_gradients(const Tensor &q_in, const Tensor &k_in,
                                                        const Tensor &v_in, const Tensor &lengths_t,
-                                                       const Tensor &out_t, const Tensor &lse_t,
+                                                       const Tensor &out_in, const Tensor &lse_t,
                                                        const Tensor &low_t, const Tensor &grad_in,
                                                        Pattern p) {
-  const Tensor q_t = for_tiles(q_in, kTilesDim), k_t = for_tiles(k_in, kTilesDim),
-               v_t = for_tiles(v_in, kTilesDim), grad_t = for_tiles(grad_in, kTilesDim);
+  const int64_t dim = padded_dim(q_in);
+  const Tensor q_t = attention_operand(q_in, dim), k_t = attention_operand(k_in, dim),
+               v_t = attention_operand(v_in, dim), out_t = attention_operand(out_in, dim),
+               grad_t = attention_operand(grad_in, dim);
   const ArrayView q = view_of(q_t), k = view_of(k_t), v = view_of(v_t), out = view_of(out_t),
                   lse = view_of(lse_t), grad = view_of(grad_t);
   const OptionalView lengths(lengths_t);
@@ -180,7 +199,8 @@ std::tuple<Tensor, Tensor, Tensor> attention_gradients(const Tensor &q_in, const
     msx::window_attention_backward(desc, out, static_cast<const float *>(lse.ptr), grad, vq, vk,
                                    vv, ctx);
   });
-  return {dq, dk, dv};
+  const int64_t given = q_in.size(-1);
+  return {without_padding(dq, given), without_padding(dk, given), without_padding(dv, given)};
 }
 
 std::optional<Tensor> present(const Tensor &t) {

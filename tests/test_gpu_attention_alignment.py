@@ -70,3 +70,25 @@ def test_steps(gpu, dtype, dim):
     want = gpu.window_attention_step(q, k, v, *mirror, n, window=300, sinks=4)
     got = gpu.window_attention_step(odd(q), odd(k), odd(v), *caches, n, window=300, sinks=4)
     assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(caches, mirror))
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 100), (BF16, 121), (BF16, 33), (F16, 6), (F32, 30), (F32, 127), (F32, 3)])
+def test_heads_between_sixteen_bytes(gpu, dtype, dim):
+    """As the same heads with zeros beyond them."""
+    q, k, v, g = operands(dim, 2, 150, 150, 4, 2, dim, dtype, "cuda")
+    per = 16 // q.element_size()
+
+    def pad(t):
+        return torch.nn.functional.pad(t, (0, -dim % per))
+
+    pattern = {"window": 40, "sinks": 3, "lengths": torch.tensor([150, 70], device="cuda")}
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = gpu.window_attention(*leaves, **pattern)
+    got = (out.detach(), *torch.autograd.grad(out, leaves, g))
+    leaves = [pad(t).requires_grad_() for t in (q, k, v)]
+    out = gpu.window_attention(*leaves, scale=dim**-0.5, **pattern)
+    want = (out.detach(), *torch.autograd.grad(out, leaves, pad(g)))
+    for a, b in zip(got, want):
+        assert a.shape[-1] == dim and a.is_contiguous() and torch.equal(a, b[..., :dim])
+    with torch.no_grad():
+        assert torch.equal(gpu.window_attention(q, k, v, **pattern), got[0])
