@@ -11,10 +11,10 @@
 // that holds it, q - p rounded once.
 //
 // Memory bounds it: the logits read and the gradient written once, 2.1 GB for
-// 4,096 rows of 131,072 bfloat16, take 425 us (5.05 TB/s, what a copy reaches;
-// 470 with the row read twice); 2,000 rows of 50,257 take 68 us (90), 65 of
-// 1,009 float32 5.6.  The loss alone reads 2,049 rows of 50,001 float16 in 40 us
-// (5.1 TB/s).
+// 4,096 rows of 131,072 bfloat16, take 430 us (5.0 TB/s, what a copy reaches, over
+// one matrix again and again as over five in turn; 470 with the row read twice), the
+// gradient alone 397; 2,000 rows of 50,257 take 71 us (90), 65 of 1,009 float32 6.0.
+// The loss alone reads 2,049 rows of 50,001 float16 in 41 us (5.0 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -39,9 +39,9 @@ struct DistillArgs {
   const float *weights;
   int64_t weights_stride;
   float scale;        // log2(e) / T: scaled logits are kept in base 2
-  float temperature;
+  float temperature;  // T^2 of a loss and T of a gradient come from it
 
-  // T^2 of a row's loss comes from these two.
+  // A row's first entry, as far as there are any.
   __device__ inline int64_t offset(int64_t r) const {
     const int64_t p = index64 ? static_cast<const int64_t *>(indptr)[r]
                               : static_cast<const int32_t *>(indptr)[r];

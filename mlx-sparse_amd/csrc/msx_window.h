@@ -44,7 +44,6 @@ constexpr int64_t max_blocks(int64_t threads) { return 0xffffffff / threads; }
 
 // Logarithms are base 2: exp2 is one instruction, and a score times log2(e)
 // costs nothing beside the scale.
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -402,9 +402,10 @@ struct TailCut {
 };
 
 // The launch that joins one part a slot takes 5 to 8 us, a tile 1 to 3, the most in
-// float32: 128 bfloat16 key blocks are not worth two parts each (2 x 1,000 tokens
-// of 8 heads of 128: 94 us, 84 whole), 45 float32 ones are worth five (3 x 517
-// tokens of 6 heads of 64: 89 us, 104 in eleven parts).
+// float32: 128 bfloat16 key blocks are not worth two parts each (a backward pass of
+// 2 x 1,000 tokens of 8 heads of 128: 92 us, 80 whole).  For float32 it says little: 45
+// key blocks (3 x 517 tokens of 6 heads of 64) take 73 us in five parts, and 70 with
+// joining held to cost nothing.
 inline double join_cost(bool float32) { return float32 ? 2.0 : 6.0; }
 
 // Costs in tiles, of which a block has `tiles`: a part more for its start and

@@ -27,9 +27,9 @@
 // cost a step of 4 x 2,048 tokens 6 %, one of 16,384 5 %.
 //
 // Bound like the forward pass by products, exponentials and LDS reads taking
-// turns; the products are under way 30 % of the time.  16,384 tokens of 16
-// heads of 128 on 8, a window of 1,024: queries 293 us, keys 384 (both about
-// 700 TFLOP/s), sinks 30, joining 9.
+// turns; the products are under way a third of the time.  16,384 tokens of 16
+// heads of 128 on 8, a window of 1,024: queries 277 us, keys 327 (790 and 840
+// TFLOP/s of what they multiply), sinks 29, joining 9.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -558,7 +558,9 @@ struct NearShape {
   static constexpr int kGroups = kInLds ? 2 : 1;  // waves of the same keys
   static constexpr int kThreads = kGroups * kWaves * kWave;
   // all but wide float32 heads fit twice (at 64: 3 to 7 % of a backward pass;
-  // a third wave spills, 145 us become 204)
+  // a third wave spills, 145 us become 204).  float32 heads of 128 do not fit once:
+  // 17 registers spill here and 42 in the far pass (4,096 tokens, 8 heads on 2,
+  // window 1,024: a training step 891 us, 178 in bfloat16)
   static constexpr int kWavesASimd = kInLds || DP <= 64 ? 2 : 1;
   static constexpr int kSub = T::kSize == 2 ? 2 : 1, kTokens = 32 * kSub;
   using Tile = QueryTile<V, DP, kTokens, kThreads>;

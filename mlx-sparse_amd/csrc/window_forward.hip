@@ -20,10 +20,11 @@
 // Bound by how a wave's matrix instructions, exponentials and LDS reads take
 // turns: a tile of 64 keys costs a wave 1,024 cycles of products, some 950 of
 // vector instructions and 2 x 16 KB of LDS, and with two waves a SIMD the
-// products are under way a third of the time, without a bank conflict.  8,192
-// tokens of 32 heads of 128 on 8, a window of 1,024: 167 us, 770 TFLOP/s of
+// products are under way 30 % of the time, without a bank conflict.  A call of 8,192
+// tokens of 32 heads of 128 on 8, a window of 1,024: 177 us, 730 TFLOP/s of
 // the work that the window needs (a large matrix product reaches 1,199); 4,099
-// on 20,001 keys, 16 heads on 8, a window of 4,096, float16: 156 us, 880.
+// on 20,001 keys, 16 heads on 8, a window of 4,096, float16: 165 us, 840, of which
+// 6 are the join's.  float32, 8,192 tokens as above: 1,270 us, 102 (a large product 153).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -8,9 +8,10 @@
 // workgroup, and over workgroups where sequences and heads are too few to fill
 // the chip; what they have is joined by exp(m - max m).
 //
-// 64 sequences of 4,100 keys, 32 heads of 128 on 8, bfloat16: 1.08 GB in 197
-// us, 5.5 TB/s (a copy moves 5.1); 37 of up to 1,001 keys, 24 heads of 96 on
-// 8: 24 us, 3.4 TB/s, of which a third is the launch.
+// 64 sequences of 4,100 keys, 32 heads of 128 on 8, bfloat16: 1.08 GB in 198
+// us, 5.4 TB/s, over one pair of caches as over six in turn (a copy moves 5.1, reading
+// and writing; float32 365 us, 5.9 TB/s); 37 of up to 1,001 keys, 24 heads of 96 on
+// 8: 25 to 27 us, 3.1 TB/s, of which a third is the launch.
 //
 // A probability enters its products as two 16-bit values, rounded and what that
 // leaves: 16 bits would add half as much again to the error of rounding the

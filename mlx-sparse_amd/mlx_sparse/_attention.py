@@ -199,11 +199,16 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale: float | Non
         Differentiable once in ``q``, ``k`` and ``v``.
 
     Operands are float32, float16 or bfloat16, of one dtype, ``dim`` at most
-    256; any strides with adjacent head values are read in place.  Scores,
-    softmax and sums are float32; 16-bit operands round probabilities to their
-    own type for the products with values, which costs no more than the
-    rounding of the result.  Gradients are summed in a fixed order; a visible
-    token that is not finite reaches those of tokens near it too.
+    256; strides with adjacent head values whose rows start at sixteen bytes
+    are read in place, others copied.  Heads above 128 do not run on the matrix
+    cores yet: 60 to 100 times slower than heads of 128, 250 and more with
+    gradients (the single-token step takes them as fast as any).
+
+    Scores, softmax and sums are float32; 16-bit operands round probabilities
+    to their own type for the products with values, which costs no more than
+    the rounding of the result.  A call with gradients keeps 16 bits more of
+    each 16-bit output for them.  Gradients are summed in a fixed order; a
+    visible token that is not finite reaches those of tokens near it too.
 
     Raises:
         TypeError: dtypes differ or are unsupported.
@@ -263,7 +268,9 @@ def window_attention_step(q, k, v, cache_k, cache_v, lengths, *, window: int, si
         q: Queries, shape ``(batch, heads, dim)``.
         k, v: The tokens' keys and values, shape ``(batch, kv_heads, dim)``.
         cache_k, cache_v: Ring caches, shape ``(batch, slots, kv_heads,
-            dim)``, updated in place; on the selected device.
+            dim)``, updated in place; on the selected device.  Rows that do not
+            start at sixteen bytes (a ``dim`` of 100 float16 values) take
+            slower kernels, one wave a query head.
         lengths: Tokens before this one, shape ``(batch,)``, int32 or int64
             (not changed: one counter serves the caches of all layers).  A
             negative length marks a slot of the batch without a sequence: its

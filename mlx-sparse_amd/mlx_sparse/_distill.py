@@ -195,7 +195,8 @@ def distill_loss(logits, teacher: CSRArray, *, temperature: float = 1.0) -> torc
             float16 or bfloat16.
         teacher: ``CSRArray`` of shape ``(tokens, vocabulary)``, ``tokens`` the
             product of the leading dimensions: the teacher's kept logits (of
-            any of the three dtypes), columns in any order.
+            any of the three dtypes), columns in any order (that of
+            ``topk``, too); a column stored twice counts twice.
         temperature: Divides both sides' logits; between 1.1e-19 and 1.8e19,
             where float32 holds its square.
 
