@@ -5,7 +5,8 @@
  * CSR SpMV (y = A x) and CSR SpMM with a dense row-major right-hand side
  * (Y = A X), with what stands next to it: solvers, the adjoint side, Matrix
  * Market input, and two operators of language models over sparse patterns
- * (window attention with sinks, distillation from a CSR teacher).  Every entry
+ * (window attention with sinks, rotary positions, attention over paged caches,
+ * distillation from a CSR teacher).  Every entry
  * point takes plain pointers and sizes; no C++ or framework type crosses it.
  *
  * Conventions
@@ -1070,6 +1071,103 @@ msx_status msx_distill_grad(const msx_distill_desc *desc, const float *lse, void
 msx_status msx_distill_loss_grad(const msx_distill_desc *desc, float *losses, void *grad,
                                  int64_t ld_grad, void *stream);
 
+/*
+ * Rotary positions.  The leading `dim` values of a head are pairs: (2 i, 2 i + 1)
+ * where interleaved, else (i, i + dim / 2).  At position p pair i is turned by
+ * turns[i] p whole turns:
+ *
+ *   (a, b) -> magnitude (a cos - b sin, a sin + b cos)
+ *
+ * and back where `inverse` (the gradient).  Values from `dim` on are copied.  Angles
+ * are worked out in 64 bits, products in float32, rounded once.
+ */
+typedef struct msx_rotation {
+  int64_t dim;         /* even, at most the head's; 0: nothing is rotated */
+  int32_t interleaved;
+  int32_t inverse;
+  double magnitude;
+  const double *turns; /* dim / 2, where the operands are */
+} msx_rotation;
+
+typedef struct msx_rotary_desc {
+  int32_t vtype; /* MSX_F32, MSX_F16 or MSX_BF16 */
+  int32_t itype; /* of starts or positions */
+  int64_t batch, tokens, heads, dim; /* dim 1 .. 256 */
+  const void *x;
+  int64_t x_strides[3];          /* (sequence, token, head), in values */
+  /* token t of sequence b is at positions[b, t], else at starts[b] + t, else at t */
+  const void *starts;            /* batch values, or NULL */
+  const void *positions;         /* or NULL */
+  int64_t position_strides[2];   /* (sequence, token) */
+  msx_rotation rotation;
+} msx_rotary_desc;
+
+/* `out` is batch x tokens x heads x dim, contiguous. */
+msx_status msx_rotary(const msx_rotary_desc *desc, void *out, void *stream);
+
+/*
+ * A paged cache.  Position j of a sequence lies in slot j % page_size of page
+ * pages[b, j / page_size].  Numbers outside [0, n_pages) are pages that are not
+ * there: nothing is written to them, and their keys are not seen; positions from
+ * width * page_size on have none.
+ */
+typedef struct msx_paged_cache {
+  int64_t n_pages, page_size, kv_heads, dim; /* width * page_size < 2^30 */
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3]; /* (page, slot, head), in values */
+  const void *pages;                  /* batch rows of `width` numbers */
+  int64_t pages_stride, width;
+  int32_t pages_itype;
+  int32_t reserved;
+} msx_paged_cache;
+
+/*
+ * Keys and values into a paged cache, the keys rotated on the way: token t of
+ * sequence b goes to position starts[b] + t (`starts` NULL: t), where t <
+ * lengths[b] (NULL: all) and starts[b] >= 0.  With heads > 0 `q_out` (batch x
+ * tokens x heads x dim, contiguous) gets the queries rotated at the same positions,
+ * zeros for tokens that are not there.  Tokens of one call go to different places;
+ * of two that do not, the values kept are any of both.
+ */
+typedef struct msx_paged_append_desc {
+  int32_t vtype, itype; /* itype: of starts and lengths */
+  int64_t batch, tokens, heads;
+  const void *q, *k, *v;
+  int64_t q_strides[3], k_strides[3], v_strides[3]; /* (sequence, token, head) */
+  const void *starts, *lengths;
+  msx_paged_cache cache;
+  msx_rotation rotation;
+} msx_paged_append_desc;
+
+msx_status msx_paged_cache_append(const msx_paged_append_desc *desc, void *q_out, void *stream);
+
+/*
+ * Attention over a paged cache.  Query t of sequence b stands at position p =
+ * starts[b] + t (`starts` NULL: t) and sees key j where j <= p and (p - j < window or
+ * j < sinks).  Queries with t >= lengths[b] (NULL: all are there), sequences with a
+ * negative start, and queries that see nothing give zeros.  `out` is batch x
+ * tokens x heads x dim, contiguous.
+ *
+ * shared_pages: the first so many pages are the same in every row of the table, those of
+ * its first row; where the queries are few, they are read once for all of them.
+ *
+ * `scratch` holds msx_paged_attention_scratch bytes at a sixteen-byte address.
+ */
+typedef struct msx_paged_attention_desc {
+  int32_t vtype, itype; /* itype: of starts and lengths */
+  int64_t batch, tokens, heads;
+  int64_t window, sinks, shared_pages;
+  double scale;
+  const void *q;
+  int64_t q_strides[3]; /* (sequence, token, head) */
+  const void *starts, *lengths;
+  msx_paged_cache cache;
+} msx_paged_attention_desc;
+
+size_t msx_paged_attention_scratch(const msx_paged_attention_desc *desc);
+msx_status msx_paged_attention(const msx_paged_attention_desc *desc, void *out, void *scratch,
+                               size_t scratch_bytes, void *stream);
+
 /* The same on the host: one row, head or token after the other, in float32
  * sums, split over `n_threads` threads (0: msx_cpu_worker_count). */
 msx_status msx_window_attention_cpu(const msx_window_attention_desc *desc, void *out, float *lse,
@@ -1084,6 +1182,10 @@ msx_status msx_window_cache_store_cpu(const msx_window_step_desc *desc, int64_t 
                                       const void *k, const int64_t *k_strides, const void *v,
                                       const int64_t *v_strides, msx_itype itype,
                                       const void *starts, const void *lengths);
+msx_status msx_rotary_cpu(const msx_rotary_desc *desc, void *out, int n_threads);
+msx_status msx_paged_cache_append_cpu(const msx_paged_append_desc *desc, void *q_out,
+                                      int n_threads);
+msx_status msx_paged_attention_cpu(const msx_paged_attention_desc *desc, void *out, int n_threads);
 msx_status msx_distill_loss_cpu(const msx_distill_desc *desc, float *losses, float *lse,
                                 int n_threads);
 msx_status msx_distill_grad_cpu(const msx_distill_desc *desc, const float *lse, void *grad,

@@ -88,6 +88,7 @@ def build(verbose: bool = True) -> Path:
                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
     py_inc = sysconfig.get_paths()["include"]
     bind_srcs = [SRC / "bindings.cpp", SRC / "bindings_operators.cpp",
+                 SRC / "bindings_paged.cpp",
                  SRC / "common" / "validate.cpp",
                  SRC / "sparse" / "csr_matvec" / "csr_matvec.cpp",
                  SRC / "sparse" / "csr_matmul" / "csr_matmul.cpp",
@@ -95,7 +96,8 @@ def build(verbose: bool = True) -> Path:
                  SRC / "sparse" / "csr_batched_matmul" / "csr_batched_matmul.cpp",
                  SRC / "sparse" / "csr_adjoint" / "csr_adjoint.cpp",
                  SRC / "linalg" / "csr_cg.cpp", SRC / "linalg" / "csr_krylov.cpp",
-                 SRC / "attention" / "window_attention.cpp", SRC / "loss" / "distill.cpp"]
+                 SRC / "attention" / "window_attention.cpp",
+                 SRC / "attention" / "paged_attention.cpp", SRC / "loss" / "distill.cpp"]
     bind_objs = []
     for s in bind_srcs:
         o = BUILD / ("bind_" + s.stem + ".o")

@@ -19,6 +19,8 @@ from mlx_sparse._ops import (
     csr_matvec,
     csr_matvec_transpose,
 )
+from mlx_sparse._paged import paged_attention, paged_cache_append
+from mlx_sparse._rotary import Rotary, rotary
 from mlx_sparse._typing import INDEX_DTYPES, VALUE_DTYPES, is_available
 
 
@@ -33,6 +35,7 @@ def capabilities() -> dict:
 __all__ = [
     "CSRArray",
     "INDEX_DTYPES",
+    "Rotary",
     "VALUE_DTYPES",
     "capabilities",
     "csr_array",
@@ -50,6 +53,9 @@ __all__ = [
     "linalg",
     "mminfo",
     "mmread",
+    "paged_attention",
+    "paged_cache_append",
+    "rotary",
     "runtime",
     "use_cpu",
     "use_device",

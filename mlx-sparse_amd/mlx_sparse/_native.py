@@ -184,6 +184,25 @@ def window_cache_store(k, v, cache_k, cache_v, starts, lengths, sinks: int) -> N
     extension().window_cache_store(k, v, cache_k, cache_v, starts, lengths, sinks)
 
 
+def rotary(x, starts, positions, rotation, inverse: bool) -> torch.Tensor:
+    """Heads rotated by their tokens' positions, or back; ``rotation``: (turns a
+    position, dim, interleaved, magnitude)."""
+    return extension().rotary(x, starts, positions, rotation, inverse)
+
+
+def paged_cache_append(k, v, cache_k, cache_v, pages, starts, lengths, rotation, q):
+    """Keys and values into a paged cache, in place; the rotated queries, or None."""
+    return extension().paged_cache_append(k, v, cache_k, cache_v, pages, starts, lengths, rotation,
+                                          q)
+
+
+def paged_attention(q, cache_k, cache_v, pages, starts, lengths, window: int, sinks: int,
+                    scale: float, shared_pages: int) -> torch.Tensor:
+    """Attention of every sequence's last tokens over its pages."""
+    return extension().paged_attention(q, cache_k, cache_v, pages, starts, lengths, window, sinks,
+                                       scale, shared_pages)
+
+
 def distill_loss(logits, data, indices, indptr, temperature: float, with_lse: bool):
     """(losses, lse or None) against a CSR teacher's kept logits."""
     return extension().distill_loss(logits, data, indices, indptr, temperature, with_lse)

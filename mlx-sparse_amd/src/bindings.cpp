@@ -739,6 +739,7 @@ PYBIND11_MODULE(_ext, m) {
         "matrix (slice_mode 0 auto, 1 off, 2 column slices per XCD, 3 LDS column panels; "
         "defer: auto's panels wait where only many products repay them).");
   bind_operators(m);
+  bind_paged(m);
   m.def("csr_matvec", &csr_matvec, py::arg("data"), py::arg("indices"), py::arg("indptr"),
         py::arg("x"), py::arg("n_rows"), py::arg("n_cols"), py::arg("plan") = py::none(),
         py::arg("n_threads") = 0, "Multiply CSR buffers by a dense vector.");

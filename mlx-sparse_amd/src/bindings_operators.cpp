@@ -17,95 +17,37 @@
 #include <tuple>
 
 #include "attention/window_attention.h"
-#include "common/torch_view.h"
-#include "common/validate.h"
+#include "bindings_operands.h"
 #include "loss/distill.h"
 #include "msx_sparse.h"
 
 namespace py = pybind11;
-using at::Tensor;
+using msx::aligned_rows;
 using msx::ArrayView;
+using msx::direct;
 using msx::DType;
+using msx::for_tiles;
+using msx::kStepDim;
+using msx::kTilesDim;
+using msx::made_direct;
+using msx::new_tensor;
+using msx::on_device;
+using msx::optional_tensor;
+using msx::OptionalView;
+using msx::present;
+using msx::real_type;
+using msx::require_writable;
+using msx::run_op;
 using msx::tensor_of;
+using msx::usable;
+using msx::usable_counts;
 using msx::view_of;
+using msx::wrap;
+using msx::written;
+using at::Tensor;
 
 namespace {
 
-// A view of a tensor that may be absent.
-struct OptionalView {
-  ArrayView view;
-  const ArrayView *get = nullptr;
-  explicit OptionalView(const Tensor &t) {
-    if (!t.defined()) return;
-    view = view_of(t);
-    get = &view;
-  }
-  OptionalView(const OptionalView &) = delete;
-  OptionalView &operator=(const OptionalView &) = delete;
-};
-
-Tensor optional_tensor(py::handle o) { return o.is_none() ? Tensor() : tensor_of(o); }
-
-Tensor new_tensor(const Tensor &like, std::initializer_list<int64_t> shape, at::ScalarType dtype) {
-  return at::empty(at::IntArrayRef(shape), at::TensorOptions().dtype(dtype).device(like.device()));
-}
-
-py::object wrap(const Tensor &t) {
-  if (!t.defined()) return py::none();
-  return py::reinterpret_steal<py::object>(THPVariable_Wrap(t));
-}
-
-// What is written in place has a place for every value.
-void require_writable(const Tensor &t, const char *name) {
-  for (int64_t i = 0; i < t.dim(); ++i)
-    if (t.size(i) > 1 && t.stride(i) == 0)
-      throw std::invalid_argument(std::string(name) +
-                                  " is written in place and cannot be an expanded tensor.");
-}
-
-// A write that torch did not make: a derivative that saved the tensor, or a view
-// of it, raises as after torch's own in-place operations.
-void written(const Tensor &t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-// Runs `fn`; without the interpreter lock where it works on the host.
-template <class Fn>
-void run_op(const ArrayView &v, Fn &&fn) {
-  std::optional<py::gil_scoped_release> nogil;
-  if (v.device < 0 && PyGILState_Check()) nogil.emplace();
-  fn();
-}
-
-// Adjacent values in the last dimension, no lazy sign.
-bool direct(const Tensor &t) {
-  return !t.is_neg() && (t.dim() == 0 || t.size(-1) < 2 || t.stride(-1) == 1);
-}
-Tensor made_direct(const Tensor &t) {
-  if (direct(t)) return t;
-  return (t.is_neg() ? t.resolve_neg() : t).contiguous();
-}
-
-// Rows at sixteen-byte addresses, as the matrix cores' kernels read them; a
-// dimension of one has no stride.
-bool aligned_rows(const Tensor &t) {
-  const auto size = static_cast<int64_t>(t.element_size());
-  bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) < 2 || t.stride(i) * size % 16 == 0);
-  return ok;
-}
-// A device operand whose layout alone would keep its call from those kernels, at
-// such addresses: copying it costs a pass over it, the kernels for any layout 80
-// times the others' and more (a slice of what `cat` was given, as its backward
-// pass hands on, is such an operand).
-constexpr int64_t kTilesDim = 128, kStepDim = 256;
-Tensor for_tiles(const Tensor &t, int64_t most_dim) {
-  const int64_t dim = t.size(-1);
-  if (!t.is_cuda() || dim > most_dim || dim * static_cast<int64_t>(t.element_size()) % 16 != 0 ||
-      aligned_rows(t))
-    return t;
-  return t.clone(at::MemoryFormat::Contiguous);
-}
 // The head dimension that those kernels take for `t`'s: whole sixteen bytes, as
 // long as zeros are a third of it at most.
 int64_t padded_dim(const Tensor &t) {
@@ -203,10 +145,6 @@ std::tuple<Tensor, Tensor, Tensor> attention_gradients(const Tensor &q_in, const
   return {without_padding(dq, given), without_padding(dk, given), without_padding(dv, given)};
 }
 
-std::optional<Tensor> present(const Tensor &t) {
-  return t.defined() ? std::optional<Tensor>(t) : std::nullopt;
-}
-
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -257,21 +195,6 @@ struct Attention : torch::autograd::Function<Attention> {
     return result;
   }
 };
-
-bool on_device(const Tensor &t, int64_t device) {
-  return device < 0 ? t.is_cpu() : t.is_cuda() && t.device().index() == device;
-}
-
-bool usable(const Tensor &t, at::ScalarType type, int64_t device) {
-  return t.scalar_type() == type && on_device(t, device) && direct(t);
-}
-
-bool real_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
-
-bool usable_counts(const Tensor &t, int64_t batch, int64_t device) {
-  return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.dim() == 1 &&
-         t.size(0) == batch && on_device(t, device) && t.is_contiguous() && !t.is_neg();
-}
 
 // A span given as plain integers in range.
 bool plain_span(py::handle window, py::handle sinks, Pattern &p) {
