@@ -1,10 +1,5 @@
 // paged_attention.hip - attention over paged caches: the entry points, and the row
 // kernel that takes every type, head dimension, alignment and page size.
-//
-// For a query at position p (sees keys [p - window + 1, p] and [0, sinks)):
-//   s_j = scale q.k_j,  out = sum_j exp(s_j) v_j / sum_j exp(s_j)
-// in one pass over the keys with the running maximum m and sum l: a larger
-// maximum m' rescales what is there by exp(m - m').
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -13,6 +8,8 @@
 #include "msx_internal.h"
 #include "msx_paged.h"
 #include "msx_paged_check.h"
+#include "msx_paged_row.h"
+#include "msx_paged_tiles.h"
 
 #pragma clang fp contract(fast)
 
@@ -20,63 +17,16 @@ namespace msx {
 namespace {
 
 constexpr int kRowWaves = 4;
-constexpr int kMaxPer = 4;  // head values a lane holds: dim <= 256
-
 // One wave a (sequence, query, head).
 template <class V>
 __global__ __launch_bounds__(kRowWaves * kWave) void paged_rows(PagedArgs a, int64_t first, int64_t rows,
                                                                 typename V::Storage *out) {
-  using S = typename V::Storage;
   __shared__ float q_lds[kRowWaves][kWindowMaxDim];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wave = threadIdx.x / kWave;
   const int64_t row = first + static_cast<int64_t>(blockIdx.x) * kRowWaves + wave;
   if (row >= rows) return;  // whole waves leave; there is no barrier below
-  const int32_t h = static_cast<int32_t>(row % a.heads);
-  const int32_t t = static_cast<int32_t>(row / a.heads % a.tokens);
-  const int64_t b = row / a.heads / a.tokens;
-  float m = -INFINITY, l = 0.0f, o[kMaxPer] = {};
-  if (t < a.length(b)) {
-    const S *q = static_cast<const S *>(a.q) + b * a.qs[0] + t * a.qs[1] + h * a.qs[2];
-    const S *k = static_cast<const S *>(a.k) + (h / a.group) * a.ks[2];
-    const S *v = static_cast<const S *>(a.v) + (h / a.group) * a.vs[2];
-    float *ql = q_lds[wave];
-    for (int d = lane; d < a.dim; d += kWave) ql[d] = V::widen(q[d]);
-    __builtin_amdgcn_wave_barrier();
-    const Keys seen = a.keys(a.start(b), t, t);
-    const int32_t n = seen.count();
-    for (int32_t c0 = 0; c0 < n; c0 += kWave) {
-      const int32_t j = seen.key(min(c0 + lane, n - 1));
-      const int32_t page = c0 + lane < n ? a.table.page(b, j) : -1, slot = a.table.slot(j);
-      float s = -INFINITY;
-      if (page >= 0) {
-        const S *from = k + page * a.ks[0] + slot * a.ks[1];
-        s = 0.0f;
-        for (int d = 0; d < a.dim; ++d) s += ql[d] * V::widen(from[d]);
-        s *= a.scale;
-      }
-      const float top = fmaxf(m, wave_max(s));
-      const float base = top == -INFINITY ? 0.0f : top;
-      const float e = page >= 0 ? exp2_fast(s - base) : 0.0f, keep = exp2_fast(m - base);
-      l = l * keep + wave_sum(e);
-      m = top;
-#pragma unroll
-      for (int r = 0; r < kMaxPer; ++r) o[r] *= keep;
-      const int32_t here = min(kWave, n - c0);
-      for (int32_t i = 0; i < here; ++i) {
-        const int32_t from_page = __shfl(page, i);
-        if (from_page < 0) continue;
-        const float w = __shfl(e, i);
-        const S *from = v + from_page * a.vs[0] + __shfl(slot, i) * a.vs[1];
-#pragma unroll
-        for (int r = 0; r < kMaxPer; ++r)
-          if (lane + kWave * r < a.dim) o[r] += w * V::widen(from[lane + kWave * r]);
-      }
-    }
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int r = 0; r < kMaxPer; ++r)
-    if (lane + kWave * r < a.dim) out[row * a.dim + lane + kWave * r] = V::narrow(o[r] * inv);
+  paged_row<V>(a, row / a.heads / a.tokens, static_cast<int32_t>(row / a.heads % a.tokens),
+               static_cast<int32_t>(row % a.heads), q_lds[wave], out);
 }
 
 PagedArgs args_of(const msx_paged_attention_desc &d) {
@@ -103,6 +53,19 @@ PagedArgs args_of(const msx_paged_attention_desc &d) {
   return a;
 }
 
+// Whether the tiles' kernels can read the operands: sixteen-byte rows at sixteen-byte
+// strides, and queries that share a kv head that 32 bits count.
+bool takes_tiles(const msx_paged_attention_desc &d) {
+  const auto size = static_cast<int64_t>(value_bytes(static_cast<msx_vtype>(d.vtype)));
+  const auto aligned = [&](const void *p, const int64_t *strides) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && strides[0] * size % 16 == 0 &&
+           strides[1] * size % 16 == 0 && strides[2] * size % 16 == 0;
+  };
+  return d.cache.dim * size % 16 == 0 &&
+         d.tokens * (d.heads / d.cache.kv_heads) <= kWindowIntMax - 256 && aligned(d.q, d.q_strides) &&
+         aligned(d.cache.k, d.cache.k_strides) && aligned(d.cache.v, d.cache.v_strides);
+}
+
 template <class Fn>
 msx_status by_vtype(int vt, Fn &&fn) {
   switch (vt) {
@@ -118,19 +81,26 @@ msx_status by_vtype(int vt, Fn &&fn) {
 using namespace msx;
 
 extern "C" size_t msx_paged_attention_scratch(const msx_paged_attention_desc *desc) {
-  if (check_paged_attention("paged_attention", desc) != MSX_OK) return 0;
-  return 0;
+  if (check_paged_attention("paged_attention", desc) != MSX_OK || desc->batch == 0 ||
+      desc->tokens == 0 || !takes_tiles(*desc))
+    return 0;
+  return paged_step_scratch(args_of(*desc));
 }
 
 extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, void *out,
                                           void *scratch, size_t scratch_bytes, void *stream) {
   clear_error();
-  (void)scratch;
-  (void)scratch_bytes;
   if (msx_status st = check_paged_attention("paged_attention", desc); st != MSX_OK) return st;
   if (desc->batch == 0 || desc->tokens == 0) return MSX_OK;
   if (out == nullptr) return fail(MSX_EINVAL, "paged_attention out is NULL.");
   const PagedArgs a = args_of(*desc);
+  if (takes_tiles(*desc)) {
+    if (scratch == nullptr || scratch_bytes < paged_step_scratch(a) ||
+        reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
+      return fail(MSX_EINVAL, "paged_attention scratch is too small or not aligned.");
+    return launch_paged_step(static_cast<msx_vtype>(desc->vtype), a, out, scratch,
+                             static_cast<hipStream_t>(stream));
+  }
   const int64_t rows = a.batch * a.tokens * a.heads;
   return by_vtype(desc->vtype, [&](auto v) {
     using V = decltype(v);

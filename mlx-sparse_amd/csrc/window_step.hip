@@ -22,62 +22,16 @@
 
 #include "msx_internal.h"
 #include "msx_window.h"
-#include "msx_window_mfma.h"
+#include "msx_step_mfma.h"
 
 #pragma clang fp contract(fast)
 
 namespace msx {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = kStepWaves;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kHeads = 16;  // query heads a workgroup
-
-template <class V>
-struct Mfma16;
-template <>
-struct Mfma16<BF16> {
-  __device__ static inline v4f mul(v4u a, v4u b, v4f c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct Mfma16<F16> {
-  __device__ static inline v4f mul(v4u a, v4u b, v4f c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct Mfma16<F32> {
-  __device__ static inline v4f mul(v4u a, v4u b, v4f c) {
-    const v4f x = __builtin_bit_cast(v4f, a), y = __builtin_bit_cast(v4f, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-    return c;
-  }
-};
-
-// Lane layout of the products: scores S^T = K Q^T, 16 keys x 16 heads, with
-// head = lane % 16 and keys 4 (lane / 16) + i; O^T = V^T P^T takes its keys in
-// that order (two 16-key tiles make the 32 of a 16-bit product).
-template <class V, int DP>
-struct StepShape {
-  static constexpr int kSize = sizeof(typename V::Storage);
-  static constexpr int kTiles = kSize == 2 ? 2 : 1;  // 16-key tiles a step
-  static constexpr int kKeys = 16 * kTiles;
-  static constexpr int kChunks = DP * kSize / 16;     // of a row
-  static constexpr int kSteps = kChunks / 4;          // four lanes a row
-  static constexpr int kVPer = kKeys * kChunks / kWave;
-  static constexpr int kPitch = kChunks * 16;
-  static constexpr int kTile = kKeys * kPitch;
-  static constexpr int kLds = std::max(kWaves * kTile, kWaves * kHeads * (DP + 4) * 4);
-
-  // 32-byte pairs permuted by row, as in the attention tiles.
-  __device__ static inline int at(int row, int chunk) {
-    constexpr int rows = kPitch >= 256 ? 1 : 256 / kPitch;
-    return row * kPitch + ((chunk ^ (((row / rows) * 2) & (kChunks - 1))) * 16);
-  }
-};
+constexpr int kHeads = kStepRows;  // query heads a workgroup
 
 // The visible slots of a sequence, numbered: sinks, then the window's.
 struct Slots {
@@ -104,9 +58,6 @@ struct Slots {
     return sinks + (r >= ring ? r - ring : r);
   }
 };
-
-// m, l and dim sums of a head over one part of the keys.
-__device__ inline int64_t part_stride(int32_t dim) { return (dim + 2 + 3) / 4 * 4; }
 
 template <class V, int DP>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void step_tiles(StepArgs a, int32_t head_tiles,
