@@ -11,17 +11,28 @@ struct StepGrid {
   int32_t groups;  // workgroups launched, as many as run at once
 };
 
-// Equal stretches of `work` steps: workgroup g takes [first(g), first(g + 1)).
+// 64-bit quotients take a workgroup some microseconds, those of 32 bits are free.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t by) {
+  if (((x | by) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(by);
+  return x / by;
+}
+
+// Equal stretches of `work`: workgroup g takes [first(g), first(g + 1)).
 struct StepShare {
-  int64_t work, groups;
-  __device__ __forceinline__ StepShare(int64_t w, int32_t launched) : work(w) {
-    // two steps a wave at least: shorter stretches cost more in joining than they gain
-    constexpr int64_t kLeast = 8;
-    groups = max(min(w / kLeast, static_cast<int64_t>(launched)), int64_t{1});
+  int64_t groups, each, more;  // the first `more` take one more
+  __device__ __forceinline__ StepShare(int64_t work, int32_t launched) {
+    groups = max(min(work / kLeast, static_cast<int64_t>(launched)), int64_t{1});
+    each = quotient(work, groups);
+    more = work - each * groups;
   }
-  __device__ __forceinline__ int64_t first(int64_t g) const { return work * g / groups; }
-  // The workgroup that takes step x: the last whose first step is not past it.
-  __device__ __forceinline__ int64_t owner(int64_t x) const { return ((x + 1) * groups - 1) / work; }
+  __device__ __forceinline__ int64_t first(int64_t g) const { return each * g + min(g, more); }
+  // The workgroup that takes x.
+  __device__ __forceinline__ int64_t owner(int64_t x) const {
+    const int64_t longer = more * (each + 1);
+    return x < longer ? quotient(x, each + 1) : more + quotient(x - longer, each);
+  }
+  // a step a wave at least
+  static constexpr int64_t kLeast = 4;
 };
 
 // The workgroups that a tile of queries was cut over; none (last < first) where one

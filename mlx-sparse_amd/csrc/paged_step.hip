@@ -38,6 +38,9 @@ struct Steps {
   int32_t sinks, window, count;  // steps over the sinks, the window's first, all (one at least)
 };
 
+// What a tile of queries costs beside its steps, in steps.
+constexpr int32_t kStart = 4;
+
 template <int kKeys>
 __device__ __forceinline__ Steps steps_of(const PagedArgs &a, int64_t b, int32_t tile) {
   Steps s;
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
   using S = typename V::Storage;
   using F = StepShape<V, DP>;
   __shared__ __attribute__((aligned(16))) char lds[F::kLds];
-  __shared__ int64_t sums[kStepWaves], found_before;
+  __shared__ int64_t sums[kStepWaves], found_first;
   __shared__ int32_t found;
   __shared__ uint32_t odd;
 
@@ -105,57 +108,65 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
 
   // this workgroup's stretch of all steps
   const int64_t entries = a.batch * grid.tiles;  // (sequence, sixteen queries)
-  const auto count_at = [&](int64_t e) -> int64_t {
-    return e < entries ? steps_of<F::kKeys>(a, e / grid.tiles, static_cast<int32_t>(e % grid.tiles)).count : 0;
+  const auto cost_at = [&](int64_t e) -> int64_t {
+    if (e >= entries) return 0;
+    const int64_t b = grid.tiles == 1 ? e : e / grid.tiles;
+    return kStart + steps_of<F::kKeys>(a, b, static_cast<int32_t>(e - b * grid.tiles)).count;
   };
-  int64_t total = 0, count = count_at(threadIdx.x), upto = running_sums(count, sums, total);
+  int64_t total = 0, cost = cost_at(threadIdx.x), upto = running_sums(cost, sums, total);
   if (entries > kThreads) {
-    int64_t mine = count;
-    for (int64_t e = threadIdx.x + kThreads; e < entries; e += kThreads) mine += count_at(e);
+    int64_t mine = cost;
+    for (int64_t e = threadIdx.x + kThreads; e < entries; e += kThreads) mine += cost_at(e);
     running_sums(mine, sums, total);
   }
-  const int64_t work = total * a.kv_heads;
-  const StepShare share(work, grid.groups);
+  const StepShare share(total * a.kv_heads, grid.groups);
   const int64_t g = blockIdx.x;
   if (g >= share.groups) return;  // whole workgroups leave
   const int64_t begin = share.first(g), end = share.first(g + 1);
   int64_t before = 0;
-  for (int64_t e0 = 0;; e0 += kThreads) {  // (every step is some entry's)
-    int64_t here = 0;
-    if (e0 > 0) {
-      count = count_at(e0 + threadIdx.x);
-      upto = running_sums(count, sums, here);
-    } else if (entries > kThreads) {
-      upto = running_sums(count, sums, here);
-    } else {
-      here = total;
+  for (int64_t e0 = 0;; e0 += kThreads) {  // (all that is to be done is some entry's)
+    int64_t here = total;
+    if (entries > kThreads) {
+      if (e0 > 0) cost = cost_at(e0 + threadIdx.x);
+      upto = running_sums(cost, sums, here);
     }
-    const int64_t low = (before + upto - count) * a.kv_heads, high = (before + upto) * a.kv_heads;
+    const int64_t low = (before + upto - cost) * a.kv_heads, high = (before + upto) * a.kv_heads;
     if (low <= begin && begin < high) {
       found = static_cast<int32_t>(e0 + threadIdx.x);
-      found_before = low;
+      found_first = low;
     }
     before += here;
     if (begin < before * a.kv_heads || e0 + kThreads >= entries) break;
   }
   __syncthreads();
-  int32_t entry = __builtin_amdgcn_readfirstlane(found);
-  int64_t entry_first = found_before;  // its first step's number
+  int32_t entry = __builtin_amdgcn_readfirstlane(found), kvh = -1;
+  int64_t x = found_first;  // where the next (entry, kv head) begins
 
-  for (int64_t x = begin; x < end;) {
-    const int64_t b = entry / grid.tiles;
-    const int32_t row_tile = static_cast<int32_t>(entry % grid.tiles);
+  while (x < end) {
+    const int64_t b = grid.tiles == 1 ? entry : entry / grid.tiles;
+    const int32_t row_tile = entry - static_cast<int32_t>(b) * grid.tiles;
     const Steps steps = uniform(steps_of<F::kKeys>(a, b, row_tile));
-    const int32_t kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>((x - entry_first) / steps.count));
-    const int64_t unit_first = entry_first + static_cast<int64_t>(kvh) * steps.count;
-    const int32_t s_begin = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(x - unit_first));
+    if (kvh < 0) {
+      kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - x, steps.count + kStart)));
+      x += static_cast<int64_t>(kvh) * (steps.count + kStart);
+    }
+    const int64_t first_step = x + kStart;
+    x = first_step + steps.count;
+    const int32_t s_begin = __builtin_amdgcn_readfirstlane(
+        static_cast<int32_t>(min(max(begin - first_step, int64_t{0}), static_cast<int64_t>(steps.count))));
     const int32_t s_end = __builtin_amdgcn_readfirstlane(
-        static_cast<int32_t>(min(end - unit_first, static_cast<int64_t>(steps.count))));
+        static_cast<int32_t>(max(min(end - first_step, static_cast<int64_t>(steps.count)), int64_t{0})));
+    const int32_t head = kvh, mine_entry = entry;
+    if (++kvh == a.kv_heads) {
+      kvh = 0;
+      ++entry;
+    }
+    if (s_begin >= s_end) continue;  // what this workgroup has of it is no step
     const auto key_of = [&](int32_t s) { return F::kKeys * (s < steps.sinks ? s : steps.window + s - steps.sinks); };
 
     // this lane's query, and what it sees
     const int32_t row = row_tile * kStepRows + lane % 16, t = row / a.group;
-    const int32_t h = kvh * a.group + row % a.group;
+    const int32_t h = head * a.group + row % a.group;
     const bool live = t <= steps.last && row < a.tokens * a.group;
     Keys mine{0, 0, -1};
     if (live) mine = a.keys(a.start(b), t, t);
@@ -171,8 +182,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
         if (live && c * 16 < bytes) qf[s] = *reinterpret_cast<const v4u *>(q + c * 16);
       }
     }
-    const char *ck = reinterpret_cast<const char *>(static_cast<const S *>(a.k) + kvh * a.ks[2]);
-    const char *cv = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + kvh * a.vs[2]);
+    const char *ck = reinterpret_cast<const char *>(static_cast<const S *>(a.k) + head * a.ks[2]);
+    const char *cv = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + head * a.vs[2]);
 
     // the page of key `lane` of a step, -1 where nobody sees it
     const auto pages_of = [&](int32_t s) {
@@ -317,11 +328,11 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
     if (threadIdx.x == 0) odd = 0;
     __syncthreads();
     const bool whole = s_begin == 0 && s_end == steps.count;
-    const int64_t unit = static_cast<int64_t>(entry) * a.kv_heads + kvh;
+    const int64_t unit = static_cast<int64_t>(mine_entry) * a.kv_heads + head;
     if (threadIdx.x == 0 && s_begin == 0)
       spans[unit] = whole ? StepSpan{0, -1}
                           : StepSpan{static_cast<int32_t>(g),
-                                     static_cast<int32_t>(share.owner(unit_first + steps.count - 1))};
+                                     static_cast<int32_t>(share.owner(first_step + steps.count - 1))};
     const float *all = reinterpret_cast<const float *>(lds);
     const int32_t rows = min(kStepRows, a.tokens * a.group - row_tile * kStepRows);
     for (int at = threadIdx.x; at < rows * DP; at += kThreads) {
@@ -343,7 +354,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
       if (whole) {
         const float value = norm == 0.0f ? 0.0f : sum / norm;
         if (!(fabsf(value) < INFINITY)) atomicOr(&odd, 1u << i);
-        out[((b * a.tokens + r / a.group) * a.heads + kvh * a.group + r % a.group) * a.dim + d] =
+        out[((b * a.tokens + r / a.group) * a.heads + head * a.group + r % a.group) * a.dim + d] =
             V::narrow(value);
       } else {
         float *part = parts + ((2 * g + (s_begin == 0 ? 1 : 0)) * kStepRows + i) * part_stride(a.dim);
@@ -359,29 +370,23 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
       const int i = __builtin_ctz(anew);
       if (i % kStepWaves != wave) continue;
       const int32_t r = row_tile * kStepRows + i;
-      paged_row<V>(a, b, r / a.group, kvh * a.group + r % a.group,
+      paged_row<V>(a, b, r / a.group, head * a.group + r % a.group,
                    reinterpret_cast<float *>(lds) + wave * DP, out);
     }
     __syncthreads();
-
-    x = unit_first + s_end;
-    if (s_end == steps.count && kvh == a.kv_heads - 1) {
-      ++entry;
-      entry_first = x;
-    }
   }
 }
 
-// A wave a (sequence, query, head) whose keys were cut over workgroups: their sums
-// in the order of the keys.
-template <class V>
-__global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a, StepGrid grid, int64_t rows,
+// A workgroup a (sequence, query, head) whose keys were cut over workgroups: their sums
+// in the order of the keys, four values a thread, every eighth part (dim 128) of
+// them; then those of the threads that have the same values, through LDS.
+template <class V, int DP>
+__global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a, StepGrid grid,
                                                        const StepSpan *spans, const float *parts,
                                                        typename V::Storage *out) {
-  __shared__ float q_lds[kStepWaves][kWindowMaxDim];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kStepWaves + wave;
-  if (row >= rows) return;  // whole waves leave; there is no barrier below
+  constexpr int kLanes = DP / 4, kBeside = kThreads / kLanes;
+  __shared__ __attribute__((aligned(16))) float lds[kBeside][DP + 4];
+  const int64_t row = blockIdx.x;
   const int32_t h = static_cast<int32_t>(row % a.heads);
   const int32_t t = static_cast<int32_t>(row / a.heads % a.tokens);
   const int64_t b = row / a.heads / a.tokens;
@@ -390,27 +395,45 @@ __global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a, StepGrid gri
   if (span.last < span.first) return;
   const int64_t stride = part_stride(a.dim);
   const int32_t n = span.last - span.first + 1;
-  // the first workgroup's last place, the others' first
-  const auto part_at = [&](int32_t s) {
-    return parts + ((2 * static_cast<int64_t>(span.first + s) + (s == 0 ? 1 : 0)) * kStepRows + i) * stride;
-  };
-  float top = -INFINITY;
-  for (int32_t s = lane; s < n; s += kWave) top = fmaxf(top, part_at(s)[a.dim]);
-  top = wave_max(top);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float norm = 0.0f;
-  for (int32_t s = lane; s < n; s += kWave) norm += part_at(s)[a.dim + 1] * exp2_fast(part_at(s)[a.dim] - base);
-  norm = wave_sum(norm);
-  bool bad = false;
-  for (int32_t d = lane; d < a.dim; d += kWave) {
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int32_t s = 0; s < n; ++s) sum += part_at(s)[d] * exp2_fast(part_at(s)[a.dim] - base);
-    const float value = norm == 0.0f ? 0.0f : sum / norm;
-    bad = bad || !(fabsf(value) < INFINITY);
-    out[row * a.dim + d] = V::narrow(value);
+  const int beside = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  float m = -INFINITY, l = 0.0f;
+  v4f o{0, 0, 0, 0};
+#pragma unroll 4
+  for (int32_t s = beside; s < n; s += kBeside) {
+    // the first workgroup's last place, the others' first
+    const float *part = parts + ((2 * static_cast<int64_t>(span.first + s) + (s == 0 ? 1 : 0)) * kStepRows + i) * stride;
+    const float part_m = part[a.dim], part_l = part[a.dim + 1];
+    v4f x{0, 0, 0, 0};
+    if (d < a.dim) x = *reinterpret_cast<const v4f *>(part + d);
+    const float top = fmaxf(m, part_m), base = top == -INFINITY ? 0.0f : top;
+    const float keep = exp2_fast(m - base), f = exp2_fast(part_m - base);
+    l = l * keep + part_l * f;
+    o = o * keep + x * f;
+    m = top;
   }
-  if (__any(bad)) paged_row<V>(a, b, t, h, q_lds[wave], out);
+  *reinterpret_cast<v4f *>(&lds[beside][d]) = o;
+  if (d == 0) {
+    lds[beside][DP] = m;
+    lds[beside][DP + 1] = l;
+  }
+  __syncthreads();
+  bool bad = false;
+  if (threadIdx.x < a.dim) {
+    float top = -INFINITY, sum = 0.0f, norm = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kBeside; ++s) top = fmaxf(top, lds[s][DP]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int s = 0; s < kBeside; ++s) {
+      const float f = exp2_fast(lds[s][DP] - base);
+      sum += lds[s][threadIdx.x] * f;
+      norm += lds[s][DP + 1] * f;
+    }
+    const float value = norm == 0.0f ? 0.0f : sum / norm;
+    bad = !(fabsf(value) < INFINITY);
+    out[row * a.dim + threadIdx.x] = V::narrow(value);
+  }
+  if (__syncthreads_or(bad) && threadIdx.x < kWave) paged_row<V>(a, b, t, h, &lds[0][0], out);
 }
 
 StepGrid grid_of(const PagedArgs &a) {
@@ -428,14 +451,14 @@ template <class V, int DP>
 msx_status run(const PagedArgs &a, void *out, void *scratch, hipStream_t stream) {
   using S = typename V::Storage;
   const StepGrid grid = grid_of(a);
-  const int64_t rows = a.batch * a.tokens * a.heads, blocks = (rows + kStepWaves - 1) / kStepWaves;
-  if (a.batch * grid.tiles > kWindowIntMax || blocks > max_blocks(kThreads))
+  const int64_t rows = a.batch * a.tokens * a.heads;
+  if (a.batch * grid.tiles > kWindowIntMax || rows > max_blocks(kThreads))
     return fail(MSX_EINVAL, "paged_attention has more rows than a grid holds.");
   auto *spans = static_cast<StepSpan *>(scratch);
   auto *parts = reinterpret_cast<float *>(static_cast<char *>(scratch) + spans_bytes(a));
   paged_step<V, DP><<<grid.groups, kThreads, 0, stream>>>(a, grid, static_cast<S *>(out), spans, parts);
-  paged_join<V><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a, grid, rows, spans, parts,
-                                                                       static_cast<S *>(out));
+  paged_join<V, DP><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(a, grid, spans, parts,
+                                                                         static_cast<S *>(out));
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
 }
