@@ -70,12 +70,15 @@ inline PageTable table_of(const msx_paged_cache &c) {
   return t;
 }
 
-// The keys that a query sees: [0, far) and [lo, hi], far <= lo.
+// The keys that a query sees: [0, far) and [lo, hi], far <= lo; of both those from
+// `from` on, where those before are another kernel's.
 struct Keys {
-  int32_t far, lo, hi;
+  int32_t far, lo, hi, from;
   __device__ __forceinline__ int32_t count() const { return far + (hi < lo ? 0 : hi - lo + 1); }
   __device__ __forceinline__ int32_t key(int32_t c) const { return c < far ? c : lo + c - far; }
-  __device__ __forceinline__ bool sees(int32_t j) const { return j <= hi && (j >= lo || j < far); }
+  __device__ __forceinline__ bool sees(int32_t j) const {
+    return j >= from && j <= hi && (j >= lo || j < far);
+  }
 };
 
 struct PagedArgs {
@@ -104,6 +107,7 @@ struct PagedArgs {
     const int64_t from = min(start, int64_t{1} << 62) + first, to = min(start, int64_t{1} << 62) + last;
     const int64_t cap = table.capacity;
     Keys k;
+    k.from = 0;
     k.hi = static_cast<int32_t>(min(to, cap - 1));
     k.lo = static_cast<int32_t>(min(max(from - window + 1, int64_t{0}), cap));
     k.far = min(min(sinks, k.lo), k.hi + 1);

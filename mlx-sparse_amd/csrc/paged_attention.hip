@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
+#include <limits>
 
 #include "msx_device.h"
 #include "msx_internal.h"
@@ -75,6 +77,70 @@ msx_status by_vtype(int vt, Fn &&fn) {
   }
 }
 
+enum class Route { kRows, kStep, kTiles, kShared };
+
+// Rows that share a kv head: up to so many a sequence go through paged_step, a read of
+// the keys for each sixteen of them.
+constexpr int64_t kFewRows = 32;
+
+Route route_of(const msx_paged_attention_desc &d) {
+  if (!takes_tiles(d)) return Route::kRows;
+  const int64_t rows = d.tokens * (d.heads / d.cache.kv_heads);
+  const bool wide = d.cache.dim > 128 ||  // (a masked score is minus infinity times the scale)
+                    !(std::fabs(static_cast<float>(d.scale)) >= std::numeric_limits<float>::min());
+  if (wide) return Route::kStep;
+  if (rows > kFewRows) return Route::kTiles;
+  if (d.shared_pages > 0 && d.batch > 1 && d.window >= d.cache.width * d.cache.page_size &&
+      d.batch * rows <= kWindowIntMax - kTileRows)
+    return Route::kShared;
+  return Route::kStep;
+}
+
+// What a call's kernels are given, and where in its scratch their parts lie.
+struct Plan {
+  Route route;
+  StepGrid step{}, tiles{};
+  TileParts step_to{}, tiles_to{};
+  size_t bytes = 0;
+
+  Plan(const msx_paged_attention_desc &d, const PagedArgs &a, void *out, void *scratch)
+      : route(route_of(d)) {
+    const int64_t rows = static_cast<int64_t>(a.tokens) * a.group, all = a.batch * a.tokens * a.heads;
+    char *base = static_cast<char *>(scratch);
+    const auto take = [&](int64_t each, int64_t count) {
+      char *p = base + bytes;
+      bytes += (static_cast<size_t>(each * count) + 255) / 256 * 256;
+      return p;
+    };
+    const int64_t part = sizeof(float) * part_stride(a.dim);
+    const auto parts_of = [&](const StepGrid &g, int64_t entries, int32_t tile_rows) {
+      TileParts to{};
+      to.out = out;
+      to.spans = reinterpret_cast<StepSpan *>(take(sizeof(StepSpan), entries * a.kv_heads));
+      to.parts = reinterpret_cast<float *>(take(part, 2 * static_cast<int64_t>(g.groups) * tile_rows));
+      if (route == Route::kShared) to.whole = reinterpret_cast<float *>(take(part, all));
+      return to;
+    };
+    // as many workgroups as run at once: registers allow two a CU, of wide heads one
+    if (route == Route::kStep || route == Route::kShared) {
+      step.tiles = static_cast<int32_t>((rows + kStepRows - 1) / kStepRows);
+      step.groups = a.dim > 128 ? 256 : 512;
+      step.from = route == Route::kShared ? static_cast<int32_t>(d.shared_pages * d.cache.page_size) : 0;
+      step_to = parts_of(step, a.batch * step.tiles, kStepRows);
+    }
+    if (route == Route::kTiles || route == Route::kShared) {
+      const int64_t together = route == Route::kShared ? a.batch * rows : rows;
+      tiles.tiles = static_cast<int32_t>((together + kTileRows - 1) / kTileRows);
+      tiles.groups = a.dim * value_bytes(static_cast<msx_vtype>(d.vtype)) > 256 ? 256 : 512;
+      tiles.from = step.from;
+      tiles_to = parts_of(tiles, route == Route::kShared ? tiles.tiles : a.batch * tiles.tiles, kTileRows);
+    }
+  }
+  PartSource source(const StepGrid &g, const TileParts &to, int32_t rows, bool batched) const {
+    return {to.spans, to.whole, to.parts, rows, g.tiles, batched};
+  }
+};
+
 }  // namespace
 }  // namespace msx
 
@@ -82,9 +148,9 @@ using namespace msx;
 
 extern "C" size_t msx_paged_attention_scratch(const msx_paged_attention_desc *desc) {
   if (check_paged_attention("paged_attention", desc) != MSX_OK || desc->batch == 0 ||
-      desc->tokens == 0 || !takes_tiles(*desc))
+      desc->tokens == 0)
     return 0;
-  return paged_step_scratch(args_of(*desc));
+  return Plan(*desc, args_of(*desc), nullptr, nullptr).bytes;
 }
 
 extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, void *out,
@@ -94,22 +160,35 @@ extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, 
   if (desc->batch == 0 || desc->tokens == 0) return MSX_OK;
   if (out == nullptr) return fail(MSX_EINVAL, "paged_attention out is NULL.");
   const PagedArgs a = args_of(*desc);
-  if (takes_tiles(*desc)) {
-    if (scratch == nullptr || scratch_bytes < paged_step_scratch(a) ||
-        reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
-      return fail(MSX_EINVAL, "paged_attention scratch is too small or not aligned.");
-    return launch_paged_step(static_cast<msx_vtype>(desc->vtype), a, out, scratch,
-                             static_cast<hipStream_t>(stream));
+  const auto s = static_cast<hipStream_t>(stream);
+  const auto vt = static_cast<msx_vtype>(desc->vtype);
+  const Plan p(*desc, a, out, scratch);
+  if (p.route == Route::kRows) {
+    const int64_t rows = a.batch * a.tokens * a.heads;
+    return by_vtype(desc->vtype, [&](auto v) {
+      using V = decltype(v);
+      constexpr int64_t kMost = max_blocks(kRowWaves * kWave) * kRowWaves;
+      for (int64_t first = 0; first < rows; first += kMost)
+        paged_rows<V><<<static_cast<unsigned>((std::min(rows - first, kMost) + kRowWaves - 1) / kRowWaves),
+                        kRowWaves * kWave, 0, s>>>(a, first, rows, static_cast<typename V::Storage *>(out));
+      const hipError_t e = hipGetLastError();
+      return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
+    });
   }
-  const int64_t rows = a.batch * a.tokens * a.heads;
-  return by_vtype(desc->vtype, [&](auto v) {
-    using V = decltype(v);
-    constexpr int64_t kMost = max_blocks(kRowWaves * kWave) * kRowWaves;
-    for (int64_t first = 0; first < rows; first += kMost)
-      paged_rows<V><<<static_cast<unsigned>((std::min(rows - first, kMost) + kRowWaves - 1) / kRowWaves),
-                      kRowWaves * kWave, 0, static_cast<hipStream_t>(stream)>>>(
-          a, first, rows, static_cast<typename V::Storage *>(out));
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
-  });
+  if (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
+    return fail(MSX_EINVAL, "paged_attention scratch is too small or not aligned.");
+  if (a.batch * std::max(p.step.tiles, p.tiles.tiles) > kWindowIntMax)
+    return fail(MSX_EINVAL, "paged_attention has more rows than a grid holds.");
+  const PartSource none{};
+  const PartSource by_step = p.source(p.step, p.step_to, kStepRows, false);
+  const PartSource by_tiles = p.source(p.tiles, p.tiles_to, kTileRows, p.route == Route::kShared);
+  if (p.route != Route::kStep)
+    if (msx_status st = launch_paged_tiles(vt, a, p.tiles, p.tiles_to, s); st != MSX_OK) return st;
+  if (p.route != Route::kTiles)
+    if (msx_status st = launch_paged_step(vt, a, p.step, p.step_to, s); st != MSX_OK) return st;
+  switch (p.route) {
+  case Route::kStep: return launch_paged_join(vt, a, by_step, none, out, s);
+  case Route::kTiles: return launch_paged_join(vt, a, by_tiles, none, out, s);
+  default: return launch_paged_join(vt, a, by_tiles, by_step, out, s);
+  }
 }

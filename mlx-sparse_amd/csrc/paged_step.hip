@@ -29,71 +29,10 @@ namespace {
 
 constexpr int kThreads = kStepWaves * kWave;
 
-// The steps of `kKeys` keys that sixteen queries take: those over the sinks,
-// then those over the window's keys.
-struct Steps {
-  Keys keys;      // that any of the queries sees
-  int32_t first;  // queries [first, last] are there, none where last < first
-  int32_t last;
-  int32_t sinks, window, count;  // steps over the sinks, the window's first, all (one at least)
-};
-
-// What a tile of queries costs beside its steps, in steps.
-constexpr int32_t kStart = 4;
-
-template <int kKeys>
-__device__ __forceinline__ Steps steps_of(const PagedArgs &a, int64_t b, int32_t tile) {
-  Steps s;
-  const int32_t rows = a.tokens * a.group;
-  const int64_t start = a.start(b);
-  s.first = tile * kStepRows / a.group;
-  s.last = min(min(tile * kStepRows + kStepRows, rows) - 1, a.length(b) * a.group - 1) / a.group;
-  if (a.length(b) == 0 || s.last < s.first) {
-    s.last = s.first - 1;
-    s.keys = Keys{0, 0, -1};
-    s.sinks = s.window = 0;
-    s.count = 1;
-    return s;
-  }
-  s.keys = a.keys(start, s.first, s.last);
-  s.sinks = (s.keys.far + kKeys - 1) / kKeys;
-  s.window = max(s.keys.lo / kKeys, s.sinks);
-  const int32_t end = s.keys.hi < s.keys.lo ? 0 : s.keys.hi / kKeys + 1;
-  s.count = max(s.sinks + max(end - s.window, 0), 1);
-  return s;
-}
-
-// The same of every lane, for scalar registers.
-__device__ __forceinline__ Steps uniform(const Steps &s) {
-  const auto one = [](int32_t x) { return __builtin_amdgcn_readfirstlane(x); };
-  return {{one(s.keys.far), one(s.keys.lo), one(s.keys.hi)}, one(s.first), one(s.last),
-          one(s.sinks), one(s.window), one(s.count)};
-}
-
-// Inclusive sums over the workgroup's threads; `total` the last one's.
-__device__ __forceinline__ int64_t running_sums(int64_t x, int64_t *lds, int64_t &total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t below = __shfl_up(x, d);
-    if (lane >= d) x += below;
-  }
-  __syncthreads();
-  if (lane == kWave - 1) lds[wave] = x;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kStepWaves; ++w) {
-    if (w < wave) x += lds[w];
-    total += lds[w];
-  }
-  return x;
-}
-
 template <class V, int DP>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedArgs a, StepGrid grid,
                                                                          typename V::Storage *out,
-                                                                         StepSpan *spans,
+                                                                         StepSpan *spans, float *whole_parts,
                                                                          float *parts) {
   using S = typename V::Storage;
   using F = StepShape<V, DP>;
@@ -111,13 +50,13 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
   const auto cost_at = [&](int64_t e) -> int64_t {
     if (e >= entries) return 0;
     const int64_t b = grid.tiles == 1 ? e : e / grid.tiles;
-    return kStart + steps_of<F::kKeys>(a, b, static_cast<int32_t>(e - b * grid.tiles)).count;
+    return kStart + steps_of<F::kKeys, kStepRows>(a, b, static_cast<int32_t>(e - b * grid.tiles), grid.from).count;
   };
-  int64_t total = 0, cost = cost_at(threadIdx.x), upto = running_sums(cost, sums, total);
+  int64_t total = 0, cost = cost_at(threadIdx.x), upto = running_sums<kStepWaves>(cost, sums, total);
   if (entries > kThreads) {
     int64_t mine = cost;
     for (int64_t e = threadIdx.x + kThreads; e < entries; e += kThreads) mine += cost_at(e);
-    running_sums(mine, sums, total);
+    running_sums<kStepWaves>(mine, sums, total);
   }
   const StepShare share(total * a.kv_heads, grid.groups);
   const int64_t g = blockIdx.x;
@@ -128,7 +67,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
     int64_t here = total;
     if (entries > kThreads) {
       if (e0 > 0) cost = cost_at(e0 + threadIdx.x);
-      upto = running_sums(cost, sums, here);
+      upto = running_sums<kStepWaves>(cost, sums, here);
     }
     const int64_t low = (before + upto - cost) * a.kv_heads, high = (before + upto) * a.kv_heads;
     if (low <= begin && begin < high) {
@@ -145,7 +84,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
   while (x < end) {
     const int64_t b = grid.tiles == 1 ? entry : entry / grid.tiles;
     const int32_t row_tile = entry - static_cast<int32_t>(b) * grid.tiles;
-    const Steps steps = uniform(steps_of<F::kKeys>(a, b, row_tile));
+    const Steps steps = uniform(steps_of<F::kKeys, kStepRows>(a, b, row_tile, grid.from));
     if (kvh < 0) {
       kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - x, steps.count + kStart)));
       x += static_cast<int64_t>(kvh) * (steps.count + kStart);
@@ -162,13 +101,13 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
       ++entry;
     }
     if (s_begin >= s_end) continue;  // what this workgroup has of it is no step
-    const auto key_of = [&](int32_t s) { return F::kKeys * (s < steps.sinks ? s : steps.window + s - steps.sinks); };
+    const auto key_of = [&](int32_t s) { return steps.template key<F::kKeys>(s); };
 
     // this lane's query, and what it sees
     const int32_t row = row_tile * kStepRows + lane % 16, t = row / a.group;
     const int32_t h = head * a.group + row % a.group;
-    const bool live = t <= steps.last && row < a.tokens * a.group;
-    Keys mine{0, 0, -1};
+    const bool live = t <= steps.last;
+    Keys mine{0, 0, -1, 0};
     if (live) mine = a.keys(a.start(b), t, t);
 
     v4u qf[F::kSteps];
@@ -328,7 +267,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
     if (threadIdx.x == 0) odd = 0;
     __syncthreads();
     const bool whole = s_begin == 0 && s_end == steps.count;
-    const int64_t unit = static_cast<int64_t>(mine_entry) * a.kv_heads + head;
+    const int64_t unit = static_cast<int64_t>(head) * entries + mine_entry;
     if (threadIdx.x == 0 && s_begin == 0)
       spans[unit] = whole ? StepSpan{0, -1}
                           : StepSpan{static_cast<int32_t>(g),
@@ -351,13 +290,14 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
         norm += from[DP + 1] * f;
       }
       const int32_t r = row_tile * kStepRows + i;
-      if (whole) {
+      const int64_t place = (b * a.tokens + r / a.group) * a.heads + head * a.group + r % a.group;
+      if (whole && whole_parts == nullptr) {
         const float value = norm == 0.0f ? 0.0f : sum / norm;
         if (!(fabsf(value) < INFINITY)) atomicOr(&odd, 1u << i);
-        out[((b * a.tokens + r / a.group) * a.heads + head * a.group + r % a.group) * a.dim + d] =
-            V::narrow(value);
+        out[place * a.dim + d] = V::narrow(value);
       } else {
-        float *part = parts + ((2 * g + (s_begin == 0 ? 1 : 0)) * kStepRows + i) * part_stride(a.dim);
+        float *part = whole ? whole_parts + place * part_stride(a.dim)
+                            : parts + ((2 * g + (s_begin == 0 ? 1 : 0)) * kStepRows + i) * part_stride(a.dim);
         part[d] = sum;
         if (d == 0) {
           part[a.dim] = top;
@@ -377,112 +317,29 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
   }
 }
 
-// A workgroup a (sequence, query, head) whose keys were cut over workgroups: their sums
-// in the order of the keys, four values a thread, every eighth part (dim 128) of
-// them; then those of the threads that have the same values, through LDS.
 template <class V, int DP>
-__global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a, StepGrid grid,
-                                                       const StepSpan *spans, const float *parts,
-                                                       typename V::Storage *out) {
-  constexpr int kLanes = DP / 4, kBeside = kThreads / kLanes;
-  __shared__ __attribute__((aligned(16))) float lds[kBeside][DP + 4];
-  const int64_t row = blockIdx.x;
-  const int32_t h = static_cast<int32_t>(row % a.heads);
-  const int32_t t = static_cast<int32_t>(row / a.heads % a.tokens);
-  const int64_t b = row / a.heads / a.tokens;
-  const int32_t r = t * a.group + h % a.group, i = r % kStepRows;
-  const StepSpan span = spans[(b * grid.tiles + r / kStepRows) * a.kv_heads + h / a.group];
-  if (span.last < span.first) return;
-  const int64_t stride = part_stride(a.dim);
-  const int32_t n = span.last - span.first + 1;
-  const int beside = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
-  float m = -INFINITY, l = 0.0f;
-  v4f o{0, 0, 0, 0};
-#pragma unroll 4
-  for (int32_t s = beside; s < n; s += kBeside) {
-    // the first workgroup's last place, the others' first
-    const float *part = parts + ((2 * static_cast<int64_t>(span.first + s) + (s == 0 ? 1 : 0)) * kStepRows + i) * stride;
-    const float part_m = part[a.dim], part_l = part[a.dim + 1];
-    v4f x{0, 0, 0, 0};
-    if (d < a.dim) x = *reinterpret_cast<const v4f *>(part + d);
-    const float top = fmaxf(m, part_m), base = top == -INFINITY ? 0.0f : top;
-    const float keep = exp2_fast(m - base), f = exp2_fast(part_m - base);
-    l = l * keep + part_l * f;
-    o = o * keep + x * f;
-    m = top;
-  }
-  *reinterpret_cast<v4f *>(&lds[beside][d]) = o;
-  if (d == 0) {
-    lds[beside][DP] = m;
-    lds[beside][DP + 1] = l;
-  }
-  __syncthreads();
-  bool bad = false;
-  if (threadIdx.x < a.dim) {
-    float top = -INFINITY, sum = 0.0f, norm = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kBeside; ++s) top = fmaxf(top, lds[s][DP]);
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int s = 0; s < kBeside; ++s) {
-      const float f = exp2_fast(lds[s][DP] - base);
-      sum += lds[s][threadIdx.x] * f;
-      norm += lds[s][DP + 1] * f;
-    }
-    const float value = norm == 0.0f ? 0.0f : sum / norm;
-    bad = !(fabsf(value) < INFINITY);
-    out[row * a.dim + threadIdx.x] = V::narrow(value);
-  }
-  if (__syncthreads_or(bad) && threadIdx.x < kWave) paged_row<V>(a, b, t, h, &lds[0][0], out);
-}
-
-StepGrid grid_of(const PagedArgs &a) {
-  StepGrid g;
-  g.tiles = static_cast<int32_t>((static_cast<int64_t>(a.tokens) * a.group + kStepRows - 1) / kStepRows);
-  g.groups = a.dim > 128 ? 256 : 512;  // what runs at once: registers allow one a CU, or two
-  return g;
-}
-
-size_t spans_bytes(const PagedArgs &a) {
-  return (sizeof(StepSpan) * static_cast<size_t>(a.batch) * grid_of(a).tiles * a.kv_heads + 255) / 256 * 256;
-}
-
-template <class V, int DP>
-msx_status run(const PagedArgs &a, void *out, void *scratch, hipStream_t stream) {
-  using S = typename V::Storage;
-  const StepGrid grid = grid_of(a);
-  const int64_t rows = a.batch * a.tokens * a.heads;
-  if (a.batch * grid.tiles > kWindowIntMax || rows > max_blocks(kThreads))
-    return fail(MSX_EINVAL, "paged_attention has more rows than a grid holds.");
-  auto *spans = static_cast<StepSpan *>(scratch);
-  auto *parts = reinterpret_cast<float *>(static_cast<char *>(scratch) + spans_bytes(a));
-  paged_step<V, DP><<<grid.groups, kThreads, 0, stream>>>(a, grid, static_cast<S *>(out), spans, parts);
-  paged_join<V, DP><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(a, grid, spans, parts,
-                                                                         static_cast<S *>(out));
+msx_status run(const PagedArgs &a, const StepGrid &grid, const TileParts &to, hipStream_t stream) {
+  paged_step<V, DP><<<grid.groups, kThreads, 0, stream>>>(a, grid, static_cast<typename V::Storage *>(to.out),
+                                                          to.spans, to.whole, to.parts);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
 }
 
 template <class V>
-msx_status by_dim(const PagedArgs &a, void *out, void *scratch, hipStream_t stream) {
-  if (a.dim <= 64) return run<V, 64>(a, out, scratch, stream);
-  if (a.dim <= 128) return run<V, 128>(a, out, scratch, stream);
-  return run<V, 256>(a, out, scratch, stream);
+msx_status by_dim(const PagedArgs &a, const StepGrid &grid, const TileParts &to, hipStream_t stream) {
+  if (a.dim <= 64) return run<V, 64>(a, grid, to, stream);
+  if (a.dim <= 128) return run<V, 128>(a, grid, to, stream);
+  return run<V, 256>(a, grid, to, stream);
 }
 
 }  // namespace
 
-size_t paged_step_scratch(const PagedArgs &a) {
-  return spans_bytes(a) +
-         sizeof(float) * 2 * grid_of(a).groups * kStepRows * static_cast<size_t>(part_stride(a.dim));
-}
-
-msx_status launch_paged_step(msx_vtype vt, const PagedArgs &a, void *out, void *scratch,
-                             hipStream_t stream) {
+msx_status launch_paged_step(msx_vtype vt, const PagedArgs &a, const StepGrid &grid,
+                             const TileParts &to, hipStream_t stream) {
   switch (vt) {
-  case MSX_F32: return by_dim<F32>(a, out, scratch, stream);
-  case MSX_F16: return by_dim<F16>(a, out, scratch, stream);
-  default: return by_dim<BF16>(a, out, scratch, stream);
+  case MSX_F32: return by_dim<F32>(a, grid, to, stream);
+  case MSX_F16: return by_dim<F16>(a, grid, to, stream);
+  default: return by_dim<BF16>(a, grid, to, stream);
   }
 }
 
