@@ -77,7 +77,7 @@ struct Keys {
   __device__ __forceinline__ int32_t count() const { return far + (hi < lo ? 0 : hi - lo + 1); }
   __device__ __forceinline__ int32_t key(int32_t c) const { return c < far ? c : lo + c - far; }
   __device__ __forceinline__ bool sees(int32_t j) const {
-    return j >= from && j <= hi && (j >= lo || j < far);
+    return (j >= from) & (j <= hi) & ((j >= lo) | (j < far));
   }
 };
 

@@ -59,6 +59,11 @@ __device__ __forceinline__ Steps uniform(const Steps &s) {
           one(s.sinks), one(s.window), one(s.count)};
 }
 
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const auto low = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int32_t>(x)));
+  return static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int32_t>(x >> 32))) << 32 | low;
+}
+
 // Inclusive sums over a workgroup of kWaves waves; `total` the last one's.
 template <int kWaves>
 __device__ __forceinline__ int64_t running_sums(int64_t x, int64_t *lds, int64_t &total) {
@@ -77,6 +82,7 @@ __device__ __forceinline__ int64_t running_sums(int64_t x, int64_t *lds, int64_t
     if (w < wave) x += lds[w];
     total += lds[w];
   }
+  total = uniform(total);
   return x;
 }
 

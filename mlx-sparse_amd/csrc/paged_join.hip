@@ -50,10 +50,10 @@ struct Parts {
 
 template <class V, int DP>
 __global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a, PartSource one, PartSource two,
-                                                       int64_t first, typename V::Storage *out) {
+                                                       typename V::Storage *out) {
   constexpr int kLanes = DP / 4, kBeside = kThreads / kLanes;
   __shared__ __attribute__((aligned(16))) float lds[kBeside][DP + 4];
-  const int64_t row = first + blockIdx.x;
+  const int64_t row = blockIdx.x;
   const int32_t h = static_cast<int32_t>(row % a.heads);
   const int32_t t = static_cast<int32_t>(row / a.heads % a.tokens);
   const int64_t b = row / a.heads / a.tokens;
@@ -101,13 +101,73 @@ __global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a, PartSource o
   if (__syncthreads_or(bad) && threadIdx.x < kWave) paged_row<V>(a, b, t, h, &lds[0][0], out);
 }
 
+// The same for many rows of few parts each: a row's parts one after the other, four
+// values a thread, kBeside rows a workgroup.
+template <class V, int DP>
+__global__ __launch_bounds__(kThreads) void paged_join_rows(PagedArgs a, PartSource one, PartSource two,
+                                                            int64_t first, int64_t rows,
+                                                            typename V::Storage *out) {
+  constexpr int kLanes = DP / 4, kBeside = kThreads / kLanes;
+  __shared__ float q_lds[kThreads / kWave][kWindowMaxDim];
+  const int64_t row = first + static_cast<int64_t>(blockIdx.x) * kBeside + threadIdx.x / kLanes;
+  const int d = threadIdx.x % kLanes * 4;
+  const int32_t h = static_cast<int32_t>(row % a.heads);
+  const int32_t t = static_cast<int32_t>(row / a.heads % a.tokens);
+  const int64_t b = row / a.heads / a.tokens;
+  bool bad = false;
+  if (row < rows) {
+    const Parts p(a, one, b, t, h), q(a, two, b, t, h);
+    const int32_t n = p.count + q.count;
+    float m = -INFINITY, l = 0.0f;
+    v4f o{0, 0, 0, 0};
+#pragma unroll 4
+    for (int32_t s = 0; s < n; ++s) {
+      const float *part = s < p.count ? p.at(s) : q.at(s - p.count);
+      const float part_m = part[a.dim], part_l = part[a.dim + 1];
+      v4f x{0, 0, 0, 0};
+      if (d < a.dim) x = *reinterpret_cast<const v4f *>(part + d);
+      const float top = fmaxf(m, part_m), base = top == -INFINITY ? 0.0f : top;
+      const float keep = exp2_fast(m - base), f = exp2_fast(part_m - base);
+      l = l * keep + part_l * f;
+      o = o * keep + x * f;
+      m = top;
+    }
+    if (n > 0 && d < a.dim) {  // (else written where it was worked out)
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = l == 0.0f ? 0.0f : o[j] / l;
+        bad = bad || !(fabsf(x[j]) < INFINITY);
+      }
+      store_four<V>(x, x, out + row * a.dim + d, nullptr);
+    }
+  }
+  uint64_t anew = __ballot(bad);
+  while (anew != 0) {
+    const int at = __builtin_ctzll(anew) / kLanes * kLanes;  // the first lane of the row's
+    anew &= ~((kLanes == kWave ? ~uint64_t{0} : (uint64_t{1} << kLanes) - 1) << at);
+    paged_row<V>(a, __shfl(b, at), __shfl(t, at), __shfl(h, at), q_lds[threadIdx.x / kWave], out);
+  }
+}
+
+// Above so many rows a row has few parts: they share 512 workgroups' stretches.  2,048 queries
+// of 16 heads in three parts each take NN us so, 64 a workgroup a row.
+constexpr int64_t kManyRows = 4096;
+
 template <class V, int DP>
 msx_status run(const PagedArgs &a, const PartSource &first, const PartSource &second, void *out,
                hipStream_t stream) {
-  const int64_t rows = a.batch * a.tokens * a.heads, most = max_blocks(kThreads);
-  for (int64_t row = 0; row < rows; row += most)
-    paged_join<V, DP><<<static_cast<unsigned>(std::min(rows - row, most)), kThreads, 0, stream>>>(
-        a, first, second, row, static_cast<typename V::Storage *>(out));
+  constexpr int64_t kBeside = kThreads / (DP / 4);
+  const int64_t rows = a.batch * a.tokens * a.heads;
+  auto *to = static_cast<typename V::Storage *>(out);
+  if (rows > kManyRows) {
+    const int64_t most = max_blocks(kThreads) * kBeside;
+    for (int64_t row = 0; row < rows; row += most)
+      paged_join_rows<V, DP><<<static_cast<unsigned>((std::min(rows - row, most) + kBeside - 1) / kBeside),
+                               kThreads, 0, stream>>>(a, first, second, row, rows, to);
+  } else {
+    paged_join<V, DP><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(a, first, second, to);
+  }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
 }

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedAr
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int place = 16 * i + k;
-          const bool seen = (there >> (place + 4 * quad) & 1) && mine.sees(j0 + place);
+          const bool seen = ((there >> (place + 4 * quad) & 1) != 0) & mine.sees(j0 + place);
           x[4 * i + k] = seen ? s[i][k] * a.scale : -INFINITY;
           top = fmaxf(top, x[4 * i + k]);
         }

@@ -49,10 +49,11 @@ __device__ __forceinline__ int32_t wave_least(int32_t v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// The rows of a tile of keys, from their pages to LDS, sixteen bytes a piece.  Whole
-// tiles go there directly: no registers on the way.  A wave's load takes a few
-// rows that follow each other; where pages hold whole such groups, their address is
-// uniform but for the lane's own offset.
+// The rows of a tile of keys and of their values, from the pages to LDS, sixteen bytes a
+// piece.  Whole tiles go there directly: no registers on the way.  A wave's load takes a
+// few rows that follow each other; where pages hold whole such groups, their address
+// is uniform but for the lane's own offset.  (Caches whose strides differ go through
+// registers: with an address for each, scalar registers run out.)
 //
 // A direct load puts lane i's piece at sixteen i bytes: the piece at place c of a row
 // is the row's chunk c ^ f(row), the permutation of TileShape::along.
@@ -67,55 +68,82 @@ struct PageLoader {
   static constexpr int kKinds = kRows % 16 == 0 ? 1 : 2;  // the permutation repeats after sixteen rows
   static_assert(kPieces % kThreads == 0 && kRows * kKinds % 16 == 0, "a thread's pieces are of one or two kinds");
   uint32_t offset[kKinds];  // of the thread's pieces from its wave's first row
-  int64_t page_step, slot_step;  // bytes
-  bool plain, grouped;           // uniform
+  bool plain, grouped;      // uniform
 
-  __device__ __forceinline__ void start(const int64_t *strides, const PageTable &table, int dim) {
-    page_step = strides[0] * T::kSize;
-    slot_step = strides[1] * T::kSize;
-    plain = kEven && dim == DP && slot_step >= 0 && slot_step * kTogether < (int64_t{1} << 31);
-    grouped = table.size % kTogether == 0;
+  __device__ __forceinline__ explicit PageLoader(const PagedArgs &a) {
+    const int64_t slot_step = a.ks[1] * T::kSize;
+    plain = kEven && a.dim == DP && slot_step >= 0 && slot_step * kTogether < (int64_t{1} << 31) &&
+            a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1];
+    grouped = a.table.size % kTogether == 0;
     const int row = threadIdx.x / T::kChunks;
 #pragma unroll
     for (int kind = 0; kind < kKinds; ++kind)
       offset[kind] = static_cast<uint32_t>(row % kTogether) * static_cast<uint32_t>(slot_step) +
                      T::logical(row + kind * kRows, threadIdx.x % T::kChunks) * 16;
   }
+  __device__ static __forceinline__ void load(const char *from, char *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from),
+                                     (__attribute__((address_space(3))) void *)(to), 16, 0, 0);
+  }
   // The kKeys keys from j on, whose pages the lanes hold, all there.
-  __device__ __forceinline__ void direct(const char *cache, const PageTable &table, int32_t pages,
-                                         int32_t j, char *tile) const {
+  __device__ __forceinline__ void direct(const PagedArgs &a, const char *k, const char *v, int32_t pages,
+                                         int32_t j, char *k_tile, char *v_tile) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const auto places = [&](int r, auto &&from) {
+      char *const to = k_tile + (r * kThreads + wave * kWave) * 16;
+      load(from(k), to);
+      load(from(v), to + (v_tile - k_tile));
+    };
+    if (grouped) {
 #pragma unroll
-    for (int r = 0; r < kPer; ++r) {
-      const char *from;
-      if (grouped) {
+      for (int r = 0; r < kPer; ++r) {
         const int row = r * kRows + wave * kTogether;
         const int64_t page = __builtin_amdgcn_readlane(pages, row);
-        from = cache + page * page_step + table.slot(j + row) * slot_step + offset[r % kKinds];
-      } else {
+        const int64_t at = (page * a.ks[0] + a.table.slot(j + row) * a.ks[1]) * T::kSize;
+        places(r, [&](const char *cache) { return cache + at + offset[r % kKinds]; });
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kPer; ++r) {
         const int row = r * kRows + threadIdx.x / T::kChunks;
         const int64_t page = __shfl(pages, row);
-        from = cache + page * page_step + table.slot(j + row) * slot_step +
-               T::logical(row, threadIdx.x % T::kChunks) * 16;
+        const int64_t at = (page * a.ks[0] + a.table.slot(j + row) * a.ks[1]) * T::kSize +
+                           T::logical(row, threadIdx.x % T::kChunks) * 16;
+        places(r, [&](const char *cache) { return cache + at; });
       }
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void *)(from),
-          (__attribute__((address_space(3))) void *)(tile + (r * kThreads + wave * kWave) * 16), 16, 0, 0);
     }
   }
-  // Zeros for those that are not.
-  __device__ __forceinline__ void each(const char *cache, const PageTable &table, int32_t pages,
-                                       int32_t j, int dim, char *tile) const {
+  // Of one cache, zeros for those that are not there.
+  __device__ __forceinline__ void each(const PagedArgs &a, const char *cache, const int64_t *strides,
+                                       int32_t pages, int32_t j, char *tile) const {
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
       const int at = threadIdx.x + r * kThreads, row = at / T::kChunks, chunk = at % T::kChunks;
       const int64_t page = __shfl(pages, row);
       if (chunk >= T::kUsed) continue;
       v4u piece = {0, 0, 0, 0};
-      if (page >= 0 && chunk * 16 < dim * T::kSize)
-        piece = *reinterpret_cast<const v4u *>(cache + page * page_step + table.slot(j + row) * slot_step + chunk * 16);
+      if (page >= 0 && chunk * 16 < a.dim * T::kSize)
+        piece = *reinterpret_cast<const v4u *>(
+            cache + (page * strides[0] + a.table.slot(j + row) * strides[1]) * T::kSize + chunk * 16);
       *reinterpret_cast<v4u *>(tile + T::along(row, chunk)) = piece;
     }
+  }
+};
+
+// Row r of those that share kv head `head`: of sequence b0, or of the batch.
+template <bool kShared>
+struct TileRow {
+  int64_t b;
+  int32_t t, h;
+  bool held;  // has a place in the results
+  __device__ __forceinline__ TileRow(const PagedArgs &a, int64_t b0, int32_t head, int32_t r) : b(b0) {
+    t = r / a.group;
+    h = head * a.group + r - t * a.group;
+    if constexpr (kShared) {
+      b = t / a.tokens;
+      t -= static_cast<int32_t>(b) * a.tokens;
+    }
+    held = b < a.batch && t < a.tokens;
   }
 };
 
@@ -186,12 +214,10 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
     }
     __syncthreads();
     entry = __builtin_amdgcn_readfirstlane(found);
-    x = kvh * total + found_first;
+    x = kvh * total + uniform(found_first);
   }
 
-  PageLoader<V, DP, F::kKeys> k_rows, v_rows;
-  k_rows.start(a.ks, a.table, a.dim);
-  v_rows.start(a.vs, a.table, a.dim);
+  const PageLoader<V, DP, F::kKeys> rows(a);
   // a negative scale moves its sign to the queries, so that the largest product is the
   // largest score
   const float scale = fabsf(a.scale);
@@ -221,18 +247,10 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
     if (s_begin >= s_end) continue;  // what this workgroup has of it is no step
 
     // this lane's row
-    const int32_t r0 = block * kTileRows + wave * kWaveRows + lane % 32;
-    int64_t b = b0;
-    int32_t t = r0 / a.group;
-    const int32_t h = head * a.group + r0 % a.group;
-    if constexpr (kShared) {
-      b = t / a.tokens;
-      t -= static_cast<int32_t>(b) * a.tokens;
-    }
-    const bool held = b < a.batch && t < a.tokens;  // has a place in the results
-    const bool live = held && t < a.length(b);
+    const TileRow<kShared> row(a, b0, head, block * kTileRows + wave * kWaveRows + lane % 32);
+    const bool live = row.held && row.t < a.length(row.b);
     Keys mine{0, 0, -1, 0};
-    if (live) mine = a.keys(a.start(b), t, t);
+    if (live) mine = a.keys(a.start(row.b), row.t, row.t);
     if constexpr (kShared) mine = Keys{0, 0, min(mine.hi, grid.from - 1), 0};
     // what the wave's rows see: all of them [all_lo, all_hi], any of them the rest
     const int32_t all_lo = -wave_least(live ? -mine.lo : 0), all_hi = wave_least(live ? mine.hi : 0x7fffffff);
@@ -241,8 +259,8 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
 
     Frag qf[kSteps];
     {
-      const char *q = reinterpret_cast<const char *>(static_cast<const S *>(a.q) + b * a.qs[0] +
-                                                     t * a.qs[1] + h * a.qs[2]);
+      const char *q = reinterpret_cast<const char *>(static_cast<const S *>(a.q) + row.b * a.qs[0] +
+                                                     row.t * a.qs[1] + row.h * a.qs[2]);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         v4u w = {0, 0, 0, 0};
@@ -264,11 +282,12 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
     const auto fetch = [&](int32_t s, int32_t pages, int parity) {
       const int32_t j = steps.template key<F::kKeys>(s);
       char *k_to = lds + parity * F::kTile, *v_to = lds + (2 + parity) * F::kTile;
-      const bool all = __ballot(pages >= 0) == kAll;
-      if (all && k_rows.plain) k_rows.direct(k_base, a.table, pages, j, k_to);
-      else k_rows.each(k_base, a.table, pages, j, a.dim, k_to);
-      if (all && v_rows.plain) v_rows.direct(v_base, a.table, pages, j, v_to);
-      else v_rows.each(v_base, a.table, pages, j, a.dim, v_to);
+      if (rows.plain && __ballot(pages >= 0) == kAll) {
+        rows.direct(a, k_base, v_base, pages, j, k_to, v_to);
+      } else {
+        rows.each(a, k_base, a.ks, pages, j, k_to);
+        rows.each(a, v_base, a.vs, pages, j, v_to);
+      }
     };
 
     v16f o[DP / 32];
@@ -278,13 +297,6 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
       for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
     float m = -INFINITY, base = 0.0f, l = 0.0f;  // l: of this lane's keys only
 
-    const auto scores = [&](uint32_t tile, int i, v16f &to) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) to[r] = 0.0f;
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st)
-        to = Mfma<V>::mul(read_rows<V>(lanes, tile, 32 * i, st), qf[st], to);
-    };
     const auto exponentials = [&](const v16f &from) {
       float e[16], sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -308,7 +320,7 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int place = 32 * i + 8 * (r / 4) + r % 4;
-            y[i][r] = (seen >> place & 1) && mine.sees(first + place) ? y[i][r] : -INFINITY;
+            y[i][r] = ((seen >> place & 1) != 0) & mine.sees(first + place) ? y[i][r] : -INFINITY;
           }
       }
       float tops[2] = {y[0][0], y[0][1]};
@@ -335,15 +347,31 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
     fetch(s_begin, pages, 0);
     sync_tiles();
     const auto step = [&](int32_t s, int parity) __attribute__((always_inline)) {
+      const int32_t j0 = steps.template key<F::kKeys>(s), j1 = j0 + F::kKeys - 1;
+      const bool seen = j0 <= any_hi && (j1 >= any_lo || j0 < any_far);
+      // (the keys are read from LDS before the next tile is asked for: a read that
+      // follows would wait for it)
+      Frag kf[F::kSub][kSteps];
+      if (seen) {
+#pragma unroll
+        for (int i = 0; i < F::kSub; ++i)
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st)
+            kf[i][st] = read_rows<V>(lanes, static_cast<uint32_t>(parity * F::kTile), 32 * i, st);
+      }
       const uint64_t there = __ballot(pages >= 0);
       pages = ahead;
       ahead = pages_of(s + 2);
       if (s + 1 < s_end) fetch(s + 1, pages, parity ^ 1);  // into the other tiles, which all waves are past
-      const int32_t j0 = steps.template key<F::kKeys>(s), j1 = j0 + F::kKeys - 1;
-      if (j0 <= any_hi && (j1 >= any_lo || j0 < any_far)) {
+      if (seen) {
         v16f y[F::kSub];
 #pragma unroll
-        for (int i = 0; i < F::kSub; ++i) scores(static_cast<uint32_t>(parity * F::kTile), i, y[i]);
+        for (int i = 0; i < F::kSub; ++i) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[i][r] = 0.0f;
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) y[i] = Mfma<V>::mul(kf[i][st], qf[st], y[i]);
+        }
         settle(j0, there, y);
 #pragma unroll
         for (int i = 0; i < F::kSub; ++i)
@@ -357,7 +385,11 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
     }
 
     l += other_half(l);
-    if (!live) {
+    // the row once more: its places would take registers all through the loop
+    int32_t again = block * kTileRows + wave * kWaveRows + lane % 32;
+    asm volatile("" : "+v"(again));
+    const TileRow<kShared> to_row(a, b0, head, again);
+    if (mine.hi < 0) {  // sees nothing
       l = 0.0f;
       m = -INFINITY;
     }
@@ -367,9 +399,10 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
       spans[unit] = all_of_it ? StepSpan{0, -1}
                               : StepSpan{static_cast<int32_t>(g),
                                          static_cast<int32_t>(share.owner(first_step + steps.count - 1))};
-    const int64_t row = (b * a.tokens + t) * a.heads + h;
+    const bool held = to_row.held;
+    const int64_t place = (to_row.b * a.tokens + to_row.t) * a.heads + to_row.h;
     if (kShared || !all_of_it) {
-      float *to = all_of_it ? whole_parts + row * part_stride(a.dim)
+      float *to = all_of_it ? whole_parts + place * part_stride(a.dim)
                             : parts + ((2 * g + (s_begin == 0 ? 1 : 0)) * kTileRows + wave * kWaveRows + lane % 32) *
                                           part_stride(a.dim);
       if (held) {
@@ -401,7 +434,7 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
             y[k] = l == 0.0f ? 0.0f : o[dt][r + k] * inv;
             odd = odd || !(fabsf(y[k]) < INFINITY);
           }
-          if (d < a.dim) store_four<V>(y, y, out + row * a.dim + d, nullptr);
+          if (d < a.dim) store_four<V>(y, y, out + place * a.dim + d, nullptr);
         }
     }
     uint64_t anew = __ballot(odd);
@@ -410,7 +443,7 @@ __global__ __launch_bounds__(kThreads, (PagedShape<V, DP>::kBlocks)) void paged_
       while (anew != 0) {  // the tiles in LDS are done with: all waves left the loop
         const int i = __builtin_ctzll(anew);
         anew &= anew - 1;
-        paged_row<V>(a, b0, __shfl(t, i), __shfl(h, i), reinterpret_cast<float *>(lds) + wave * kWindowMaxDim, out);
+        paged_row<V>(a, b0, __shfl(to_row.t, i), __shfl(to_row.h, i), reinterpret_cast<float *>(lds) + wave * kWindowMaxDim, out);
       }
       __syncthreads();
     }

@@ -294,9 +294,13 @@ msx_status launch(const Rows &rows, const Turning &how, int64_t tokens, int32_t 
   s.heads = heads;
   s.units = Unit<V, E, kInterleaved>::units(how.r, dim);
   const int32_t groups = kThreads / s.units;
-  s.side = std::min(heads, groups);
+  // Where there are heads for 256 CUs' threads four times over, a thread takes four of a
+  // token's, its loads in flight together and its angles worked out once; a few tokens
+  // are spread over as many workgroups as their heads give.
+  const bool many = tokens * heads * s.units >= int64_t{4} * 256 * 1024;
+  s.side = std::min(many ? (heads + 3) / 4 : heads, groups);
   s.per_block = groups / s.side;
-  s.parts = 1;
+  s.parts = many ? 1 : (heads + s.side - 1) / s.side;
   const int64_t most = max_blocks(kThreads) / s.parts * s.per_block;
   for (int64_t first = 0; first < tokens; first += most) {
     const int64_t here = std::min(tokens - first, most);
