@@ -1,0 +1,500 @@
+// msx_paged_block.h - many queries against the same pages, chunks of prompts and the
+// queries of a batch against the pages that it shares: what a workgroup does.
+//
+// A wave takes 32 rows (a row is a query and head; those of a query that share a kv
+// head follow each other), a workgroup four such units, which share the tiles of
+// keys in LDS.  Per tile: S^T = K Q^T, the running maximum and sum, O^T += V^T P^T,
+// as in window_forward.hip; the next tile's rows are on their way to LDS meanwhile,
+// the numbers of the pages after those in registers.  A row's probabilities are rounded
+// to the operands' 16 bits for the second product, unnormalised and at most
+// 2^8: their errors are independent and no larger than the output's own rounding.
+//
+// As in msx_paged_step.h each workgroup takes an equal stretch of all tiles, numbered by
+// kv head, sequence and unit; of its first and last unit it may have a part, which
+// paged_join joins.
+#pragma once
+
+#include "msx_paged.h"
+#include "msx_paged_row.h"
+#include "msx_paged_tiles.h"
+#include "msx_window_mfma.h"
+
+#pragma clang fp contract(fast)
+
+namespace msx {
+
+constexpr int kTileWaves = kTileRows / 32;
+constexpr int kTileThreads = kTileWaves * kWave;
+
+template <class V, int DP>
+struct PagedShape {
+  using T = TileShape<V, DP>;
+  static constexpr int kSub = T::kSize == 2 ? 2 : 1;  // 32-key parts of a tile
+  static constexpr int kKeys = 32 * kSub;
+  static constexpr int kTile = kKeys * T::kPitch;
+  static constexpr int kLds = 4 * kTile;  // K and V, twice
+  // workgroups a CU: two hide each other's waits; wide float32 heads need the
+  // registers of one
+  static constexpr int kBlocks = T::kRowBytes > 256 ? 1 : 2;
+};
+
+__device__ __forceinline__ int32_t wave_least(int32_t v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = min(v, __shfl_xor(v, d));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// The rows of a tile of keys and of their values, from the pages to LDS, sixteen bytes a
+// piece.  Whole tiles go there directly: no registers on the way.  A wave's load takes a
+// few rows that follow each other; where pages hold whole such groups, their address
+// is uniform but for the lane's own offset.  (Caches whose strides differ go through
+// registers: with an address for each, scalar registers run out.)
+//
+// A direct load puts lane i's piece at sixteen i bytes: the piece at place c of a row
+// is the row's chunk c ^ f(row), the permutation of TileShape::along.
+template <class V, int DP, int kKeys>
+struct PageLoader {
+  using T = TileShape<V, DP>;
+  static constexpr int kPieces = kKeys * T::kChunks;
+  static constexpr int kPer = kPieces / kTileThreads;
+  static constexpr int kRows = kTileThreads / T::kChunks;     // between a thread's pieces
+  static constexpr int kTogether = kWave / T::kChunks;    // rows of a wave's load
+  static constexpr bool kEven = T::kUsed == T::kChunks;
+  static constexpr int kKinds = kRows % 16 == 0 ? 1 : 2;  // the permutation repeats after sixteen rows
+  static_assert(kPieces % kTileThreads == 0 && kRows * kKinds % 16 == 0, "a thread's pieces are of one or two kinds");
+  uint32_t offset[kKinds];  // of the thread's pieces from its wave's first row
+  bool plain, grouped;      // uniform
+
+  __device__ __forceinline__ explicit PageLoader(const PagedArgs &a) {
+    const int64_t slot_step = a.ks[1] * T::kSize;
+    plain = kEven && a.dim == DP && slot_step >= 0 && slot_step * kTogether < (int64_t{1} << 31) &&
+            a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1];
+    grouped = a.table.size % kTogether == 0;
+    const int row = threadIdx.x / T::kChunks;
+#pragma unroll
+    for (int kind = 0; kind < kKinds; ++kind)
+      offset[kind] = static_cast<uint32_t>(row % kTogether) * static_cast<uint32_t>(slot_step) +
+                     T::logical(row + kind * kRows, threadIdx.x % T::kChunks) * 16;
+  }
+  __device__ static __forceinline__ void load(const char *from, char *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from),
+                                     (__attribute__((address_space(3))) void *)(to), 16, 0, 0);
+  }
+  // The kKeys keys from j on, whose pages the lanes hold, all there.
+  __device__ __forceinline__ void direct(const PagedArgs &a, const char *k, const char *v, int32_t pages,
+                                         int32_t j, char *k_tile, char *v_tile) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const auto places = [&](int r, auto &&from) {
+      char *const to = k_tile + (r * kTileThreads + wave * kWave) * 16;
+      load(from(k), to);
+      load(from(v), to + (v_tile - k_tile));
+    };
+    if (grouped) {
+#pragma unroll
+      for (int r = 0; r < kPer; ++r) {
+        const int row = r * kRows + wave * kTogether;
+        const int64_t page = __builtin_amdgcn_readlane(pages, row);
+        const int64_t at = (page * a.ks[0] + a.table.slot(j + row) * a.ks[1]) * T::kSize;
+        places(r, [&](const char *cache) { return cache + at + offset[r % kKinds]; });
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kPer; ++r) {
+        const int row = r * kRows + threadIdx.x / T::kChunks;
+        const int64_t page = __shfl(pages, row);
+        const int64_t at = (page * a.ks[0] + a.table.slot(j + row) * a.ks[1]) * T::kSize +
+                           T::logical(row, threadIdx.x % T::kChunks) * 16;
+        places(r, [&](const char *cache) { return cache + at; });
+      }
+    }
+  }
+  // Of one cache, zeros for those that are not there.
+  __device__ __forceinline__ void each(const PagedArgs &a, const char *cache, const int64_t *strides,
+                                       int32_t pages, int32_t j, char *tile) const {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const int at = threadIdx.x + r * kTileThreads, row = at / T::kChunks, chunk = at % T::kChunks;
+      const int64_t page = __shfl(pages, row);
+      if (chunk >= T::kUsed) continue;
+      v4u piece = {0, 0, 0, 0};
+      if (page >= 0 && chunk * 16 < a.dim * T::kSize)
+        piece = *reinterpret_cast<const v4u *>(
+            cache + (page * strides[0] + a.table.slot(j + row) * strides[1]) * T::kSize + chunk * 16);
+      *reinterpret_cast<v4u *>(tile + T::along(row, chunk)) = piece;
+    }
+  }
+};
+
+// The probabilities of 32 keys as the second product takes them: rounded to the operands' type,
+// or for shared pages rounded and what that leaves, which costs nothing there
+// (64 sequences behind 8,192 tokens wait for loads) and gives the results their own rounding
+// alone, as the sequences' own keys do.
+template <class V, bool kTwice>
+struct Probabilities {
+  Column<V> high;
+  __device__ __forceinline__ explicit Probabilities(const float (&p)[16]) : high(p) {}
+  template <int kBlocks>
+  __device__ __forceinline__ void times(const TileLanes<V, kBlocks * 32> &lanes, uint32_t tile, int row0,
+                                        v16f (&acc)[kBlocks]) const {
+    mul_transposed<V>(lanes, tile, row0, high, acc);
+  }
+};
+template <class V>
+struct Probabilities<V, true> {
+  Column<V> high, low;
+  __device__ __forceinline__ explicit Probabilities(const float (&p)[16]) : high(p), low(left(p, high)) {}
+  template <int kBlocks>
+  __device__ __forceinline__ void times(const TileLanes<V, kBlocks * 32> &lanes, uint32_t tile, int row0,
+                                        v16f (&acc)[kBlocks]) const {
+    using Frag = typename Mfma<V>::Frag;
+#pragma unroll
+    for (int dt = 0; dt < kBlocks; ++dt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        v4s part[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) part[t] = read_transposed(lanes.column_at(tile, row0, 16 * k + 8 * t, dt));
+        const auto lo = __builtin_bit_cast(v2u, part[0]), hi = __builtin_bit_cast(v2u, part[1]);
+        const auto a = __builtin_bit_cast(Frag, (v4u{lo[0], lo[1], hi[0], hi[1]}));
+        acc[dt] = Mfma<V>::mul(a, high.b[k], acc[dt]);
+        acc[dt] = Mfma<V>::mul(a, low.b[k], acc[dt]);
+      }
+  }
+
+ private:
+  __device__ static __forceinline__ Column<V> left(const float (&p)[16], const Column<V> &taken) {
+    float rest[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const v4u w = __builtin_bit_cast(v4u, taken.b[k]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t pair = w[j];
+        rest[8 * k + 2 * j] = p[8 * k + 2 * j] - V::widen(static_cast<uint16_t>(pair));
+        rest[8 * k + 2 * j + 1] = p[8 * k + 2 * j + 1] - V::widen(static_cast<uint16_t>(pair >> 16));
+      }
+    }
+    return Column<V>(rest);
+  }
+};
+
+// Row r of those that share kv head `head`: of sequence b0, or of the batch.
+template <bool kShared>
+struct TileRow {
+  int64_t b;
+  int32_t t, h;
+  bool held;  // has a place in the results
+  __device__ __forceinline__ TileRow(const PagedArgs &a, int64_t b0, int32_t head, int32_t r) : b(b0) {
+    t = r / a.group;
+    h = head * a.group + r - t * a.group;
+    if constexpr (kShared) {
+      b = t / a.tokens;
+      t -= static_cast<int32_t>(b) * a.tokens;
+    }
+    held = b < a.batch && t < a.tokens;
+  }
+};
+
+// kShared: rows are those of the whole batch, keys those of the pages that it shares
+// (grid.from of them, listed in the table's first row), and all results are parts.
+// Workgroup `id` of grid.groups; `lds`: PagedShape's kLds bytes at a multiple of 1,024.
+template <class V, int DP, bool kShared>
+__device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid &grid, uint32_t id, const TileParts &to,
+                                              char *lds, StretchLds &own) {
+  using S = typename V::Storage;
+  using F = PagedShape<V, DP>;
+  using T = TileShape<V, DP>;
+  using Frag = typename Mfma<V>::Frag;
+  constexpr int kSteps = DP / Mfma<V>::kDepth;
+  auto *const out = static_cast<S *>(to.out);
+  const TileLanes<V, DP> lanes(lds);
+
+  const int lane = threadIdx.x % kWave, half = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+
+  // this workgroup's stretch of all tiles: numbered by kv head, then (sequence, unit)
+  const int64_t entries = kShared ? grid.tiles : a.batch * grid.tiles;
+  const int32_t shared_count = (grid.from + F::kKeys - 1) / F::kKeys;
+  const auto cost_at = [&](int64_t e) -> int64_t {
+    if (e >= entries) return 0;
+    const int64_t b = quotient(e, grid.tiles);
+    return kStart + steps_of<F::kKeys, kTileRows>(a, b, static_cast<int32_t>(e - b * grid.tiles), 0).count;
+  };
+  int64_t total = 0, cost = 0, upto = 0;
+  if constexpr (kShared) {
+    total = entries * (shared_count + kStart);
+  } else {
+    cost = cost_at(threadIdx.x);
+    upto = running_sums<kTileWaves>(cost, own.sums, total);
+    if (entries > kTileThreads) {
+      int64_t mine = cost;
+      for (int64_t e = threadIdx.x + kTileThreads; e < entries; e += kTileThreads) mine += cost_at(e);
+      running_sums<kTileWaves>(mine, own.sums, total);
+    }
+  }
+  const StepShare share(total * a.kv_heads, grid.groups);
+  if (id >= share.groups) return;  // whole workgroups leave
+  const int64_t g = xcd_order(id, static_cast<uint32_t>(share.groups));
+  const int64_t begin = share.first(g), end = share.first(g + 1);
+  int32_t kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin, total)));
+  int32_t entry;
+  int64_t x;  // where the next (kv head, entry) begins
+  if constexpr (kShared) {
+    entry = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - kvh * total, shared_count + kStart)));
+    x = kvh * total + static_cast<int64_t>(entry) * (shared_count + kStart);
+  } else {
+    const int64_t at = begin - kvh * total;
+    int64_t before = 0;
+    for (int64_t e0 = 0;; e0 += kTileThreads) {  // (all that is to be done is some entry's)
+      int64_t here = total;
+      if (entries > kTileThreads) {
+        if (e0 > 0) cost = cost_at(e0 + threadIdx.x);
+        else cost = cost_at(threadIdx.x);
+        upto = running_sums<kTileWaves>(cost, own.sums, here);
+      }
+      if (before + upto - cost <= at && at < before + upto) {
+        own.found = static_cast<int32_t>(e0 + threadIdx.x);
+        own.found_first = before + upto - cost;
+      }
+      before += here;
+      if (at < before || e0 + kTileThreads >= entries) break;
+    }
+    __syncthreads();
+    entry = __builtin_amdgcn_readfirstlane(own.found);
+    x = kvh * total + uniform(own.found_first);
+  }
+
+  const PageLoader<V, DP, F::kKeys> rows(a);
+  // a negative scale moves its sign to the queries, so that the largest product is the
+  // largest score
+  const float scale = fabsf(a.scale);
+
+  while (x < end) {
+    const int64_t b0 = kShared ? 0 : quotient(entry, grid.tiles);
+    const int32_t block = kShared ? entry : entry - static_cast<int32_t>(b0) * grid.tiles;
+    Steps steps;
+    if constexpr (kShared) {
+      steps.keys = Keys{0, 0, grid.from - 1, 0};
+      steps.sinks = steps.window = 0;
+      steps.count = shared_count;
+    } else {
+      steps = uniform(steps_of<F::kKeys, kTileRows>(a, b0, block, 0));
+    }
+    const int64_t first_step = x + kStart;
+    x = first_step + steps.count;
+    const int32_t s_begin = __builtin_amdgcn_readfirstlane(
+        static_cast<int32_t>(min(max(begin - first_step, int64_t{0}), static_cast<int64_t>(steps.count))));
+    const int32_t s_end = __builtin_amdgcn_readfirstlane(
+        static_cast<int32_t>(max(min(end - first_step, static_cast<int64_t>(steps.count)), int64_t{0})));
+    const int32_t head = kvh, this_entry = entry;
+    if (++entry == entries) {
+      entry = 0;
+      ++kvh;
+    }
+    if (s_begin >= s_end) continue;  // what this workgroup has of it is no step
+
+    // this lane's row
+    const TileRow<kShared> row(a, b0, head, block * kTileRows + wave * 32 + lane % 32);
+    const bool live = row.held && row.t < a.length(row.b);
+    Keys mine{0, 0, -1, 0};
+    if (live) mine = a.keys(a.start(row.b), row.t, row.t);
+    if constexpr (kShared) mine = Keys{0, 0, min(mine.hi, grid.from - 1), 0};
+    // what the wave's rows see: all of them [all_lo, all_hi], any of them the rest
+    const int32_t all_lo = -wave_least(live ? -mine.lo : 0), all_hi = wave_least(live ? mine.hi : 0x7fffffff);
+    const int32_t any_hi = -wave_least(live ? -mine.hi : 1), any_lo = wave_least(live ? mine.lo : 0x7fffffff);
+    const int32_t any_far = -wave_least(live ? -mine.far : 0);
+
+    Frag qf[kSteps];
+    {
+      const char *q = reinterpret_cast<const char *>(static_cast<const S *>(a.q) + row.b * a.qs[0] +
+                                                     row.t * a.qs[1] + row.h * a.qs[2]);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        v4u w = {0, 0, 0, 0};
+        const int chunk = 2 * s + half;
+        if (live && chunk * 16 < a.dim * T::kSize) w = *reinterpret_cast<const v4u *>(q + chunk * 16);
+        if (a.scale < 0.0f) w ^= Mfma<V>::kSign;
+        qf[s] = __builtin_bit_cast(Frag, w);
+      }
+    }
+    const char *k_base = reinterpret_cast<const char *>(static_cast<const S *>(a.k) + head * a.ks[2]);
+    const char *v_base = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + head * a.vs[2]);
+
+    // the page of key `lane` of a tile, -1 where nobody sees it
+    const auto pages_of = [&](int32_t s) {
+      const int32_t j = steps.template key<F::kKeys>(s) + lane;
+      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? a.table.page(b0, j) : -1;
+    };
+    constexpr uint64_t kAll = F::kKeys == 64 ? ~uint64_t{0} : (uint64_t{1} << F::kKeys) - 1;
+    const auto fetch = [&](int32_t s, int32_t pages, int parity) {
+      const int32_t j = steps.template key<F::kKeys>(s);
+      char *k_to = lds + parity * F::kTile, *v_to = lds + (2 + parity) * F::kTile;
+      if (rows.plain && __ballot(pages >= 0) == kAll) {
+        rows.direct(a, k_base, v_base, pages, j, k_to, v_to);
+      } else {
+        rows.each(a, k_base, a.ks, pages, j, k_to);
+        rows.each(a, v_base, a.vs, pages, j, v_to);
+      }
+    };
+
+    v16f o[DP / 32];
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+    float m = -INFINITY, base = 0.0f, l = 0.0f;  // l: of this lane's keys only
+
+    const auto exponentials = [&](const v16f &from) {
+      float e[16], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        e[r] = exp2_fast(from[r] * scale - base);
+        sum[r % 2] += e[r];
+      }
+      l += sum[0] + sum[1];
+      return Probabilities<V, kShared && T::kSize == 2>(e);
+    };
+    // masks the scores of the tile at j0 and moves the maximum.  It is moved only where
+    // it has grown by more than 2^8: until then exponentials up to 2^8 stand
+    // beside sums of their own scale.
+    const auto settle = [&](int32_t j0, uint64_t there, v16f (&y)[F::kSub]) {
+      const bool whole = there == kAll && j0 >= all_lo && j0 + F::kKeys - 1 <= all_hi;
+      if (!whole) {
+        const uint64_t seen = there >> (4 * half);
+        const int32_t first = j0 + 4 * half;
+#pragma unroll
+        for (int i = 0; i < F::kSub; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int place = 32 * i + 8 * (r / 4) + r % 4;
+            y[i][r] = (((seen >> place & 1) != 0) & mine.sees(first + place)) ? y[i][r] : -INFINITY;
+          }
+      }
+      float tops[2] = {y[0][0], y[0][1]};
+#pragma unroll
+      for (int i = 0; i < F::kSub; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) tops[r % 2] = fmaxf(tops[r % 2], y[i][r]);
+      float top = fmaxf(tops[0], tops[1]);
+      top = fmaxf(top, other_half(top)) * scale;
+      if (__any(top > m + 8.0f)) {
+        const float grown = fmaxf(m, top);
+        const float shrink = grown == -INFINITY ? 1.0f : exp2_fast(m - grown);
+        m = grown;
+        base = m == -INFINITY ? 0.0f : m;
+        l *= shrink;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= shrink;
+      }
+    };
+
+    int32_t pages = pages_of(s_begin), ahead = pages_of(s_begin + 1);
+    fetch(s_begin, pages, 0);
+    sync_tiles();
+    const auto step = [&](int32_t s, int parity) __attribute__((always_inline)) {
+      const int32_t j0 = steps.template key<F::kKeys>(s), j1 = j0 + F::kKeys - 1;
+      const bool seen = j0 <= any_hi && (j1 >= any_lo || j0 < any_far);
+      // (the keys are read from LDS before the next tile is asked for: a read that
+      // follows would wait for it)
+      Frag kf[F::kSub][kSteps];
+      if (seen) {
+#pragma unroll
+        for (int i = 0; i < F::kSub; ++i)
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st)
+            kf[i][st] = read_rows<V>(lanes, static_cast<uint32_t>(parity * F::kTile), 32 * i, st);
+      }
+      const uint64_t there = __ballot(pages >= 0);
+      pages = ahead;
+      ahead = pages_of(s + 2);
+      if (s + 1 < s_end) fetch(s + 1, pages, parity ^ 1);  // into the other tiles, which all waves are past
+      if (seen) {
+        v16f y[F::kSub];
+#pragma unroll
+        for (int i = 0; i < F::kSub; ++i) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[i][r] = 0.0f;
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) y[i] = Mfma<V>::mul(kf[i][st], qf[st], y[i]);
+        }
+        settle(j0, there, y);
+#pragma unroll
+        for (int i = 0; i < F::kSub; ++i)
+          exponentials(y[i]).times(lanes, static_cast<uint32_t>((2 + parity) * F::kTile), 32 * i, o);
+      }
+      sync_tiles();
+    };
+    for (int32_t s = s_begin; s < s_end; s += 2) {
+      step(s, 0);
+      if (s + 1 < s_end) step(s + 1, 1);
+    }
+
+    l += other_half(l);
+    // the row once more: its places would take registers all through the loop
+    int32_t again = block * kTileRows + wave * 32 + lane % 32;
+    asm volatile("" : "+v"(again));
+    const TileRow<kShared> to_row(a, b0, head, again);
+    if (mine.hi < 0) {  // sees nothing
+      l = 0.0f;
+      m = -INFINITY;
+    }
+    const bool all_of_it = s_begin == 0 && s_end == steps.count;
+    const int64_t unit = static_cast<int64_t>(head) * entries + this_entry;
+    if (threadIdx.x == 0 && s_begin == 0)
+      to.spans[unit] = all_of_it ? StepSpan{0, -1}
+                              : StepSpan{static_cast<int32_t>(g),
+                                         static_cast<int32_t>(share.owner(first_step + steps.count - 1))};
+    const bool held = to_row.held;
+    const int64_t place = (to_row.b * a.tokens + to_row.t) * a.heads + to_row.h;
+    if (kShared || !all_of_it) {
+      float *part = all_of_it ? to.whole + place * part_stride(a.dim)
+                            : to.parts + ((2 * g + (s_begin == 0 ? 1 : 0)) * kTileRows + wave * 32 + lane % 32) *
+                                          part_stride(a.dim);
+      if (held) {
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            const int d = dt * 32 + 2 * r + 4 * half;
+            if (d < a.dim) *reinterpret_cast<v4f *>(part + d) = v4f{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]};
+          }
+        if (half == 0) {
+          part[a.dim] = m;
+          part[a.dim + 1] = l;
+        }
+      }
+      continue;  // (the last tile's waits are behind all waves)
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bool odd = false;  // something is not finite: the row is computed anew
+    if (held) {
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const int d = dt * 32 + 2 * r + 4 * half;
+          float y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            y[k] = l == 0.0f ? 0.0f : o[dt][r + k] * inv;
+            odd = odd || !(fabsf(y[k]) < INFINITY);
+          }
+          if (d < a.dim) store_four<V>(y, y, out + place * a.dim + d, nullptr);
+        }
+    }
+    uint64_t anew = __ballot(odd);
+    anew = (anew | anew >> 32) & 0xffffffffu;
+    if (__syncthreads_or(anew != 0)) {
+      while (anew != 0) {  // the tiles in LDS are done with: all waves left the loop
+        const int i = __builtin_ctzll(anew);
+        anew &= anew - 1;
+        paged_row<V>(a, b0, __shfl(to_row.t, i), __shfl(to_row.h, i), reinterpret_cast<float *>(lds) + wave * kWindowMaxDim, out);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+}  // namespace msx

@@ -125,14 +125,26 @@ struct TileParts {
   float *whole, *parts;
 };
 
+// What a workgroup has in LDS beside its tiles.
+struct StretchLds {
+  int64_t sums[4], found_first;
+  int32_t found;
+  uint32_t odd;  // rows whose results are not finite
+};
+
+constexpr int32_t kTileRows = 128;  // queries a workgroup, where they are many
+
 // paged_step.hip, paged_tiles.hip: rows and caches at sixteen-byte addresses and strides.
-// Tiles of kStepRows and kTileRows queries; paged_tiles with grid.from > 0 takes the keys
-// before it, of the pages that the batch shares, and needs heads of 128 at most.
-constexpr int32_t kTileRows = 128;
+// Grids of tiles of kStepRows and kTileRows queries; the latter need heads of 128 at most.
+// launch_paged_shared: `tiles` those of the batch against the keys before tiles.from, of the
+// pages that it shares, `step` those of each sequence against the keys from there on.
 msx_status launch_paged_step(msx_vtype vt, const PagedArgs &a, const StepGrid &grid,
                              const TileParts &to, hipStream_t stream);
 msx_status launch_paged_tiles(msx_vtype vt, const PagedArgs &a, const StepGrid &grid,
                               const TileParts &to, hipStream_t stream);
+msx_status launch_paged_shared(msx_vtype vt, const PagedArgs &a, const StepGrid &tiles,
+                               const TileParts &tiles_to, const StepGrid &step,
+                               const TileParts &step_to, hipStream_t stream);
 
 // Parts of one kernel, as paged_join reads them.
 struct PartSource {

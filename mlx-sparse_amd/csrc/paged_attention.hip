@@ -124,14 +124,14 @@ struct Plan {
     // as many workgroups as run at once: registers allow two a CU, of wide heads one
     if (route == Route::kStep || route == Route::kShared) {
       step.tiles = static_cast<int32_t>((rows + kStepRows - 1) / kStepRows);
-      step.groups = a.dim > 128 ? 256 : 512;
+      step.groups = a.dim > 128 || route == Route::kShared ? 256 : 512;
       step.from = route == Route::kShared ? static_cast<int32_t>(d.shared_pages * d.cache.page_size) : 0;
       step_to = parts_of(step, a.batch * step.tiles, kStepRows);
     }
     if (route == Route::kTiles || route == Route::kShared) {
       const int64_t together = route == Route::kShared ? a.batch * rows : rows;
       tiles.tiles = static_cast<int32_t>((together + kTileRows - 1) / kTileRows);
-      tiles.groups = a.dim * value_bytes(static_cast<msx_vtype>(d.vtype)) > 256 ? 256 : 512;
+      tiles.groups = route == Route::kShared || a.dim * value_bytes(static_cast<msx_vtype>(d.vtype)) > 256 ? 256 : 512;
       tiles.from = step.from;
       tiles_to = parts_of(tiles, route == Route::kShared ? tiles.tiles : a.batch * tiles.tiles, kTileRows);
     }
@@ -182,10 +182,13 @@ extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, 
   const PartSource none{};
   const PartSource by_step = p.source(p.step, p.step_to, kStepRows, false);
   const PartSource by_tiles = p.source(p.tiles, p.tiles_to, kTileRows, p.route == Route::kShared);
-  if (p.route != Route::kStep)
-    if (msx_status st = launch_paged_tiles(vt, a, p.tiles, p.tiles_to, s); st != MSX_OK) return st;
-  if (p.route != Route::kTiles)
-    if (msx_status st = launch_paged_step(vt, a, p.step, p.step_to, s); st != MSX_OK) return st;
+  msx_status st;
+  switch (p.route) {
+  case Route::kStep: st = launch_paged_step(vt, a, p.step, p.step_to, s); break;
+  case Route::kTiles: st = launch_paged_tiles(vt, a, p.tiles, p.tiles_to, s); break;
+  default: st = launch_paged_shared(vt, a, p.tiles, p.tiles_to, p.step, p.step_to, s); break;
+  }
+  if (st != MSX_OK) return st;
   switch (p.route) {
   case Route::kStep: return launch_paged_join(vt, a, by_step, none, out, s);
   case Route::kTiles: return launch_paged_join(vt, a, by_tiles, none, out, s);

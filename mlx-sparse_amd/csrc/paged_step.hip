@@ -1,28 +1,9 @@
-// paged_step.hip - a few queries of every sequence against its pages.
-//
-// Bound by memory: every visible key and value is read once, 2 flops a byte, query
-// and head.  The queries and heads that share a kv head (sixteen at a time) share
-// each read, as the sixteen columns of matrix products; a wave takes 32 keys (16 in
-// float32) after the other, with the next ones in flight and their pages' numbers
-// a step ahead of them, and keeps running maximum, sum and output of its own.
-//
-// Sequences differ in length, and the host knows none of them.  The steps of all
-// (sequence, sixteen queries, kv head) are numbered through, and each workgroup takes
-// an equal stretch of them, whatever it begins and ends in: every workgroup adds
-// up the batch's lengths to find its own.  Of a stretch only the first and the last tile
-// of queries can be another's as well; what it has of them goes to two places
-// of scratch, and paged_join adds those up in the order of the keys.
+// paged_step.hip - a few queries of every sequence against its pages; see
+// msx_paged_step.h.
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
-
 #include "msx_internal.h"
-#include "msx_paged.h"
-#include "msx_paged_row.h"
-#include "msx_paged_tiles.h"
-#include "msx_step_mfma.h"
-
-#pragma clang fp contract(fast)
+#include "msx_paged_step.h"
 
 namespace msx {
 namespace {
@@ -30,297 +11,15 @@ namespace {
 constexpr int kThreads = kStepWaves * kWave;
 
 template <class V, int DP>
-__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedArgs a, StepGrid grid,
-                                                                         typename V::Storage *out,
-                                                                         StepSpan *spans, float *whole_parts,
-                                                                         float *parts) {
-  using S = typename V::Storage;
-  using F = StepShape<V, DP>;
-  __shared__ __attribute__((aligned(16))) char lds[F::kLds];
-  __shared__ int64_t sums[kStepWaves], found_first;
-  __shared__ int32_t found;
-  __shared__ uint32_t odd;
-
-  const int lane = threadIdx.x % kWave, quad = lane / 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int bytes = a.dim * F::kSize;
-
-  // this workgroup's stretch of all steps
-  const int64_t entries = a.batch * grid.tiles;  // (sequence, sixteen queries)
-  const auto cost_at = [&](int64_t e) -> int64_t {
-    if (e >= entries) return 0;
-    const int64_t b = grid.tiles == 1 ? e : e / grid.tiles;
-    return kStart + steps_of<F::kKeys, kStepRows>(a, b, static_cast<int32_t>(e - b * grid.tiles), grid.from).count;
-  };
-  int64_t total = 0, cost = cost_at(threadIdx.x), upto = running_sums<kStepWaves>(cost, sums, total);
-  if (entries > kThreads) {
-    int64_t mine = cost;
-    for (int64_t e = threadIdx.x + kThreads; e < entries; e += kThreads) mine += cost_at(e);
-    running_sums<kStepWaves>(mine, sums, total);
-  }
-  const StepShare share(total * a.kv_heads, grid.groups);
-  const int64_t g = blockIdx.x;
-  if (g >= share.groups) return;  // whole workgroups leave
-  const int64_t begin = share.first(g), end = share.first(g + 1);
-  int64_t before = 0;
-  for (int64_t e0 = 0;; e0 += kThreads) {  // (all that is to be done is some entry's)
-    int64_t here = total;
-    if (entries > kThreads) {
-      if (e0 > 0) cost = cost_at(e0 + threadIdx.x);
-      upto = running_sums<kStepWaves>(cost, sums, here);
-    }
-    const int64_t low = (before + upto - cost) * a.kv_heads, high = (before + upto) * a.kv_heads;
-    if (low <= begin && begin < high) {
-      found = static_cast<int32_t>(e0 + threadIdx.x);
-      found_first = low;
-    }
-    before += here;
-    if (begin < before * a.kv_heads || e0 + kThreads >= entries) break;
-  }
-  __syncthreads();
-  int32_t entry = __builtin_amdgcn_readfirstlane(found), kvh = -1;
-  int64_t x = found_first;  // where the next (entry, kv head) begins
-
-  while (x < end) {
-    const int64_t b = grid.tiles == 1 ? entry : entry / grid.tiles;
-    const int32_t row_tile = entry - static_cast<int32_t>(b) * grid.tiles;
-    const Steps steps = uniform(steps_of<F::kKeys, kStepRows>(a, b, row_tile, grid.from));
-    if (kvh < 0) {
-      kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - x, steps.count + kStart)));
-      x += static_cast<int64_t>(kvh) * (steps.count + kStart);
-    }
-    const int64_t first_step = x + kStart;
-    x = first_step + steps.count;
-    const int32_t s_begin = __builtin_amdgcn_readfirstlane(
-        static_cast<int32_t>(min(max(begin - first_step, int64_t{0}), static_cast<int64_t>(steps.count))));
-    const int32_t s_end = __builtin_amdgcn_readfirstlane(
-        static_cast<int32_t>(max(min(end - first_step, static_cast<int64_t>(steps.count)), int64_t{0})));
-    const int32_t head = kvh, mine_entry = entry;
-    if (++kvh == a.kv_heads) {
-      kvh = 0;
-      ++entry;
-    }
-    if (s_begin >= s_end) continue;  // what this workgroup has of it is no step
-    const auto key_of = [&](int32_t s) { return steps.template key<F::kKeys>(s); };
-
-    // this lane's query, and what it sees
-    const int32_t row = row_tile * kStepRows + lane % 16, t = row / a.group;
-    const int32_t h = head * a.group + row % a.group;
-    const bool live = t <= steps.last;
-    Keys mine{0, 0, -1, 0};
-    if (live) mine = a.keys(a.start(b), t, t);
-
-    v4u qf[F::kSteps];
-    {
-      const char *q = reinterpret_cast<const char *>(static_cast<const S *>(a.q) + b * a.qs[0] +
-                                                     t * a.qs[1] + h * a.qs[2]);
-#pragma unroll
-      for (int s = 0; s < F::kSteps; ++s) {
-        const int c = 4 * s + quad;
-        qf[s] = v4u{0, 0, 0, 0};
-        if (live && c * 16 < bytes) qf[s] = *reinterpret_cast<const v4u *>(q + c * 16);
-      }
-    }
-    const char *ck = reinterpret_cast<const char *>(static_cast<const S *>(a.k) + head * a.ks[2]);
-    const char *cv = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + head * a.vs[2]);
-
-    // the page of key `lane` of a step, -1 where nobody sees it
-    const auto pages_of = [&](int32_t s) {
-      const int32_t j = key_of(s) + lane;
-      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? a.table.page(b, j) : -1;
-    };
-    v4u kf[F::kTiles][F::kSteps], vf[F::kVPer];
-    const auto fetch_k = [&](int32_t s, int32_t pages) {
-#pragma unroll
-      for (int i = 0; i < F::kTiles; ++i) {
-        const int place = 16 * i + lane % 16;
-        const int64_t page = __shfl(pages, place);
-        const char *from = ck + (page * a.ks[0] + a.table.slot(key_of(s) + place) * a.ks[1]) * F::kSize;
-#pragma unroll
-        for (int c = 0; c < F::kSteps; ++c) {
-          const int chunk = 4 * c + quad;
-          kf[i][c] = v4u{0, 0, 0, 0};
-          if (page >= 0 && chunk * 16 < bytes) kf[i][c] = *reinterpret_cast<const v4u *>(from + chunk * 16);
-        }
-      }
-    };
-    const auto fetch_v = [&](int32_t s, int32_t pages) {
-#pragma unroll
-      for (int r = 0; r < F::kVPer; ++r) {
-        const int at = lane + r * kWave, chunk = at % F::kChunks, place = at / F::kChunks;
-        const int64_t page = __shfl(pages, place);
-        const char *from = cv + (page * a.vs[0] + a.table.slot(key_of(s) + place) * a.vs[1]) * F::kSize;
-        vf[r] = v4u{0, 0, 0, 0};
-        if (page >= 0 && chunk * 16 < bytes) vf[r] = *reinterpret_cast<const v4u *>(from + chunk * 16);
-      }
-    };
-
-    char *tile = lds + wave * F::kTile;
-    v4f o[DP / 16];
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) o[d] = v4f{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
-
-    int32_t step = s_begin + wave;
-    int32_t pages = pages_of(step), ahead = pages_of(step + kStepWaves);
-    if (step < s_end) {
-      fetch_k(step, pages);
-      fetch_v(step, pages);
-    }
-    for (; step < s_end; step += kStepWaves) {
-      v4f s[F::kTiles];
-#pragma unroll
-      for (int i = 0; i < F::kTiles; ++i) {
-        s[i] = v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < F::kSteps; ++c) s[i] = Mfma16<V>::mul(kf[i][c], qf[c], s[i]);
-      }
-      const uint32_t there = static_cast<uint32_t>(__ballot(pages >= 0));
-      const bool more = step + kStepWaves < s_end;
-      pages = ahead;
-      ahead = pages_of(step + 2 * kStepWaves);
-      if (more) fetch_k(step + kStepWaves, pages);
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int r = 0; r < F::kVPer; ++r) {
-        const int at = lane + r * kWave;
-        *reinterpret_cast<v4u *>(tile + F::at(at / F::kChunks, at % F::kChunks)) = vf[r];
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (more) fetch_v(step + kStepWaves, pages);
-
-      float x[F::kTiles * 4], top = -INFINITY;
-      const int32_t j0 = key_of(step) + 4 * quad;
-#pragma unroll
-      for (int i = 0; i < F::kTiles; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int place = 16 * i + k;
-          const bool seen = ((there >> (place + 4 * quad) & 1) != 0) & mine.sees(j0 + place);
-          x[4 * i + k] = seen ? s[i][k] * a.scale : -INFINITY;
-          top = fmaxf(top, x[4 * i + k]);
-        }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float grown = fmaxf(m, top);
-      const float base = grown == -INFINITY ? 0.0f : grown;
-      if (__any(grown > m)) {
-        const float shrink = exp2_fast(m - base);
-        l *= shrink;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) o[d] *= shrink;
-      }
-      m = grown;
-#pragma unroll
-      for (int k = 0; k < F::kTiles * 4; ++k) {
-        x[k] = exp2_fast(x[k] - base);
-        l += x[k];
-      }
-      if constexpr (F::kSize == 2) {
-        v4u p, low;  // rounded, and what that leaves: the output has its own rounding alone
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t pair = Mfma<V>::pack(x[2 * k], x[2 * k + 1]);
-          p[k] = pair;
-          low[k] = Mfma<V>::pack(x[2 * k] - V::widen(static_cast<uint16_t>(pair)),
-                                 x[2 * k + 1] - V::widen(static_cast<uint16_t>(pair >> 16)));
-        }
-        const int i = lane % 16;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-          v4s part[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int place = 16 * k + 4 * quad + i / 4, column = d * 16 + (i % 4) * 4;
-            part[k] = read_transposed(tile + F::at(place, column / 8) + (column % 8) * 2);
-          }
-          const auto lo = __builtin_bit_cast(v2u, part[0]), hi = __builtin_bit_cast(v2u, part[1]);
-          const v4u values{lo[0], lo[1], hi[0], hi[1]};
-          o[d] = Mfma16<V>::mul(values, p, o[d]);
-          o[d] = Mfma16<V>::mul(values, low, o[d]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int d = 0; d < DP / 16; ++d) {
-            const int place = 4 * quad + i, column = d * 16 + lane % 16;
-            const float v = *reinterpret_cast<const float *>(tile + F::at(place, column / 4) + (column % 4) * 4);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[i], o[d], 0, 0, 0);
-          }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-
-    // the waves' parts, joined: a row of DP sums, m and l a query and wave
-    __syncthreads();
-    float *own = reinterpret_cast<float *>(lds) + (wave * kStepRows + lane % 16) * (DP + 4);
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) *reinterpret_cast<v4f *>(own + 16 * d + 4 * quad) = o[d];
-    if (quad == 0) {
-      own[DP] = m;
-      own[DP + 1] = l;
-    }
-    if (threadIdx.x == 0) odd = 0;
-    __syncthreads();
-    const bool whole = s_begin == 0 && s_end == steps.count;
-    const int64_t unit = static_cast<int64_t>(head) * entries + mine_entry;
-    if (threadIdx.x == 0 && s_begin == 0)
-      spans[unit] = whole ? StepSpan{0, -1}
-                          : StepSpan{static_cast<int32_t>(g),
-                                     static_cast<int32_t>(share.owner(first_step + steps.count - 1))};
-    const float *all = reinterpret_cast<const float *>(lds);
-    const int32_t rows = min(kStepRows, a.tokens * a.group - row_tile * kStepRows);
-    for (int at = threadIdx.x; at < rows * DP; at += kThreads) {
-      const int i = at / DP, d = at % DP;
-      if (d >= a.dim) continue;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kStepWaves; ++w) top = fmaxf(top, all[(w * kStepRows + i) * (DP + 4) + DP]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, norm = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kStepWaves; ++w) {
-        const float *from = all + (w * kStepRows + i) * (DP + 4);
-        const float f = exp2_fast(from[DP] - base);
-        sum += from[d] * f;
-        norm += from[DP + 1] * f;
-      }
-      const int32_t r = row_tile * kStepRows + i;
-      const int64_t place = (b * a.tokens + r / a.group) * a.heads + head * a.group + r % a.group;
-      if (whole && whole_parts == nullptr) {
-        const float value = norm == 0.0f ? 0.0f : sum / norm;
-        if (!(fabsf(value) < INFINITY)) atomicOr(&odd, 1u << i);
-        out[place * a.dim + d] = V::narrow(value);
-      } else {
-        float *part = whole ? whole_parts + place * part_stride(a.dim)
-                            : parts + ((2 * g + (s_begin == 0 ? 1 : 0)) * kStepRows + i) * part_stride(a.dim);
-        part[d] = sum;
-        if (d == 0) {
-          part[a.dim] = top;
-          part[a.dim + 1] = norm;
-        }
-      }
-    }
-    __syncthreads();
-    for (uint32_t anew = odd; anew != 0; anew &= anew - 1) {
-      const int i = __builtin_ctz(anew);
-      if (i % kStepWaves != wave) continue;
-      const int32_t r = row_tile * kStepRows + i;
-      paged_row<V>(a, b, r / a.group, head * a.group + r % a.group,
-                   reinterpret_cast<float *>(lds) + wave * DP, out);
-    }
-    __syncthreads();
-  }
+__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedArgs a, StepGrid grid, TileParts to) {
+  __shared__ __attribute__((aligned(16))) char lds[StepShape<V, DP>::kLds];
+  __shared__ StretchLds own;
+  step_stretch<V, DP>(a, grid, blockIdx.x, to, lds, own);
 }
 
 template <class V, int DP>
 msx_status run(const PagedArgs &a, const StepGrid &grid, const TileParts &to, hipStream_t stream) {
-  paged_step<V, DP><<<grid.groups, kThreads, 0, stream>>>(a, grid, static_cast<typename V::Storage *>(to.out),
-                                                          to.spans, to.whole, to.parts);
+  paged_step<V, DP><<<grid.groups, kThreads, 0, stream>>>(a, grid, to);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
 }
