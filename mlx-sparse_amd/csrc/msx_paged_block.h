@@ -63,10 +63,11 @@ struct PageLoader {
   static constexpr int kKinds = kRows % 16 == 0 ? 1 : 2;  // the permutation repeats after sixteen rows
   static_assert(kPieces % kTileThreads == 0 && kRows * kKinds % 16 == 0, "a thread's pieces are of one or two kinds");
   uint32_t offset[kKinds];  // of the thread's pieces from its wave's first row
-  bool plain, grouped;      // uniform
+  int64_t page_step, slot_step;  // of both caches, in bytes
+  bool plain, grouped;           // uniform
 
-  __device__ __forceinline__ explicit PageLoader(const PagedArgs &a) {
-    const int64_t slot_step = a.ks[1] * T::kSize;
+  __device__ __forceinline__ explicit PageLoader(const PagedArgs &a)
+      : page_step(a.ks[0] * T::kSize), slot_step(a.ks[1] * T::kSize) {
     plain = kEven && a.dim == DP && slot_step >= 0 && slot_step * kTogether < (int64_t{1} << 31) &&
             a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1];
     grouped = a.table.size % kTogether == 0;
@@ -76,12 +77,19 @@ struct PageLoader {
       offset[kind] = static_cast<uint32_t>(row % kTogether) * static_cast<uint32_t>(slot_step) +
                      T::logical(row + kind * kRows, threadIdx.x % T::kChunks) * 16;
   }
+  // The thread, for what is worked out where it is needed: the addresses of ways that a tile
+  // seldom takes would otherwise be kept in registers.
+  __device__ static __forceinline__ int this_thread() {
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    return thread;
+  }
   __device__ static __forceinline__ void load(const char *from, char *to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from),
                                      (__attribute__((address_space(3))) void *)(to), 16, 0, 0);
   }
   // The kKeys keys from j on, whose pages the lanes hold, all there.
-  __device__ __forceinline__ void direct(const PagedArgs &a, const char *k, const char *v, int32_t pages,
+  __device__ __forceinline__ void direct(const PageTable &table, const char *k, const char *v, int32_t pages,
                                          int32_t j, char *k_tile, char *v_tile) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const auto places = [&](int r, auto &&from) {
@@ -94,16 +102,16 @@ struct PageLoader {
       for (int r = 0; r < kPer; ++r) {
         const int row = r * kRows + wave * kTogether;
         const int64_t page = __builtin_amdgcn_readlane(pages, row);
-        const int64_t at = (page * a.ks[0] + a.table.slot(j + row) * a.ks[1]) * T::kSize;
+        const int64_t at = page * page_step + table.slot(j + row) * slot_step;
         places(r, [&](const char *cache) { return cache + at + offset[r % kKinds]; });
       }
     } else {
+      const int thread = this_thread();
 #pragma unroll
       for (int r = 0; r < kPer; ++r) {
-        const int row = r * kRows + threadIdx.x / T::kChunks;
+        const int row = r * kRows + thread / T::kChunks;
         const int64_t page = __shfl(pages, row);
-        const int64_t at = (page * a.ks[0] + a.table.slot(j + row) * a.ks[1]) * T::kSize +
-                           T::logical(row, threadIdx.x % T::kChunks) * 16;
+        const int64_t at = page * page_step + table.slot(j + row) * slot_step + T::logical(row, thread % T::kChunks) * 16;
         places(r, [&](const char *cache) { return cache + at; });
       }
     }
@@ -111,9 +119,10 @@ struct PageLoader {
   // Of one cache, zeros for those that are not there.
   __device__ __forceinline__ void each(const PagedArgs &a, const char *cache, const int64_t *strides,
                                        int32_t pages, int32_t j, char *tile) const {
+    const int thread = this_thread();
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const int at = threadIdx.x + r * kTileThreads, row = at / T::kChunks, chunk = at % T::kChunks;
+      const int at = thread + r * kTileThreads, row = at / T::kChunks, chunk = at % T::kChunks;
       const int64_t page = __shfl(pages, row);
       if (chunk >= T::kUsed) continue;
       v4u piece = {0, 0, 0, 0};
@@ -125,58 +134,83 @@ struct PageLoader {
   }
 };
 
-// The probabilities of 32 keys as the second product takes them: rounded to the operands' type,
-// or for shared pages rounded and what that leaves, which costs nothing there
-// (64 sequences behind 8,192 tokens wait for loads) and gives the results their own rounding
-// alone, as the sequences' own keys do.
-template <class V, bool kTwice>
-struct Probabilities {
-  Column<V> high;
-  __device__ __forceinline__ explicit Probabilities(const float (&p)[16]) : high(p) {}
-  template <int kBlocks>
-  __device__ __forceinline__ void times(const TileLanes<V, kBlocks * 32> &lanes, uint32_t tile, int row0,
-                                        v16f (&acc)[kBlocks]) const {
-    mul_transposed<V>(lanes, tile, row0, high, acc);
-  }
-};
-template <class V>
-struct Probabilities<V, true> {
-  Column<V> high, low;
-  __device__ __forceinline__ explicit Probabilities(const float (&p)[16]) : high(p), low(left(p, high)) {}
-  template <int kBlocks>
-  __device__ __forceinline__ void times(const TileLanes<V, kBlocks * 32> &lanes, uint32_t tile, int row0,
-                                        v16f (&acc)[kBlocks]) const {
-    using Frag = typename Mfma<V>::Frag;
+// The values of 32 keys, from LDS as the second product takes them.
+template <class V, int DP>
+struct ValueColumns {
+  using Frag = typename Mfma<V>::Frag;
+  Frag a[DP / 32][2];
+  __device__ __forceinline__ void read(const TileLanes<V, DP> &lanes, uint32_t tile, int row0) {
 #pragma unroll
-    for (int dt = 0; dt < kBlocks; ++dt)
+    for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         v4s part[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) part[t] = read_transposed(lanes.column_at(tile, row0, 16 * k + 8 * t, dt));
         const auto lo = __builtin_bit_cast(v2u, part[0]), hi = __builtin_bit_cast(v2u, part[1]);
-        const auto a = __builtin_bit_cast(Frag, (v4u{lo[0], lo[1], hi[0], hi[1]}));
-        acc[dt] = Mfma<V>::mul(a, high.b[k], acc[dt]);
-        acc[dt] = Mfma<V>::mul(a, low.b[k], acc[dt]);
+        a[dt][k] = __builtin_bit_cast(Frag, (v4u{lo[0], lo[1], hi[0], hi[1]}));
       }
   }
-
- private:
-  __device__ static __forceinline__ Column<V> left(const float (&p)[16], const Column<V> &taken) {
+  // acc += V^T P, P rounded to the operands' type, or with `twice` that and what it leaves:
+  // shared pages wait for loads, so that this costs nothing there and gives the results
+  // their own rounding alone, as the sequences' own keys do.
+  template <bool twice>
+  __device__ __forceinline__ void times(const float (&p)[16], v16f (&acc)[DP / 32]) const {
+    const Column<V> high(p);
     float rest[16];
+    if constexpr (twice) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const v4u w = __builtin_bit_cast(v4u, taken.b[k]);
+      for (int k = 0; k < 2; ++k) {
+        const v4u w = __builtin_bit_cast(v4u, high.b[k]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t pair = w[j];
-        rest[8 * k + 2 * j] = p[8 * k + 2 * j] - V::widen(static_cast<uint16_t>(pair));
-        rest[8 * k + 2 * j + 1] = p[8 * k + 2 * j + 1] - V::widen(static_cast<uint16_t>(pair >> 16));
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t pair = w[j];
+          rest[8 * k + 2 * j] = p[8 * k + 2 * j] - V::widen(static_cast<uint16_t>(pair));
+          rest[8 * k + 2 * j + 1] = p[8 * k + 2 * j + 1] - V::widen(static_cast<uint16_t>(pair >> 16));
+        }
       }
     }
-    return Column<V>(rest);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) acc[dt] = Mfma<V>::mul(a[dt][k], high.b[k], acc[dt]);
+    if constexpr (twice) {
+      const Column<V> low(rest);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) acc[dt] = Mfma<V>::mul(a[dt][k], low.b[k], acc[dt]);
+    }
   }
 };
+template <int DP>
+struct ValueColumns<F32, DP> {
+  float a[16][DP / 32];
+  __device__ __forceinline__ void read(const TileLanes<F32, DP> &lanes, uint32_t tile, int row0) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+        a[r][dt] = read_lds<float>(lanes.column_at(tile, row0, 8 * (r / 4) + r % 4, dt));
+  }
+  template <bool>
+  __device__ __forceinline__ void times(const float (&p)[16], v16f (&acc)[DP / 32]) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[r][dt], p[r], acc[dt], 0, 0, 0);
+  }
+};
+
+// The launch's first argument, read anew: what a unit needs of it once would otherwise be kept in
+// scalar registers through the loop over its keys, and there are too few (280 spilled to
+// vector registers, which are as scarce, at heads of 128).
+__device__ __forceinline__ const PagedArgs &kernel_args() {
+  auto p = (const __attribute__((address_space(4))) PagedArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PagedArgs *)p;
+}
 
 // Row r of those that share kv head `head`: of sequence b0, or of the batch.
 template <bool kShared>
@@ -197,9 +231,9 @@ struct TileRow {
 
 // kShared: rows are those of the whole batch, keys those of the pages that it shares
 // (grid.from of them, listed in the table's first row), and all results are parts.
-// Workgroup `id` of grid.groups; `lds`: PagedShape's kLds bytes at a multiple of 1,024.
+// Workgroup `id` of grid.groups; `args`: the launch's first argument; `lds`: PagedShape's kLds bytes at a multiple of 1,024.
 template <class V, int DP, bool kShared>
-__device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid &grid, uint32_t id, const TileParts &to,
+__device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepGrid &grid, uint32_t id, const TileParts &to,
                                               char *lds, StretchLds &own) {
   using S = typename V::Storage;
   using F = PagedShape<V, DP>;
@@ -213,12 +247,12 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 
   // this workgroup's stretch of all tiles: numbered by kv head, then (sequence, unit)
-  const int64_t entries = kShared ? grid.tiles : a.batch * grid.tiles;
+  const int64_t entries = kShared ? grid.tiles : args.batch * grid.tiles;
   const int32_t shared_count = (grid.from + F::kKeys - 1) / F::kKeys;
   const auto cost_at = [&](int64_t e) -> int64_t {
     if (e >= entries) return 0;
     const int64_t b = quotient(e, grid.tiles);
-    return kStart + steps_of<F::kKeys, kTileRows>(a, b, static_cast<int32_t>(e - b * grid.tiles), 0).count;
+    return kStart + steps_of<F::kKeys, kTileRows>(args, b, static_cast<int32_t>(e - b * grid.tiles), 0).count;
   };
   int64_t total = 0, cost = 0, upto = 0;
   if constexpr (kShared) {
@@ -232,7 +266,7 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid
       running_sums<kTileWaves>(mine, own.sums, total);
     }
   }
-  const StepShare share(total * a.kv_heads, grid.groups);
+  const StepShare share(total * args.kv_heads, grid.groups);
   if (id >= share.groups) return;  // whole workgroups leave
   const int64_t g = xcd_order(id, static_cast<uint32_t>(share.groups));
   const int64_t begin = share.first(g), end = share.first(g + 1);
@@ -264,12 +298,13 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid
     x = kvh * total + uniform(own.found_first);
   }
 
-  const PageLoader<V, DP, F::kKeys> rows(a);
+  const PageLoader<V, DP, F::kKeys> rows(args);
   // a negative scale moves its sign to the queries, so that the largest product is the
   // largest score
-  const float scale = fabsf(a.scale);
+  const float scale = fabsf(args.scale);
 
   while (x < end) {
+    const PagedArgs &a = kernel_args();
     const int64_t b0 = kShared ? 0 : quotient(entry, grid.tiles);
     const int32_t block = kShared ? entry : entry - static_cast<int32_t>(b0) * grid.tiles;
     Steps steps;
@@ -320,17 +355,20 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid
     const char *k_base = reinterpret_cast<const char *>(static_cast<const S *>(a.k) + head * a.ks[2]);
     const char *v_base = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + head * a.vs[2]);
 
+    PageTable table = a.table;  // of this sequence
+    table.pages = static_cast<const char *>(table.pages) + b0 * table.stride * (table.wide ? 8 : 4);
+
     // the page of key `lane` of a tile, -1 where nobody sees it
     const auto pages_of = [&](int32_t s) {
       const int32_t j = steps.template key<F::kKeys>(s) + lane;
-      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? a.table.page(b0, j) : -1;
+      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? table.page(0, j) : -1;
     };
-    constexpr uint64_t kAll = F::kKeys == 64 ? ~uint64_t{0} : (uint64_t{1} << F::kKeys) - 1;
+    constexpr uint64_t kAll = ~uint64_t{0} >> (64 - F::kKeys);
     const auto fetch = [&](int32_t s, int32_t pages, int parity) {
       const int32_t j = steps.template key<F::kKeys>(s);
       char *k_to = lds + parity * F::kTile, *v_to = lds + (2 + parity) * F::kTile;
       if (rows.plain && __ballot(pages >= 0) == kAll) {
-        rows.direct(a, k_base, v_base, pages, j, k_to, v_to);
+        rows.direct(table, k_base, v_base, pages, j, k_to, v_to);
       } else {
         rows.each(a, k_base, a.ks, pages, j, k_to);
         rows.each(a, v_base, a.vs, pages, j, v_to);
@@ -344,15 +382,14 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid
       for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
     float m = -INFINITY, base = 0.0f, l = 0.0f;  // l: of this lane's keys only
 
-    const auto exponentials = [&](const v16f &from) {
-      float e[16], sum[2] = {0.0f, 0.0f};
+    const auto exponentials = [&](const v16f &from, float (&e)[16]) {
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         e[r] = exp2_fast(from[r] * scale - base);
         sum[r % 2] += e[r];
       }
       l += sum[0] + sum[1];
-      return Probabilities<V, kShared && T::kSize == 2>(e);
     };
     // masks the scores of the tile at j0 and moves the maximum.  It is moved only where
     // it has grown by more than 2^8: until then exponentials up to 2^8 stand
@@ -396,33 +433,42 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &a, const StepGrid
     const auto step = [&](int32_t s, int parity) __attribute__((always_inline)) {
       const int32_t j0 = steps.template key<F::kKeys>(s), j1 = j0 + F::kKeys - 1;
       const bool seen = j0 <= any_hi && (j1 >= any_lo || j0 < any_far);
-      // (the keys are read from LDS before the next tile is asked for: a read that
-      // follows would wait for it)
-      Frag kf[F::kSub][kSteps];
-      if (seen) {
-#pragma unroll
-        for (int i = 0; i < F::kSub; ++i)
-#pragma unroll
-          for (int st = 0; st < kSteps; ++st)
-            kf[i][st] = read_rows<V>(lanes, static_cast<uint32_t>(parity * F::kTile), 32 * i, st);
-      }
       const uint64_t there = __ballot(pages >= 0);
       pages = ahead;
       ahead = pages_of(s + 2);
-      if (s + 1 < s_end) fetch(s + 1, pages, parity ^ 1);  // into the other tiles, which all waves are past
-      if (seen) {
+      const bool more = s + 1 < s_end;
+      // (into the other tiles, which all waves are past; after this tile is read from LDS, since a
+      // read that followed would wait for the loads)
+      if (!seen) {
+        if (more) fetch(s + 1, pages, parity ^ 1);
+      } else {
         v16f y[F::kSub];
+        {
+          Frag kf[F::kSub][kSteps];
 #pragma unroll
-        for (int i = 0; i < F::kSub; ++i) {
+          for (int i = 0; i < F::kSub; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) y[i][r] = 0.0f;
+            for (int st = 0; st < kSteps; ++st)
+              kf[i][st] = read_rows<V>(lanes, static_cast<uint32_t>(parity * F::kTile), 32 * i, st);
 #pragma unroll
-          for (int st = 0; st < kSteps; ++st) y[i] = Mfma<V>::mul(kf[i][st], qf[st], y[i]);
+          for (int i = 0; i < F::kSub; ++i) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[i][r] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) y[i] = Mfma<V>::mul(kf[i][st], qf[st], y[i]);
+          }
         }
+        ValueColumns<V, DP> values;
+        values.read(lanes, static_cast<uint32_t>((2 + parity) * F::kTile), 0);
+        if (more) fetch(s + 1, pages, parity ^ 1);
         settle(j0, there, y);
 #pragma unroll
-        for (int i = 0; i < F::kSub; ++i)
-          exponentials(y[i]).times(lanes, static_cast<uint32_t>((2 + parity) * F::kTile), 32 * i, o);
+        for (int i = 0; i < F::kSub; ++i) {
+          float e[16];
+          exponentials(y[i], e);
+          if (i > 0) values.read(lanes, static_cast<uint32_t>((2 + parity) * F::kTile), 32 * i);
+          values.template times<kShared && T::kSize == 2>(e, o);
+        }
       }
       sync_tiles();
     };
