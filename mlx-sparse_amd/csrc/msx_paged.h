@@ -36,23 +36,31 @@ __device__ inline int64_t count_of(const void *counts, int32_t wide, int64_t b, 
 // The caches and the table of their pages, as the kernels take them.
 struct PageTable {
   const void *pages;
-  int64_t stride, n_pages;
+  int64_t stride;
+  int32_t n_pages;
   int32_t wide;  // numbers of 64 bits
   int32_t size;  // tokens a page
   int32_t capacity;
   FastDiv by_size;
 
-  // The page of entry e of row b, or -1 for one that is not there.
-  __device__ __forceinline__ int32_t entry(int64_t b, int32_t e) const {
-    const int64_t at = b * stride + e;
-    const int64_t page = wide ? static_cast<const int64_t *>(pages)[at]
-                              : static_cast<const int32_t *>(pages)[at];
-    return page >= 0 && page < n_pages ? static_cast<int32_t>(page) : -1;
+  // A page's number as it is loaded, to be looked at where it is wanted: looked at
+  // once it is asked for, each would be waited for.
+  struct Number {
+    int32_t low, high;
+  };
+  __device__ static __forceinline__ Number none() { return {-1, 0}; }
+  // of position j of row b, 0 <= j < capacity
+  __device__ __forceinline__ Number number(int64_t b, int32_t j) const {
+    const int64_t at = b * stride + static_cast<int32_t>(by_size(j));
+    if (!wide) return {static_cast<const int32_t *>(pages)[at], 0};
+    const int2 both = static_cast<const int2 *>(pages)[at];
+    return {both.x, both.y};
   }
-  // of position j of sequence b, 0 <= j < capacity
-  __device__ __forceinline__ int32_t page(int64_t b, int32_t j) const {
-    return entry(b, static_cast<int32_t>(by_size(j)));
+  // The page, or -1 for one that is not there.
+  __device__ __forceinline__ int32_t checked(Number n) const {
+    return ((static_cast<uint32_t>(n.low) < static_cast<uint32_t>(n_pages)) & (n.high == 0)) ? n.low : -1;
   }
+  __device__ __forceinline__ int32_t page(int64_t b, int32_t j) const { return checked(number(b, j)); }
   __device__ __forceinline__ int32_t slot(int32_t j) const {
     return j - static_cast<int32_t>(by_size(j)) * size;
   }
@@ -62,7 +70,7 @@ inline PageTable table_of(const msx_paged_cache &c) {
   PageTable t;
   t.pages = c.pages;
   t.stride = c.pages_stride;
-  t.n_pages = c.n_pages;
+  t.n_pages = static_cast<int32_t>(c.n_pages);
   t.wide = c.pages_itype == MSX_I64;
   t.size = static_cast<int32_t>(c.page_size);
   t.capacity = static_cast<int32_t>(c.width * c.page_size);

@@ -63,18 +63,18 @@ struct PageLoader {
   static constexpr int kKinds = kRows % 16 == 0 ? 1 : 2;  // the permutation repeats after sixteen rows
   static_assert(kPieces % kTileThreads == 0 && kRows * kKinds % 16 == 0, "a thread's pieces are of one or two kinds");
   uint32_t offset[kKinds];  // of the thread's pieces from its wave's first row
-  int64_t page_step, slot_step;  // of both caches, in bytes
-  bool plain, grouped;           // uniform
+  uint32_t page_step, slot_step;  // of both caches, in bytes
+  bool plain, grouped;            // uniform
 
   __device__ __forceinline__ explicit PageLoader(const PagedArgs &a)
-      : page_step(a.ks[0] * T::kSize), slot_step(a.ks[1] * T::kSize) {
-    plain = kEven && a.dim == DP && slot_step >= 0 && slot_step * kTogether < (int64_t{1} << 31) &&
-            a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1];
+      : page_step(static_cast<uint32_t>(a.ks[0] * T::kSize)), slot_step(static_cast<uint32_t>(a.ks[1] * T::kSize)) {
+    plain = kEven && a.dim == DP && a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1] && a.ks[0] * T::kSize == page_step &&
+            a.ks[1] * T::kSize == slot_step && a.ks[1] * T::kSize * kTogether < (int64_t{1} << 31);
     grouped = a.table.size % kTogether == 0;
     const int row = threadIdx.x / T::kChunks;
 #pragma unroll
     for (int kind = 0; kind < kKinds; ++kind)
-      offset[kind] = static_cast<uint32_t>(row % kTogether) * static_cast<uint32_t>(slot_step) +
+      offset[kind] = static_cast<uint32_t>(row % kTogether) * slot_step +
                      T::logical(row + kind * kRows, threadIdx.x % T::kChunks) * 16;
   }
   // The thread, for what is worked out where it is needed: the addresses of ways that a tile
@@ -91,28 +91,31 @@ struct PageLoader {
   // The kKeys keys from j on, whose pages the lanes hold, all there.
   __device__ __forceinline__ void direct(const PageTable &table, const char *k, const char *v, int32_t pages,
                                          int32_t j, char *k_tile, char *v_tile) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const auto places = [&](int r, auto &&from) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    // where key `lane` lies: worked out by all lanes at once, a scalar a row group would take
+    // ten times the instructions
+    const uint64_t place = static_cast<uint64_t>(static_cast<uint32_t>(pages)) * page_step +
+                           static_cast<uint64_t>(static_cast<uint32_t>(table.slot(j + lane))) * slot_step;
+    const auto low = static_cast<int32_t>(place), high = static_cast<int32_t>(place >> 32);
+    const auto both = [&](int r, uint64_t at, uint32_t more) {
       char *const to = k_tile + (r * kTileThreads + wave * kWave) * 16;
-      load(from(k), to);
-      load(from(v), to + (v_tile - k_tile));
+      load(k + at + more, to);
+      load(v + at + more, to + (v_tile - k_tile));
     };
     if (grouped) {
 #pragma unroll
       for (int r = 0; r < kPer; ++r) {
         const int row = r * kRows + wave * kTogether;
-        const int64_t page = __builtin_amdgcn_readlane(pages, row);
-        const int64_t at = page * page_step + table.slot(j + row) * slot_step;
-        places(r, [&](const char *cache) { return cache + at + offset[r % kKinds]; });
+        both(r, static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(high, row))) << 32 |
+                    static_cast<uint32_t>(__builtin_amdgcn_readlane(low, row)), offset[r % kKinds]);
       }
     } else {
       const int thread = this_thread();
 #pragma unroll
       for (int r = 0; r < kPer; ++r) {
         const int row = r * kRows + thread / T::kChunks;
-        const int64_t page = __shfl(pages, row);
-        const int64_t at = page * page_step + table.slot(j + row) * slot_step + T::logical(row, thread % T::kChunks) * 16;
-        places(r, [&](const char *cache) { return cache + at; });
+        both(r, static_cast<uint64_t>(static_cast<uint32_t>(__shfl(high, row))) << 32 |
+                    static_cast<uint32_t>(__shfl(low, row)), T::logical(row, thread % T::kChunks) * 16);
       }
     }
   }
@@ -358,10 +361,10 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     PageTable table = a.table;  // of this sequence
     table.pages = static_cast<const char *>(table.pages) + b0 * table.stride * (table.wide ? 8 : 4);
 
-    // the page of key `lane` of a tile, -1 where nobody sees it
-    const auto pages_of = [&](int32_t s) {
+    // the page of key `lane` of a tile, none where nobody sees it
+    const auto numbers_of = [&](int32_t s) {
       const int32_t j = steps.template key<F::kKeys>(s) + lane;
-      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? table.page(0, j) : -1;
+      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? table.number(0, j) : PageTable::none();
     };
     constexpr uint64_t kAll = ~uint64_t{0} >> (64 - F::kKeys);
     const auto fetch = [&](int32_t s, int32_t pages, int parity) {
@@ -427,15 +430,16 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
       }
     };
 
-    int32_t pages = pages_of(s_begin), ahead = pages_of(s_begin + 1);
+    int32_t pages = table.checked(numbers_of(s_begin));
+    PageTable::Number ahead = numbers_of(s_begin + 1);
     fetch(s_begin, pages, 0);
     sync_tiles();
     const auto step = [&](int32_t s, int parity) __attribute__((always_inline)) {
       const int32_t j0 = steps.template key<F::kKeys>(s), j1 = j0 + F::kKeys - 1;
       const bool seen = j0 <= any_hi && (j1 >= any_lo || j0 < any_far);
       const uint64_t there = __ballot(pages >= 0);
-      pages = ahead;
-      ahead = pages_of(s + 2);
+      pages = table.checked(ahead);
+      ahead = numbers_of(s + 2);
       const bool more = s + 1 < s_end;
       // (into the other tiles, which all waves are past; after this tile is read from LDS, since a
       // read that followed would wait for the loads)

@@ -115,10 +115,10 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     const char *ck = reinterpret_cast<const char *>(static_cast<const S *>(a.k) + head * a.ks[2]);
     const char *cv = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + head * a.vs[2]);
 
-    // the page of key `lane` of a step, -1 where nobody sees it
-    const auto pages_of = [&](int32_t s) {
+    // the page of key `lane` of a step, none where nobody sees it
+    const auto numbers_of = [&](int32_t s) {
       const int32_t j = key_of(s) + lane;
-      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? a.table.page(b, j) : -1;
+      return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? a.table.number(b, j) : PageTable::none();
     };
     v4u kf[F::kTiles][F::kSteps], vf[F::kVPer];
     const auto fetch_k = [&](int32_t s, int32_t pages) {
@@ -153,7 +153,8 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
 
     int32_t step = s_begin + wave;
-    int32_t pages = pages_of(step), ahead = pages_of(step + kStepWaves);
+    int32_t pages = a.table.checked(numbers_of(step));
+    PageTable::Number ahead = numbers_of(step + kStepWaves);
     if (step < s_end) {
       fetch_k(step, pages);
       fetch_v(step, pages);
@@ -168,8 +169,8 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       }
       const uint32_t there = static_cast<uint32_t>(__ballot(pages >= 0));
       const bool more = step + kStepWaves < s_end;
-      pages = ahead;
-      ahead = pages_of(step + 2 * kStepWaves);
+      pages = a.table.checked(ahead);
+      ahead = numbers_of(step + 2 * kStepWaves);
       if (more) fetch_k(step + kStepWaves, pages);
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
