@@ -206,6 +206,27 @@ struct ValueColumns<F32, DP> {
   }
 };
 
+// The most and least of a workgroup's threads.
+__device__ __forceinline__ void extremes(int32_t &most, int32_t &least, StretchLds &own) {
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) {
+    most = max(most, __shfl_xor(most, d));
+    least = min(least, __shfl_xor(least, d));
+  }
+  if (threadIdx.x % kWave == 0) {
+    own.most[threadIdx.x / kWave] = most;
+    own.least[threadIdx.x / kWave] = least;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kTileWaves; ++w) {
+    most = max(most, own.most[w]);
+    least = min(least, own.least[w]);
+  }
+  most = __builtin_amdgcn_readfirstlane(most);
+  least = __builtin_amdgcn_readfirstlane(least);
+}
+
 // The launch's first argument, read anew: what a unit needs of it once would otherwise be kept in
 // scalar registers through the loop over its keys, and there are too few (280 spilled to
 // vector registers, which are as scarce, at heads of 128).
@@ -252,41 +273,56 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
   // this workgroup's stretch of all tiles: numbered by kv head, then (sequence, unit)
   const int64_t entries = kShared ? grid.tiles : args.batch * grid.tiles;
   const int32_t shared_count = (grid.from + F::kKeys - 1) / F::kKeys;
-  const auto cost_at = [&](int64_t e) -> int64_t {
-    if (e >= entries) return 0;
+  const auto count_at = [&](int64_t e) -> int32_t {
     const int64_t b = quotient(e, grid.tiles);
-    return kStart + steps_of<F::kKeys, kTileRows>(args, b, static_cast<int32_t>(e - b * grid.tiles), 0).count;
+    return steps_of<F::kKeys, kTileRows>(args, b, static_cast<int32_t>(e - b * grid.tiles), 0).count;
   };
-  int64_t total = 0, cost = 0, upto = 0;
-  if constexpr (kShared) {
-    total = entries * (shared_count + kStart);
-  } else {
-    cost = cost_at(threadIdx.x);
-    upto = running_sums<kTileWaves>(cost, own.sums, total);
-    if (entries > kTileThreads) {
-      int64_t mine = cost;
-      for (int64_t e = threadIdx.x + kTileThreads; e < entries; e += kTileThreads) mine += cost_at(e);
-      running_sums<kTileWaves>(mine, own.sums, total);
+  const auto cost_at = [&](int64_t e) -> int64_t { return e < entries ? kStart + count_at(e) : 0; };
+  int64_t total = entries * (shared_count + kStart), cost = 0, upto = 0;
+  int32_t most = shared_count, least = shared_count;
+  if constexpr (!kShared) {
+    int64_t mine = 0;
+    most = 0;
+    least = 0x7fffffff;
+    for (int64_t e = threadIdx.x; e < entries; e += kTileThreads) {
+      const int32_t count = count_at(e);
+      if (e < kTileThreads) cost = kStart + count;
+      mine += kStart + count;
+      most = max(most, count);
+      least = min(least, count);
     }
+    upto = running_sums<kTileWaves>(mine, own.sums, total);
+    extremes(most, least, own);
   }
-  const StepShare share(total * args.kv_heads, grid.groups);
+  // Units that are nearly as long and fill the workgroups are cut alike: their workgroups then
+  // read the same keys at the same time, through their XCD's L2 (2,048 queries on 18,432 keys: of
+  // 1.54 GB that missed it 0.14 did, 393 to 367 us).
+  const int64_t units = entries * args.kv_heads;
+  const int64_t parts = units <= grid.groups ? quotient(grid.groups, units) : 1;
+  const bool even = least >= parts && total * 16 >= entries * (most + kStart) * 15 &&
+                    (units <= grid.groups ? units * parts * 10 >= int64_t{grid.groups} * 9
+                                          : units - quotient(units, grid.groups) * grid.groups == 0);
+  const int64_t unit_cost = quotient(most + kStart + parts - 1, parts) * parts;  // where even
+  if (even) total = entries * unit_cost;
+  const StepShare share = even ? StepShare(total * args.kv_heads, min(units * parts, int64_t{grid.groups}))
+                               : StepShare(total * args.kv_heads, grid.groups);
   if (id >= share.groups) return;  // whole workgroups leave
   const int64_t g = xcd_order(id, static_cast<uint32_t>(share.groups));
   const int64_t begin = share.first(g), end = share.first(g + 1);
   int32_t kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin, total)));
   int32_t entry;
   int64_t x;  // where the next (kv head, entry) begins
-  if constexpr (kShared) {
-    entry = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - kvh * total, shared_count + kStart)));
-    x = kvh * total + static_cast<int64_t>(entry) * (shared_count + kStart);
+  if (kShared || even) {
+    const int64_t each = even ? unit_cost : shared_count + kStart;
+    entry = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - kvh * total, each)));
+    x = kvh * total + entry * each;
   } else {
     const int64_t at = begin - kvh * total;
     int64_t before = 0;
     for (int64_t e0 = 0;; e0 += kTileThreads) {  // (all that is to be done is some entry's)
       int64_t here = total;
       if (entries > kTileThreads) {
-        if (e0 > 0) cost = cost_at(e0 + threadIdx.x);
-        else cost = cost_at(threadIdx.x);
+        cost = cost_at(e0 + threadIdx.x);
         upto = running_sums<kTileWaves>(cost, own.sums, here);
       }
       if (before + upto - cost <= at && at < before + upto) {
@@ -318,12 +354,19 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     } else {
       steps = uniform(steps_of<F::kKeys, kTileRows>(a, b0, block, 0));
     }
-    const int64_t first_step = x + kStart;
-    x = first_step + steps.count;
-    const int32_t s_begin = __builtin_amdgcn_readfirstlane(
-        static_cast<int32_t>(min(max(begin - first_step, int64_t{0}), static_cast<int64_t>(steps.count))));
-    const int32_t s_end = __builtin_amdgcn_readfirstlane(
-        static_cast<int32_t>(max(min(end - first_step, static_cast<int64_t>(steps.count)), int64_t{0})));
+    const int64_t first = x;
+    int64_t from, upto_step;
+    if (even) {
+      x += unit_cost;
+      from = quotient(max(begin - first, int64_t{0}) * steps.count, unit_cost);
+      upto_step = quotient(min(end - first, unit_cost) * steps.count, unit_cost);
+    } else {
+      x += kStart + steps.count;
+      from = max(begin - first - kStart, int64_t{0});
+      upto_step = min(end - first - kStart, static_cast<int64_t>(steps.count));
+    }
+    const int32_t s_begin = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(min(from, static_cast<int64_t>(steps.count))));
+    const int32_t s_end = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(max(upto_step, int64_t{0})));
     const int32_t head = kvh, this_entry = entry;
     if (++entry == entries) {
       entry = 0;
@@ -495,7 +538,7 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     if (threadIdx.x == 0 && s_begin == 0)
       to.spans[unit] = all_of_it ? StepSpan{0, -1}
                               : StepSpan{static_cast<int32_t>(g),
-                                         static_cast<int32_t>(share.owner(first_step + steps.count - 1))};
+                                         static_cast<int32_t>(share.owner(x - 1))};
     const bool held = to_row.held;
     const int64_t place = (to_row.b * a.tokens + to_row.t) * a.heads + to_row.h;
     if (kShared || !all_of_it) {

@@ -95,8 +95,9 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t by) {
 // Equal stretches of `work`: workgroup g takes [first(g), first(g + 1)).
 struct StepShare {
   int64_t groups, each, more;  // the first `more` take one more
-  __device__ __forceinline__ StepShare(int64_t work, int32_t launched) {
-    groups = max(min(work / kLeast, static_cast<int64_t>(launched)), int64_t{1});
+  __device__ __forceinline__ StepShare(int64_t work, int32_t launched)
+      : StepShare(work, max(min(work / kLeast, static_cast<int64_t>(launched)), int64_t{1})) {}
+  __device__ __forceinline__ StepShare(int64_t work, int64_t n) : groups(n) {
     each = quotient(work, groups);
     more = work - each * groups;
   }
@@ -128,6 +129,7 @@ struct TileParts {
 // What a workgroup has in LDS beside its tiles.
 struct StretchLds {
   int64_t sums[4], found_first;
+  int32_t most[4], least[4];
   int32_t found;
   uint32_t odd;  // rows whose results are not finite
 };
