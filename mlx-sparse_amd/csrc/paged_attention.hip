@@ -83,6 +83,30 @@ enum class Route { kRows, kStep, kTiles, kShared };
 // the keys for each sixteen of them.
 constexpr int64_t kFewRows = 32;
 
+// Whether the shared pages are worth kernels of their own.  Reading them for each sequence takes
+// their bytes at 5 TB/s; once for all of them, the products of 128 queries a tile at what
+// paged_tiles reaches at such sizes, or the bytes once, some 8 us for more workgroups' starts
+// and a second set of parts to join, and the sequences' own keys half the chip.  Measured,
+// without and with, in us, one token a sequence:
+//   32 heads of 128 on 8, bfloat16   4 sequences of 1,024 shared keys 15.5 18.0, 4,096 23.4 18.3;
+//                                    64 of 64 24.2 31.6, 256 28.6 33.9, 1,024 51.6 38.2, 16,384 589 51
+//   8 heads of 64 on 2, float16      64 of 256 15.1 17.8, 4,096 31.8 22.0
+//   16 heads of 128, float32         2 of 16,384 96 166, 8 283 167; 64 of 256 67.9 70.9, 1,024 164 67
+bool shares(const msx_paged_attention_desc &d, int64_t rows) {
+  const msx_paged_cache &c = d.cache;
+  // (with a window few sequences see much of what they share)
+  if (d.shared_pages == 0 || d.batch < 2 || d.window < c.width * c.page_size ||
+      d.batch * rows > kWindowIntMax - kTileRows)
+    return false;
+  const double keys = static_cast<double>(d.shared_pages * c.page_size * c.kv_heads);
+  const double size = static_cast<double>(value_bytes(static_cast<msx_vtype>(d.vtype)));
+  const double once = keys * c.dim * 2 * size / 5e6, rate = d.vtype == MSX_F32 ? 80e6 : 500e6;
+  const double products = static_cast<double>((d.batch * rows + kTileRows - 1) / kTileRows) * kTileRows * keys *
+                          c.dim * 4 / rate;
+  const double own = 0.01 * static_cast<double>(d.batch * c.kv_heads * ((rows + kStepRows - 1) / kStepRows));
+  return std::max(once, products) + 8 + own < once * static_cast<double>(d.batch);
+}
+
 Route route_of(const msx_paged_attention_desc &d) {
   if (!takes_tiles(d)) return Route::kRows;
   const int64_t rows = d.tokens * (d.heads / d.cache.kv_heads);
@@ -90,10 +114,7 @@ Route route_of(const msx_paged_attention_desc &d) {
                     !(std::fabs(static_cast<float>(d.scale)) >= std::numeric_limits<float>::min());
   if (wide) return Route::kStep;
   if (rows > kFewRows) return Route::kTiles;
-  if (d.shared_pages > 0 && d.batch > 1 && d.window >= d.cache.width * d.cache.page_size &&
-      d.batch * rows <= kWindowIntMax - kTileRows)
-    return Route::kShared;
-  return Route::kStep;
+  return shares(d, rows) ? Route::kShared : Route::kStep;
 }
 
 // What a call's kernels are given, and where in its scratch their parts lie.

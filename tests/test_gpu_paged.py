@@ -141,6 +141,57 @@ def test_all_pages_shared(gpu):
     paged_case(gpu, "cuda", torch.float32, [63, 40, 50, 60], shared=4, width=4, dim=64)
 
 
+def behind(size, pages, batch=64, low=-9, high=90):
+    """Starts of a batch behind a prefix that is long enough to be read once for all."""
+    gen = torch.Generator().manual_seed(size + pages)
+    starts = (pages * size + torch.randint(low, high, (batch,), generator=gen)).tolist()
+    starts[0] = starts[17] = -1
+    return starts
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size,pages,dim,tokens", [(16, 140, 128, 1), (24, 130, 96, 2), (5, 841, 64, 1),
+                                                   (64, 65, 32, 4), (16, 200, 80, 1)])
+def test_read_once(gpu, dtype, size, pages, dim, tokens):
+    paged_case(gpu, "cuda", dtype, behind(size, pages), shared=pages, size=size, dim=dim, tokens=tokens,
+               heads=4, kv_heads=2)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(5, 5), (24, 1)])
+def test_read_once_heads(gpu, heads, kv_heads):
+    paged_case(gpu, "cuda", torch.bfloat16, behind(16, 260), shared=260, dim=64, heads=heads,
+               kv_heads=kv_heads, layout="packed")
+
+
+def test_read_once_with_what_is_not_there(gpu):
+    starts = behind(16, 140)
+    paged_case(gpu, "cuda", torch.float16, starts, shared=140, dim=128, heads=4, kv_heads=2, sinks=3,
+               tokens=3, lengths=[3, 0, 1, 2] * 16, holes=[(b, 7) for b in range(64)] + [(5, 141)])
+    # no sequence goes on behind the prefix, some end within it
+    paged_case(gpu, "cuda", torch.float16, behind(16, 140, low=-900, high=-1), shared=140, dim=128,
+               heads=4, kv_heads=2)
+
+
+def test_read_once_values(gpu):
+    """Infinite values that all see; and of two drafts' own one that the first does not."""
+    def change(q, ck, cv, table):
+        cv[table[1, 3], 2, :, 5] = float("inf")
+        j = starts[1] + 1
+        ck[table[1, j // 16], j % 16], cv[table[1, j // 16], j % 16] = float("nan"), float("-inf")
+
+    starts = behind(16, 140, low=0)
+    out, (value, tol) = paged_case(gpu, "cuda", torch.bfloat16, starts, shared=140, dim=128, heads=4,
+                                   kv_heads=2, tokens=2, change=change)
+    live = [b for b, s in enumerate(starts) if s >= 0]
+    rest = [d for d in range(128) if d != 5]
+    assert (out[live, 0, :, 5] == math.inf).all() and out[1, 1].isnan().all()
+    live.remove(1)
+    got, want = (t[live][..., rest] for t in (out, value))
+    check(got, (want, tol[live][..., rest]), "values beside")
+    check(out[1, :1][..., rest], (value[1, :1][..., rest], tol[1, :1][..., rest].nan_to_num(posinf=0)),
+          "the first draft")
+
+
 # -- what is not there ---------------------------------------------------------
 @pytest.mark.parametrize("tokens", [1, 3, 80])
 @pytest.mark.parametrize("shared", [0, 2])
@@ -247,8 +298,9 @@ def test_prompt_then_steps(gpu, dtype, window, sinks, chunk, size):
 
 def serving(gpu, dtype=torch.bfloat16, batch=5, shared=2, size=16, heads=8, kv_heads=2, dim=64):
     gen = torch.Generator().manual_seed(6)
-    starts = [shared * size + n for n in (3, 40, 0, 200, 17)][:batch]
-    width = 20
+    starts = [shared * size + n for n in (3, 40, 0, 200, 17)] * (batch // 5 + 1)
+    starts = starts[:batch]
+    width = shared + 18
     total, table = table_for(gen, [width * size] * batch, size, width, shared=shared)
     state = {n: normal(gen, dtype, "cuda", batch, 1, h, dim)
              for n, h in (("q", heads), ("k", kv_heads), ("v", kv_heads))}
@@ -263,10 +315,10 @@ def one_step(gpu, s, shared):
     return gpu.paged_attention(q, s["ck"], s["cv"], s["pages"], starts=s["starts"], shared_pages=shared)
 
 
-@pytest.mark.parametrize("shared", [0, 2])
+@pytest.mark.parametrize("shared", [0, 2, 140])
 def test_captured_and_replayed(gpu, shared):
     """Two graphs of the same steps, replayed in turn with eager work between."""
-    s = serving(gpu)
+    s = serving(gpu, batch=64, shared=140) if shared > 2 else serving(gpu)
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
@@ -288,17 +340,18 @@ def test_captured_and_replayed(gpu, shared):
         torch.cuda.synchronize()
 
 
-def test_on_two_streams_at_once(gpu):
-    states = [serving(gpu) for _ in range(2)]
+@pytest.mark.parametrize("shared", [2, 140])
+def test_on_two_streams_at_once(gpu, shared):
+    states = [serving(gpu, batch=64 if shared > 2 else 5, shared=shared) for _ in range(2)]
     states[1]["q"].mul_(-2)
-    want = [one_step(gpu, s, 2) for s in states]
+    want = [one_step(gpu, s, shared) for s in states]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in states]
     got = [[], []]
     for _ in range(5):
         for stream, s, g in zip(streams, states, got):
             with torch.cuda.stream(stream):
-                g.append(one_step(gpu, s, 2))
+                g.append(one_step(gpu, s, shared))
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(x, w) for x in g)
