@@ -24,13 +24,20 @@
 
 namespace msx {
 
-// Workgroup g of grid.groups.  `lds`: StepShape's kLds bytes at a sixteen-byte address.
-template <class V, int DP>
+template <class V, int DP, int kWaves>
+constexpr int step_lds() {
+  return std::max(kWaves * StepShape<V, DP>::kTile, kWaves * kStepRows * (DP + 4) * 4);
+}
+
+// Workgroup g of grid.groups.  `lds`: step_lds bytes at a sixteen-byte address.
+// Where grid.whole (a workgroup of eight waves always is) it has all keys of one tile.
+template <class V, int DP, int kWaves = kStepWaves>
 __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid &grid, int64_t g, const TileParts &to,
                                              char *lds, StretchLds &own) {
   using S = typename V::Storage;
   using F = StepShape<V, DP>;
-  constexpr int kThreads = kStepWaves * kWave;
+  constexpr int kThreads = kWaves * kWave;
+  constexpr bool kAlwaysWhole = kWaves != kStepWaves;
   auto *const out = static_cast<S *>(to.out);
 
   const int lane = threadIdx.x % kWave, quad = lane / 16;
@@ -44,35 +51,45 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     const int64_t b = grid.tiles == 1 ? e : e / grid.tiles;
     return kStart + steps_of<F::kKeys, kStepRows>(a, b, static_cast<int32_t>(e - b * grid.tiles), grid.from).count;
   };
-  int64_t total = 0, cost = cost_at(threadIdx.x), upto = running_sums<kStepWaves>(cost, own.sums, total);
-  if (entries > kThreads) {
-    int64_t mine = cost;
-    for (int64_t e = threadIdx.x + kThreads; e < entries; e += kThreads) mine += cost_at(e);
-    running_sums<kStepWaves>(mine, own.sums, total);
-  }
-  const StepShare share(total * a.kv_heads, grid.groups);
-  if (g >= share.groups) return;  // whole workgroups leave
-  const int64_t begin = share.first(g), end = share.first(g + 1);
-  int64_t before = 0;
-  for (int64_t e0 = 0;; e0 += kThreads) {  // (all that is to be done is some entry's)
-    int64_t here = total;
+  int32_t entry, kvh = -1;
+  int64_t begin = 0, end = 0, x = 0;  // x: where the next (entry, kv head) begins
+  StepShare share(0, int64_t{1});
+  const bool whole_grid = kAlwaysWhole || grid.whole;
+  if (whole_grid) {
+    entry = static_cast<int32_t>(quotient(g, a.kv_heads));
+    kvh = static_cast<int32_t>(g - entry * static_cast<int64_t>(a.kv_heads));
+  } else {
+    int64_t total = 0, cost = cost_at(threadIdx.x), upto = running_sums<kWaves>(cost, own.sums, total);
     if (entries > kThreads) {
-      if (e0 > 0) cost = cost_at(e0 + threadIdx.x);
-      upto = running_sums<kStepWaves>(cost, own.sums, here);
+      int64_t mine = cost;
+      for (int64_t e = threadIdx.x + kThreads; e < entries; e += kThreads) mine += cost_at(e);
+      running_sums<kWaves>(mine, own.sums, total);
     }
-    const int64_t low = (before + upto - cost) * a.kv_heads, high = (before + upto) * a.kv_heads;
-    if (low <= begin && begin < high) {
-      own.found = static_cast<int32_t>(e0 + threadIdx.x);
-      own.found_first = low;
+    share = StepShare(total * a.kv_heads, grid.groups);
+    if (g >= share.groups) return;  // whole workgroups leave
+    begin = share.first(g);
+    end = share.first(g + 1);
+    int64_t before = 0;
+    for (int64_t e0 = 0;; e0 += kThreads) {  // (all that is to be done is some entry's)
+      int64_t here = total;
+      if (entries > kThreads) {
+        if (e0 > 0) cost = cost_at(e0 + threadIdx.x);
+        upto = running_sums<kWaves>(cost, own.sums, here);
+      }
+      const int64_t low = (before + upto - cost) * a.kv_heads, high = (before + upto) * a.kv_heads;
+      if (low <= begin && begin < high) {
+        own.found = static_cast<int32_t>(e0 + threadIdx.x);
+        own.found_first = low;
+      }
+      before += here;
+      if (begin < before * a.kv_heads || e0 + kThreads >= entries) break;
     }
-    before += here;
-    if (begin < before * a.kv_heads || e0 + kThreads >= entries) break;
+    __syncthreads();
+    entry = __builtin_amdgcn_readfirstlane(own.found);
+    x = uniform(own.found_first);
   }
-  __syncthreads();
-  int32_t entry = __builtin_amdgcn_readfirstlane(own.found), kvh = -1;
-  int64_t x = uniform(own.found_first);  // where the next (entry, kv head) begins
 
-  while (x < end) {
+  for (;;) {
     const int64_t b = grid.tiles == 1 ? entry : entry / grid.tiles;
     const int32_t row_tile = entry - static_cast<int32_t>(b) * grid.tiles;
     const Steps steps = uniform(steps_of<F::kKeys, kStepRows>(a, b, row_tile, grid.from));
@@ -82,6 +99,7 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     }
     const int64_t first_step = x + kStart;
     x = first_step + steps.count;
+    if (whole_grid) end = x;
     const int32_t s_begin = __builtin_amdgcn_readfirstlane(
         static_cast<int32_t>(min(max(begin - first_step, int64_t{0}), static_cast<int64_t>(steps.count))));
     const int32_t s_end = __builtin_amdgcn_readfirstlane(
@@ -91,7 +109,10 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       kvh = 0;
       ++entry;
     }
-    if (s_begin >= s_end) continue;  // what this workgroup has of it is no step
+    if (s_begin >= s_end) {  // what this workgroup has of it is no step
+      if (x >= end) break;
+      continue;
+    }
     const auto key_of = [&](int32_t s) { return steps.template key<F::kKeys>(s); };
 
     // this lane's query, and what it sees
@@ -154,12 +175,12 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
 
     int32_t step = s_begin + wave;
     int32_t pages = a.table.checked(numbers_of(step));
-    PageTable::Number ahead = numbers_of(step + kStepWaves);
+    PageTable::Number ahead = numbers_of(step + kWaves);
     if (step < s_end) {
       fetch_k(step, pages);
       fetch_v(step, pages);
     }
-    for (; step < s_end; step += kStepWaves) {
+    for (; step < s_end; step += kWaves) {
       v4f s[F::kTiles];
 #pragma unroll
       for (int i = 0; i < F::kTiles; ++i) {
@@ -168,10 +189,10 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
         for (int c = 0; c < F::kSteps; ++c) s[i] = Mfma16<V>::mul(kf[i][c], qf[c], s[i]);
       }
       const uint32_t there = static_cast<uint32_t>(__ballot(pages >= 0));
-      const bool more = step + kStepWaves < s_end;
+      const bool more = step + kWaves < s_end;
       pages = a.table.checked(ahead);
-      ahead = numbers_of(step + 2 * kStepWaves);
-      if (more) fetch_k(step + kStepWaves, pages);
+      ahead = numbers_of(step + 2 * kWaves);
+      if (more) fetch_k(step + kWaves, pages);
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int r = 0; r < F::kVPer; ++r) {
@@ -180,7 +201,7 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      if (more) fetch_v(step + kStepWaves, pages);
+      if (more) fetch_v(step + kWaves, pages);
 
       float x[F::kTiles * 4], top = -INFINITY;
       const int32_t j0 = key_of(step) + 4 * quad;
@@ -260,7 +281,7 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     __syncthreads();
     const bool whole = s_begin == 0 && s_end == steps.count;
     const int64_t unit = static_cast<int64_t>(head) * entries + mine_entry;
-    if (threadIdx.x == 0 && s_begin == 0)
+    if (threadIdx.x == 0 && s_begin == 0 && !whole_grid)
       to.spans[unit] = whole ? StepSpan{0, -1}
                           : StepSpan{static_cast<int32_t>(g),
                                      static_cast<int32_t>(share.owner(first_step + steps.count - 1))};
@@ -271,11 +292,11 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       if (d >= a.dim) continue;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kStepWaves; ++w) top = fmaxf(top, all[(w * kStepRows + i) * (DP + 4) + DP]);
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, all[(w * kStepRows + i) * (DP + 4) + DP]);
       const float base = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f, norm = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kStepWaves; ++w) {
+      for (int w = 0; w < kWaves; ++w) {
         const float *from = all + (w * kStepRows + i) * (DP + 4);
         const float f = exp2_fast(from[DP] - base);
         sum += from[d] * f;
@@ -300,11 +321,12 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     __syncthreads();
     for (uint32_t anew = own.odd; anew != 0; anew &= anew - 1) {
       const int i = __builtin_ctz(anew);
-      if (i % kStepWaves != wave) continue;
+      if (i % kWaves != wave) continue;
       const int32_t r = row_tile * kStepRows + i;
       paged_row<V>(a, b, r / a.group, head * a.group + r % a.group,
                    reinterpret_cast<float *>(lds) + wave * DP, out);
     }
+    if (x >= end) break;
     __syncthreads();
   }
 }

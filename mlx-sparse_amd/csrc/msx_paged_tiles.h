@@ -11,6 +11,8 @@ struct StepGrid {
   int32_t tiles;   // of queries: of a sequence and kv head
   int32_t groups;  // workgroups launched, as many as run at once
   int32_t from;    // the first key
+  int32_t whole;   // a workgroup a tile of queries and kv head, all of its keys
+  int32_t waves;   // of a workgroup: eight where whole and few, else four
 };
 
 // The steps of `kKeys` keys that a tile of queries takes: those over the sinks, then
@@ -128,7 +130,7 @@ struct TileParts {
 
 // What a workgroup has in LDS beside its tiles.
 struct StretchLds {
-  int64_t sums[4], found_first;
+  int64_t sums[8], found_first;
   int32_t most[4], least[4];
   int32_t found;
   uint32_t odd;  // rows whose results are not finite

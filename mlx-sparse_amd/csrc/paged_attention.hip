@@ -137,6 +137,7 @@ struct Plan {
     const auto parts_of = [&](const StepGrid &g, int64_t entries, int32_t tile_rows) {
       TileParts to{};
       to.out = out;
+      if (g.whole) return to;
       to.spans = reinterpret_cast<StepSpan *>(take(sizeof(StepSpan), entries * a.kv_heads));
       to.parts = reinterpret_cast<float *>(take(part, 2 * static_cast<int64_t>(g.groups) * tile_rows));
       if (route == Route::kShared) to.whole = reinterpret_cast<float *>(take(part, all));
@@ -146,6 +147,8 @@ struct Plan {
     if (route == Route::kStep || route == Route::kShared) {
       step.tiles = static_cast<int32_t>((rows + kStepRows - 1) / kStepRows);
       step.groups = a.dim > 128 || route == Route::kShared ? 256 : 512;
+      step.waves = kStepWaves;
+      if (route == Route::kStep) whole(d, a);
       step.from = route == Route::kShared ? static_cast<int32_t>(d.shared_pages * d.cache.page_size) : 0;
       step_to = parts_of(step, a.batch * step.tiles, kStepRows);
     }
@@ -156,6 +159,25 @@ struct Plan {
       tiles.from = step.from;
       tiles_to = parts_of(tiles, route == Route::kShared ? tiles.tiles : a.batch * tiles.tiles, kTileRows);
     }
+  }
+  // Few keys a sequence: a workgroup takes all of a tile's, of eight waves where the chip has
+  // room, and nothing is to be joined, which takes 5 us and more.  What it costs is a round more
+  // for every 32 keys a wave (16 in float32), of 1.7 us for rows of 128 bytes, 2.9 of 256, 4 of 512.
+  // Measured, cut and whole, in us, one token of sequences of as many keys:
+  //   8 heads of 64 on 2, float16      1 of 512 12.5 8.0, 1,024 12.6 11.5, 2,048 12.5 18.2; 300 of 512 33.1 20.5
+  //   32 heads of 128 on 8, bfloat16   1 of 512 14.1 11.5, 1,024 14.2 17.4; 64 of 512 33.4 27.3
+  //   16 heads of 128, float32         8 of 256 20.6 15.3, 512 27.0 23.9; 64 of 256 57.9 53.9
+  void whole(const msx_paged_attention_desc &d, const PagedArgs &a) {
+    const int64_t units = a.batch * step.tiles * a.kv_heads;
+    const int64_t held = std::min<int64_t>(a.table.capacity, a.window + a.sinks + a.tokens);
+    const int64_t row = a.dim * static_cast<int64_t>(value_bytes(static_cast<msx_vtype>(d.vtype)));
+    const bool few = units <= 256 && a.dim <= 128;
+    const int32_t waves = few ? 8 : kStepWaves;
+    const int64_t round = waves * (d.vtype == MSX_F32 ? 16 : 32), rounds = (held + round - 1) / round;
+    if (units > max_blocks(8 * kWave) || rounds > (!few || row <= 128 ? 4 : row <= 256 ? 3 : 2)) return;
+    step.whole = 1;
+    step.waves = waves;
+    step.groups = static_cast<int32_t>(units);
   }
   PartSource source(const StepGrid &g, const TileParts &to, int32_t rows, bool batched) const {
     return {to.spans, to.whole, to.parts, rows, g.tiles, batched};
@@ -196,7 +218,7 @@ extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, 
       return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
     });
   }
-  if (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
+  if (p.bytes > 0 && (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0))
     return fail(MSX_EINVAL, "paged_attention scratch is too small or not aligned.");
   if (a.batch * std::max(p.step.tiles, p.tiles.tiles) > kWindowIntMax)
     return fail(MSX_EINVAL, "paged_attention has more rows than a grid holds.");
@@ -205,7 +227,10 @@ extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, 
   const PartSource by_tiles = p.source(p.tiles, p.tiles_to, kTileRows, p.route == Route::kShared);
   msx_status st;
   switch (p.route) {
-  case Route::kStep: st = launch_paged_step(vt, a, p.step, p.step_to, s); break;
+  case Route::kStep:
+    st = launch_paged_step(vt, a, p.step, p.step_to, s);
+    if (p.step.whole) return st;
+    break;
   case Route::kTiles: st = launch_paged_tiles(vt, a, p.tiles, p.tiles_to, s); break;
   default: st = launch_paged_shared(vt, a, p.tiles, p.tiles_to, p.step, p.step_to, s); break;
   }

@@ -8,18 +8,24 @@
 namespace msx {
 namespace {
 
-constexpr int kThreads = kStepWaves * kWave;
-
-template <class V, int DP>
-__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void paged_step(PagedArgs a, StepGrid grid, TileParts to) {
-  __shared__ __attribute__((aligned(16))) char lds[StepShape<V, DP>::kLds];
+template <class V, int DP, int kWaves>
+__global__ __launch_bounds__(kWaves * kWave, DP > 128 || kWaves > 4 ? 1 : 2) void paged_step(PagedArgs a, StepGrid grid,
+                                                                                            TileParts to) {
+  __shared__ __attribute__((aligned(16))) char lds[step_lds<V, DP, kWaves>()];
   __shared__ StretchLds own;
-  step_stretch<V, DP>(a, grid, blockIdx.x, to, lds, own);
+  step_stretch<V, DP, kWaves>(a, grid, blockIdx.x, to, lds, own);
 }
 
 template <class V, int DP>
 msx_status run(const PagedArgs &a, const StepGrid &grid, const TileParts &to, hipStream_t stream) {
-  paged_step<V, DP><<<grid.groups, kThreads, 0, stream>>>(a, grid, to);
+  if constexpr (DP <= 128) {
+    if (grid.waves == 8) {
+      paged_step<V, DP, 8><<<grid.groups, 8 * kWave, 0, stream>>>(a, grid, to);
+      const hipError_t e = hipGetLastError();
+      return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
+    }
+  }
+  paged_step<V, DP, kStepWaves><<<grid.groups, kStepWaves * kWave, 0, stream>>>(a, grid, to);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, "paged_attention");
 }

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kTileThreads, (PagedShape<V, DP>::kBlocks)) void pa
   constexpr int kStepDim = DP <= 64 ? 64 : 128;
   static_assert(kTileThreads == kStepWaves * kWave, "one launch");
   __shared__ __attribute__((aligned(1024))) char
-      lds[std::max(PagedShape<V, DP>::kLds, StepShape<V, kStepDim>::kLds)];
+      lds[std::max(PagedShape<V, DP>::kLds, step_lds<V, kStepDim, kStepWaves>())];
   __shared__ StretchLds own;
   if (blockIdx.x < static_cast<uint32_t>(tiles.groups))
     tiles_stretch<V, DP, true>(a, tiles, blockIdx.x, tiles_to, lds, own);
