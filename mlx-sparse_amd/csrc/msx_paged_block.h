@@ -29,7 +29,7 @@ constexpr int kTileThreads = kTileWaves * kWave;
 template <class V, int DP>
 struct PagedShape {
   using T = TileShape<V, DP>;
-  static constexpr int kSub = T::kSize == 2 ? 2 : 1;  // 32-key parts of a tile
+  static constexpr int kSub = T::kSize == 2 && DP <= 128 ? 2 : 1;  // 32-key parts of a tile
   static constexpr int kKeys = 32 * kSub;
   static constexpr int kTile = kKeys * T::kPitch;
   static constexpr int kLds = 4 * kTile;  // K and V, twice
@@ -59,23 +59,29 @@ struct PageLoader {
   static constexpr int kPer = kPieces / kTileThreads;
   static constexpr int kRows = kTileThreads / T::kChunks;     // between a thread's pieces
   static constexpr int kTogether = kWave / T::kChunks;    // rows of a wave's load
-  static constexpr bool kEven = T::kUsed == T::kChunks;
   static constexpr int kKinds = kRows % 16 == 0 ? 1 : 2;  // the permutation repeats after sixteen rows
   static_assert(kPieces % kTileThreads == 0 && kRows * kKinds % 16 == 0, "a thread's pieces are of one or two kinds");
   uint32_t offset[kKinds];  // of the thread's pieces from its wave's first row
   uint32_t page_step, slot_step;  // of both caches, in bytes
+  int32_t dim;
   bool plain, grouped;            // uniform
 
   __device__ __forceinline__ explicit PageLoader(const PagedArgs &a)
-      : page_step(static_cast<uint32_t>(a.ks[0] * T::kSize)), slot_step(static_cast<uint32_t>(a.ks[1] * T::kSize)) {
-    plain = kEven && a.dim == DP && a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1] && a.ks[0] * T::kSize == page_step &&
+      : page_step(static_cast<uint32_t>(a.ks[0] * T::kSize)), slot_step(static_cast<uint32_t>(a.ks[1] * T::kSize)), dim(a.dim) {
+    plain = a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1] && a.ks[0] * T::kSize == page_step &&
             a.ks[1] * T::kSize == slot_step && a.ks[1] * T::kSize * kTogether < (int64_t{1} << 31);
     grouped = a.table.size % kTogether == 0;
     const int row = threadIdx.x / T::kChunks;
 #pragma unroll
     for (int kind = 0; kind < kKinds; ++kind)
       offset[kind] = static_cast<uint32_t>(row % kTogether) * slot_step +
-                     T::logical(row + kind * kRows, threadIdx.x % T::kChunks) * 16;
+                     chunk_at(row + kind * kRows, threadIdx.x % T::kChunks, a.dim) * 16;
+  }
+  // The chunk that goes to a place of a row.  Beyond the head's values it is the head's first:
+  // there queries are zero and results are not kept.
+  __device__ static __forceinline__ int chunk_at(int row, int place, int dim) {
+    const int chunk = T::logical(row, place);
+    return chunk * 16 < dim * T::kSize ? chunk : 0;
   }
   // The thread, for what is worked out where it is needed: the addresses of ways that a tile
   // seldom takes would otherwise be kept in registers.
@@ -115,7 +121,7 @@ struct PageLoader {
       for (int r = 0; r < kPer; ++r) {
         const int row = r * kRows + thread / T::kChunks;
         both(r, static_cast<uint64_t>(static_cast<uint32_t>(__shfl(high, row))) << 32 |
-                    static_cast<uint32_t>(__shfl(low, row)), T::logical(row, thread % T::kChunks) * 16);
+                    static_cast<uint32_t>(__shfl(low, row)), chunk_at(row, thread % T::kChunks, dim) * 16);
       }
     }
   }
@@ -255,7 +261,7 @@ struct TileRow {
 
 // kShared: rows are those of the whole batch, keys those of the pages that it shares
 // (grid.from of them, listed in the table's first row), and all results are parts.
-// Workgroup `id` of grid.groups; `args`: the launch's first argument; `lds`: PagedShape's kLds bytes at a multiple of 1,024.
+// Where grid.whole a workgroup has all keys of one unit.  Workgroup `id` of grid.groups; `args`: the launch's first argument; `lds`: PagedShape's kLds bytes at a multiple of 1,024.
 template <class V, int DP, bool kShared>
 __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepGrid &grid, uint32_t id, const TileParts &to,
                                               char *lds, StretchLds &own) {
@@ -278,63 +284,73 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     return steps_of<F::kKeys, kTileRows>(args, b, static_cast<int32_t>(e - b * grid.tiles), 0).count;
   };
   const auto cost_at = [&](int64_t e) -> int64_t { return e < entries ? kStart + count_at(e) : 0; };
-  int64_t total = entries * (shared_count + kStart), cost = 0, upto = 0;
-  int32_t most = shared_count, least = shared_count;
-  if constexpr (!kShared) {
-    int64_t mine = 0;
-    most = 0;
-    least = 0x7fffffff;
-    for (int64_t e = threadIdx.x; e < entries; e += kTileThreads) {
-      const int32_t count = count_at(e);
-      if (e < kTileThreads) cost = kStart + count;
-      mine += kStart + count;
-      most = max(most, count);
-      least = min(least, count);
-    }
-    upto = running_sums<kTileWaves>(mine, own.sums, total);
-    extremes(most, least, own);
-  }
-  // Units that are nearly as long and fill the workgroups are cut alike: their workgroups then
-  // read the same keys at the same time, through their XCD's L2 (2,048 queries on 18,432 keys: of
-  // 1.54 GB that missed it 0.14 did, 393 to 367 us).
-  const int64_t units = entries * args.kv_heads;
-  const int64_t parts = units <= grid.groups ? quotient(grid.groups, units) : 1;
-  const bool even = least >= parts && total * 16 >= entries * (most + kStart) * 15 &&
-                    (units <= grid.groups ? units * parts * 10 >= int64_t{grid.groups} * 9
-                                          : units - quotient(units, grid.groups) * grid.groups == 0);
-  const int64_t unit_cost = quotient(most + kStart + parts - 1, parts) * parts;  // where even
-  if (even) total = entries * unit_cost;
-  const StepShare share = even ? StepShare(total * args.kv_heads, min(units * parts, int64_t{grid.groups}))
-                               : StepShare(total * args.kv_heads, grid.groups);
-  if (id >= share.groups) return;  // whole workgroups leave
-  const int64_t g = xcd_order(id, static_cast<uint32_t>(share.groups));
-  const int64_t begin = share.first(g), end = share.first(g + 1);
-  int32_t kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin, total)));
-  int32_t entry;
-  int64_t x;  // where the next (kv head, entry) begins
-  if (kShared || even) {
-    const int64_t each = even ? unit_cost : shared_count + kStart;
-    entry = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - kvh * total, each)));
-    x = kvh * total + entry * each;
+  bool even = false;
+  int64_t unit_cost = 1, g = 0, begin = 0, end = 0, x = 0;  // x: where the next (kv head, entry) begins
+  int32_t kvh, entry;
+  StepShare share(0, int64_t{1});
+  if (!kShared && grid.whole) {
+    g = xcd_order(id, static_cast<uint32_t>(grid.groups));
+    kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(g, entries)));
+    // (a prompt's last queries see most: they begin first)
+    entry = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(entries - 1 - (g - kvh * entries)));
   } else {
-    const int64_t at = begin - kvh * total;
-    int64_t before = 0;
-    for (int64_t e0 = 0;; e0 += kTileThreads) {  // (all that is to be done is some entry's)
-      int64_t here = total;
-      if (entries > kTileThreads) {
-        cost = cost_at(e0 + threadIdx.x);
-        upto = running_sums<kTileWaves>(cost, own.sums, here);
+    int64_t total = entries * (shared_count + kStart), cost = 0, upto = 0;
+    int32_t most = shared_count, least = shared_count;
+    if constexpr (!kShared) {
+      int64_t mine = 0;
+      most = 0;
+      least = 0x7fffffff;
+      for (int64_t e = threadIdx.x; e < entries; e += kTileThreads) {
+        const int32_t count = count_at(e);
+        if (e < kTileThreads) cost = kStart + count;
+        mine += kStart + count;
+        most = max(most, count);
+        least = min(least, count);
       }
-      if (before + upto - cost <= at && at < before + upto) {
-        own.found = static_cast<int32_t>(e0 + threadIdx.x);
-        own.found_first = before + upto - cost;
-      }
-      before += here;
-      if (at < before || e0 + kTileThreads >= entries) break;
+      upto = running_sums<kTileWaves>(mine, own.sums, total);
+      extremes(most, least, own);
     }
-    __syncthreads();
-    entry = __builtin_amdgcn_readfirstlane(own.found);
-    x = kvh * total + uniform(own.found_first);
+    // Units that are nearly as long and fill the workgroups are cut alike: their workgroups then
+    // read the same keys at the same time, through their XCD's L2 (2,048 queries on 18,432 keys: of
+    // 1.54 GB that missed it 0.14 did, 393 to 367 us).
+    const int64_t units = entries * args.kv_heads;
+    const int64_t parts = units <= grid.groups ? quotient(grid.groups, units) : 1;
+    even = least >= parts && total * 16 >= entries * (most + kStart) * 15 &&
+                      (units <= grid.groups ? units * parts * 10 >= int64_t{grid.groups} * 9
+                                            : units - quotient(units, grid.groups) * grid.groups == 0);
+    unit_cost = quotient(most + kStart + parts - 1, parts) * parts;  // where even
+    if (even) total = entries * unit_cost;
+    share = even ? StepShare(total * args.kv_heads, min(units * parts, int64_t{grid.groups}))
+                 : StepShare(total * args.kv_heads, grid.groups);
+    if (id >= share.groups) return;  // whole workgroups leave
+    g = xcd_order(id, static_cast<uint32_t>(share.groups));
+    begin = share.first(g);
+    end = share.first(g + 1);
+    kvh = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin, total)));
+    if (kShared || even) {
+      const int64_t each = even ? unit_cost : shared_count + kStart;
+      entry = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(quotient(begin - kvh * total, each)));
+      x = kvh * total + entry * each;
+    } else {
+      const int64_t at = begin - kvh * total;
+      int64_t before = 0;
+      for (int64_t e0 = 0;; e0 += kTileThreads) {  // (all that is to be done is some entry's)
+        int64_t here = total;
+        if (entries > kTileThreads) {
+          cost = cost_at(e0 + threadIdx.x);
+          upto = running_sums<kTileWaves>(cost, own.sums, here);
+        }
+        if (before + upto - cost <= at && at < before + upto) {
+          own.found = static_cast<int32_t>(e0 + threadIdx.x);
+          own.found_first = before + upto - cost;
+        }
+        before += here;
+        if (at < before || e0 + kTileThreads >= entries) break;
+      }
+      __syncthreads();
+      entry = __builtin_amdgcn_readfirstlane(own.found);
+      x = kvh * total + uniform(own.found_first);
+    }
   }
 
   const PageLoader<V, DP, F::kKeys> rows(args);
@@ -342,7 +358,7 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
   // largest score
   const float scale = fabsf(args.scale);
 
-  while (x < end) {
+  for (bool more = (!kShared && grid.whole) || x < end; more;) {
     const PagedArgs &a = kernel_args();
     const int64_t b0 = kShared ? 0 : quotient(entry, grid.tiles);
     const int32_t block = kShared ? entry : entry - static_cast<int32_t>(b0) * grid.tiles;
@@ -362,11 +378,13 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
       upto_step = quotient(min(end - first, unit_cost) * steps.count, unit_cost);
     } else {
       x += kStart + steps.count;
+      if (!kShared && grid.whole) end = x;
       from = max(begin - first - kStart, int64_t{0});
       upto_step = min(end - first - kStart, static_cast<int64_t>(steps.count));
     }
     const int32_t s_begin = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(min(from, static_cast<int64_t>(steps.count))));
     const int32_t s_end = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(max(upto_step, int64_t{0})));
+    more = x < end;
     const int32_t head = kvh, this_entry = entry;
     if (++entry == entries) {
       entry = 0;
@@ -483,11 +501,11 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
       const uint64_t there = __ballot(pages >= 0);
       pages = table.checked(ahead);
       ahead = numbers_of(s + 2);
-      const bool more = s + 1 < s_end;
+      const bool next = s + 1 < s_end;
       // (into the other tiles, which all waves are past; after this tile is read from LDS, since a
       // read that followed would wait for the loads)
       if (!seen) {
-        if (more) fetch(s + 1, pages, parity ^ 1);
+        if (next) fetch(s + 1, pages, parity ^ 1);
       } else {
         v16f y[F::kSub];
         {
@@ -507,7 +525,7 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
         }
         ValueColumns<V, DP> values;
         values.read(lanes, static_cast<uint32_t>((2 + parity) * F::kTile), 0);
-        if (more) fetch(s + 1, pages, parity ^ 1);
+        if (next) fetch(s + 1, pages, parity ^ 1);
         settle(j0, there, y);
 #pragma unroll
         for (int i = 0; i < F::kSub; ++i) {
@@ -535,7 +553,7 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     }
     const bool all_of_it = s_begin == 0 && s_end == steps.count;
     const int64_t unit = static_cast<int64_t>(head) * entries + this_entry;
-    if (threadIdx.x == 0 && s_begin == 0)
+    if (threadIdx.x == 0 && s_begin == 0 && (kShared || !grid.whole))
       to.spans[unit] = all_of_it ? StepSpan{0, -1}
                               : StepSpan{static_cast<int32_t>(g),
                                          static_cast<int32_t>(share.owner(x - 1))};

@@ -43,8 +43,9 @@ struct StepShape {
   static constexpr int kSize = sizeof(typename V::Storage);
   static constexpr int kTiles = kSize == 2 ? 2 : 1;  // 16-key tiles a step
   static constexpr int kKeys = 16 * kTiles;
-  static constexpr int kChunks = DP * kSize / 16;     // of a row
-  static constexpr int kSteps = kChunks / 4;          // four lanes a row
+  static constexpr int kUsed = DP * kSize / 16;       // chunks of a row
+  static constexpr int kChunks = kUsed <= 4 ? 4 : kUsed <= 8 ? 8 : kUsed <= 16 ? 16 : kUsed <= 32 ? 32 : 64;  // and its pitch
+  static constexpr int kSteps = kUsed / 4;            // four lanes a row
   static constexpr int kVPer = kKeys * kChunks / kWave;
   static constexpr int kPitch = kChunks * 16;
   static constexpr int kTile = kKeys * kPitch;

@@ -80,8 +80,13 @@ msx_status by_vtype(int vt, Fn &&fn) {
 enum class Route { kRows, kStep, kTiles, kShared };
 
 // Rows that share a kv head: up to so many a sequence go through paged_step, a read of
-// the keys for each sixteen of them.
+// the keys for each sixteen of them; more in 16 bits through paged_tiles, where the second read
+// would be long.  Measured, by tiles and by steps, in us, heads of 128:
+//   bfloat16   5 tokens of 16 heads on 4: 32 of 4,000 keys 27.7 32.9; 8 of 32 on 8: 1 of 30,000 37.9 55.1,
+//              17 of 3 on 3: 8 of 2,000 21.7 17.7
+//   float32    5 of 16 on 4: 32 of 4,000 61.6 48.1; 8 of 32 on 8: 1 of 30,000 155 92
 constexpr int64_t kFewRows = 32;
+constexpr int64_t kLongRead = int64_t{48} << 20;  // bytes that the table has room for
 
 // Whether the shared pages are worth kernels of their own.  Reading them for each sequence takes
 // their bytes at 5 TB/s; once for all of them, the products of 128 queries a tile at what
@@ -107,13 +112,22 @@ bool shares(const msx_paged_attention_desc &d, int64_t rows) {
   return std::max(once, products) + 8 + own < once * static_cast<double>(d.batch);
 }
 
+// The most keys that a query of this call may see.
+int64_t held_keys(const msx_paged_attention_desc &d) {
+  const int64_t wide = int64_t{1} << 40;  // no sequence is as long
+  return std::min(d.cache.width * d.cache.page_size,
+                  std::min(d.window, wide) + std::min(d.sinks, wide) + d.tokens);
+}
+
 Route route_of(const msx_paged_attention_desc &d) {
   if (!takes_tiles(d)) return Route::kRows;
   const int64_t rows = d.tokens * (d.heads / d.cache.kv_heads);
-  const bool wide = d.cache.dim > 128 ||  // (a masked score is minus infinity times the scale)
+  const bool wide = (d.cache.dim > 128 && d.vtype == MSX_F32) ||  // (a masked score is minus infinity times the scale)
                     !(std::fabs(static_cast<float>(d.scale)) >= std::numeric_limits<float>::min());
   if (wide) return Route::kStep;
   if (rows > kFewRows) return Route::kTiles;
+  const int64_t held = held_keys(d), read = d.batch * d.cache.kv_heads * held * d.cache.dim * 4;
+  if (rows > kStepRows && d.vtype != MSX_F32 && held > 512 && read >= kLongRead) return Route::kTiles;
   return shares(d, rows) ? Route::kShared : Route::kStep;
 }
 
@@ -157,6 +171,7 @@ struct Plan {
       tiles.tiles = static_cast<int32_t>((together + kTileRows - 1) / kTileRows);
       tiles.groups = route == Route::kShared || a.dim * value_bytes(static_cast<msx_vtype>(d.vtype)) > 256 ? 256 : 512;
       tiles.from = step.from;
+      if (route == Route::kTiles) whole_tiles(d, a);
       tiles_to = parts_of(tiles, route == Route::kShared ? tiles.tiles : a.batch * tiles.tiles, kTileRows);
     }
   }
@@ -169,15 +184,26 @@ struct Plan {
   //   16 heads of 128, float32         8 of 256 20.6 15.3, 512 27.0 23.9; 64 of 256 57.9 53.9
   void whole(const msx_paged_attention_desc &d, const PagedArgs &a) {
     const int64_t units = a.batch * step.tiles * a.kv_heads;
-    const int64_t held = std::min<int64_t>(a.table.capacity, a.window + a.sinks + a.tokens);
     const int64_t row = a.dim * static_cast<int64_t>(value_bytes(static_cast<msx_vtype>(d.vtype)));
     const bool few = units <= 256 && a.dim <= 128;
     const int32_t waves = few ? 8 : kStepWaves;
-    const int64_t round = waves * (d.vtype == MSX_F32 ? 16 : 32), rounds = (held + round - 1) / round;
+    const int64_t round = waves * (d.vtype == MSX_F32 ? 16 : 32), rounds = (held_keys(d) + round - 1) / round;
     if (units > max_blocks(8 * kWave) || rounds > (!few || row <= 128 ? 4 : row <= 256 ? 3 : 2)) return;
     step.whole = 1;
     step.waves = waves;
     step.groups = static_cast<int32_t>(units);
+  }
+  // The same of tiles of 128 queries.  Measured, cut and whole, in us, 16 heads on 4:
+  //   bfloat16, heads of 64    300 tokens 24.0 13.3, 512 19.9 16.7, 64 on 1,000 20.1 26.3; 8 x 1,000 67 57
+  //             heads of 128   512 tokens 25.6 22.9, 64 on 1,000 23.8 34.4; 8 x 1,000 102 81
+  //             heads of 256   128 tokens 30.0 21.5, 512 35.6 43.5; 4 x 512 66.0 46.5
+  //   float32, heads of 64     128 tokens 25.8 17.4, 300 29.5 31.5; 8 x 1,000 196 220
+  void whole_tiles(const msx_paged_attention_desc &d, const PagedArgs &a) {
+    const int64_t units = a.batch * tiles.tiles * a.kv_heads;
+    const int64_t few = d.vtype == MSX_F32 ? 128 : a.dim <= 128 ? 512 : 256;
+    if (units > max_blocks(256) || held_keys(d) > (units >= 512 ? 2 * few : few)) return;
+    tiles.whole = 1;
+    tiles.groups = static_cast<int32_t>(units);
   }
   PartSource source(const StepGrid &g, const TileParts &to, int32_t rows, bool batched) const {
     return {to.spans, to.whole, to.parts, rows, g.tiles, batched};
@@ -231,7 +257,10 @@ extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, 
     st = launch_paged_step(vt, a, p.step, p.step_to, s);
     if (p.step.whole) return st;
     break;
-  case Route::kTiles: st = launch_paged_tiles(vt, a, p.tiles, p.tiles_to, s); break;
+  case Route::kTiles:
+    st = launch_paged_tiles(vt, a, p.tiles, p.tiles_to, s);
+    if (p.tiles.whole) return st;
+    break;
   default: st = launch_paged_shared(vt, a, p.tiles, p.tiles_to, p.step, p.step_to, s); break;
   }
   if (st != MSX_OK) return st;

@@ -32,7 +32,9 @@ msx_status run(const PagedArgs &a, const StepGrid &grid, const TileParts &to, hi
 
 template <class V>
 msx_status by_dim(const PagedArgs &a, const StepGrid &grid, const TileParts &to, hipStream_t stream) {
+  if (a.dim <= 32) return run<V, 32>(a, grid, to, stream);
   if (a.dim <= 64) return run<V, 64>(a, grid, to, stream);
+  if (a.dim <= 96) return run<V, 96>(a, grid, to, stream);
   if (a.dim <= 128) return run<V, 128>(a, grid, to, stream);
   return run<V, 256>(a, grid, to, stream);
 }

@@ -26,15 +26,14 @@ __global__ __launch_bounds__(kTileThreads, (PagedShape<V, DP>::kBlocks)) void pa
 template <class V, int DP>
 __global__ __launch_bounds__(kTileThreads, (PagedShape<V, DP>::kBlocks)) void paged_shared(
     PagedArgs a, StepGrid tiles, TileParts tiles_to, StepGrid step, TileParts step_to) {
-  constexpr int kStepDim = DP <= 64 ? 64 : 128;
   static_assert(kTileThreads == kStepWaves * kWave, "one launch");
   __shared__ __attribute__((aligned(1024))) char
-      lds[std::max(PagedShape<V, DP>::kLds, step_lds<V, kStepDim, kStepWaves>())];
+      lds[std::max(PagedShape<V, DP>::kLds, step_lds<V, DP, kStepWaves>())];
   __shared__ StretchLds own;
   if (blockIdx.x < static_cast<uint32_t>(tiles.groups))
     tiles_stretch<V, DP, true>(a, tiles, blockIdx.x, tiles_to, lds, own);
   else
-    step_stretch<V, kStepDim>(a, step, blockIdx.x - tiles.groups, step_to, lds, own);
+    step_stretch<V, DP>(a, step, blockIdx.x - tiles.groups, step_to, lds, own);
 }
 
 template <class V, int DP>
@@ -54,7 +53,9 @@ msx_status by_dim(const PagedArgs &a, const StepGrid &tiles, const TileParts &ti
   if (a.dim <= 32) return run<V, 32>(a, tiles, tiles_to, step, step_to, stream);
   if (a.dim <= 64) return run<V, 64>(a, tiles, tiles_to, step, step_to, stream);
   if (a.dim <= 96) return run<V, 96>(a, tiles, tiles_to, step, step_to, stream);
-  return run<V, 128>(a, tiles, tiles_to, step, step_to, stream);
+  if (a.dim <= 128) return run<V, 128>(a, tiles, tiles_to, step, step_to, stream);
+  if constexpr (sizeof(typename V::Storage) == 2) return run<V, 256>(a, tiles, tiles_to, step, step_to, stream);
+  return fail(MSX_EINVAL, "paged_attention tiles take float32 heads of 128 at most.");
 }
 
 msx_status by_type(msx_vtype vt, const PagedArgs &a, const StepGrid &tiles, const TileParts &tiles_to,
