@@ -37,6 +37,10 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
   using S = typename V::Storage;
   using F = StepShape<V, DP>;
   constexpr int kThreads = kWaves * kWave;
+  // steps of a row's sixty-four bytes that every head of this kernel has
+  constexpr int kSure = (DP <= 128 ? DP - 32 : 128) * F::kSize / 64;
+  constexpr uint32_t kAll = static_cast<uint32_t>((uint64_t{1} << F::kKeys) - 1);
+  const bool alike = a.ks[0] == a.vs[0] && a.ks[1] == a.vs[1];
   constexpr bool kAlwaysWhole = kWaves != kStepWaves;
   auto *const out = static_cast<S *>(to.out);
 
@@ -133,6 +137,10 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
         if (live && c * 16 < bytes) qf[s] = *reinterpret_cast<const v4u *>(q + c * 16);
       }
     }
+    // all of the tile's queries that are there see [all_lo, all_hi]
+    const int32_t first_t = row_tile * kStepRows / a.group;
+    const int32_t all_lo = __builtin_amdgcn_readfirstlane(a.keys(a.start(b), steps.last, steps.last).lo);
+    const int32_t all_hi = steps.keys.hi - (steps.last - first_t);
     const char *ck = reinterpret_cast<const char *>(static_cast<const S *>(a.k) + head * a.ks[2]);
     const char *cv = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + head * a.vs[2]);
 
@@ -142,29 +150,46 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       return s < s_end && lane < F::kKeys && steps.keys.sees(j) ? a.table.number(b, j) : PageTable::none();
     };
     v4u kf[F::kTiles][F::kSteps], vf[F::kVPer];
-    const auto fetch_k = [&](int32_t s, int32_t pages) {
+    // Where the keys of a step lie, a key a lane, and their values.  Those that nobody sees are given the
+    // first one's place: their weight is zero, and no load asks whether it may.
+    struct Places {
+      uint64_t k, v;
+    };
+    const auto places_of = [&](int32_t s, int32_t pages, uint32_t there) {
+      const auto slot = static_cast<uint32_t>(a.table.slot(key_of(s) + lane)), page = static_cast<uint32_t>(pages);
+      const auto at = [&](const int64_t *strides) {
+        const uint64_t place = (static_cast<uint64_t>(strides[0]) * page + static_cast<uint64_t>(strides[1]) * slot) * F::kSize;
+        const int first = __builtin_ctz(there);
+        const auto low = __builtin_amdgcn_readlane(static_cast<int32_t>(place), first);
+        const auto high = __builtin_amdgcn_readlane(static_cast<int32_t>(place >> 32), first);
+        return pages >= 0 ? place : static_cast<uint64_t>(static_cast<uint32_t>(high)) << 32 | static_cast<uint32_t>(low);
+      };
+      Places p;
+      p.k = at(a.ks);
+      p.v = alike ? p.k : at(a.vs);
+      return p;
+    };
+    const auto of_key = [](uint64_t places, int key) {
+      const auto low = static_cast<uint32_t>(__shfl(static_cast<int32_t>(places), key));
+      return static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int32_t>(places >> 32), key))) << 32 | low;
+    };
+    const auto fetch_k = [&](const Places &places) {
 #pragma unroll
       for (int i = 0; i < F::kTiles; ++i) {
-        const int place = 16 * i + lane % 16;
-        const int64_t page = __shfl(pages, place);
-        const char *from = ck + (page * a.ks[0] + a.table.slot(key_of(s) + place) * a.ks[1]) * F::kSize;
+        const char *from = ck + of_key(places.k, 16 * i + lane % 16) + quad * 16;
 #pragma unroll
         for (int c = 0; c < F::kSteps; ++c) {
-          const int chunk = 4 * c + quad;
-          kf[i][c] = v4u{0, 0, 0, 0};
-          if (page >= 0 && chunk * 16 < bytes) kf[i][c] = *reinterpret_cast<const v4u *>(from + chunk * 16);
+          // beyond the head's values its first: queries are zero there
+          const int more = c < kSure || (4 * c + quad) * 16 < bytes ? 64 * c : -quad * 16;
+          kf[i][c] = *reinterpret_cast<const v4u *>(from + more);
         }
       }
     };
-    const auto fetch_v = [&](int32_t s, int32_t pages) {
+    const auto fetch_v = [&](const Places &places) {
+      const int chunk = lane % F::kChunks * 16 < bytes ? lane % F::kChunks * 16 : 0;  // (nor are such sums kept)
 #pragma unroll
-      for (int r = 0; r < F::kVPer; ++r) {
-        const int at = lane + r * kWave, chunk = at % F::kChunks, place = at / F::kChunks;
-        const int64_t page = __shfl(pages, place);
-        const char *from = cv + (page * a.vs[0] + a.table.slot(key_of(s) + place) * a.vs[1]) * F::kSize;
-        vf[r] = v4u{0, 0, 0, 0};
-        if (page >= 0 && chunk * 16 < bytes) vf[r] = *reinterpret_cast<const v4u *>(from + chunk * 16);
-      }
+      for (int r = 0; r < F::kVPer; ++r)
+        vf[r] = *reinterpret_cast<const v4u *>(cv + of_key(places.v, (lane + r * kWave) / F::kChunks) + chunk);
     };
 
     char *tile = lds + wave * F::kTile;
@@ -174,46 +199,69 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
 
     int32_t step = s_begin + wave;
-    int32_t pages = a.table.checked(numbers_of(step));
     PageTable::Number ahead = numbers_of(step + kWaves);
-    if (step < s_end) {
-      fetch_k(step, pages);
-      fetch_v(step, pages);
+    uint32_t there;  // keys of a step that somebody sees
+    {
+      const int32_t pages = a.table.checked(numbers_of(step));
+      there = static_cast<uint32_t>(__ballot(pages >= 0));
+      if (there != 0) {
+        const Places places = places_of(step, pages, there);
+        fetch_k(places);
+        fetch_v(places);
+      }
     }
     for (; step < s_end; step += kWaves) {
+      const uint32_t here = there;
       v4f s[F::kTiles];
+      if (here != 0) {
 #pragma unroll
-      for (int i = 0; i < F::kTiles; ++i) {
-        s[i] = v4f{0, 0, 0, 0};
+        for (int i = 0; i < F::kTiles; ++i) {
+          s[i] = v4f{0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < F::kSteps; ++c) s[i] = Mfma16<V>::mul(kf[i][c], qf[c], s[i]);
+          for (int c = 0; c < F::kSteps; ++c) s[i] = Mfma16<V>::mul(kf[i][c], qf[c], s[i]);
+        }
       }
-      const uint32_t there = static_cast<uint32_t>(__ballot(pages >= 0));
-      const bool more = step + kWaves < s_end;
-      pages = a.table.checked(ahead);
+      const int32_t pages = a.table.checked(ahead);
+      there = static_cast<uint32_t>(__ballot(pages >= 0));
       ahead = numbers_of(step + 2 * kWaves);
-      if (more) fetch_k(step + kWaves, pages);
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int r = 0; r < F::kVPer; ++r) {
-        const int at = lane + r * kWave;
-        *reinterpret_cast<v4u *>(tile + F::at(at / F::kChunks, at % F::kChunks)) = vf[r];
+      Places places{0, 0};
+      if (there != 0) {
+        places = places_of(step + kWaves, pages, there);
+        fetch_k(places);
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (more) fetch_v(step + kWaves, pages);
+      if (here != 0) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < F::kVPer; ++r) {
+          const int at = lane + r * kWave;
+          *reinterpret_cast<v4u *>(tile + F::at(at / F::kChunks, at % F::kChunks)) = vf[r];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+      if (there != 0) fetch_v(places);
+      if (here == 0) continue;
 
       float x[F::kTiles * 4], top = -INFINITY;
-      const int32_t j0 = key_of(step) + 4 * quad;
+      const int32_t j0 = key_of(step);
+      if (here == kAll && j0 >= all_lo && j0 + F::kKeys - 1 <= all_hi) {
 #pragma unroll
-      for (int i = 0; i < F::kTiles; ++i)
+        for (int i = 0; i < F::kTiles; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int place = 16 * i + k;
-          const bool seen = ((there >> (place + 4 * quad) & 1) != 0) & mine.sees(j0 + place);
-          x[4 * i + k] = seen ? s[i][k] * a.scale : -INFINITY;
-          top = fmaxf(top, x[4 * i + k]);
-        }
+          for (int k = 0; k < 4; ++k) x[4 * i + k] = s[i][k] * a.scale;
+      } else {
+        const uint32_t mine_here = here >> (4 * quad);
+#pragma unroll
+        for (int i = 0; i < F::kTiles; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int place = 16 * i + k;
+            const bool seen = ((mine_here >> place & 1) != 0) & mine.sees(j0 + 4 * quad + place);
+            x[4 * i + k] = seen ? s[i][k] * a.scale : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < F::kTiles * 4; ++k) top = fmaxf(top, x[k]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float grown = fmaxf(m, top);
@@ -267,6 +315,10 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    if (!live) {
+      l = 0.0f;
+      m = -INFINITY;
+    }
 
     // the waves' parts, joined: a row of DP sums, m and l a query and wave
     __syncthreads();
