@@ -294,10 +294,12 @@ msx_status launch(const Rows &rows, const Turning &how, int64_t tokens, int32_t 
   s.heads = heads;
   s.units = Unit<V, E, kInterleaved>::units(how.r, dim);
   const int32_t groups = kThreads / s.units;
-  // Where there are heads for 256 CUs' threads four times over, a thread takes four of a
-  // token's, its loads in flight together and its angles worked out once; a few tokens
-  // are spread over as many workgroups as their heads give.
-  const bool many = tokens * heads * s.units >= int64_t{4} * 256 * 1024;
+  // A thread takes four of a token's heads, its loads in flight together and their angles
+  // worked out once, where that leaves a workgroup a CU (bf16 appends of 512 tokens' 32 + 16
+  // heads of 128, interleaved: 7.0 us, a head a thread 7.5; of 1,024 7.3 and 11.3; of 8,192
+  // 31 and 63).  Fewer tokens are spread over as many workgroups as their heads give, for
+  // which both ways take less than the call itself.
+  const bool many = tokens * heads * s.units >= int64_t{4} * 256 * kThreads;
   s.side = std::min(many ? (heads + 3) / 4 : heads, groups);
   s.per_block = groups / s.side;
   s.parts = many ? 1 : (heads + s.side - 1) / s.side;
