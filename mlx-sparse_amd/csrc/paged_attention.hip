@@ -131,6 +131,12 @@ Route route_of(const msx_paged_attention_desc &d) {
   return shares(d, rows) ? Route::kShared : Route::kStep;
 }
 
+// Whether tiles of queries are as few as the kernels count.
+bool countable(const msx_paged_attention_desc &d) {
+  const int64_t rows = d.tokens * (d.heads / d.cache.kv_heads);
+  return !takes_tiles(d) || d.batch * ((rows + kStepRows - 1) / kStepRows) <= kWindowIntMax;
+}
+
 // What a call's kernels are given, and where in its scratch their parts lie.
 struct Plan {
   Route route;
@@ -217,7 +223,7 @@ using namespace msx;
 
 extern "C" size_t msx_paged_attention_scratch(const msx_paged_attention_desc *desc) {
   if (check_paged_attention("paged_attention", desc) != MSX_OK || desc->batch == 0 ||
-      desc->tokens == 0)
+      desc->tokens == 0 || !countable(*desc))
     return 0;
   return Plan(*desc, args_of(*desc), nullptr, nullptr).bytes;
 }
@@ -228,6 +234,7 @@ extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, 
   if (msx_status st = check_paged_attention("paged_attention", desc); st != MSX_OK) return st;
   if (desc->batch == 0 || desc->tokens == 0) return MSX_OK;
   if (out == nullptr) return fail(MSX_EINVAL, "paged_attention out is NULL.");
+  if (!countable(*desc)) return fail(MSX_EINVAL, "paged_attention has more rows than its kernels count.");
   const PagedArgs a = args_of(*desc);
   const auto s = static_cast<hipStream_t>(stream);
   const auto vt = static_cast<msx_vtype>(desc->vtype);
@@ -246,8 +253,6 @@ extern "C" msx_status msx_paged_attention(const msx_paged_attention_desc *desc, 
   }
   if (p.bytes > 0 && (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0))
     return fail(MSX_EINVAL, "paged_attention scratch is too small or not aligned.");
-  if (a.batch * std::max(p.step.tiles, p.tiles.tiles) > kWindowIntMax)
-    return fail(MSX_EINVAL, "paged_attention has more rows than a grid holds.");
   const PartSource none{};
   const PartSource by_step = p.source(p.step, p.step_to, kStepRows, false);
   const PartSource by_tiles = p.source(p.tiles, p.tiles_to, kTileRows, p.route == Route::kShared);

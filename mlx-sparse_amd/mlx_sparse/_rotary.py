@@ -55,7 +55,8 @@ class Rotary:
 
     The frequencies are put on the selected device when the object is made; on
     another one the first call there copies them (not while a graph is
-    captured).
+    captured).  Like any operand the object lives until work that was given to
+    other streams with it is done, and as long as a captured graph that reads it.
     """
 
     __slots__ = ("_dim", "_interleaved", "_magnitude", "_frequencies", "_held")
@@ -133,6 +134,10 @@ class Rotary:
         if held is None:
             turns = self._frequencies / (2 * math.pi)
             if device >= 0:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(
+                        "Rotary has no frequencies on this device, and none can be copied while a "
+                        "graph is captured: make it, or call it once, on the device before.")
                 turns = turns.to(torch.device("cuda", device))
             held = (turns, self._dim, self._interleaved, self._magnitude)
             self._held[device] = held
