@@ -9,6 +9,11 @@
 // to the operands' 16 bits for the second product, unnormalised and at most
 // 2^8: their errors are independent and no larger than the output's own rounding.
 //
+// Bound by products, exponentials and LDS reads taking turns, two waves a SIMD, at the clocks that power
+// allows: 2,048 queries on 18,432 keys, 16 heads of 128 on 8, float16, 355 us, 821 TFLOP/s where a
+// large matrix product reaches 1,080; 1,024 on 8,192, 16 heads on 4, bfloat16, 97 us (663), float32
+// 620 (104 of 153).  64 sequences' queries against 8,192 shared keys: 36 us with their own keys beside.
+//
 // As in msx_paged_step.h each workgroup takes an equal stretch of all tiles, numbered by
 // kv head, sequence and unit; of its first and last unit it may have a part, which
 // paged_join joins.

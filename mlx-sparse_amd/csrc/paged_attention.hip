@@ -93,10 +93,10 @@ constexpr int64_t kLongRead = int64_t{48} << 20;  // bytes that the table has ro
 // paged_tiles reaches at such sizes, or the bytes once, some 8 us for more workgroups' starts
 // and a second set of parts to join, and the sequences' own keys half the chip.  Measured,
 // without and with, in us, one token a sequence:
-//   32 heads of 128 on 8, bfloat16   4 sequences of 1,024 shared keys 15.5 18.0, 4,096 23.4 18.3;
-//                                    64 of 64 24.2 31.6, 256 28.6 33.9, 1,024 51.6 38.2, 16,384 589 51
-//   8 heads of 64 on 2, float16      64 of 256 15.1 17.8, 4,096 31.8 22.0
-//   16 heads of 128, float32         2 of 16,384 96 166, 8 283 167; 64 of 256 67.9 70.9, 1,024 164 67
+//   32 heads of 128 on 8, bfloat16   4 sequences of 1,024 shared keys 15.2 18.0, 4,096 22.4 17.9;
+//                                    64 of 64 12.9 31.6, 256 17.2 33.9, 1,024 42.5 38.9, 16,384 558 53
+//   8 heads of 64 on 2, float16      64 of 256 8.6 17.8, 4,096 28.7 21.9
+//   16 heads of 128, float32         2 of 16,384 98 166, 8 286 169; 64 of 256 60.5 70.4, 1,024 140 66
 bool shares(const msx_paged_attention_desc &d, int64_t rows) {
   const msx_paged_cache &c = d.cache;
   // (with a window few sequences see much of what they share)
