@@ -14,8 +14,8 @@
 // of queries can be another's as well; what it has of them goes to two places
 // of scratch, and paged_join adds those up in the order of the keys.
 //
-// One token of 131,072 keys, 32 heads of 128 on 8, bfloat16: 108 us, 5.0 TB/s; 64 sequences of up
-// to 16,384, cold, 120 us with joining (4.4 TB/s); 32 of 4,000, 16 heads on 4, 52 us (5.1); 32 of
+// One token of 131,072 keys, 32 heads of 128 on 8, bfloat16: 101 us, 5.3 TB/s; 64 sequences of up
+// to 16,384, cold, 113 us with joining (4.9 TB/s); 32 of 4,000, 16 heads on 4, 52 us (5.1); 32 of
 // 4,000 in float32, heads of 256, 193 us (5.4).  Rows of 64 bytes move half lines: 33 us for heads
 // of 32, what heads of 64 take.  Two workgroups a CU are what registers allow; for heads of 64 at most,
 // where they would allow four, one took up to 60 % more, three or four 25 % less to 20 more.
@@ -37,7 +37,8 @@ constexpr int step_lds() {
 
 // Workgroup g of grid.groups.  `lds`: step_lds bytes at a sixteen-byte address.
 // Where grid.whole (a workgroup of eight waves always is) it has all keys of one tile.
-template <class V, int DP, int kWaves = kStepWaves>
+// kPast: keys and values go past the caches.
+template <class V, int DP, int kWaves = kStepWaves, bool kPast = false>
 __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid &grid, int64_t g, const TileParts &to,
                                              char *lds, StretchLds &own) {
   using S = typename V::Storage;
@@ -179,6 +180,10 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       const auto low = static_cast<uint32_t>(__shfl(static_cast<int32_t>(places), key));
       return static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int32_t>(places >> 32), key))) << 32 | low;
     };
+    const auto piece = [](const char *from) {
+      if constexpr (kPast) return __builtin_nontemporal_load(reinterpret_cast<const v4u *>(from));
+      return *reinterpret_cast<const v4u *>(from);
+    };
     const auto fetch_k = [&](const Places &places) {
 #pragma unroll
       for (int i = 0; i < F::kTiles; ++i) {
@@ -187,7 +192,7 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
         for (int c = 0; c < F::kSteps; ++c) {
           // beyond the head's values its first: queries are zero there
           const int more = c < kSure || (4 * c + quad) * 16 < bytes ? 64 * c : -quad * 16;
-          kf[i][c] = *reinterpret_cast<const v4u *>(from + more);
+          kf[i][c] = piece(from + more);
         }
       }
     };
@@ -195,7 +200,7 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       const int chunk = lane % F::kChunks * 16 < bytes ? lane % F::kChunks * 16 : 0;  // (nor are such sums kept)
 #pragma unroll
       for (int r = 0; r < F::kVPer; ++r)
-        vf[r] = *reinterpret_cast<const v4u *>(cv + of_key(places.v, (lane + r * kWave) / F::kChunks) + chunk);
+        vf[r] = piece(cv + of_key(places.v, (lane + r * kWave) / F::kChunks) + chunk);
     };
 
     char *tile = lds + wave * F::kTile;

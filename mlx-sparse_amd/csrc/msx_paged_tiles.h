@@ -13,6 +13,7 @@ struct StepGrid {
   int32_t from;    // the first key
   int32_t whole;   // a workgroup a tile of queries and kv head, all of its keys
   int32_t waves;   // of a workgroup: eight where whole and few, else four
+  int32_t past;    // steps that are cut: past the caches, where that pays
 };
 
 // The steps of `kKeys` keys that a tile of queries takes: those over the sinks, then

@@ -119,6 +119,17 @@ int64_t held_keys(const msx_paged_attention_desc &d) {
                   std::min(d.window, wide) + std::min(d.sinks, wide) + d.tokens);
 }
 
+// The bytes of as many keys and values, of one sequence and kv head.
+int64_t held_bytes(const msx_paged_attention_desc &d) {
+  return 2 * held_keys(d) * d.cache.dim * static_cast<int64_t>(value_bytes(static_cast<msx_vtype>(d.vtype)));
+}
+
+// Keys that are read once go past the caches where there may be more of them than the Infinity Cache holds
+// (256 MB) from one call to the next: 64 sequences of up to 16,384 tokens, 32 heads of 128 on 8, bfloat16, 125 us
+// to 113; one of 131,072 114.5 to 107; 300 of 2,048 439 to 403; 60 of 1,500 in float32 150 to 136.  What is there
+// is read faster from it: 262 MB of 32 of 4,000 keys, 52 us so, 58 past it.
+constexpr int64_t kCached = int64_t{320} << 20;
+
 Route route_of(const msx_paged_attention_desc &d) {
   if (!takes_tiles(d)) return Route::kRows;
   const int64_t rows = d.tokens * (d.heads / d.cache.kv_heads);
@@ -169,6 +180,8 @@ struct Plan {
       step.groups = a.dim > 128 || route == Route::kShared ? 256 : 512;
       step.waves = kStepWaves;
       if (route == Route::kStep) whole(d, a);
+      step.past = route == Route::kStep && !step.whole && step.tiles == 1 &&
+                  held_bytes(d) * d.batch * d.cache.kv_heads > kCached;
       step.from = route == Route::kShared ? static_cast<int32_t>(d.shared_pages * d.cache.page_size) : 0;
       step_to = parts_of(step, a.batch * step.tiles, kStepRows);
     }
@@ -195,7 +208,7 @@ struct Plan {
   //   32 of 256 on 8, bfloat16         8 of 500 23.0 20.9, up to 22.2 16.9; 30 of 500 27.8 38.7, up to 22.2 24.2
   void whole(const msx_paged_attention_desc &d, const PagedArgs &a) {
     const int64_t units = a.batch * step.tiles * a.kv_heads;
-    const int64_t bytes = held_keys(d) * a.dim * static_cast<int64_t>(value_bytes(static_cast<msx_vtype>(d.vtype)));
+    const int64_t bytes = held_bytes(d) / 2;
     if (units > max_blocks(8 * kWave) ||
         bytes > (units <= 128 ? (d.vtype == MSX_F32 ? 128 << 10 : 192 << 10) : a.dim > 128 ? 128 << 10 : 224 << 10))
       return;
