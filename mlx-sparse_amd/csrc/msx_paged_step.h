@@ -14,7 +14,7 @@
 // of queries can be another's as well; what it has of them goes to two places
 // of scratch, and paged_join adds those up in the order of the keys.
 //
-// One token of 131,072 keys, 32 heads of 128 on 8, bfloat16: 101 us, 5.3 TB/s; 64 sequences of up
+// One token of 131,072 keys, 32 heads of 128 on 8, bfloat16: 103 us, 5.2 TB/s; 64 sequences of up
 // to 16,384, cold, 113 us with joining (4.9 TB/s); 32 of 4,000, 16 heads on 4, 52 us (5.1); 32 of
 // 4,000 in float32, heads of 256, 193 us (5.4).  Rows of 64 bytes move half lines: 33 us for heads
 // of 32, what heads of 64 take.  Two workgroups a CU are what registers allow; for heads of 64 at most,

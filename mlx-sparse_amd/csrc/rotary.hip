@@ -9,7 +9,7 @@
 // that their angles are worked out once.
 //
 // Bound by memory, calls of a few tokens by the launch.  16,384 tokens of 40 heads of 128,
-// bfloat16: 65 us, 5.2 TB/s read and written, a copy's rate; 129 of 10 of 80, float32: 3.4 us.
+// bfloat16: 59 us, 5.7 TB/s read and written, more than a copy; 129 of 10 of 80, float32: 3.4 us.
 // Appended: 64 tokens' 48 heads 4.5 us; 5 prompts of up to 2,049 tokens, 32 heads, float16, 17 us
 // (4.0 TB/s).  Heads of which a half (interleaved, the rotated part) is no multiple of sixteen
 // bytes go a value a thread, at 1.3 to 3 times that.
@@ -58,13 +58,23 @@ __device__ __forceinline__ void turn(double t, float magnitude, float &cosine, f
   sine = static_cast<float>(n & 2 ? -b * T(magnitude) : b * T(magnitude));
 }
 
-// E adjacent values, as they lie in memory.
+// E adjacent values, as they lie in memory; kPast: past the caches.
 template <class V, int E>
 struct Values {
   using S = typename V::Storage;
   using Raw = std::conditional_t<E == 1, S, v4u>;
-  __device__ static __forceinline__ Raw load(const S *p) { return *reinterpret_cast<const Raw *>(p); }
-  __device__ static __forceinline__ void store(S *p, Raw r) { *reinterpret_cast<Raw *>(p) = r; }
+  template <bool kPast>
+  __device__ static __forceinline__ Raw load(const S *p) {
+    if constexpr (kPast) return __builtin_nontemporal_load(reinterpret_cast<const Raw *>(p));
+    return *reinterpret_cast<const Raw *>(p);
+  }
+  template <bool kPast>
+  __device__ static __forceinline__ void store(S *p, Raw r) {
+    if constexpr (kPast)
+      __builtin_nontemporal_store(r, reinterpret_cast<Raw *>(p));
+    else
+      *reinterpret_cast<Raw *>(p) = r;
+  }
   __device__ static __forceinline__ void widen(Raw r, float (&x)[E]) {
     if constexpr (E == 1) {
       x[0] = V::widen(r);
@@ -254,7 +264,7 @@ struct Split {
   int32_t parts;      // of a token's heads, a workgroup each
 };
 
-template <class V, int E, bool kInterleaved, class Rows>
+template <class V, int E, bool kInterleaved, bool kPast, class Rows>
 __global__ __launch_bounds__(kThreads) void rotate_rows(Rows rows, Turning how, Split s, int64_t first) {
   using U = Unit<V, E, kInterleaved>;
   using Raw = typename U::Raw;
@@ -279,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void rotate_rows(Rows rows, Turning how, 
 #pragma unroll
       for (int k = 0; k < U::kVectors; ++k) {
         raw[j][k] = Raw{};
-        if (!place[j].zero) raw[j][k] = Values<V, E>::load(place[j].from + unit.at[k]);
+        if (!place[j].zero) raw[j][k] = Values<V, E>::template load<kPast>(place[j].from + unit.at[k]);
       }
     }
 #pragma unroll
@@ -287,10 +297,15 @@ __global__ __launch_bounds__(kThreads) void rotate_rows(Rows rows, Turning how, 
       if (place[j].to == nullptr) continue;
       if (unit.rotated && place[j].rotated && !place[j].zero) unit.apply(raw[j]);
 #pragma unroll
-      for (int k = 0; k < U::kVectors; ++k) Values<V, E>::store(place[j].to + unit.at[k], raw[j][k]);
+      for (int k = 0; k < U::kVectors; ++k) Values<V, E>::template store<kPast>(place[j].to + unit.at[k], raw[j][k]);
     }
   }
 }
+
+// More values, read and written, than the Infinity Cache (256 MB) holds until the next reader go past the
+// caches, in us: of 40 heads of 128, bfloat16, 16,384 tokens (336 MB) 65 to 59, 24,000 91 to 82; 8,192 of 20
+// (84 MB) 14.8 and 16.4, 13,300 of 40 (272 MB) 44 and 47, 14,200 (291 MB) 47 and 50, in float32 55 and 53.
+constexpr int64_t kCached = int64_t{288} << 20;
 
 template <class V, int E, bool kInterleaved, class Rows>
 msx_status launch(const Rows &rows, const Turning &how, int64_t tokens, int32_t heads, int32_t dim,
@@ -312,8 +327,14 @@ msx_status launch(const Rows &rows, const Turning &how, int64_t tokens, int32_t 
   const int64_t most = max_blocks(kThreads) / s.parts * s.per_block;
   for (int64_t first = 0; first < tokens; first += most) {
     const int64_t here = std::min(tokens - first, most);
-    rotate_rows<V, E, kInterleaved><<<static_cast<unsigned>((here + s.per_block - 1) / s.per_block * s.parts),
-                                      kThreads, 0, stream>>>(rows, how, s, first);
+    const auto blocks = static_cast<unsigned>((here + s.per_block - 1) / s.per_block * s.parts);
+    if constexpr (E > 1) {
+      if (2 * tokens * heads * dim * static_cast<int64_t>(sizeof(typename V::Storage)) > kCached) {
+        rotate_rows<V, E, kInterleaved, true><<<blocks, kThreads, 0, stream>>>(rows, how, s, first);
+        continue;
+      }
+    }
+    rotate_rows<V, E, kInterleaved, false><<<blocks, kThreads, 0, stream>>>(rows, how, s, first);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MSX_OK : hip_fail(e, op);
