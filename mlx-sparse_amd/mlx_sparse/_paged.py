@@ -123,6 +123,9 @@ def paged_attention(q, cache_k, cache_v, pages, *, starts=None, lengths=None,
             kernels, a wave a query and head.
         pages: The table, shape ``(batch, pages of a sequence)``, int32 or int64.
             Pages that no position up to the last query's needs may be anything.
+            Lengths are not read on the host: how the work is cut goes by the
+            table's width, so that short sequences are served fastest from a table
+            that is cut to the longest (``pages[:, :n]``, no copy).
         starts: Tokens of each sequence before the first query, shape
             ``(batch,)``, int32 or int64; zero by default.  A negative start
             marks a slot of the batch without a sequence: it gives zeros.

@@ -213,7 +213,8 @@ def rotary(x, rotation: Rotary, *, starts=None, positions=None) -> torch.Tensor:
         Shape and dtype of ``x``, differentiable in ``x`` to any order.
 
     Angles are worked out in 64 bits (positions of a million lose nothing),
-    products in float32, rounded once.
+    products in float32, rounded once.  A backward pass is captured into a graph
+    as any of torch's is: no eager graph of ``x`` may be alive meanwhile.
     """
     if not isinstance(rotation, Rotary):
         raise TypeError(f"rotary expects a Rotary, got {type(rotation).__name__}.")

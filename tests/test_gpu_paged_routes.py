@@ -103,3 +103,12 @@ def test_tables_of_one_row_for_all(gpu):
         got = gpu.paged_attention(q, ck, cv, table[:1].cuda().expand(70, -1), starts=starts,
                                   shared_pages=shared)
         check(got, attention(q, ck, cv, table, [130] * 70), f"shared {shared}")
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 128), (BF16, 128), (BF16, 200), (BF16, 256),
+                                       (torch.float32, 120), (torch.float32, 128)])
+@pytest.mark.parametrize("tokens,window", [(1, None), (3, None), (1, 2**41)])
+def test_tables_of_more_than_the_cache_holds(gpu, dtype, dim, tokens, window):
+    """Wide tables of which little is filled: keys that are read past the caches."""
+    paged_case(gpu, "cuda", dtype, [0, 40, -1, 700, 2500, 33], tokens=tokens, heads=8, kv_heads=2, dim=dim,
+               width=6000, window=window, lengths=[tokens, 1, 1, tokens, tokens, 0])
