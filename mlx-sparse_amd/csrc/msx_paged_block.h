@@ -6,8 +6,8 @@
 // keys in LDS.  Per tile: S^T = K Q^T, the running maximum and sum, O^T += V^T P^T,
 // as in window_forward.hip; the next tile's rows are on their way to LDS meanwhile,
 // the numbers of the pages after those in registers.  A row's probabilities are rounded
-// to the operands' 16 bits for the second product, unnormalised and at most
-// 2^8: their errors are independent and no larger than the output's own rounding.
+// to the operands' 16 bits for the second product, unnormalised, at most 2^8 (float16: 2^15):
+// their errors are independent and no larger than the output's own rounding.
 //
 // Bound by products, exponentials and LDS reads taking turns, two waves a SIMD, at the clocks that power
 // allows: 2,048 queries on 18,432 keys, 16 heads of 128 on 8, float16, 355 us, 821 TFLOP/s where a
@@ -461,8 +461,12 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
       l += sum[0] + sum[1];
     };
     // masks the scores of the tile at j0 and moves the maximum.  It is moved only where
-    // it has grown by more than 2^8: until then exponentials up to 2^8 stand
-    // beside sums of their own scale.
+    // it has grown by more than 2^kLag: until then exponentials up to 2^kLag times those of its
+    // scale stand beside sums of their own.  Float16's range holds that beside the weights below (see
+    // kWeightsUp), 1,024 queries on 8,192 keys of scores that vary by a nat, and by three, in us:
+    //   heads of 128   2^8 99.5 100.5, 2^4 99.1 101.8, 2^2 100.1 103.4, 2 102.1 104.1, 1 104.1 105.2
+    //   heads of 256       257   264       257   276       267   288    282   297      307   307
+    constexpr float kLag = kWeightsUp<V> > 0.0f ? 2.0f : 8.0f, kUp = std::max(kWeightsUp<V> - kLag, 0.0f);
     const auto settle = [&](int32_t j0, uint64_t there, v16f (&y)[F::kSub]) {
       const bool whole = there == kAll && j0 >= all_lo && j0 + F::kKeys - 1 <= all_hi;
       if (!whole) {
@@ -483,8 +487,8 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
         for (int r = 0; r < 16; ++r) tops[r % 2] = fmaxf(tops[r % 2], y[i][r]);
       float top = fmaxf(tops[0], tops[1]);
       top = fmaxf(top, other_half(top)) * scale;
-      if (__any(top > m + 8.0f)) {
-        const float grown = fmaxf(m, top);
+      if (__any(top > m + (kUp + kLag))) {
+        const float grown = fmaxf(m, top - kUp);
         const float shrink = grown == -INFINITY ? 1.0f : exp2_fast(m - grown);
         m = grown;
         base = m == -INFINITY ? 0.0f : m;

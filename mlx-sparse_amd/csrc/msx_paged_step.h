@@ -275,7 +275,7 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
       for (int k = 0; k < F::kTiles * 4; ++k) top = fmaxf(top, x[k]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float grown = fmaxf(m, top);
+      const float grown = fmaxf(m, top - kWeightsUp<V>);
       const float base = grown == -INFINITY ? 0.0f : grown;
       if (__any(grown > m)) {
         const float shrink = exp2_fast(m - base);
@@ -290,7 +290,7 @@ __device__ __forceinline__ void step_stretch(const PagedArgs &a, const StepGrid 
         l += x[k];
       }
       if constexpr (F::kSize == 2) {
-        v4u p, low;  // rounded, and what that leaves: the output has its own rounding alone
+        v4u p, low;  // rounded, and what that leaves: of a weight 2^-22 at most in float16, 2^-16 in bfloat16
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t pair = Mfma<V>::pack(x[2 * k], x[2 * k + 1]);

@@ -58,6 +58,16 @@ struct StepShape {
   }
 };
 
+// Weights of paged attention are 2^(score - m), their sums kept beside that m, which may be any
+// number near the row's largest score.  Float16 ends at 2^-24: were m that score, a weight below
+// 2^-25 of the largest would be nothing, and many of those may be all that a row adds up to (a
+// first key that takes the softmax and whose value is nothing).  So m is as far below it as
+// leaves the largest weight 2^15: of a weight w beside the largest, 1, rounding takes 2^-11 w or
+// 2^-40, whichever is more, and of one in two values 2^-22 w or 2^-40.  (In tiles, whose m
+// may be two lower still, 2^-38.)
+template <class V>
+constexpr float kWeightsUp = V::kType == MSX_F16 ? 15.0f : 0.0f;
+
 // m, l and dim sums of a query over one part of the keys.
 __host__ __device__ inline int64_t part_stride(int32_t dim) { return (dim + 2 + 3) / 4 * 4; }
 
