@@ -402,7 +402,8 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     const bool live = row.held && row.t < a.length(row.b);
     Keys mine{0, 0, -1, 0};
     if (live) mine = a.keys(a.start(row.b), row.t, row.t);
-    if constexpr (kShared) mine = Keys{0, 0, min(mine.hi, grid.from - 1), 0};
+    // (a window as wide as the table still hides keys from queries that stand behind it)
+    if constexpr (kShared) mine.hi = min(mine.hi, grid.from - 1);
     // what the wave's rows see: all of them [all_lo, all_hi], any of them the rest
     const int32_t all_lo = -wave_least(live ? -mine.lo : 0), all_hi = wave_least(live ? mine.hi : 0x7fffffff);
     const int32_t any_hi = -wave_least(live ? -mine.hi : 1), any_lo = wave_least(live ? mine.lo : 0x7fffffff);

@@ -99,7 +99,7 @@ constexpr int64_t kLongRead = int64_t{48} << 20;  // bytes that the table has ro
 //   16 heads of 128, float32         2 of 16,384 98 166, 8 286 169; 64 of 256 60.5 70.4, 1,024 140 66
 bool shares(const msx_paged_attention_desc &d, int64_t rows) {
   const msx_paged_cache &c = d.cache;
-  // (with a window few sequences see much of what they share)
+  // (with a window narrower than the table few sequences see much of what they share)
   if (d.shared_pages == 0 || d.batch < 2 || d.window < c.width * c.page_size ||
       d.batch * rows > kWindowIntMax - kTileRows)
     return false;

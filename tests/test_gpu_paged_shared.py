@@ -1,0 +1,30 @@
+"""Pages that a batch shares, read once for all: what each query sees of them."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from _paged_checks import paged_case
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def past_the_table(capacity):
+    """Starts of a batch some of which have outgrown a table of so many places, one by so much
+    that it sees nothing of it."""
+    starts = [capacity - 90 + 3 * b for b in range(64)]
+    starts[3], starts[4], starts[5] = -1, 2 * capacity + 40, 2 * capacity - 30
+    return starts
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,sinks,beyond", [(1, 0, 0), (1, 3, 0), (3, 0, 0), (3, 40, 0), (1, 0, 50)])
+@pytest.mark.parametrize("shared", [0, 140, 146])
+def test_a_window_of_the_table(gpu, dtype, tokens, sinks, beyond, shared):
+    """Windows as wide as the table hide keys of it from queries that stand behind it."""
+    capacity = 146 * 16
+    paged_case(gpu, "cuda", dtype, past_the_table(capacity), tokens=tokens, window=capacity + beyond,
+               sinks=sinks, shared=shared, width=146, dim=64, heads=4, kv_heads=2)
+
