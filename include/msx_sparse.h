@@ -1148,8 +1148,9 @@ msx_status msx_paged_cache_append(const msx_paged_append_desc *desc, void *q_out
  * negative start, and queries that see nothing give zeros.  `out` is batch x
  * tokens x heads x dim, contiguous.
  *
- * shared_pages: the first so many pages are the same in every row of the table, those of
- * its first row; where the queries are few, they are read once for all of them.
+ * shared_pages: the first so many pages are the same in every row of the table (rows of
+ * sequences that have no query here need not hold them); where the queries are few, they are
+ * read once for all of them.
  *
  * `scratch` holds msx_paged_attention_scratch bytes at a sixteen-byte address.
  */

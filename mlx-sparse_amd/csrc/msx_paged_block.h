@@ -264,9 +264,21 @@ struct TileRow {
   }
 };
 
+// The first sequence that has queries here (0 where none has): slots without one need not hold
+// the pages that the batch shares.
+__device__ __forceinline__ int32_t first_live(const PagedArgs &a) {
+  for (int64_t b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int64_t b = b0 + threadIdx.x % kWave;
+    const uint64_t live = __ballot(b < a.batch && a.length(b) > 0);
+    if (live != 0) return static_cast<int32_t>(b0) + __builtin_ctzll(live);
+  }
+  return 0;
+}
+
 // kShared: rows are those of the whole batch, keys those of the pages that it shares
-// (grid.from of them, listed in the table's first row), and all results are parts.
-// Where grid.whole a workgroup has all keys of one unit.  Workgroup `id` of grid.groups; `args`: the launch's first argument; `lds`: PagedShape's kLds bytes at a multiple of 1,024.
+// (grid.from of them, as the first sequence's row of the table lists them), and all results are parts.
+// Where grid.whole a workgroup has all keys of one unit.  Workgroup `id` of grid.groups; `args`: the
+// launch's first argument; `lds`: PagedShape's kLds bytes at a multiple of 1,024.
 template <class V, int DP, bool kShared>
 __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepGrid &grid, uint32_t id, const TileParts &to,
                                               char *lds, StretchLds &own) {
@@ -358,6 +370,7 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     }
   }
 
+  const int32_t lister = kShared ? __builtin_amdgcn_readfirstlane(first_live(args)) : 0;
   const PageLoader<V, DP, F::kKeys> rows(args);
   // a negative scale moves its sign to the queries, so that the largest product is the
   // largest score
@@ -426,7 +439,7 @@ __device__ __forceinline__ void tiles_stretch(const PagedArgs &args, const StepG
     const char *v_base = reinterpret_cast<const char *>(static_cast<const S *>(a.v) + head * a.vs[2]);
 
     PageTable table = a.table;  // of this sequence
-    table.pages = static_cast<const char *>(table.pages) + b0 * table.stride * (table.wide ? 8 : 4);
+    table.pages = static_cast<const char *>(table.pages) + (kShared ? lister : b0) * table.stride * (table.wide ? 8 : 4);
 
     // the page of key `lane` of a tile, none where nobody sees it
     const auto numbers_of = [&](int32_t s) {

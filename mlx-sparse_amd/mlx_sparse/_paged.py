@@ -134,8 +134,8 @@ def paged_attention(q, cache_k, cache_v, pages, *, starts=None, lengths=None,
         window: Keys a query sees, its own position included; all by default.
         sinks: First keys that stay visible.
         scale: Factor of the scores, ``dim ** -0.5`` by default.
-        shared_pages: The first so many pages of every row of the table are the same,
-            those of its first row (slots without a sequence need not have
+        shared_pages: The first so many pages of every row of the table are the same
+            (slots without a sequence, or with no query here, need not have
             them): a batch behind one long instruction.  Few queries a
             sequence then read them once for all.
 

@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from _attention_reference import check
 from _paged_checks import paged_case
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +29,25 @@ def test_a_window_of_the_table(gpu, dtype, tokens, sinks, beyond, shared):
     paged_case(gpu, "cuda", dtype, past_the_table(capacity), tokens=tokens, window=capacity + beyond,
                sinks=sinks, shared=shared, width=146, dim=64, heads=4, kv_heads=2)
 
+
+
+@pytest.mark.parametrize("missing", [-1, 10**6, 5])
+@pytest.mark.parametrize("empty,batch,ended", [(1, 64, False), (63, 64, True), (64, 130, False), (100, 130, True),
+                                               (64, 64, False)])
+def test_first_slots_without_a_sequence(gpu, missing, empty, batch, ended):
+    """Slots that have emptied, or have no query here, name no pages, or other ones."""
+    starts = [2240 + 5 * b % 77 for b in range(batch)]
+    lengths = [1] * batch
+    for b in range(empty):
+        if ended and b % 2 == 0:
+            lengths[b] = 0
+        else:
+            starts[b] = -1
+
+    def change(q, ck, cv, table):
+        table[:empty] = missing
+
+    out, want = paged_case(gpu, "cuda", torch.bfloat16, starts, lengths=lengths, shared=140, dim=64, heads=4, kv_heads=2,
+                           change=change)
+    assert (out[:empty] == 0).all() and (empty == batch or out[empty:].abs().max() > 0)
+    check(out, want, f"{empty} of {batch}")
