@@ -197,21 +197,28 @@ struct Plan {
   // Few keys a sequence: a workgroup takes all of a tile's, of eight waves where the chip has
   // room, and nothing is to be joined, which takes 5 us and more.  The longest sequence then
   // takes 4.5 us and, for every 32 KB of its keys and as many of values, 1.8 (0.8 more in float32,
-  // whose products are slower), which few workgroups would share better; many fill the chip anyway.
+  // whose products are slower), which few workgroups would share better; from 129 on they fill the
+  // chip anyway, those of heads above 128, one a CU, up to four rounds of it.
   // Measured, cut and whole, in us, one token of sequences of as many keys, or of up to as many:
   //   8 heads of 64 on 2, bfloat16     1 of 1,000 13.1 10.6, 1,500 13.4 13.0, 2,000 13.5 15.7
-  //   32 of 64 on 8, bfloat16          30 of 1,500 29.6 19.4, up to 15.4 13.3; 3,000 43.9 34.1, up to 19.8 20.6
+  //   32 of 64 on 8, bfloat16          30 of 1,500 29.6 19.4, up to 15.4 13.3; 3,000 43.9 34.1, up to 19.8 20.6;
+  //                                    300 of 1,500 178 194, up to 60 39
   //   32 of 128 on 8, bfloat16         1 of 700 14.1 12.5, 1,000 14.1 15.0; 30 of 700 28.6 18.9, up to 16.4 12.9,
   //                                    1,500 44.3 32.1, up to 18.2 19.6; 128 of 1,000 107 102, up to 38.8 31.9
   //   32 of 64 on 8, float32           8 of 500 15.8 13.7, 1,000 21.4 21.9, up to 14.5 21.2; 30 of 700 30.8 18.6,
   //                                    up to 17.2 16.2, 1,000 37.1 24.0, up to 20.2 21.3
-  //   32 of 256 on 8, bfloat16         8 of 500 23.0 20.9, up to 22.2 16.9; 30 of 500 27.8 38.7, up to 22.2 24.2
+  //   32 of 256 on 8, bfloat16         8 of 300 17.3 18.5, 500 21.1 23.2, up to 16.9 22.2; 16 of 500 27.2 24.0, up to
+  //                                    17.1 22.2; 30 of 500 38.6 28.0, up to 24.0 22.2; 60 of 500 58.9 51.7, up to
+  //                                    32.7 27.0; 128 of 500 116 116, up to 58 55; 300 of 500 251 267, up to 107 118
   void whole(const msx_paged_attention_desc &d, const PagedArgs &a) {
     const int64_t units = a.batch * step.tiles * a.kv_heads;
     const int64_t bytes = held_bytes(d) / 2;
-    if (units > max_blocks(8 * kWave) ||
-        bytes > (units <= 128 ? (d.vtype == MSX_F32 ? 128 << 10 : 192 << 10) : a.dim > 128 ? 128 << 10 : 224 << 10))
-      return;
+    int64_t most = 224 << 10;
+    if (a.dim > 128)
+      most = units > 128 && units <= 1024 ? 256 << 10 : 128 << 10;
+    else if (units <= 128)
+      most = d.vtype == MSX_F32 ? 128 << 10 : 192 << 10;
+    if (units > max_blocks(8 * kWave) || bytes > most) return;
     step.whole = 1;
     step.waves = units <= 256 && a.dim <= 128 ? 8 : kStepWaves;
     step.groups = static_cast<int32_t>(units);
