@@ -4,9 +4,10 @@
  * This is the drop-in boundary for mlx-sparse's sparse x dense hot path:
  * CSR SpMV (y = A x) and CSR SpMM with a dense row-major right-hand side
  * (Y = A X), with what stands next to it: solvers, the adjoint side, Matrix
- * Market input, and two operators of language models over sparse patterns
- * (window attention with sinks, rotary positions, attention over paged caches,
- * distillation from a CSR teacher).  Every entry
+ * Market input, two operators of language models over sparse patterns (window
+ * attention with sinks, distillation from a CSR teacher), and what models with
+ * full attention need beside them (rotary positions, paged caches and the
+ * attention over them).  Every entry
  * point takes plain pointers and sizes; no C++ or framework type crosses it.
  *
  * Conventions

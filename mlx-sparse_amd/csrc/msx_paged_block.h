@@ -10,9 +10,12 @@
 // their errors are independent and no larger than the output's own rounding.
 //
 // Bound by products, exponentials and LDS reads taking turns, two waves a SIMD, at the clocks that power
-// allows: 2,048 queries on 18,432 keys, 16 heads of 128 on 8, float16, 355 us, 821 TFLOP/s where a
-// large matrix product reaches 1,080; 1,024 on 8,192, 16 heads on 4, bfloat16, 97 us (663), float32
-// 620 (104 of 153).  64 sequences' queries against 8,192 shared keys: 36 us with their own keys beside.
+// allows: 2,048 queries on 18,432 keys, 16 heads of 128 on 8, float16, 361 us, 809 TFLOP/s where a
+// large matrix product reaches 1,080; 1,024 on 8,192, 16 heads on 4, bfloat16, 95 us (681), float32
+// 616 (105 of 153).  What a score takes beside its products is the same for narrow heads, whose
+// matrix cores wait for it: bfloat16 heads of 32 270 TFLOP/s, of 64 450, of 80 474, of 96 576; those of
+// 256, a wave a SIMD and 32 keys a tile, 501.  64 sequences' queries against 8,192 shared keys: 36 us with
+// their own keys beside.
 //
 // As in msx_paged_step.h each workgroup takes an equal stretch of all tiles, numbered by
 // kv head, sequence and unit; of its first and last unit it may have a part, which

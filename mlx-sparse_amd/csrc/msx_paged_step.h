@@ -16,9 +16,11 @@
 //
 // One token of 131,072 keys, 32 heads of 128 on 8, bfloat16: 103 us, 5.2 TB/s; 64 sequences of up
 // to 16,384, cold, 113 us with joining (4.9 TB/s); 32 of 4,000, 16 heads on 4, 52 us (5.1); 32 of
-// 4,000 in float32, heads of 256, 193 us (5.4).  Rows of 64 bytes move half lines: 33 us for heads
-// of 32, what heads of 64 take.  Two workgroups a CU are what registers allow; for heads of 64 at most,
-// where they would allow four, one took up to 60 % more, three or four 25 % less to 20 more.
+// 4,000 in float32, heads of 256, 193 us (5.4).  Rows that end within a line of 128 bytes move the
+// lines that two kv heads share once for each, their workgroups lying on different XCDs: 16-bit heads of 32
+// take 33 us, of 80 50 and of 96 49, where heads of 64 take 34 and of 128 52.  Two workgroups a CU are what
+// registers allow; for heads of 64 at most, where they would allow four, one took up to 60 % more, three or
+// four 25 % less to 20 more.
 #pragma once
 
 #include "msx_paged.h"

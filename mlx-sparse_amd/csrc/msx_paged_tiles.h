@@ -140,7 +140,8 @@ struct StretchLds {
 constexpr int32_t kTileRows = 128;  // queries a workgroup, where they are many
 
 // paged_step.hip, paged_tiles.hip: rows and caches at sixteen-byte addresses and strides.
-// Grids of tiles of kStepRows and kTileRows queries; the latter need heads of 128 at most.
+// Grids of tiles of kStepRows and kTileRows queries; the latter take float32 heads of 128 at most,
+// 16-bit heads of 256.
 // launch_paged_shared: `tiles` those of the batch against the keys before tiles.from, of the
 // pages that it shares, `step` those of each sequence against the keys from there on.
 msx_status launch_paged_step(msx_vtype vt, const PagedArgs &a, const StepGrid &grid,

@@ -12,7 +12,8 @@
 // bfloat16: 59 us, 5.7 TB/s read and written, more than a copy; 129 of 10 of 80, float32: 3.4 us.
 // Appended: 64 tokens' 48 heads 4.5 us; 5 prompts of up to 2,049 tokens, 32 heads, float16, 17 us
 // (4.0 TB/s).  Heads of which a half (interleaved, the rotated part) is no multiple of sixteen
-// bytes go a value a thread, at 1.3 to 3 times that.
+// bytes go a value a thread: 8,192 tokens of 20 heads of 128, 62 values rotated, 30 us in bfloat16 and 29.5
+// in float32 where whole heads take 14.8 and 26; 4,096 tokens of 16 + 4 appended 30 where they take 11 and 17.5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

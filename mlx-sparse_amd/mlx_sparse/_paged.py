@@ -142,7 +142,13 @@ def paged_attention(q, cache_k, cache_v, pages, *, starts=None, lengths=None,
     Returns:
         Shape and dtype of ``q``.  Not differentiable.
 
-    Scores, softmax and sums are float32.
+    Scores, softmax and sums are float32.  16-bit operands round the softmax's
+    weights for the product with the values: to two numbers of their own type,
+    so that the result has its own rounding alone, where up to 16 queries and
+    heads share a kv head (17 to 32 where the tables together hold little) and
+    over shared pages; to one, which adds about as much as the rounding of the result,
+    where more do.  In float16 a weight below ``2**-38`` of a row's largest may
+    count as nothing.
     """
     name = "paged_attention"
     if _transformed():

@@ -45,7 +45,9 @@ class Rotary:
             et al., 2023), frequencies that turn more than ``ramp[1]`` times
             within the ``trained`` positions stay, those below ``ramp[0]``
             are divided by ``factor``, those between go from one to the
-            other, and ``magnitude`` is ``0.1 ln(factor) + 1``.
+            other in proportion to their turns, and ``magnitude`` is ``0.1
+            ln(factor) + 1``.  (Models whose ramp goes by the pairs' numbers,
+            between rounded bounds, take ``frequencies``.)
         factor: See ``scaling``.
         trained: Positions trained on ("yarn").
         ramp: Turns within them ("yarn").

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from _attention_reference import check
-from _paged_checks import paged_case
+from _paged_checks import normal, paged_case, table_for
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -51,3 +51,32 @@ def test_first_slots_without_a_sequence(gpu, missing, empty, batch, ended):
                            change=change)
     assert (out[:empty] == 0).all() and (empty == batch or out[empty:].abs().max() > 0)
     check(out, want, f"{empty} of {batch}")
+
+
+def test_slots_that_empty_between_replays(gpu):
+    """A captured call finds the pages where they are when it is replayed."""
+    gen = torch.Generator().manual_seed(4)
+    total, table = table_for(gen, [2300] * 64, 16, 144, shared=140)
+    ck, cv = (normal(gen, torch.bfloat16, "cuda", total, 16, 2, 64) for _ in range(2))
+    q = normal(gen, torch.bfloat16, "cuda", 64, 1, 4, 64)
+    pages = table.int().cuda()
+    starts = (2240 + torch.arange(64) % 50).cuda()
+
+    def attend():
+        return gpu.paged_attention(q, ck, cv, pages, starts=starts, shared_pages=140)
+
+    attend()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend()
+    graph.replay()
+    full = out.clone()
+    for empty in (1, 2, 40):
+        starts[:empty] = -1
+        pages[:empty] = -1
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[:empty] == 0).all() and torch.equal(out, attend())
+        # (the others' parts are the same; what is joined with them is cut another way)
+        assert (out[empty:].float() - full[empty:].float()).abs().max() <= 2.0**-7 * full.abs().max()
