@@ -207,7 +207,7 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, scale: float | Non
     Scores, softmax and sums are float32; 16-bit operands round probabilities
     to their own type for the products with values, which costs no more than
     the rounding of the result (in float16 one below ``2**-25`` of a row's
-    largest counts as nothing).  A call with gradients keeps 16 bits more of
+    largest may count as nothing).  A call with gradients keeps 16 bits more of
     each 16-bit output for them.  Gradients are summed in a fixed order; a
     visible token that is not finite reaches those of tokens near it too.
 
